@@ -42,22 +42,26 @@ def _nvcc() -> str:
     raise RuntimeError("nvcc not found")
 
 
-def _newest_header() -> float:
-    hdrs = list(CSRC.glob("*.cuh")) + list(CSRC.glob("*.h")) + list(CSRC.glob("*.inc"))
-    hdrs.append(HERE.parent / "include" / "dsdpa.h")
-    return max(h.stat().st_mtime for h in hdrs)
+def _newest_source(src: Path, dep: Path) -> float:
+    """Newest of src and the repository's headers that nvcc found it to include (infinite while that is not known)."""
+    if not dep.exists():
+        return float("inf")
+    files = [Path(f) for f in dep.read_text().replace("\\\n", " ").split(":", 1)[1].split()]
+    own = [f for f in files if HERE.parent in f.resolve().parents] + [src]
+    return max(f.stat().st_mtime if f.exists() else float("inf") for f in own)
 
 
-def _compile(src: Path, force: bool, hdr_time: float, checked: bool = False) -> Path:
+def _compile(src: Path, force: bool, checked: bool = False) -> Path:
     out_dir = OBJ / "checked" if checked else OBJ
     obj = out_dir / (src.stem + ".o")
     # -DNAME=value pairs for experiments and for the checked debug build
-    if not force and obj.exists() and obj.stat().st_mtime >= max(src.stat().st_mtime, hdr_time):
+    dep = out_dir / (src.stem + ".d")
+    if not force and obj.exists() and obj.stat().st_mtime >= _newest_source(src, dep):
         return obj
     extra = os.environ.get("DSDPA_NVCC_EXTRA", "").split()   # e.g. -DDSDPA_FWD_UNROLL=4, for experiments
     if checked:
         extra = extra + ["-DDSDPA_BOUNDS_CHECK"]
-    cmd = [_nvcc(), *NVCC_FLAGS, *extra, "-I", str(CSRC), "-c", str(src), "-o", str(obj)]
+    cmd = [_nvcc(), *NVCC_FLAGS, *extra, "-I", str(CSRC), "-MD", "-MF", str(dep), "-c", str(src), "-o", str(obj)]
     res = subprocess.run(cmd, capture_output=True, text=True)
     (out_dir / (src.stem + ".ptxas.log")).write_text(res.stderr)
     if res.returncode != 0:
@@ -77,11 +81,10 @@ def build(force: bool = False, jobs: int | None = None, checked: bool = True) ->
     (OBJ / "checked").mkdir(parents=True, exist_ok=True)
     srcs = sorted(CSRC.glob("*.cu"))
     probe_srcs = sorted((CSRC / "probes").glob("*.cu"))
-    hdr_time = _newest_header()
     work = [(s, False) for s in srcs + probe_srcs] + ([(s, True) for s in srcs] if checked else [])
     jobs = jobs or min(len(work), os.cpu_count() or 4)
     with ThreadPoolExecutor(max_workers=jobs) as pool:
-        objs = list(pool.map(lambda w: _compile(w[0], force, hdr_time, w[1]), work))
+        objs = list(pool.map(lambda w: _compile(w[0], force, w[1]), work))
     n, m = len(srcs), len(srcs) + len(probe_srcs)
     _link(LIB, objs[:n], force)
     _link(PROBES_LIB, objs[n:m], force)
