@@ -40,6 +40,12 @@ FLAG_SCATTER_GLOBAL = 0x4
 FLAG_SCATTER = 0x8
 FLAG_ROUNDED_WEIGHTS = 0x10
 
+# flags of dsdpa_masked_problem
+MASKED_CAUSAL = 0x1
+
+# drafted tokens of one dsdpa_tree_forward (DSDPA_TREE_MAX)
+TREE_MAX = 64
+
 # limit of dsdpa_backward_static_scratch (DSDPA_STATIC_SCRATCH_BYTES)
 STATIC_SCRATCH_BYTES = 64 << 20
 
@@ -66,6 +72,13 @@ EXPORTS = (
     "dsdpa_selftest_bounded_wait",
     "dsdpa_build_is_checked",
     "dsdpa_describe_plan",
+    "dsdpa_masked_forward",
+    "dsdpa_masked_backward_workspace_bytes",
+    "dsdpa_masked_backward",
+    "dsdpa_tree_workspace_bytes",
+    "dsdpa_tree_forward",
+    "dsdpa_cache_weights",
+    "dsdpa_cache_evict",
 )
 
 
@@ -81,6 +94,26 @@ class Problem(ctypes.Structure):
 class Mirrors(ctypes.Structure):
     """Mirror of ``struct dsdpa_mirrors``: second destinations of out, dq, dk, dv (0 = none)."""
     _fields_ = [("out", ctypes.c_void_p), ("dq", ctypes.c_void_p), ("dk", ctypes.c_void_p), ("dv", ctypes.c_void_p)]
+
+
+class MaskedProblem(ctypes.Structure):
+    """Mirror of ``struct dsdpa_masked_problem``."""
+    _fields_ = ([(n, ctypes.c_int) for n in ("B", "Hq", "Hkv", "Lq", "Lk", "D")] +
+                [("sm_scale", ctypes.c_float), ("softcap", ctypes.c_float), ("dtype", ctypes.c_int), ("flags", ctypes.c_uint)] +
+                [("stride_" + n, ctypes.c_longlong * 3) for n in ("q", "k", "v", "out", "dout", "dq", "dk", "dv")] +
+                [("stride_visible", ctypes.c_longlong)])
+
+
+class CacheProblem(ctypes.Structure):
+    """Mirror of ``struct dsdpa_cache_problem``."""
+    _fields_ = ([(n, ctypes.c_int) for n in ("B", "Hq", "Hkv", "T", "D", "pages", "page_size", "table_width", "slots")] +
+                [("sm_scale", ctypes.c_float), ("softcap", ctypes.c_float), ("dtype", ctypes.c_int), ("flags", ctypes.c_uint)] +
+                [("stride_" + n, ctypes.c_longlong * 3) for n in ("q", "k", "v")])
+
+
+class CacheTree(ctypes.Structure):
+    """Mirror of ``struct dsdpa_cache_tree`` (0: not given)."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("parents", "drafted", "positions", "start", "slopes")]
 
 
 class DsdpaError(RuntimeError):
@@ -140,6 +173,16 @@ def lib() -> ctypes.CDLL:
     L.dsdpa_build_is_checked.restype = ci
     L.dsdpa_describe_plan.argtypes = [pp, ctypes.c_char_p, ctypes.c_size_t]
     L.dsdpa_describe_plan.restype = ci
+    mp, cp, tp, sz = ctypes.POINTER(MaskedProblem), ctypes.POINTER(CacheProblem), ctypes.POINTER(CacheTree), ctypes.c_size_t
+    for name, restype, argtypes in (
+            ("dsdpa_masked_forward", ci, [mp] + [vp] * 7 + [ci, vp]),
+            ("dsdpa_masked_backward_workspace_bytes", sz, [mp]),
+            ("dsdpa_masked_backward", ci, [mp] + [vp] * 12 + [sz, ci, vp]),
+            ("dsdpa_tree_workspace_bytes", sz, [cp]),
+            ("dsdpa_tree_forward", ci, [cp, tp] + [vp] * 8 + [sz, ci, vp]),
+            ("dsdpa_cache_weights", ci, [cp, tp] + [vp] * 7 + [ci, vp]),
+            ("dsdpa_cache_evict", ci, [cp] + [vp] * 6 + [ci] * 3 + [vp, ci] + [vp] * 4 + [ci, vp])):
+        getattr(L, name).restype, getattr(L, name).argtypes = restype, argtypes
     _lib = L
     return L
 

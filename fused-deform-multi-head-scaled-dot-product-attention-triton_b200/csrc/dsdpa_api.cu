@@ -5,6 +5,7 @@
 #include <cstring>
 #include <atomic>
 
+#include "dsdpa_host.h"
 #include "dsdpa_launch.cuh"
 
 namespace dsdpa {
@@ -240,21 +241,6 @@ static bool use_two_pass(const dsdpa_problem& p, const GatherPlan& g) {
     return knobs().bwd_two_pass != 0;
 }
 
-static bool misaligned(const void* p) { return ((uintptr_t)p & 15u) != 0; }
-
-struct DeviceGuard {
-    int prev = -1;
-    cudaError_t err = cudaSuccess;
-    explicit DeviceGuard(int device) {
-        err = cudaGetDevice(&prev);
-        if (err == cudaSuccess && prev != device) err = cudaSetDevice(device);
-    }
-    ~DeviceGuard() {
-        int cur = -1;
-        if (prev >= 0 && cudaGetDevice(&cur) == cudaSuccess && cur != prev) (void)cudaSetDevice(prev);
-    }
-};
-
 // A mirror may lie in another GPU's memory: kernels launched on `device` (the current device)
 // must be allowed to store to it, or the first store faults.  Looked up once per pair of devices.
 static int ensure_mirror_access(const void* ptr, int device) {
@@ -296,6 +282,10 @@ static cudaError_t error_word_ptr(int device, int** out) {
     return cudaSuccess;
 }
 
+// For the library's other translation units.
+cudaError_t device_error_word(int device, int** out) { return error_word_ptr(device, out); }
+void count_launches(int n) { g_launches += (unsigned long long)n; }
+
 // ---- copy of a finished result to its mirror (scatter forms of the backward only) ---
 __global__ void __launch_bounds__(512) copy16_kernel(const uint4* __restrict__ src, uint4* __restrict__ dst, size_t n16) {
     for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < n16; i += (size_t)gridDim.x * blockDim.x)
@@ -330,7 +320,7 @@ const char* dsdpa_status_string(int status) {
         case DSDPA_ERR_DEVICE_TIMEOUT: return "a bounded wait inside a kernel gave up";
         case DSDPA_ERR_TOO_LARGE: return "problem exceeds the maximum of this entry point";
         case DSDPA_ERR_PEER_ACCESS: return "a mirror lies in memory the launching device cannot store to";
-        case DSDPA_ERR_DEVICE_BOUNDS: return "a kernel of the checked build computed an index out of range (access skipped)";
+        case DSDPA_ERR_DEVICE_BOUNDS: return "an index out of range (access skipped): a kernel of the checked build computed it, or a page table or tree holds it";
         default: return "unknown status";
     }
 }

@@ -1,0 +1,220 @@
+// C ABI of the paged cache's operators: argument checks and launches.  Declarations are in include/dsdpa.h.
+#include <math.h>
+
+#include "dsdpa_evict.cuh"
+#include "dsdpa_host.h"
+
+namespace dsdpa {
+namespace {
+
+constexpr int kRowWarps = 8;
+
+template <typename T>
+__global__ void __launch_bounds__(kRowWarps * 32) tree_rows_kernel(const CacheParams p) {
+    const long long r = (long long)blockIdx.x * kRowWarps + threadIdx.x / 32;
+    if (r < (long long)p.B * p.Hq * p.T) exact_row_tree<T>(p, (int)(r / p.T / p.Hq), (int)(r / p.T % p.Hq), (int)(r % p.T));
+}
+
+// One warp sums one key's weights over the tokens and heads.
+template <typename T>
+__global__ void __launch_bounds__(kRowWarps * 32) weights_rows_kernel(const CacheParams p) {
+    const int lane = threadIdx.x & 31;
+    const long long per = (long long)p.width * p.page_size;
+    const long long r = (long long)blockIdx.x * kRowWarps + threadIdx.x / 32;
+    if (r >= (long long)p.B * p.Hkv * per) return;
+    const int j = (int)(r % per), hk = (int)(r / per % p.Hkv), b = (int)(r / per / p.Hkv);
+    const int n = cached_keys(p, b), real = drafted_tokens(p, b);
+    if (j >= n + real) return;
+    const int index = j / p.page_size, page = page_of(p.table, p.width, p.pages, p.err, b, index);
+    if (page < 0) return;
+    float k[8], sum = 0.0f;
+    load_row<T>(row_of<T>(p.k, p.sk, 0, hk, j - index * p.page_size) + page * p.sk[0], p.D, lane, k);
+    const int base = first_position(p, b, n);
+    int at = j;
+    if (j >= n) at = base + depth_of(tokens_above(p, b, j - n));
+    else if (p.positions) at = __ldg(p.positions + ((long long)b * p.Hkv + hk) * p.slots + j);
+    for (int t = 0; t < real; ++t) {
+        if (p.take && !p.take[(long long)b * p.T + t]) continue;
+        const unsigned long long above = tokens_above(p, b, t);
+        if (j >= n && !(above >> (j - n) & 1)) continue;
+        const int pos = base + depth_of(above);
+        for (int g = 0; g < p.group; ++g) {
+            const int h = hk * p.group + g;
+            float q[8];
+            load_row<T>(row_of<T>(p.q, p.sq, b, h, t), p.D, lane, q);
+            float s = soft_cap(p.sm_scale * warp_sum(dot8(q, k)), p.cap);
+            if (p.slopes) s -= __ldg(p.slopes + h) * fabsf((float)(pos - at));
+            const float lse = p.lse[((long long)b * p.Hq + h) * p.T + t];
+            if (lse != kNegInf) sum += exp2f(s * kLog2e - lse);
+        }
+    }
+    if (lane == 0) p.weights[((long long)b * p.Hkv + hk) * p.slots + j] += sum;
+}
+
+int check(const dsdpa_cache_problem* p) {
+    if (!p) return DSDPA_ERR_NULL_POINTER;
+    if (p->dtype != DSDPA_F32 && p->dtype != DSDPA_BF16 && p->dtype != DSDPA_F16) return DSDPA_ERR_BAD_DTYPE;
+    if (p->D < 8 || p->D > 256 || p->D % 8) return DSDPA_ERR_BAD_HEAD_DIM;
+    if (p->B <= 0 || p->Hkv <= 0 || p->pages <= 0 || p->page_size <= 0 || p->table_width <= 0) return DSDPA_ERR_BAD_SHAPE;
+    if ((long long)p->table_width * p->page_size > (1ll << 30) || (long long)p->B * p->Hkv >= (1ll << 20)) return DSDPA_ERR_BAD_SHAPE;
+    if (p->flags) return DSDPA_ERR_BAD_FLAGS;
+    const int e = p->dtype == DSDPA_F32 ? 4 : 2;
+    for (int i = 0; i < 3; ++i)
+        if (p->stride_k[i] < 0 || p->stride_v[i] < 0 || p->stride_k[i] * e % 16 || p->stride_v[i] * e % 16) return DSDPA_ERR_MISALIGNED;
+    return DSDPA_OK;
+}
+int check_tokens(const dsdpa_cache_problem* p) {
+    const int st = check(p);
+    if (st != DSDPA_OK) return st;
+    if (p->Hq <= 0 || p->Hq % p->Hkv || (long long)p->B * p->Hq >= (1ll << 24) || p->T <= 0) return DSDPA_ERR_BAD_SHAPE;
+    if (p->T > kTreeMax) return DSDPA_ERR_TOO_LARGE;
+    if (!isfinite(p->sm_scale) || !isfinite(p->softcap)) return DSDPA_ERR_BAD_SHAPE;
+    const int e = p->dtype == DSDPA_F32 ? 4 : 2;
+    for (int i = 0; i < 3; ++i)
+        if (p->stride_q[i] < 0 || p->stride_q[i] * e % 16) return DSDPA_ERR_MISALIGNED;
+    return DSDPA_OK;
+}
+bool odd4(const void* p) { return ((uintptr_t)p & 3) != 0; }
+bool odd_tree(const dsdpa_cache_tree* t) {
+    return t && (odd4(t->parents) || odd4(t->drafted) || odd4(t->positions) || odd4(t->start) || odd4(t->slopes));
+}
+
+CacheParams params(const dsdpa_cache_problem& p, const dsdpa_cache_tree* t, const void* q, const void* k, const void* v,
+                   const int* table, const int* lens, int* err) {
+    CacheParams c{};
+    c.q = q; c.k = k; c.v = v; c.table = table; c.lens = lens;
+    if (t) { c.parents = t->parents; c.drafted = t->drafted; c.positions = t->positions; c.start = t->start; c.slopes = t->slopes; }
+    c.B = p.B; c.Hq = p.Hq; c.Hkv = p.Hkv; c.group = p.Hq / p.Hkv; c.T = p.T; c.D = p.D;
+    c.pages = p.pages; c.page_size = p.page_size; c.width = p.table_width; c.slots = p.slots;
+    c.sm_scale = p.sm_scale;
+    c.cap = p.softcap > 0.0f ? p.softcap : 0.0f;
+    for (int i = 0; i < 3; ++i) { c.sq[i] = p.stride_q[i]; c.sk[i] = p.stride_k[i]; c.sv[i] = p.stride_v[i]; }
+    c.err = err;
+    return c;
+}
+
+template <typename T>
+cudaError_t tree_forward(const CacheParams& p, cudaStream_t s) {
+    const long long rows = (long long)p.B * p.Hq * p.T;
+    tree_rows_kernel<T><<<(unsigned)((rows + kRowWarps - 1) / kRowWarps), kRowWarps * 32, 0, s>>>(p);
+    count_launches(1);
+    return cudaGetLastError();
+}
+template <typename T>
+cudaError_t weights_add(const CacheParams& p, cudaStream_t s) {
+    const long long rows = (long long)p.B * p.Hkv * p.width * p.page_size;
+    weights_rows_kernel<T><<<(unsigned)((rows + kRowWarps - 1) / kRowWarps), kRowWarps * 32, 0, s>>>(p);
+    count_launches(1);
+    return cudaGetLastError();
+}
+
+}  // namespace
+}  // namespace dsdpa
+
+using namespace dsdpa;
+
+extern "C" {
+
+size_t dsdpa_tree_workspace_bytes(const dsdpa_cache_problem* p) {
+    (void)p;
+    return 0;
+}
+
+int dsdpa_tree_forward(const dsdpa_cache_problem* p, const dsdpa_cache_tree* tree, const void* q, const void* k_pages,
+                       const void* v_pages, const int* page_table, const int* lens, void* out, float* lse,
+                       void* workspace, size_t workspace_bytes, int device, void* stream) {
+    const int st = check_tokens(p);
+    if (st != DSDPA_OK) return st;
+    if (!q || !k_pages || !v_pages || !page_table || !lens || !out || !lse) return DSDPA_ERR_NULL_POINTER;
+    if (misaligned(q) || misaligned(k_pages) || misaligned(v_pages) || misaligned(out) || misaligned(workspace) ||
+        odd4(page_table) || odd4(lens) || odd4(lse) || odd_tree(tree))
+        return DSDPA_ERR_MISALIGNED;
+    if (tree && tree->positions && p->slots < p->table_width * p->page_size) return DSDPA_ERR_BAD_SHAPE;
+    const size_t need = dsdpa_tree_workspace_bytes(p);
+    if (need > 0 && (!workspace || workspace_bytes < need)) return DSDPA_ERR_WORKSPACE;
+    DeviceGuard guard(device);
+    if (guard.err != cudaSuccess) return report_cuda_failure(guard.err);
+    int* err = nullptr;
+    cudaError_t e = device_error_word(device, &err);
+    if (e != cudaSuccess) return report_cuda_failure(e);
+    CacheParams c = params(*p, tree, q, k_pages, v_pages, page_table, lens, err);
+    c.out = out;
+    c.lse = lse;
+    switch (p->dtype) {
+        case DSDPA_F32: e = tree_forward<float>(c, (cudaStream_t)stream); break;
+        case DSDPA_BF16: e = tree_forward<__nv_bfloat16>(c, (cudaStream_t)stream); break;
+        default: e = tree_forward<__half>(c, (cudaStream_t)stream); break;
+    }
+    return e == cudaSuccess ? DSDPA_OK : report_cuda_failure(e);
+}
+
+int dsdpa_cache_weights(const dsdpa_cache_problem* p, const dsdpa_cache_tree* tree, const void* q, const float* lse,
+                        const void* k_pages, const int* page_table, const int* lens, const unsigned char* take,
+                        float* weights, int device, void* stream) {
+    const int st = check_tokens(p);
+    if (st != DSDPA_OK) return st;
+    if (!q || !lse || !k_pages || !page_table || !lens || !weights) return DSDPA_ERR_NULL_POINTER;
+    if (misaligned(q) || misaligned(k_pages) || odd4(lse) || odd4(page_table) || odd4(lens) || odd4(weights) || odd_tree(tree))
+        return DSDPA_ERR_MISALIGNED;
+    if (p->slots < p->table_width * p->page_size) return DSDPA_ERR_BAD_SHAPE;
+    DeviceGuard guard(device);
+    if (guard.err != cudaSuccess) return report_cuda_failure(guard.err);
+    int* err = nullptr;
+    cudaError_t e = device_error_word(device, &err);
+    if (e != cudaSuccess) return report_cuda_failure(e);
+    CacheParams c = params(*p, tree, q, k_pages, nullptr, page_table, lens, err);
+    c.lse = const_cast<float*>(lse);
+    c.take = take;
+    c.weights = weights;
+    switch (p->dtype) {
+        case DSDPA_F32: e = weights_add<float>(c, (cudaStream_t)stream); break;
+        case DSDPA_BF16: e = weights_add<__nv_bfloat16>(c, (cudaStream_t)stream); break;
+        default: e = weights_add<__half>(c, (cudaStream_t)stream); break;
+    }
+    return e == cudaSuccess ? DSDPA_OK : report_cuda_failure(e);
+}
+
+int dsdpa_cache_evict(const dsdpa_cache_problem* p, void* k_pages, void* v_pages, const int* page_table, const int* lens,
+                      const float* weights, const int* positions, int keep, int sinks, int recent,
+                      const int* out_table, int out_width, int* kept, int* new_lens, float* new_weights,
+                      int* new_positions, int device, void* stream) {
+    const int st = check(p);
+    if (st != DSDPA_OK) return st;
+    if (!k_pages || !v_pages || !page_table || !lens || !weights || !out_table || !kept || !new_lens || !new_weights)
+        return DSDPA_ERR_NULL_POINTER;
+    if (new_weights == weights || (new_positions && new_positions == positions)) return DSDPA_ERR_BAD_SHAPE;
+    if (misaligned(k_pages) || misaligned(v_pages) || odd4(page_table) || odd4(lens) || odd4(weights) || odd4(positions) ||
+        odd4(out_table) || odd4(kept) || odd4(new_lens) || odd4(new_weights) || odd4(new_positions))
+        return DSDPA_ERR_MISALIGNED;
+    if (p->slots < p->table_width * p->page_size || keep <= 0 || sinks < 0 || recent < 0 || sinks > keep || recent > keep - sinks)
+        return DSDPA_ERR_BAD_SHAPE;
+    // the kept keys have to find room in out_table, and in a row of weights
+    if (out_width <= 0 || (long long)out_width * p->page_size > (1ll << 30)) return DSDPA_ERR_BAD_SHAPE;
+    const long long most = (long long)p->table_width * p->page_size < keep ? (long long)p->table_width * p->page_size : keep;
+    if ((long long)out_width * p->page_size < most) return DSDPA_ERR_BAD_SHAPE;
+    DeviceGuard guard(device);
+    if (guard.err != cudaSuccess) return report_cuda_failure(guard.err);
+    int* err = nullptr;
+    cudaError_t e = device_error_word(device, &err);
+    if (e != cudaSuccess) return report_cuda_failure(e);
+    const int es = p->dtype == DSDPA_F32 ? 4 : 2;
+    EvictParams v{};
+    v.k = (char*)k_pages; v.v = (char*)v_pages;
+    v.table = page_table; v.lens = lens; v.positions = positions; v.out_table = out_table; v.weights = weights;
+    v.kept = kept; v.new_lens = new_lens; v.new_positions = new_positions; v.new_weights = new_weights;
+    v.B = p->B; v.Hkv = p->Hkv; v.pages = p->pages; v.page_size = p->page_size; v.width = p->table_width;
+    v.out_width = out_width; v.slots = p->slots; v.keep = keep; v.sinks = sinks; v.recent = recent;
+    v.row_bytes = p->D * es;
+    for (int i = 0; i < 3; ++i) { v.sk[i] = p->stride_k[i] * es; v.sv[i] = p->stride_v[i] * es; }
+    v.err = err;
+    cudaStream_t s = (cudaStream_t)stream;
+    evict_select_kernel<<<(unsigned)(p->B * p->Hkv), kSelectThreads, 0, s>>>(v);
+    if ((e = cudaGetLastError()) != cudaSuccess) return report_cuda_failure(e);
+    const unsigned slices = (unsigned)((v.row_bytes + 63) / 64);
+    evict_move_kernel<<<(unsigned)(p->B * p->Hkv) * 2 * slices, kMoveThreads, 0, s>>>(v);
+    if ((e = cudaGetLastError()) != cudaSuccess) return report_cuda_failure(e);
+    count_launches(2);
+    return DSDPA_OK;
+}
+
+}  // extern "C"

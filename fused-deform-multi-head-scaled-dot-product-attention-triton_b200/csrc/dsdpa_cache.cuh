@@ -1,0 +1,114 @@
+// Paged key/value cache: where a key's row lies, what a drafted token sees, and one drafted token's
+// result computed by one warp that visits the keys it sees only (the definition written out; the
+// tiled kernel hands it the rows that came out non-finite).
+#pragma once
+
+#include "dsdpa_masked.cuh"
+
+namespace dsdpa {
+
+constexpr int kTreeMax = DSDPA_TREE_MAX;
+
+struct CacheParams {
+    const void *q, *k, *v;
+    const int *table, *lens, *parents, *drafted, *positions, *start;
+    const float* slopes;
+    void* out;
+    float* lse;                // tree: written; weights: read
+    int B, Hq, Hkv, group, T, D;
+    int pages, page_size, width, slots;
+    float sm_scale, cap;
+    long long sq[3], sk[3], sv[3];
+    int* err;
+    // weights
+    const unsigned char* take;
+    float* weights;
+};
+
+// Keys that sequence b has cached, and its real drafted tokens.  Numbers that a table cannot hold are
+// cut to what it holds, and reported.
+__device__ __forceinline__ int cached_keys(const CacheParams& p, int b) {
+    const int n = __ldg(p.lens + b), room = p.width * p.page_size;
+    if (n > room) atomicCAS(p.err, 0, kErrBounds);
+    return max(0, min(n, room));
+}
+__device__ __forceinline__ int drafted_tokens(const CacheParams& p, int b) {
+    return p.drafted ? max(0, min(__ldg(p.drafted + b), p.T)) : p.T;
+}
+// The page of key number n of sequence b; -1 (and a report) where the table has no valid one.
+__device__ __forceinline__ int page_of(const int* table, int width, int pages, int* err, int b, int index) {
+    int page = -1;
+    if (index < width) page = __ldg(table + (long long)b * width + index);
+    if ((unsigned)page >= (unsigned)pages) {
+        atomicCAS(err, 0, kErrBounds);
+        return -1;
+    }
+    return page;
+}
+
+// The tokens that token t sees (bit u: token u), itself among them, from its chain of parents; its
+// depth is their number less one.  Every step goes to an earlier token, so the walk ends.
+__device__ __forceinline__ unsigned long long tokens_above(const CacheParams& p, int b, int t) {
+    if (!p.parents) return t == 63 ? ~0ull : (1ull << (t + 1)) - 1;
+    unsigned long long seen = 1ull << t;
+    int at = t;
+    while (true) {
+        const int up = __ldg(p.parents + (long long)b * p.T + at);
+        if (up < -1 || up >= at) atomicCAS(p.err, 0, kErrBounds);
+        if (up < 0 || up >= at) return seen;
+        seen |= 1ull << up;
+        at = up;
+    }
+}
+__device__ __forceinline__ int depth_of(unsigned long long above) { return __popcll(above) - 1; }
+__device__ __forceinline__ int first_position(const CacheParams& p, int b, int n) { return p.start ? __ldg(p.start + b) : n; }
+
+// out and lse of one drafted token, by one warp.
+template <typename T>
+__device__ __noinline__ void exact_row_tree(const CacheParams& p, int b, int h, int t) {
+    const int lane = threadIdx.x & 31, hk = h / p.group;
+    const int n = cached_keys(p, b), real = drafted_tokens(p, b);
+    const float slope = p.slopes ? __ldg(p.slopes + h) : 0.0f;
+    float q[8], acc[8] = {}, m = kNegInf, l = 0.0f;
+    if (t < real) {
+        const unsigned long long above = tokens_above(p, b, t);
+        const int base = first_position(p, b, n), pos = base + depth_of(above);
+        load_row<T>(row_of<T>(p.q, p.sq, b, h, t), p.D, lane, q);
+        int page = -1, page_index = -1;
+        for (int j = 0; j < n + real; ++j) {
+            if (j >= n && !(above >> (j - n) & 1)) continue;
+            const int index = j / p.page_size;
+            if (index != page_index) {
+                page_index = index;
+                page = page_of(p.table, p.width, p.pages, p.err, b, index);
+            }
+            if (page < 0) continue;
+            const int slot = j - index * p.page_size;
+            float k[8], v[8];
+            load_row<T>(row_of<T>(p.k, p.sk, 0, hk, slot) + page * p.sk[0], p.D, lane, k);
+            load_row<T>(row_of<T>(p.v, p.sv, 0, hk, slot) + page * p.sv[0], p.D, lane, v);
+            float s = soft_cap(p.sm_scale * warp_sum(dot8(q, k)), p.cap);
+            if (p.slopes) {
+                int at = j;
+                if (j >= n) at = base + depth_of(tokens_above(p, b, j - n));
+                else if (p.positions) at = __ldg(p.positions + ((long long)b * p.Hkv + hk) * p.slots + j);
+                s -= slope * fabsf((float)(pos - at));
+            }
+            s *= kLog2e;
+            if (s == kNegInf) continue;
+            const float m2 = fmaxf(m, s), c = exp2f(m - m2), w = exp2f(s - m2);
+            l = fmaf(l, c, w);
+            m = m2;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[e] = fmaf(acc[e], c, w * v[e]);
+        }
+    }
+    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] *= inv;
+    const long long row = ((long long)b * p.Hq + h) * p.T + t;
+    if (lane * 8 < p.D) store8<T>((T*)p.out + row * p.D + lane * 8, acc);
+    if (lane == 0) p.lse[row] = l != 0.0f ? m + log2f(l) : kNegInf;
+}
+
+}  // namespace dsdpa

@@ -1,0 +1,33 @@
+// What the library's C-ABI translation units share on the host side.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "../../include/dsdpa.h"
+
+namespace dsdpa {
+
+// dsdpa_api.cu: record a failed CUDA call (what dsdpa_last_cuda_error() returns); returns DSDPA_ERR_CUDA
+int report_cuda_failure(int cuda_error);
+// dsdpa_api.cu: the device's error word (what dsdpa_device_error() reads), `device` being current
+cudaError_t device_error_word(int device, int** out);
+// dsdpa_api.cu: kernels launched, for dsdpa_kernel_launches()
+void count_launches(int n);
+
+inline bool misaligned(const void* p) { return ((uintptr_t)p & 15u) != 0; }
+
+struct DeviceGuard {
+    int prev = -1;
+    cudaError_t err = cudaSuccess;
+    explicit DeviceGuard(int device) {
+        err = cudaGetDevice(&prev);
+        if (err == cudaSuccess && prev != device) err = cudaSetDevice(device);
+    }
+    ~DeviceGuard() {
+        int cur = -1;
+        if (prev >= 0 && cudaGetDevice(&cur) == cudaSuccess && cur != prev) (void)cudaSetDevice(prev);
+    }
+};
+
+}  // namespace dsdpa

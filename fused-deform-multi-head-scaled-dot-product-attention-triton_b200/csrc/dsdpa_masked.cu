@@ -1,0 +1,170 @@
+// C ABI of masked attention: argument checks and launches.  Declarations are in include/dsdpa.h.
+#include <math.h>
+
+#include "dsdpa_host.h"
+#include "dsdpa_masked.cuh"
+
+namespace dsdpa {
+namespace {
+
+constexpr int kRowWarps = 8;   // rows of a block of the row kernels, one warp each
+
+template <typename T>
+__global__ void __launch_bounds__(kRowWarps * 32) masked_rows_forward(const MaskedParams p) {
+    const long long n = (long long)p.B * p.Hq * p.Lq;
+    for (long long r = (long long)blockIdx.x * kRowWarps + threadIdx.x / 32; r < n; r += (long long)gridDim.x * kRowWarps)
+        exact_row_forward<T>(p, (int)(r / p.Lq / p.Hq), (int)(r / p.Lq % p.Hq), (int)(r % p.Lq));
+}
+template <typename T>
+__global__ void __launch_bounds__(kRowWarps * 32) masked_rows_dq(const MaskedParams p) {
+    const long long n = (long long)p.B * p.Hq * p.Lq;
+    for (long long r = (long long)blockIdx.x * kRowWarps + threadIdx.x / 32; r < n; r += (long long)gridDim.x * kRowWarps)
+        exact_row_dq<T>(p, (int)(r / p.Lq / p.Hq), (int)(r / p.Lq % p.Hq), (int)(r % p.Lq));
+}
+template <typename T>
+__global__ void __launch_bounds__(kRowWarps * 32) masked_rows_dkdv(const MaskedParams p) {
+    const long long n = (long long)p.B * p.Hkv * p.Lk;
+    for (long long r = (long long)blockIdx.x * kRowWarps + threadIdx.x / 32; r < n; r += (long long)gridDim.x * kRowWarps)
+        exact_row_dkdv<T>(p, (int)(r / p.Lk / p.Hkv), (int)(r / p.Lk % p.Hkv), (int)(r % p.Lk));
+}
+
+unsigned row_blocks(long long rows) {
+    const long long b = (rows + kRowWarps - 1) / kRowWarps;
+    return (unsigned)(b < (1ll << 30) ? b : (1ll << 30));
+}
+
+int check(const dsdpa_masked_problem* p) {
+    if (!p) return DSDPA_ERR_NULL_POINTER;
+    if (p->dtype != DSDPA_F32 && p->dtype != DSDPA_BF16 && p->dtype != DSDPA_F16) return DSDPA_ERR_BAD_DTYPE;
+    if (p->D < 8 || p->D > 256 || p->D % 8) return DSDPA_ERR_BAD_HEAD_DIM;
+    if (p->B <= 0 || p->Hq <= 0 || p->Hkv <= 0 || p->Hq % p->Hkv || p->Lq < 0 || p->Lk < 0) return DSDPA_ERR_BAD_SHAPE;
+    // positions are exact in fp32 and tile counts fit the grid
+    if (p->Lq > (1 << 24) || p->Lk > (1 << 24) || (long long)p->B * p->Hq >= (1ll << 24)) return DSDPA_ERR_BAD_SHAPE;
+    if (p->flags & ~DSDPA_MASKED_CAUSAL) return DSDPA_ERR_BAD_FLAGS;
+    if (!isfinite(p->sm_scale) || !isfinite(p->softcap)) return DSDPA_ERR_BAD_SHAPE;
+    return DSDPA_OK;
+}
+
+bool bad_stride(const long long (&st)[3], int dtype) {
+    for (long long s : st)
+        if (s < 0 || (s * (dtype == DSDPA_F32 ? 4 : 2)) % 16) return true;
+    return false;
+}
+
+MaskedParams params(const dsdpa_masked_problem& p, const void* q, const void* k, const void* v, const int* visible,
+                    const float* slopes, int* err) {
+    MaskedParams m{};
+    m.q = q; m.k = k; m.v = v;
+    m.visible = (const int2*)visible;
+    m.slopes = slopes;
+    m.B = p.B; m.Hq = p.Hq; m.Hkv = p.Hkv; m.group = p.Hq / p.Hkv; m.Lq = p.Lq; m.Lk = p.Lk; m.D = p.D;
+    m.causal = (p.flags & DSDPA_MASKED_CAUSAL) != 0;
+    m.sm_scale = p.sm_scale;
+    m.cap = p.softcap > 0.0f ? p.softcap : 0.0f;
+    m.s_visible = p.stride_visible / 2;
+    m.err = err;
+    for (int i = 0; i < 3; ++i) {
+        m.sq[i] = p.stride_q[i]; m.sk[i] = p.stride_k[i]; m.sv[i] = p.stride_v[i];
+        m.so[i] = p.stride_out[i]; m.sdo[i] = p.stride_dout[i];
+        m.sdq[i] = p.stride_dq[i]; m.sdk[i] = p.stride_dk[i]; m.sdv[i] = p.stride_dv[i];
+    }
+    return m;
+}
+
+template <typename T>
+cudaError_t forward(const MaskedParams& p, cudaStream_t s) {
+    masked_rows_forward<T><<<row_blocks((long long)p.B * p.Hq * p.Lq), kRowWarps * 32, 0, s>>>(p);
+    count_launches(1);
+    return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t backward(const MaskedParams& p, cudaStream_t s) {
+    if (p.Lq > 0) {
+        masked_rows_dq<T><<<row_blocks((long long)p.B * p.Hq * p.Lq), kRowWarps * 32, 0, s>>>(p);
+        count_launches(1);
+    }
+    if (p.Lk > 0) {
+        masked_rows_dkdv<T><<<row_blocks((long long)p.B * p.Hkv * p.Lk), kRowWarps * 32, 0, s>>>(p);
+        count_launches(1);
+    }
+    return cudaGetLastError();
+}
+
+size_t delta_bytes(const dsdpa_masked_problem& p) { return (((size_t)p.B * p.Hq * p.Lq * 4) + 255) & ~(size_t)255; }
+
+}  // namespace
+}  // namespace dsdpa
+
+using namespace dsdpa;
+
+extern "C" {
+
+int dsdpa_masked_forward(const dsdpa_masked_problem* p, const void* q, const void* k, const void* v, const int* visible,
+                         const float* slopes, void* out, float* lse, int device, void* stream) {
+    int st = check(p);
+    if (st != DSDPA_OK) return st;
+    if (p->Lq == 0) return DSDPA_OK;
+    if (!q || !out || !lse || (p->Lk > 0 && (!k || !v))) return DSDPA_ERR_NULL_POINTER;
+    if (misaligned(q) || misaligned(k) || misaligned(v) || misaligned(out) || ((uintptr_t)visible & 7) ||
+        ((uintptr_t)lse & 3) || ((uintptr_t)slopes & 3))
+        return DSDPA_ERR_MISALIGNED;
+    if (bad_stride(p->stride_q, p->dtype) || bad_stride(p->stride_k, p->dtype) || bad_stride(p->stride_v, p->dtype) ||
+        bad_stride(p->stride_out, p->dtype) || p->stride_visible % 2)
+        return DSDPA_ERR_MISALIGNED;
+    DeviceGuard guard(device);
+    if (guard.err != cudaSuccess) return report_cuda_failure(guard.err);
+    int* err = nullptr;
+    cudaError_t e = device_error_word(device, &err);
+    if (e != cudaSuccess) return report_cuda_failure(e);
+    MaskedParams m = params(*p, q, k, v, visible, slopes, err);
+    m.out = out;
+    m.lse = lse;
+    switch (p->dtype) {
+        case DSDPA_F32: e = forward<float>(m, (cudaStream_t)stream); break;
+        case DSDPA_BF16: e = forward<__nv_bfloat16>(m, (cudaStream_t)stream); break;
+        default: e = forward<__half>(m, (cudaStream_t)stream); break;
+    }
+    return e == cudaSuccess ? DSDPA_OK : report_cuda_failure(e);
+}
+
+size_t dsdpa_masked_backward_workspace_bytes(const dsdpa_masked_problem* p) {
+    return check(p) == DSDPA_OK ? delta_bytes(*p) : 0;
+}
+
+int dsdpa_masked_backward(const dsdpa_masked_problem* p, const void* q, const void* k, const void* v, const int* visible,
+                          const float* slopes, const void* out, const float* lse, const void* dout, void* dq, void* dk,
+                          void* dv, void* workspace, size_t workspace_bytes, int device, void* stream) {
+    int st = check(p);
+    if (st != DSDPA_OK) return st;
+    if (p->Lq == 0 && p->Lk == 0) return DSDPA_OK;
+    if ((p->Lq > 0 && (!q || !out || !lse || !dout || !dq)) || (p->Lk > 0 && (!k || !v || !dk || !dv)))
+        return DSDPA_ERR_NULL_POINTER;
+    if (misaligned(q) || misaligned(k) || misaligned(v) || misaligned(out) || misaligned(dout) || misaligned(dq) ||
+        misaligned(dk) || misaligned(dv) || misaligned(workspace) || ((uintptr_t)visible & 7) || ((uintptr_t)lse & 3) ||
+        ((uintptr_t)slopes & 3))
+        return DSDPA_ERR_MISALIGNED;
+    if (bad_stride(p->stride_q, p->dtype) || bad_stride(p->stride_k, p->dtype) || bad_stride(p->stride_v, p->dtype) ||
+        bad_stride(p->stride_out, p->dtype) || bad_stride(p->stride_dout, p->dtype) || bad_stride(p->stride_dq, p->dtype) ||
+        bad_stride(p->stride_dk, p->dtype) || bad_stride(p->stride_dv, p->dtype) || p->stride_visible % 2)
+        return DSDPA_ERR_MISALIGNED;
+    const size_t need = dsdpa_masked_backward_workspace_bytes(p);
+    if (need > 0 && (!workspace || workspace_bytes < need)) return DSDPA_ERR_WORKSPACE;
+    DeviceGuard guard(device);
+    if (guard.err != cudaSuccess) return report_cuda_failure(guard.err);
+    int* err = nullptr;
+    cudaError_t e = device_error_word(device, &err);
+    if (e != cudaSuccess) return report_cuda_failure(e);
+    MaskedParams m = params(*p, q, k, v, visible, slopes, err);
+    m.out_in = out; m.lse = (float*)lse; m.dout = dout;
+    m.dq = dq; m.dk = dk; m.dv = dv;
+    m.delta = (float*)workspace;
+    switch (p->dtype) {
+        case DSDPA_F32: e = backward<float>(m, (cudaStream_t)stream); break;
+        case DSDPA_BF16: e = backward<__nv_bfloat16>(m, (cudaStream_t)stream); break;
+        default: e = backward<__half>(m, (cudaStream_t)stream); break;
+    }
+    return e == cudaSuccess ? DSDPA_OK : report_cuda_failure(e);
+}
+
+}  // extern "C"

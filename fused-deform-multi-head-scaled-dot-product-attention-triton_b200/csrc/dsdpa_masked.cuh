@@ -1,0 +1,200 @@
+// Masked attention over a sequence: parameters, the score function, and one row's results computed
+// by one warp that visits visible keys (or queries) only.
+//
+// The row functions are the definition written out: any storage type, any head dimension that is a
+// multiple of 8, any mask.  The tiled kernels multiply whole tiles, where a masked probability of zero
+// meets whatever the masked row holds; a row that comes out non-finite there is computed again here,
+// so that NaN or infinity in a place that a query does not see never reaches its results.
+#pragma once
+
+#include "dsdpa_common.cuh"
+
+namespace dsdpa {
+
+struct MaskedParams {
+    const void *q, *k, *v, *out_in, *dout;
+    void *out, *dq, *dk, *dv;
+    float* lse;          // forward: written; backward: read
+    float* delta;        // backward: sum_d out dout, [B, Hq, Lq]
+    const int2* visible; // or null
+    const float* slopes; // or null
+    int B, Hq, Hkv, group, Lq, Lk, D;
+    int causal;
+    float sm_scale, cap; // cap <= 0: none
+    long long sq[3], sk[3], sv[3], so[3], sdo[3], sdq[3], sdk[3], sdv[3];
+    long long s_visible; // in int2
+    int* err;
+};
+
+constexpr float kNegInf = -__builtin_huge_valf();
+
+// Keys [x, y) that query i of batch element b sees; x >= y: none.
+__device__ __forceinline__ int2 key_range(const MaskedParams& p, int b, int i) {
+    int lo = 0, hi = p.Lk;
+    if (p.visible) {
+        const int2 r = __ldg(p.visible + b * p.s_visible + i);
+        lo = max(lo, r.x);
+        hi = min(hi, r.y);
+    }
+    if (p.causal) hi = min(hi, i + (p.Lk - p.Lq) + 1);
+    return make_int2(lo, hi);
+}
+
+__device__ __forceinline__ float warp_sum(float x) { return group_sum<32>(x); }
+
+// cap tanh(x / cap): CUDA's tanhf, whose error is a few units in the last place of the result.
+__device__ __forceinline__ float soft_cap(float x, float cap) { return cap > 0.0f ? cap * tanhf(x / cap) : x; }
+
+// Eight consecutive elements of a row, as fp32.
+template <typename T> __device__ __forceinline__ void load8(const T* p, float (&f)[8]) {
+    unpack16(ldg128_nc(p), f, (T*)nullptr);
+}
+template <> __device__ __forceinline__ void load8<float>(const float* p, float (&f)[8]) {
+    float a[4], b[4];
+    unpack16(ldg128_nc(p), a, (float*)nullptr);
+    unpack16(ldg128_nc(p + 4), b, (float*)nullptr);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { f[e] = a[e]; f[4 + e] = b[e]; }
+}
+template <typename T> __device__ __forceinline__ void store8(T* p, const float (&f)[8]) {
+    stg128(p, pack16(f, (T*)nullptr));
+}
+template <> __device__ __forceinline__ void store8<float>(float* p, const float (&f)[8]) {
+    const float a[4] = { f[0], f[1], f[2], f[3] }, b[4] = { f[4], f[5], f[6], f[7] };
+    stg128(p, pack16(a, (float*)nullptr));
+    stg128(p + 4, pack16(b, (float*)nullptr));
+}
+__device__ __forceinline__ float dot8(const float (&a)[8], const float (&b)[8]) {
+    float s = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s = fmaf(a[e], b[e], s);
+    return s;
+}
+
+template <typename T>
+__device__ __forceinline__ const T* row_of(const void* base, const long long (&st)[3], int b, int h, long long i) {
+    return (const T*)base + b * st[0] + h * st[1] + i * st[2];
+}
+template <typename T>
+__device__ __forceinline__ T* row_of(void* base, const long long (&st)[3], int b, int h, long long i) {
+    return (T*)base + b * st[0] + h * st[1] + i * st[2];
+}
+
+// Lane l of the warp holds elements 8l .. 8l+7 of a row; lanes behind the row hold zeros and load nothing.
+template <typename T>
+__device__ __forceinline__ void load_row(const T* row, int D, int lane, float (&f)[8]) {
+    if (lane * 8 < D) load8<T>(row + lane * 8, f);
+    else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = 0.0f;
+    }
+}
+
+// out and lse of one query, by one warp.
+template <typename T>
+__device__ __noinline__ void exact_row_forward(const MaskedParams& p, int b, int h, int i) {
+    const int lane = threadIdx.x & 31, hk = h / p.group;
+    const int2 r = key_range(p, b, i);
+    const int pos = i + (p.Lk - p.Lq);
+    const float slope = p.slopes ? __ldg(p.slopes + h) : 0.0f;
+    float q[8], acc[8] = {}, m = kNegInf, l = 0.0f;
+    load_row<T>(row_of<T>(p.q, p.sq, b, h, i), p.D, lane, q);
+    for (int j = r.x; j < r.y; ++j) {
+        float k[8], v[8];
+        load_row<T>(row_of<T>(p.k, p.sk, b, hk, j), p.D, lane, k);
+        load_row<T>(row_of<T>(p.v, p.sv, b, hk, j), p.D, lane, v);
+        float s = soft_cap(p.sm_scale * warp_sum(dot8(q, k)), p.cap);
+        if (p.slopes) s -= slope * fabsf((float)(pos - j));
+        s *= kLog2e;
+        if (s == kNegInf) continue;               // weight zero, whatever v holds
+        const float m2 = fmaxf(m, s), c = exp2f(m - m2), w = exp2f(s - m2);
+        l = fmaf(l, c, w);
+        m = m2;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[e] = fmaf(acc[e], c, w * v[e]);
+    }
+    const float inv = l != 0.0f ? 1.0f / l : 0.0f;   // a NaN sum stays NaN
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] *= inv;
+    if (lane * 8 < p.D) store8<T>(row_of<T>(p.out, p.so, b, h, i) + lane * 8, acc);
+    if (lane == 0) p.lse[((long long)b * p.Hq + h) * p.Lq + i] = l != 0.0f ? m + log2f(l) : kNegInf;
+}
+
+// p and d(loss)/d(sm_scale q.k) of one (query, key) pair; x = q.k, dp = dout.v
+__device__ __forceinline__ void pair_grad(const MaskedParams& p, float x, float dp, float lse, float delta, float slope,
+                                          int dist, float& w, float& ds) {
+    const float y = soft_cap(p.sm_scale * x, p.cap);
+    float s = y;
+    if (p.slopes) s -= slope * fabsf((float)dist);
+    w = lse == kNegInf ? 0.0f : exp2f(s * kLog2e - lse);
+    ds = w == 0.0f ? 0.0f : w * (dp - delta);
+    if (p.cap > 0.0f) {
+        const float t = y / p.cap;
+        ds *= 1.0f - t * t;
+    }
+}
+
+// dq of one query, by one warp; also the query's delta, which the other functions read.
+template <typename T>
+__device__ __noinline__ void exact_row_dq(const MaskedParams& p, int b, int h, int i) {
+    const int lane = threadIdx.x & 31, hk = h / p.group;
+    const int2 r = key_range(p, b, i);
+    const int pos = i + (p.Lk - p.Lq);
+    const float slope = p.slopes ? __ldg(p.slopes + h) : 0.0f;
+    const long long row = ((long long)b * p.Hq + h) * p.Lq + i;
+    const float lse = p.lse[row];
+    float q[8], o[8], go[8], acc[8] = {};
+    load_row<T>(row_of<T>(p.q, p.sq, b, h, i), p.D, lane, q);
+    load_row<T>(row_of<T>(p.out_in, p.so, b, h, i), p.D, lane, o);
+    load_row<T>(row_of<T>(p.dout, p.sdo, b, h, i), p.D, lane, go);
+    const float delta = r.x < r.y ? warp_sum(dot8(o, go)) : 0.0f;
+    for (int j = r.x; j < r.y; ++j) {
+        float k[8], v[8], w, ds;
+        load_row<T>(row_of<T>(p.k, p.sk, b, hk, j), p.D, lane, k);
+        load_row<T>(row_of<T>(p.v, p.sv, b, hk, j), p.D, lane, v);
+        pair_grad(p, warp_sum(dot8(q, k)), warp_sum(dot8(go, v)), lse, delta, slope, pos - j, w, ds);
+        if (w == 0.0f) continue;
+        ds *= p.sm_scale;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[e] = fmaf(ds, k[e], acc[e]);
+    }
+    if (lane * 8 < p.D) store8<T>(row_of<T>(p.dq, p.sdq, b, h, i) + lane * 8, acc);
+    if (lane == 0) p.delta[row] = delta;
+}
+
+// dk and dv of one key, summed over the query heads that share it, by one warp.
+template <typename T>
+__device__ __noinline__ void exact_row_dkdv(const MaskedParams& p, int b, int hk, int j) {
+    const int lane = threadIdx.x & 31;
+    float k[8], v[8], ak[8] = {}, av[8] = {};
+    load_row<T>(row_of<T>(p.k, p.sk, b, hk, j), p.D, lane, k);
+    load_row<T>(row_of<T>(p.v, p.sv, b, hk, j), p.D, lane, v);
+    const int first = p.causal ? max(0, j - (p.Lk - p.Lq)) : 0;
+    for (int g = 0; g < p.group; ++g) {
+        const int h = hk * p.group + g;
+        const float slope = p.slopes ? __ldg(p.slopes + h) : 0.0f;
+        for (int i = first; i < p.Lq; ++i) {
+            const int2 r = key_range(p, b, i);
+            if (j < r.x || j >= r.y) continue;
+            const long long row = ((long long)b * p.Hq + h) * p.Lq + i;
+            float q[8], go[8], w, ds;
+            load_row<T>(row_of<T>(p.q, p.sq, b, h, i), p.D, lane, q);
+            load_row<T>(row_of<T>(p.dout, p.sdo, b, h, i), p.D, lane, go);
+            pair_grad(p, warp_sum(dot8(q, k)), warp_sum(dot8(go, v)), p.lse[row], p.delta[row], slope,
+                      i + (p.Lk - p.Lq) - j, w, ds);
+            if (w == 0.0f) continue;
+            ds *= p.sm_scale;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                ak[e] = fmaf(ds, q[e], ak[e]);
+                av[e] = fmaf(w, go[e], av[e]);
+            }
+        }
+    }
+    if (lane * 8 < p.D) {
+        store8<T>(row_of<T>(p.dk, p.sdk, b, hk, j) + lane * 8, ak);
+        store8<T>(row_of<T>(p.dv, p.sdv, b, hk, j) + lane * 8, av);
+    }
+}
+
+}  // namespace dsdpa

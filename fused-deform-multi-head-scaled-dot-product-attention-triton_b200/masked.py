@@ -1,0 +1,215 @@
+"""Attention over a sequence: ``masked_sdpa(q, k, v, sm_scale, ...)``.
+
+Scores may be capped by a tanh and get a bias that falls with distance; which keys a query sees is given
+as one range of keys per query (documents, prefixes, windows, padding: ``visible_ranges``) and ``causal``.
+The device work is libdeform_sdpa.so's, through the C ABI of ``include/dsdpa.h``, which has the formulas.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import cabi, op
+
+
+def _usable(t):
+    """Rows contiguous and 16-byte aligned, no dimension broadcast: what the kernels read as it lies."""
+    e = t.element_size()
+    return (t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and
+            all(st > 0 and st * e % 16 == 0 for st, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1) and
+            all(st * e % 16 == 0 and st >= 0 for st in t.stride()[:-1]))
+
+
+def _as_rows(t):
+    t = t.detach()
+    if not _usable(t):
+        t = t.contiguous()
+        if t.data_ptr() % 16:
+            t = t.clone()
+    return t
+
+
+def _check_inputs(q, k, v, sm_scale, softcap, visible, slopes, name):
+    if not (q.is_cuda and k.is_cuda and v.is_cuda):
+        raise RuntimeError(f"{name}: tensors must live on a CUDA device (there is no CPU path)")
+    if q.dim() != 4 or k.dim() != 4:
+        raise ValueError(f"{name}: q must be [B, heads, Lq, D], k and v [B, kv_heads, Lk, D]")
+    if k.shape != v.shape:
+        raise ValueError(f"{name}: k and v shapes differ: {tuple(k.shape)}, {tuple(v.shape)}")
+    if not (q.dtype == k.dtype == v.dtype):
+        raise ValueError(f"{name}: q, k, v dtypes differ")
+    if q.dtype not in op._DTYPES:
+        raise NotImplementedError(f"{name}: unsupported dtype {q.dtype}")
+    if not (q.device == k.device == v.device):
+        raise ValueError(f"{name}: tensors are on different devices")
+    B, Hq, Lq, D = q.shape
+    if k.shape[0] != B or k.shape[3] != D:
+        raise ValueError(f"{name}: q {tuple(q.shape)} and k {tuple(k.shape)} do not fit")
+    if k.shape[1] == 0 or Hq % k.shape[1]:
+        raise ValueError(f"{name}: {Hq} query heads are no multiple of {k.shape[1]} key/value heads")
+    if D % 8 or not 8 <= D <= 256:
+        raise ValueError(f"{name}: head dim {D} is not a multiple of 8 in 8 .. 256")
+    _check_numbers(sm_scale, softcap, name)
+    _check_slopes(slopes, Hq, q.device, name)
+    if visible is not None:
+        if visible.dtype != torch.int32 or visible.shape[-2:] != (Lq, 2) or \
+                not (visible.dim() == 2 or (visible.dim() == 3 and visible.shape[0] in (1, B))):
+            raise ValueError(f"{name}: visible must be int32 [B, Lq, 2] (or [Lq, 2]), got {visible.dtype} {tuple(visible.shape)}")
+        if visible.device != q.device:
+            raise ValueError(f"{name}: visible is on another device")
+
+
+def _check_numbers(sm_scale, softcap, name):
+    if not math.isfinite(sm_scale) or not math.isfinite(softcap) or softcap < 0:
+        raise ValueError(f"{name}: sm_scale must be finite and softcap finite and not negative")
+
+
+def _check_slopes(slopes, heads, device, name):
+    if slopes is None:
+        return
+    if slopes.requires_grad:
+        raise ValueError(f"{name}: slopes get no gradient; pass slopes.detach()")
+    if slopes.dtype != torch.float32 or tuple(slopes.shape) != (heads,) or slopes.device != device:
+        raise ValueError(f"{name}: slopes must be fp32 [{heads}] on {device}")
+
+
+def _mask_args(q, visible, slopes):
+    """visible and slopes as the library takes them, and the batch stride of visible."""
+    stride = 0
+    if visible is not None:
+        if visible.dim() == 2:
+            visible = visible.unsqueeze(0)
+        if visible.shape[0] == 1 or visible.stride(0) == 0:
+            visible = visible[:1]
+        visible = visible.contiguous()
+        if visible.data_ptr() % 8:
+            visible = visible.clone()
+        stride = 0 if visible.shape[0] == 1 else visible.stride(0)
+    return visible, slopes.contiguous() if slopes is not None else None, stride
+
+
+def _problem(q, k, sm_scale, softcap, causal, stride_visible, /, **rows):
+    prob = cabi.MaskedProblem(q.shape[0], q.shape[1], k.shape[1], q.shape[2], k.shape[2], q.shape[3], float(sm_scale),
+                              float(softcap), op._DTYPES[q.dtype], cabi.MASKED_CAUSAL if causal else 0)
+    for name, t in rows.items():
+        setattr(prob, "stride_" + name, (ctypes.c_longlong * 3)(*t.stride()[:3]))
+    prob.stride_visible = stride_visible
+    return prob
+
+
+def masked_forward_raw(q, k, v, sm_scale=None, *, causal=False, visible=None, softcap=0.0, slopes=None):
+    """Forward through the C ABI.  Returns ``(out, lse)``, lse fp32 [B, heads, Lq] in base 2; no autograd.
+
+    Arguments as for ``masked_sdpa``."""
+    sm_scale = q.shape[-1] ** -0.5 if sm_scale is None else float(sm_scale)
+    _check_inputs(q, k, v, sm_scale, softcap, visible, slopes, "masked_sdpa")
+    q, k, v = _as_rows(q), _as_rows(k), _as_rows(v)
+    out = torch.empty_like(q)
+    lse = torch.empty(q.shape[:3], device=q.device, dtype=torch.float32)
+    if lse.numel() == 0:
+        return out, lse
+    visible, slopes, stride = _mask_args(q, visible, slopes)
+    prob = _problem(q, k, sm_scale, softcap, causal, stride, q=q, k=k, v=v, out=out)
+    stream = torch.cuda.current_stream(q.device).cuda_stream
+    p = op._ptr
+    cabi.check(cabi.lib().dsdpa_masked_forward(ctypes.byref(prob), p(q), p(k), p(v), p(visible), p(slopes), p(out), p(lse),
+                                               q.device.index, ctypes.c_void_p(stream)))
+    return out, lse
+
+
+def masked_backward_raw(q, k, v, out, lse, dout, sm_scale=None, *, causal=False, visible=None, softcap=0.0, slopes=None):
+    """Backward through the C ABI.  Returns ``(dq, dk, dv)``; ``out`` and ``lse`` are the forward's."""
+    sm_scale = q.shape[-1] ** -0.5 if sm_scale is None else float(sm_scale)
+    _check_inputs(q, k, v, sm_scale, softcap, visible, slopes, "masked_sdpa")
+    if out.shape != q.shape or dout.shape != q.shape or lse.shape != q.shape[:3]:
+        raise ValueError("masked_sdpa: out, dout and lse must have the shapes of the forward's results")
+    if out.dtype != q.dtype or lse.dtype != torch.float32 or not (out.device == lse.device == dout.device == q.device):
+        raise ValueError("masked_sdpa: out and lse must be the forward's results")
+    q, k, v, out, dout = _as_rows(q), _as_rows(k), _as_rows(v), _as_rows(out), _as_rows(dout.to(q.dtype))
+    lse = lse.contiguous()
+    dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+    if q.shape[0] == 0 or q.shape[1] == 0 or (q.shape[2] == 0 and k.shape[2] == 0):
+        return dq, dk, dv
+    visible, slopes, stride = _mask_args(q, visible, slopes)
+    prob = _problem(q, k, sm_scale, softcap, causal, stride, q=q, k=k, v=v, out=out, dout=dout, dq=dq, dk=dk, dv=dv)
+    L = cabi.lib()
+    n = int(L.dsdpa_masked_backward_workspace_bytes(ctypes.byref(prob)))
+    ws = torch.empty(n, device=q.device, dtype=torch.uint8) if n else None
+    stream = torch.cuda.current_stream(q.device).cuda_stream
+    p = op._ptr
+    cabi.check(L.dsdpa_masked_backward(ctypes.byref(prob), p(q), p(k), p(v), p(visible), p(slopes), p(out), p(lse), p(dout),
+                                       p(dq), p(dk), p(dv), p(ws), n, q.device.index, ctypes.c_void_p(stream)))
+    return dq, dk, dv
+
+
+class _MaskedSDPA(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, sm_scale, causal, visible, softcap, slopes):
+        out, lse = masked_forward_raw(q, k, v, sm_scale, causal=causal, visible=visible, softcap=softcap, slopes=slopes)
+        ctx.save_for_backward(q, k, v, out, lse, visible, slopes)
+        ctx.sm_scale, ctx.causal, ctx.softcap = sm_scale, causal, softcap
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        q, k, v, out, lse, visible, slopes = ctx.saved_tensors
+        dq, dk, dv = masked_backward_raw(q, k, v, out, lse, dout, ctx.sm_scale, causal=ctx.causal, visible=visible,
+                                         softcap=ctx.softcap, slopes=slopes)
+        if op.check_device_errors:
+            cabi.check(cabi.lib().dsdpa_device_error(q.device.index))
+        return dq, dk, dv, None, None, None, None, None
+
+
+def masked_sdpa(q, k, v, sm_scale=None, *, causal=False, visible=None, softcap=0.0, slopes=None):
+    """Attention of q [B, heads, Lq, D] over k, v [B, kv_heads, Lk, D]; returns out, of q's shape.
+
+    ``sm_scale``: factor of q.k, ``D ** -0.5`` by default.  ``causal``: query i sees keys up to ``i + Lk - Lq``.
+    ``visible``: int32 [B, Lq, 2] (or [Lq, 2], the same for every batch element): query i sees keys
+    ``lo <= j < hi`` only.  ``softcap``: scores become ``softcap * tanh(score / softcap)``; 0: none.
+    ``slopes``: fp32 [heads]; ``slopes[h] * |i + Lk - Lq - j|`` is taken off the (capped) scores.
+    Query heads in groups of ``heads // kv_heads`` share a key/value head.  D is a multiple of 8 up to 256.
+    A query that sees no key gives zeros; keys it does not see have no part in its result, whatever they
+    hold.  Gradients for q, k and v, bit-reproducible."""
+    sm_scale = q.shape[-1] ** -0.5 if sm_scale is None else float(sm_scale)
+    return _MaskedSDPA.apply(q, k, v, sm_scale, bool(causal), visible, float(softcap), slopes)
+
+
+def visible_ranges(lengths, total=None, *, prefix=0, causal=True, window=None, device=None):
+    """``visible`` of ``masked_sdpa`` for self-attention over packed documents: int32 [total, 2] from the lengths of
+    the documents that lie one behind the other (a list, or a list of such lists for a batch: [B, total, 2]).
+
+    A token sees its own document only: all of it, or with ``causal`` what lies before it and itself.  The
+    first ``prefix`` tokens of every document (a number, or one per document) see one another in any case.
+    ``window``: not further back than that many tokens, itself among them.  Tokens behind the last document,
+    up to ``total``, are padding and see nothing."""
+    if len(lengths) and isinstance(lengths[0], (list, tuple)):
+        if total is None:
+            total = max(sum(x) for x in lengths)
+        each = prefix if isinstance(prefix, (list, tuple)) else [prefix] * len(lengths)
+        if len(each) != len(lengths):
+            raise ValueError("visible_ranges: prefix does not fit the batch")
+        return torch.stack([visible_ranges(x, total, prefix=f, causal=causal, window=window, device=device)
+                            for x, f in zip(lengths, each)])
+    used = sum(lengths)
+    total = used if total is None else int(total)
+    if any(n < 0 for n in lengths) or used > total:
+        raise ValueError(f"visible_ranges: lengths {lengths} do not fit {total} tokens")
+    if window is not None and window < 1:
+        raise ValueError("visible_ranges: window must be at least 1")
+    fixes = list(prefix) if isinstance(prefix, (list, tuple)) else [prefix] * len(lengths)
+    if len(fixes) != len(lengths) or any(f < 0 for f in fixes):
+        raise ValueError("visible_ranges: prefix must be one number, or one per document, not negative")
+    n = torch.tensor(list(lengths), dtype=torch.int64)
+    start = torch.repeat_interleave(torch.cumsum(n, 0) - n, n)
+    end = start + torch.repeat_interleave(n, n)
+    fix = torch.minimum(start + torch.repeat_interleave(torch.tensor(fixes, dtype=torch.int64), n), end)
+    at = torch.arange(used)
+    hi = torch.maximum(at + 1, torch.where(at < fix, fix, start)) if causal else end
+    lo = start if window is None else torch.where(at < fix, start, torch.maximum(start, at + 1 - window))
+    out = torch.zeros(total, 2, dtype=torch.int32)
+    out[:used, 0], out[:used, 1] = lo.int(), hi.int()
+    return out.to(device) if device is not None else out

@@ -47,8 +47,9 @@ typedef enum dsdpa_status {
     DSDPA_ERR_DEVICE_TIMEOUT = 9,  /* a bounded wait inside a kernel gave up (dsdpa_device_error) */
     DSDPA_ERR_TOO_LARGE = 10,      /* beyond a stated maximum of the entry point */
     DSDPA_ERR_PEER_ACCESS = 11,    /* a mirror lies in memory the launching device cannot store to */
-    DSDPA_ERR_DEVICE_BOUNDS = 12   /* checked build only: a kernel computed an index out of range and
-                                      skipped the access (dsdpa_device_error) */
+    DSDPA_ERR_DEVICE_BOUNDS = 12   /* an index out of range, its access skipped (dsdpa_device_error): one
+                                      that a kernel computed (checked build only), or one that a page
+                                      table or a tree of drafted tokens holds */
 } dsdpa_status;
 
 typedef enum dsdpa_dtype {
@@ -235,8 +236,8 @@ int dsdpa_last_cuda_error(void);
 /*
  * Synchronises `device` and returns DSDPA_ERR_DEVICE_TIMEOUT if any kernel of this
  * library recorded that a bounded wait ran out since the last call (clearing the
- * record), DSDPA_ERR_DEVICE_BOUNDS if a kernel of the checked build found an index out of
- * range, DSDPA_OK otherwise.  A kernel that gave up returns without writing its results, and
+ * record), DSDPA_ERR_DEVICE_BOUNDS if a kernel of the checked build, or one that reads a page
+ * table or a tree, found an index out of range, DSDPA_OK otherwise.  A kernel that gave up returns without writing its results, and
  * nothing else reports that: callers who need to know poll this function.
  */
 int dsdpa_device_error(int device);
@@ -258,6 +259,129 @@ int dsdpa_build_is_checked(void);
  * terminated) with a one-line description (paths, tile sizes, shared memory).
  */
 int dsdpa_describe_plan(const dsdpa_problem* p, char* text, size_t cap);
+
+/* ================================================================================================
+ * Sequence attention and its key/value cache.  (No counterpart in the reference, whose one operator
+ * attends over sampled pixels; these attend over the sequence that such features are part of.)
+ *
+ * Scores, for query i of head h and key j of the key/value head that h's group shares:
+ *     x = sm_scale q_i.k_j     y = softcap tanh(x / softcap) where softcap > 0, else x
+ *     s = y - slopes[h] |position(i) - position(j)|      (slopes NULL: s = y)
+ *     p = softmax of s over the visible keys,  out_i = sum_j p_ij v_j,  lse = log2 sum_j exp(s_ij)
+ * A query that sees no key gives out = 0 and lse = -inf, and zero gradients; so does one all of
+ * whose scores are -inf.  Keys that a query does not see have no part in its results, whatever
+ * they hold, NaN and infinity included; nor have queries that do not see a key in its gradients.
+ * Strides are in elements; the last dimension (D) is contiguous.  Row starts are 16-byte aligned:
+ * stride * element size is a multiple of 16 and so is every address.  D is a multiple of 8 up to 256.
+ * Hq is a multiple of Hkv; query heads h*Hq/Hkv .. (h+1)*Hq/Hkv - 1 share key/value head h.
+ * ============================================================================================== */
+
+/* flags of dsdpa_masked_problem */
+#define DSDPA_MASKED_CAUSAL 0x1u   /* query i sees keys j <= i + Lk - Lq only */
+
+typedef struct dsdpa_masked_problem {
+    int B, Hq, Hkv;
+    int Lq, Lk;              /* 0 is allowed */
+    int D;
+    float sm_scale, softcap; /* softcap <= 0: no cap */
+    int dtype;               /* of q, k, v, out, dout, dq, dk, dv */
+    unsigned flags;
+    long long stride_q[3], stride_k[3], stride_v[3];     /* batch, head, row */
+    long long stride_out[3], stride_dout[3];
+    long long stride_dq[3], stride_dk[3], stride_dv[3];
+    long long stride_visible;                            /* batch stride of `visible`, in 32-bit words */
+} dsdpa_masked_problem;
+
+/*
+ * Attention over a sequence.  position(i) = i + Lk - Lq for queries, position(j) = j for keys.
+ * visible: NULL, or int32 [B][Lq][2], 8-byte aligned: query i sees keys lo <= j < hi only (clipped to
+ *          [0, Lk); lo >= hi: none).  This is how documents, prefixes, windows and padding are given.
+ * slopes:  NULL, or fp32 [Hq].
+ * out is written with stride_out, lse is [B, Hq, Lq] contiguous.
+ */
+int dsdpa_masked_forward(const dsdpa_masked_problem* p, const void* q, const void* k, const void* v,
+                         const int* visible, const float* slopes, void* out, float* lse, int device, void* stream);
+
+/* Bytes of scratch dsdpa_masked_backward needs (its contents need no preparation). */
+size_t dsdpa_masked_backward_workspace_bytes(const dsdpa_masked_problem* p);
+
+/*
+ * Gradients of dsdpa_masked_forward, given its out and lse.  dk and dv are summed over the query
+ * heads that share them.  Bit-reproducible: every result has one writer and a fixed order of sums.
+ */
+int dsdpa_masked_backward(const dsdpa_masked_problem* p, const void* q, const void* k, const void* v,
+                          const int* visible, const float* slopes, const void* out, const float* lse, const void* dout,
+                          void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes, int device, void* stream);
+
+/*
+ * A paged key/value cache.  A pool of `pages` pages holds page_size keys each: row (page, head, slot)
+ * of k_pages at stride_k.  Sequence b's key number n lies in slot n % page_size of page
+ * page_table[b*table_width + n / page_size].  lens[b] keys are cached and seen by every query of b;
+ * the T drafted tokens' own keys are keys lens[b] .. lens[b]+T-1.
+ * A page number outside [0, pages), or a key number beyond the table, is not read: the key counts as
+ * absent, and dsdpa_device_error() answers DSDPA_ERR_DEVICE_BOUNDS once.
+ */
+typedef struct dsdpa_cache_problem {
+    int B, Hq, Hkv, T, D;
+    int pages, page_size, table_width;
+    int slots;               /* row length of weights and positions: at least table_width * page_size */
+    float sm_scale, softcap;
+    int dtype;               /* of q, k_pages, v_pages, out */
+    unsigned flags;          /* 0 */
+    long long stride_q[3];                /* batch, head, token */
+    long long stride_k[3], stride_v[3];   /* page, head, slot */
+} dsdpa_cache_problem;
+
+/* What the drafted tokens are (any pointer may be NULL). */
+typedef struct dsdpa_cache_tree {
+    const int* parents;   /* [B, T]: the drafted token (an earlier one) that t follows, -1: none.  t sees the
+                             cached keys, itself and the tokens above it.  NULL: t follows t - 1.  A value
+                             outside [-1, t) is taken for -1 and reported as above */
+    const int* drafted;   /* [B]: tokens of the sequence's T that are real; the others' results are those of
+                             a query that sees no key.  NULL: all */
+    const int* positions; /* [B, Hkv, slots]: position of each cached key.  NULL: its number */
+    const int* start;     /* [B]: position of a drafted token without parent.  NULL: lens[b].  A token below
+                             another has the next position */
+    const float* slopes;  /* fp32 [Hq] */
+} dsdpa_cache_tree;
+
+#define DSDPA_TREE_MAX 64   /* drafted tokens of a call */
+
+/*
+ * Attention of T drafted tokens (1 .. DSDPA_TREE_MAX, one: ordinary decoding) over a cache.
+ * out [B, Hq, T, D] and lse [B, Hq, T] are contiguous.
+ */
+size_t dsdpa_tree_workspace_bytes(const dsdpa_cache_problem* p);
+int dsdpa_tree_forward(const dsdpa_cache_problem* p, const dsdpa_cache_tree* tree, const void* q, const void* k_pages,
+                       const void* v_pages, const int* page_table, const int* lens, void* out, float* lse,
+                       void* workspace, size_t workspace_bytes, int device, void* stream);
+
+/*
+ * Accumulated attention weight: weights[b, h, n] += sum over the query heads of h's group and the tokens t
+ * with take[b, t] != 0 (take NULL: all real ones) of p_tn, p from the lse that dsdpa_tree_forward gave.
+ * weights is fp32 [B, Hkv, slots]; one writer per element, fixed order of sums.
+ */
+int dsdpa_cache_weights(const dsdpa_cache_problem* p, const dsdpa_cache_tree* tree, const void* q, const float* lse,
+                        const void* k_pages, const int* page_table, const int* lens, const unsigned char* take,
+                        float* weights, int device, void* stream);
+
+/*
+ * Eviction.  Sequences longer than `keep` keep, for every key/value head by itself, their first `sinks`
+ * keys, their last `recent` ones and the heaviest of those between (equal weights: the lowest number;
+ * NaN is lighter than any number), `keep` in all and in their order; others keep everything.
+ *   kept        int32 [B, Hkv, keep]: numbers of the kept keys, ascending, -1 behind the last
+ *   new_lens    int32 [B]
+ *   new_weights fp32 [B, Hkv, slots]: the kept keys' weights, 0 behind the last
+ *   new_positions int32 [B, Hkv, slots] or NULL: positions (NULL: numbers) of the kept keys, 0 behind
+ * Their rows of k_pages and v_pages are copied to keys 0 .. new_lens-1 of out_table [B, out_width].  Where
+ * out_table is page_table itself the sequence is compacted in place.  Otherwise the pages of out_table hold
+ * none of the sequences' keys, and the old rows stay as they were.  Rows behind the last kept one
+ * are left as they were.  p->T, Hq, sm_scale and softcap play no part.
+ */
+int dsdpa_cache_evict(const dsdpa_cache_problem* p, void* k_pages, void* v_pages, const int* page_table, const int* lens,
+                      const float* weights, const int* positions, int keep, int sinks, int recent,
+                      const int* out_table, int out_width, int* kept, int* new_lens, float* new_weights,
+                      int* new_positions, int device, void* stream);
 
 #ifdef __cplusplus
 }
