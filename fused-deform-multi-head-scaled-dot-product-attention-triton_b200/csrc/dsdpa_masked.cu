@@ -1,10 +1,34 @@
 // C ABI of masked attention: argument checks and launches.  Declarations are in include/dsdpa.h.
+#include <cudaTypedefs.h>
 #include <math.h>
 
 #include "dsdpa_host.h"
 #include "dsdpa_masked.cuh"
+#include "dsdpa_masked_launch.h"
 
 namespace dsdpa {
+
+cudaError_t tensor_map_16(CUtensorMap* map, int dtype, const void* base, int D, int rows, int L, int H, int B, const long long (&stride)[3]) {
+    // a driver call, reached through the runtime: the library links no driver library
+    static PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
+    if (!encode) {
+        void* fn = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        const cudaError_t e = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &found);
+        if (e != cudaSuccess) return e;
+        if (!fn || found != cudaDriverEntryPointSuccess) return cudaErrorNotSupported;
+        encode = (PFN_cuTensorMapEncodeTiled_v12000)fn;
+    }
+    const cuuint64_t dims[4] = { (cuuint64_t)D, (cuuint64_t)L, (cuuint64_t)H, (cuuint64_t)B };
+    const cuuint64_t strides[3] = { L > 1 ? (cuuint64_t)stride[2] * 2 : 16, H > 1 ? (cuuint64_t)stride[1] * 2 : 16,
+                                    B > 1 ? (cuuint64_t)stride[0] * 2 : 16 };
+    const cuuint32_t box[4] = { 64, (cuuint32_t)rows, 1, 1 }, step[4] = { 1, 1, 1, 1 };
+    const CUresult r = encode(map, dtype == DSDPA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                              const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
 namespace {
 
 constexpr int kRowWarps = 8;   // rows of a block of the row kernels, one warp each
@@ -45,11 +69,15 @@ int check(const dsdpa_masked_problem* p) {
     return DSDPA_OK;
 }
 
-bool bad_stride(const long long (&st)[3], int dtype) {
-    for (long long s : st)
-        if (s < 0 || (s * (dtype == DSDPA_F32 ? 4 : 2)) % 16) return true;
+// Strides of dimensions that have one element do not matter.
+bool bad_stride(const long long (&st)[3], int dtype, int B, int H, int L) {
+    const int n[3] = { B, H, L };
+    for (int i = 0; i < 3; ++i)
+        if (n[i] > 1 && (st[i] <= 0 || (st[i] * (dtype == DSDPA_F32 ? 4 : 2)) % 16)) return true;
     return false;
 }
+bool bad_q(const long long (&st)[3], const dsdpa_masked_problem* p) { return bad_stride(st, p->dtype, p->B, p->Hq, p->Lq); }
+bool bad_k(const long long (&st)[3], const dsdpa_masked_problem* p) { return bad_stride(st, p->dtype, p->B, p->Hkv, p->Lk); }
 
 MaskedParams params(const dsdpa_masked_problem& p, const void* q, const void* k, const void* v, const int* visible,
                     const float* slopes, int* err) {
@@ -71,8 +99,19 @@ MaskedParams params(const dsdpa_masked_problem& p, const void* q, const void* k,
     return m;
 }
 
+// The tensor-core kernels take 16-bit storage with up to 128 elements a row; the row kernels the rest.
+template <typename T>
+bool on_tensor_cores(const MaskedParams& p) {
+    return DtypeOf<T>::value != DSDPA_F32 && p.D <= 128 && p.Lq > 0 && p.Lk > 0;
+}
+
 template <typename T>
 cudaError_t forward(const MaskedParams& p, cudaStream_t s) {
+    if constexpr (DtypeOf<T>::value != DSDPA_F32)
+        if (on_tensor_cores<T>(p)) {
+            count_launches(1);
+            return launch_masked_fwd_tc<T>(p, s);
+        }
     masked_rows_forward<T><<<row_blocks((long long)p.B * p.Hq * p.Lq), kRowWarps * 32, 0, s>>>(p);
     count_launches(1);
     return cudaGetLastError();
@@ -109,8 +148,7 @@ int dsdpa_masked_forward(const dsdpa_masked_problem* p, const void* q, const voi
     if (misaligned(q) || misaligned(k) || misaligned(v) || misaligned(out) || ((uintptr_t)visible & 7) ||
         ((uintptr_t)lse & 3) || ((uintptr_t)slopes & 3))
         return DSDPA_ERR_MISALIGNED;
-    if (bad_stride(p->stride_q, p->dtype) || bad_stride(p->stride_k, p->dtype) || bad_stride(p->stride_v, p->dtype) ||
-        bad_stride(p->stride_out, p->dtype) || p->stride_visible % 2)
+    if (bad_q(p->stride_q, p) || bad_k(p->stride_k, p) || bad_k(p->stride_v, p) || bad_q(p->stride_out, p) || p->stride_visible % 2)
         return DSDPA_ERR_MISALIGNED;
     DeviceGuard guard(device);
     if (guard.err != cudaSuccess) return report_cuda_failure(guard.err);
@@ -144,9 +182,8 @@ int dsdpa_masked_backward(const dsdpa_masked_problem* p, const void* q, const vo
         misaligned(dk) || misaligned(dv) || misaligned(workspace) || ((uintptr_t)visible & 7) || ((uintptr_t)lse & 3) ||
         ((uintptr_t)slopes & 3))
         return DSDPA_ERR_MISALIGNED;
-    if (bad_stride(p->stride_q, p->dtype) || bad_stride(p->stride_k, p->dtype) || bad_stride(p->stride_v, p->dtype) ||
-        bad_stride(p->stride_out, p->dtype) || bad_stride(p->stride_dout, p->dtype) || bad_stride(p->stride_dq, p->dtype) ||
-        bad_stride(p->stride_dk, p->dtype) || bad_stride(p->stride_dv, p->dtype) || p->stride_visible % 2)
+    if (bad_q(p->stride_q, p) || bad_k(p->stride_k, p) || bad_k(p->stride_v, p) || bad_q(p->stride_out, p) || bad_q(p->stride_dout, p) ||
+        bad_q(p->stride_dq, p) || bad_k(p->stride_dk, p) || bad_k(p->stride_dv, p) || p->stride_visible % 2)
         return DSDPA_ERR_MISALIGNED;
     const size_t need = dsdpa_masked_backward_workspace_bytes(p);
     if (need > 0 && (!workspace || workspace_bytes < need)) return DSDPA_ERR_WORKSPACE;
