@@ -118,7 +118,9 @@ cudaError_t forward(const MaskedParams& p, cudaStream_t s) {
 }
 
 template <typename T>
-cudaError_t backward(const MaskedParams& p, cudaStream_t s) {
+cudaError_t backward(const MaskedParams& p, void* workspace, cudaStream_t s) {
+    if constexpr (DtypeOf<T>::value != DSDPA_F32)
+        if (on_tensor_cores<T>(p)) return launch_masked_bwd_tc<T>(p, workspace, s);
     if (p.Lq > 0) {
         masked_rows_dq<T><<<row_blocks((long long)p.B * p.Hq * p.Lq), kRowWarps * 32, 0, s>>>(p);
         count_launches(1);
@@ -130,7 +132,10 @@ cudaError_t backward(const MaskedParams& p, cudaStream_t s) {
     return cudaGetLastError();
 }
 
-size_t delta_bytes(const dsdpa_masked_problem& p) { return (((size_t)p.B * p.Hq * p.Lq * 4) + 255) & ~(size_t)255; }
+size_t backward_bytes(const dsdpa_masked_problem& p) {
+    const MaskedBwdSpace w = masked_bwd_space(p.dtype, p.B, p.Hq, p.Hkv, p.Lq);
+    return p.dtype != DSDPA_F32 && p.D <= 128 ? w.bytes : w.stats;
+}
 
 }  // namespace
 }  // namespace dsdpa
@@ -167,7 +172,7 @@ int dsdpa_masked_forward(const dsdpa_masked_problem* p, const void* q, const voi
 }
 
 size_t dsdpa_masked_backward_workspace_bytes(const dsdpa_masked_problem* p) {
-    return check(p) == DSDPA_OK ? delta_bytes(*p) : 0;
+    return check(p) == DSDPA_OK ? backward_bytes(*p) : 0;
 }
 
 int dsdpa_masked_backward(const dsdpa_masked_problem* p, const void* q, const void* k, const void* v, const int* visible,
@@ -197,9 +202,9 @@ int dsdpa_masked_backward(const dsdpa_masked_problem* p, const void* q, const vo
     m.dq = dq; m.dk = dk; m.dv = dv;
     m.delta = (float*)workspace;
     switch (p->dtype) {
-        case DSDPA_F32: e = backward<float>(m, (cudaStream_t)stream); break;
-        case DSDPA_BF16: e = backward<__nv_bfloat16>(m, (cudaStream_t)stream); break;
-        default: e = backward<__half>(m, (cudaStream_t)stream); break;
+        case DSDPA_F32: e = backward<float>(m, workspace, (cudaStream_t)stream); break;
+        case DSDPA_BF16: e = backward<__nv_bfloat16>(m, workspace, (cudaStream_t)stream); break;
+        default: e = backward<__half>(m, workspace, (cudaStream_t)stream); break;
     }
     return e == cudaSuccess ? DSDPA_OK : report_cuda_failure(e);
 }

@@ -1,0 +1,550 @@
+// Backward of masked attention on the tensor cores, 16-bit storage, head dimensions up to 128: two kernels,
+// both of which compute the scores again.
+//
+//   masked_dq_kernel    a block has 128 queries of one head and goes over their keys:
+//                         S = q k^T, dP = dout v^T, dS = P (dP - delta), dq += dS k
+//   masked_dkdv_kernel  a block has 128 keys of one key/value head and goes over the queries that see them, of all
+//                       heads of the group:  S^T = k q^T, dP^T = v dout^T, dv += P^T dout, dk += dS^T q
+//
+// Every gradient has one writer and one order of sums, so two runs give the same bits; the price, against
+// one kernel that adds dq up with atomics, is seven products a tile pair instead of five.  P and dS go to
+// tensor memory in the storage type, as operands; everything before them and every sum is fp32.  For
+// fp16 dS is scaled by a power of two (of the largest |dout|, of the row or of the whole group), since
+// a loss that is scaled far down would take it out of the type's range.
+// Both kernels: 8 warps of elementwise work (a thread has one row and 64 of its 128 columns), one warp of
+// TMA loads, one that issues the matrix instructions.
+#pragma once
+
+#include "dsdpa_masked_fwd.cuh"
+
+namespace dsdpa {
+
+constexpr int kBwdThreads = 320;
+
+// What masked_dq_kernel leaves for masked_dkdv_kernel, in whole tiles of 128 queries.
+struct BwdStats {
+    float2* stats;    // [B, Hq, tiles * 128]: lse (+inf: no weight) and delta
+    int2* ranges;     // [B, tiles * 128]: visible keys
+    int4* tiles;      // [B, tiles]: least lo, largest hi over rows that see something; largest lo, least hi over all rows
+    unsigned* amax;   // [B, Hkv]: exponent field of the largest |dout| (fp16)
+    int n;            // tiles of a sequence
+};
+
+// 2^-e for numbers in [2^e, 2^(e+1)), from their exponent field; 1 for zero, infinity and NaN.
+__device__ __forceinline__ float scale_down(unsigned e) {
+    return e == 0 || e >= 254 ? 1.0f : __uint_as_float((unsigned)(254 - e) << 23);
+}
+
+// The weight of one pair from its product qk; `slope` gets the factor that the cap's derivative puts on ds.
+template <bool CAP, bool BIAS>
+__device__ __forceinline__ float pair_weight(float qk, const ScoreConsts& c, float slope2, float dist, float lse, float& slope) {
+    float s;
+    if (CAP) {
+        const float r = rcp_approx(1.0f + fast_exp2(qk * c.cap_in));
+        s = fmaf(-2.0f * c.cap_out, r, c.cap_out) - lse;
+        slope = 4.0f * fmaf(-r, r, r);              // 1 - tanh^2
+    } else {
+        s = fmaf(qk, c.scale2, -lse);
+        slope = 1.0f;
+    }
+    if (BIAS) s = fmaf(-slope2, fabsf(dist), s);
+    return fast_exp2(s);
+}
+
+// d[128 x HD] (+)= w[128 x 128] b[128 x HD]; w's halves lie in columns 0 .. 31 and 64 .. 95 of its region, each
+// where the half of the scores was that the same threads have read.
+template <int HD>
+__device__ __forceinline__ void mma_halves(uint32_t d, uint32_t w, uint32_t b, uint32_t idesc, bool add) {
+#pragma unroll
+    for (int s = 0; s < 8; ++s)
+        mma_ts(d, w + (s & 3) * 8 + (s >> 2) * 64, smem_desc(b + s * 2048, 128 * 128), idesc, add || s > 0);
+}
+
+template <typename T, int HD, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(kBwdThreads, 1)
+masked_dq_kernel(const __grid_constant__ MaskedParams p, const __grid_constant__ BwdStats st, const __grid_constant__ CUtensorMap mq,
+                 const __grid_constant__ CUtensorMap mdo, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
+                 int negate) {
+    using L = FwdLayout<HD>;     // q and dout where the forward has its two tiles, then the ring of k and v tiles
+    constexpr bool kScaled = DtypeOf<T>::value == DSDPA_F16;
+    extern __shared__ char smem_raw[];
+    const uint32_t smem = (smem_addr(smem_raw) + 1023u) & ~1023u;
+    const uint32_t sm_q = smem, sm_do = smem + L::kTileBytes, sm_ring = smem + 2 * L::kTileBytes, bars = sm_ring + L::kStages * L::kTileBytes;
+    const uint32_t bar_q = bars, bar_s = bars + 8, bar_dp = bars + 24, bar_ds = bars + 32, bar_done = bars + 40, bar_full = bars + 48,
+                   bar_empty = bar_full + 8 * L::kStages, slot = bar_empty + 8 * L::kStages;
+    __shared__ int s_lo, s_hi, s_lomax, s_himin;
+    __shared__ float s_part[2][kTileQ];
+    __shared__ unsigned char s_big[2][kTileQ];
+    __shared__ unsigned s_bad[8];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int bh = blockIdx.x % (p.B * p.Hq), b = bh / p.Hq, h = bh % p.Hq, hk = h / p.group;
+    const int qt = st.n - 1 - (int)(blockIdx.x / (p.B * p.Hq)), q0 = qt * kTileQ;
+
+    if (tid == 0) {
+        s_lo = 0x7fffffff; s_hi = 0; s_lomax = -1; s_himin = 0x7fffffff;
+        mbar_init(bar_q, 1);
+        mbar_init(bar_s, 1);
+        mbar_init(bar_s + 8, 1);
+        mbar_init(bar_dp, 1);
+        mbar_init(bar_ds, 8);
+        mbar_init(bar_done, 1);
+        for (int i = 0; i < L::kStages; ++i) { mbar_init(bar_full + 8 * i, 1); mbar_init(bar_empty + 8 * i, 1); }
+        fence_mbar_init();
+    }
+    if (warp == 9) tmem_alloc(slot, 512);
+    __syncthreads();
+    const int half = warp >> 2, in_tile = (warp & 3) * 32 + lane, row = q0 + in_tile;
+    int2 r = make_int2(0, 0);
+    int lo_most = -1, hi_least = 0x7fffffff;
+    if (warp < 8) {
+        if (row < p.Lq) {
+            r = key_range(p, b, row);
+            if (r.x >= r.y) r = make_int2(0, 0);
+            lo_most = r.x;
+            hi_least = r.y;
+        }
+        const int lo = warp_min(r.x < r.y ? r.x : 0x7fffffff), hi = warp_max(r.y);
+        lo_most = warp_max(lo_most);
+        hi_least = warp_min(hi_least);
+        if (lane == 0 && half == 0) {
+            atomicMin(&s_lo, lo);
+            atomicMax(&s_hi, hi);
+            atomicMax(&s_lomax, lo_most);
+            atomicMin(&s_himin, hi_least);
+        }
+        // delta = out.dout: each half of the threads has half of the row
+        float part = 0.0f;
+        unsigned big = 0;
+        if (r.x < r.y) {
+            const T* o = row_of<T>(p.out_in, p.so, b, h, row);
+            const T* g = row_of<T>(p.dout, p.sdo, b, h, row);
+#pragma unroll
+            for (int x = 0; x < HD / 2; x += 8) {
+                const int d = half * (HD / 2) + x;
+                if (d < p.D) {
+                    float a[8], e[8];
+                    load8<T>(o + d, a);
+                    load8<T>(g + d, e);
+                    part += dot8(a, e);
+                    if (kScaled) {
+#pragma unroll
+                        for (int y = 0; y < 8; ++y) big = max(big, __float_as_uint(e[y]) & 0x7fffffffu);
+                    }
+                }
+            }
+        }
+        s_part[half][in_tile] = part;
+        s_big[half][in_tile] = (unsigned char)(big >> 23);
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    uint32_t tmem;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(slot));
+    const int first = s_hi > 0 ? s_lo / kTileK : 0, n = s_hi > 0 ? (s_hi + kTileK - 1) / kTileK - first : 0;
+    if (tid == 0 && h == 0) st.tiles[(long long)b * st.n + qt] = make_int4(s_lo, s_hi, s_lomax, s_himin);
+
+    if (warp == 8) {
+        if (elect_one() && n > 0) {
+            mbar_expect_tx(bar_q, 2 * L::kTileBytes);
+#pragma unroll
+            for (int x = 0; x < HD / kPanel; ++x) {
+                tma_load_4d(sm_q + x * 128 * 128, &mq, x * kPanel, q0, h, b, bar_q);
+                tma_load_4d(sm_do + x * 128 * 128, &mdo, x * kPanel, q0, h, b, bar_q);
+            }
+            int at = 0, ph = 1;
+            bool ok = true;
+            for (int i = 0; i < n && ok; ++i)
+#pragma unroll
+                for (int kv = 0; kv < 2; ++kv) {
+                    if (!mbar_wait_bounded(bar_empty + 8 * at, ph, p.err)) { ok = false; break; }
+                    const uint32_t dst = sm_ring + at * L::kTileBytes, full = bar_full + 8 * at;
+                    mbar_expect_tx(full, L::kTileBytes);
+#pragma unroll
+                    for (int x = 0; x < HD / kPanel; ++x)
+                        tma_load_4d(dst + x * 128 * 128, kv ? &mv : &mk, x * kPanel, (first + i) * kTileK, hk, b, full);
+                    if (++at == L::kStages) { at = 0; ph ^= 1; }
+                }
+        }
+    } else if (warp == 9) {
+        if (elect_one() && n > 0) {
+            // columns: S of even and of odd key blocks (dS in their place), dP, dq
+            const uint32_t id_s = mma_desc<T>(kTileK, false, negate != 0), id_dp = mma_desc<T>(kTileK, false), id_dq = mma_desc<T>(HD, true);
+            const uint32_t t_dp = tmem + 256, t_dq = tmem + 384;
+            bool ok = mbar_wait_bounded(bar_q, 0, p.err);
+            auto tile = [&](int e) { return sm_ring + (uint32_t)(e % L::kStages) * L::kTileBytes; };     // entry e: k of block e/2, or v
+            auto arrived = [&](int e) { return mbar_wait_bounded(bar_full + 8 * (e % L::kStages), (e / L::kStages) & 1, p.err); };
+            auto score = [&](int i) {
+                if (!arrived(2 * i)) return false;
+                mma_rows<HD>(tmem + (i & 1) * kTileK, sm_q, tile(2 * i), kTileK, id_s);
+                mma_commit(bar_s + 8 * (i & 1));
+                return true;
+            };
+            auto dprod = [&](int i) {
+                if (!arrived(2 * i + 1)) return false;
+                mma_rows<HD>(t_dp, sm_do, tile(2 * i + 1), kTileK, id_dp);
+                mma_commit(bar_dp);
+                mma_commit(bar_empty + 8 * ((2 * i + 1) % L::kStages));
+                return true;
+            };
+            ok = ok && score(0) && dprod(0) && (n < 2 || score(1));
+            for (int i = 0; i < n && ok; ++i) {
+                if (!(ok = mbar_wait_bounded(bar_ds, i & 1, p.err))) break;
+                tc_fence_after();
+                if (i + 1 < n && !(ok = dprod(i + 1))) break;
+                mma_halves<HD>(t_dq, tmem + (i & 1) * kTileK, tile(2 * i), id_dq, i > 0);
+                mma_commit(bar_empty + 8 * ((2 * i) % L::kStages));
+                if (i + 2 < n) ok = score(i + 2);
+            }
+            if (ok) mma_commit(bar_done);
+        }
+    } else {
+        const uint32_t lanes = (uint32_t)(warp & 3) << 21;
+        ScoreConsts c;
+        c.scale2 = fabsf(p.sm_scale) * kLog2e;
+        c.cap_in = CAP ? 2.0f * c.scale2 / p.cap : 0.0f;
+        c.cap_out = CAP ? p.cap * kLog2e : 0.0f;
+        const float slope2 = BIAS ? __ldg(p.slopes + h) * kLog2e : 0.0f;
+        const bool sees = r.x < r.y;
+        const float delta = s_part[0][in_tile] + s_part[1][in_tile];
+        const unsigned big = max((unsigned)s_big[0][in_tile], (unsigned)s_big[1][in_tile]);
+        const float sigma = kScaled ? scale_down(big) : 1.0f;
+        const long long at = (long long)bh * p.Lq + row;
+        float lse = sees ? p.lse[at] : kNegInf;
+        if (lse == kNegInf) lse = -kNegInf;                 // weight exp2(s - inf) = 0
+        if (half == 0) {
+            st.stats[(long long)bh * st.n * kTileQ + row] = make_float2(lse, delta);
+            if (h == 0) st.ranges[(long long)b * st.n * kTileQ + row] = r;
+            if (row < p.Lq) p.delta[at] = delta;
+            if (kScaled) {
+                const unsigned top = __reduce_max_sync(0xffffffffu, big);
+                if (lane == 0) atomicMax(st.amax + b * p.Hkv + hk, top);
+            }
+        }
+        const float ndelta = -delta * sigma;
+        const int pos = row + (p.Lk - p.Lq);
+        bool ok = true;
+        for (int i = 0; i < n; ++i) {
+            const uint32_t s_at = tmem + (i & 1) * kTileK + half * 64 + lanes, d_at = tmem + 256 + half * 64 + lanes;
+            float w[64];
+            if (!mbar_wait_bounded(bar_s + 8 * (i & 1), (i >> 1) & 1, p.err)) { ok = false; break; }
+            tc_fence_after();
+            tmem_ld32(s_at, w);
+            tmem_ld32(s_at + 32, w + 32);
+            tmem_wait_ld();
+            const int n0 = (first + i) * kTileK + half * 64;
+            const float d0 = (float)(pos - n0);
+            const bool partial = lo_most > n0 || hi_least < n0 + 64;
+            const int a = r.x - n0, e = r.y - n0;
+#pragma unroll
+            for (int x = 0; x < 64; ++x) {
+                float slope, v = pair_weight<CAP, BIAS>(w[x], c, slope2, d0 - (float)x, lse, slope);
+                w[x] = CAP ? v * slope : v;
+            }
+            if (partial) {
+#pragma unroll
+                for (int x = 0; x < 64; ++x) w[x] = x >= a && x < e ? w[x] : 0.0f;
+            }
+            if (!mbar_wait_bounded(bar_dp, i & 1, p.err)) { ok = false; break; }
+            tc_fence_after();
+#pragma unroll
+            for (int x = 0; x < 64; x += 32) {
+                float d[32];
+                uint32_t o[16];
+                tmem_ld32(d_at + x, d);
+                tmem_wait_ld();
+#pragma unroll
+                for (int y = 0; y < 32; y += 2) {
+                    const float u0 = kScaled ? fmaf(d[y], sigma, ndelta) : d[y] + ndelta;
+                    const float u1 = kScaled ? fmaf(d[y + 1], sigma, ndelta) : d[y + 1] + ndelta;
+                    o[y / 2] = pack2<T>(w[x + y] * u0, w[x + y + 1] * u1);
+                }
+                tmem_st16(s_at + x / 2, o);
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_ds);
+        }
+        if (ok && n > 0) ok = mbar_wait_bounded(bar_done, 0, p.err);
+        if (ok) {
+            tc_fence_after();
+            const float back = p.sm_scale / sigma;         // sigma is a power of two
+            bool fine = true;
+#pragma unroll
+            for (int x = 0; x < HD / 2; x += 32) {
+                float o[32];
+                const int d0 = half * (HD / 2) + x;
+                if (n > 0) {
+                    tmem_ld32(tmem + 384 + d0 + lanes, o);
+                    tmem_wait_ld();
+                }
+                if (row < p.Lq) {
+                    T* out = row_of<T>(p.dq, p.sdq, b, h, row) + d0;
+#pragma unroll
+                    for (int y = 0; y < 32; y += 8) {
+                        float v[8];
+#pragma unroll
+                        for (int z = 0; z < 8; ++z) {
+                            v[z] = n > 0 ? o[y + z] * back : 0.0f;
+                            fine = fine && fabsf(v[z]) <= 3.0e38f;
+                        }
+                        if (d0 + y < p.D) stg128(out + y, pack16(v, (T*)nullptr));
+                    }
+                }
+            }
+            const unsigned bad = __ballot_sync(0xffffffffu, row < p.Lq && !fine);
+            if (lane == 0) s_bad[warp] = bad;
+        } else if (lane == 0) s_bad[warp] = 0;
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 9) tmem_free(tmem, 512);
+    // rows that something non-finite reached: once more, from the keys they see alone
+    if (n > 0 && warp < 4) {
+        unsigned bad = s_bad[warp] | s_bad[warp + 4];
+        while (bad) {
+            const int at = __ffs(bad) - 1;
+            bad &= bad - 1;
+            exact_row_dq<T>(p, b, h, row - lane + at);
+        }
+    }
+}
+
+template <int HD>
+struct DkdvLayout {
+    static constexpr int kTileBytes = 128 * HD * 2;
+    static constexpr int kRowBytes = 128 * 8;                       // stats, or ranges, of a tile
+    static constexpr int kStage = 2 * kTileBytes + 2 * kRowBytes;   // q, dout, stats, ranges
+    static constexpr int kSmem = 2 * kTileBytes + 2 * kStage + 1024 + 256;
+};
+
+template <typename T, int HD, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(kBwdThreads, 1)
+masked_dkdv_kernel(const __grid_constant__ MaskedParams p, const __grid_constant__ BwdStats st, const __grid_constant__ CUtensorMap mq,
+                   const __grid_constant__ CUtensorMap mdo, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
+                   int negate) {
+    using L = DkdvLayout<HD>;
+    constexpr bool kScaled = DtypeOf<T>::value == DSDPA_F16;
+    extern __shared__ char smem_raw[];
+    const uint32_t smem = (smem_addr(smem_raw) + 1023u) & ~1023u;
+    const uint32_t sm_k = smem, sm_v = smem + L::kTileBytes, sm_q = smem + 2 * L::kTileBytes;    // q and dout of both stages first
+    const uint32_t sm_rows = sm_q + 4 * L::kTileBytes, bars = sm_rows + 4 * L::kRowBytes;
+    const uint32_t bar_kv = bars, bar_qf = bars + 8, bar_qe = bars + 24, bar_of = bars + 40, bar_oe = bars + 56, bar_s = bars + 72,
+                   bar_dp = bars + 80, bar_p = bars + 88, bar_ds = bars + 96, bar_done = bars + 104, slot = bars + 112;
+    __shared__ int s_first, s_end;
+    __shared__ unsigned s_bad[8];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int bh = blockIdx.x % (p.B * p.Hkv), b = bh / p.Hkv, hk = bh % p.Hkv;
+    const int k0 = (int)(blockIdx.x / (p.B * p.Hkv)) * kTileK;       // first keys first: with a causal mask most queries see them
+    auto tile_q = [&](int e) { return sm_q + (uint32_t)(e & 1) * 2 * L::kTileBytes; };
+    auto tile_do = [&](int e) { return tile_q(e) + L::kTileBytes; };
+    auto tile_rows = [&](int e) { return sm_rows + (uint32_t)(e & 1) * 2 * L::kRowBytes; };
+
+    if (tid == 0) {
+        s_first = 0x7fffffff; s_end = 0;
+        mbar_init(bar_kv, 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(bar_qf + 8 * i, 1);
+            mbar_init(bar_qe + 8 * i, 1);
+            mbar_init(bar_of + 8 * i, 1);
+            mbar_init(bar_oe + 8 * i, 1);
+        }
+        mbar_init(bar_s, 1);
+        mbar_init(bar_dp, 1);
+        mbar_init(bar_p, 8);
+        mbar_init(bar_ds, 8);
+        mbar_init(bar_done, 1);
+        fence_mbar_init();
+    }
+    if (warp == 9) tmem_alloc(slot, 512);
+    __syncthreads();
+    // the query tiles between the first and the last that see any of these keys
+    int lo = 0x7fffffff, hi = 0;
+    for (int i = tid; i < st.n; i += kBwdThreads) {
+        const int4 t = st.tiles[(long long)b * st.n + i];
+        if (t.x < k0 + kTileK && t.y > k0) { lo = min(lo, i); hi = max(hi, i + 1); }
+    }
+    lo = warp_min(lo);
+    hi = warp_max(hi);
+    if (lane == 0) { atomicMin(&s_first, lo); atomicMax(&s_end, hi); }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    uint32_t tmem;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(slot));
+    const int first = s_first, span = s_end > 0 ? s_end - first : 0, n = span * p.group;
+
+    if (warp == 8) {
+        if (elect_one() && n > 0) {
+            mbar_expect_tx(bar_kv, 2 * L::kTileBytes);
+#pragma unroll
+            for (int x = 0; x < HD / kPanel; ++x) {
+                tma_load_4d(sm_k + x * 128 * 128, &mk, x * kPanel, k0, hk, b, bar_kv);
+                tma_load_4d(sm_v + x * 128 * 128, &mv, x * kPanel, k0, hk, b, bar_kv);
+            }
+            bool ok = true;
+            for (int e = 0; e < n && ok; ++e) {
+                const int h = hk * p.group + e / span, q0 = (first + e % span) * kTileQ;
+                const uint32_t ph = ((e >> 1) & 1) ^ 1, full = bar_qf + 8 * (e & 1), dfull = bar_of + 8 * (e & 1);
+                if (!(ok = mbar_wait_bounded(bar_qe + 8 * (e & 1), ph, p.err))) break;
+                mbar_expect_tx(full, L::kTileBytes + 2 * L::kRowBytes);
+#pragma unroll
+                for (int x = 0; x < HD / kPanel; ++x) tma_load_4d(tile_q(e) + x * 128 * 128, &mq, x * kPanel, q0, h, b, full);
+                bulk_g2s(tile_rows(e), st.stats + ((long long)b * p.Hq + h) * st.n * kTileQ + q0, L::kRowBytes, full);
+                bulk_g2s(tile_rows(e) + L::kRowBytes, st.ranges + (long long)b * st.n * kTileQ + q0, L::kRowBytes, full);
+                if (!(ok = mbar_wait_bounded(bar_oe + 8 * (e & 1), ph, p.err))) break;
+                mbar_expect_tx(dfull, L::kTileBytes);
+#pragma unroll
+                for (int x = 0; x < HD / kPanel; ++x) tma_load_4d(tile_do(e) + x * 128 * 128, &mdo, x * kPanel, q0, h, b, dfull);
+            }
+        }
+    } else if (warp == 9) {
+        if (elect_one() && n > 0) {
+            // columns: S^T (P^T in its place), dP^T (dS^T in its place), dv, dk
+            const uint32_t id_s = mma_desc<T>(kTileQ, false, negate != 0), id_dp = mma_desc<T>(kTileQ, false), id_g = mma_desc<T>(HD, true);
+            const uint32_t t_dp = tmem + 128, t_dv = tmem + 256, t_dk = tmem + 384;
+            bool ok = mbar_wait_bounded(bar_kv, 0, p.err);
+            auto score = [&](int e) {
+                if (!mbar_wait_bounded(bar_qf + 8 * (e & 1), (e >> 1) & 1, p.err)) return false;
+                mma_rows<HD>(tmem, sm_k, tile_q(e), kTileQ, id_s);
+                mma_commit(bar_s);
+                return true;
+            };
+            auto dprod = [&](int e) {
+                if (!mbar_wait_bounded(bar_of + 8 * (e & 1), (e >> 1) & 1, p.err)) return false;
+                mma_rows<HD>(t_dp, sm_v, tile_do(e), kTileQ, id_dp);
+                mma_commit(bar_dp);
+                return true;
+            };
+            ok = ok && score(0) && dprod(0);
+            for (int e = 0; e < n && ok; ++e) {
+                if (!(ok = mbar_wait_bounded(bar_p, e & 1, p.err))) break;
+                tc_fence_after();
+                mma_halves<HD>(t_dv, tmem, tile_do(e), id_g, e > 0);
+                mma_commit(bar_oe + 8 * (e & 1));
+                if (e + 1 < n && !(ok = score(e + 1))) break;
+                if (!(ok = mbar_wait_bounded(bar_ds, e & 1, p.err))) break;
+                tc_fence_after();
+                mma_halves<HD>(t_dk, t_dp, tile_q(e), id_g, e > 0);
+                mma_commit(bar_qe + 8 * (e & 1));
+                if (e + 1 < n) ok = dprod(e + 1);
+            }
+            if (ok) mma_commit(bar_done);
+        }
+    } else {
+        const uint32_t lanes = (uint32_t)(warp & 3) << 21;
+        const int half = warp >> 2, in_tile = (warp & 3) * 32 + lane, key = k0 + in_tile;
+        ScoreConsts c;
+        c.scale2 = fabsf(p.sm_scale) * kLog2e;
+        c.cap_in = CAP ? 2.0f * c.scale2 / p.cap : 0.0f;
+        c.cap_out = CAP ? p.cap * kLog2e : 0.0f;
+        const float sigma = kScaled ? scale_down(st.amax[bh]) : 1.0f;
+        const uint32_t s_at = tmem + half * 64 + lanes, d_at = s_at + 128;
+        bool ok = true;
+        for (int e = 0; e < n; ++e) {
+            const int qt = first + e % span, q0 = qt * kTileQ + half * 64;
+            const float slope2 = BIAS ? __ldg(p.slopes + hk * p.group + e / span) * kLog2e : 0.0f;
+            const int4 t = __ldg(st.tiles + (long long)b * st.n + qt);
+            const bool partial = t.z > k0 || t.w < k0 + kTileK;
+            const uint32_t stats = tile_rows(e) + half * 64 * 8, ranges = stats + L::kRowBytes;
+            const float d0 = (float)(q0 + (p.Lk - p.Lq) - key);
+            float w[64];
+            if (!mbar_wait_bounded(bar_qf + 8 * (e & 1), (e >> 1) & 1, p.err) || !mbar_wait_bounded(bar_s, e & 1, p.err)) { ok = false; break; }
+            tc_fence_after();
+            tmem_ld32(s_at, w);
+            tmem_ld32(s_at + 32, w + 32);
+            tmem_wait_ld();
+#pragma unroll
+            for (int x = 0; x < 64; x += 32) {
+                uint32_t o[16];
+#pragma unroll
+                for (int y = 0; y < 32; y += 2) {
+                    const uint4 q = lds128(stats + (x + y) * 8);       // lse, delta of two queries
+                    float g0, g1;
+                    float v0 = pair_weight<CAP, BIAS>(w[x + y], c, slope2, d0 + (float)(x + y), __uint_as_float(q.x), g0);
+                    float v1 = pair_weight<CAP, BIAS>(w[x + y + 1], c, slope2, d0 + (float)(x + y + 1), __uint_as_float(q.z), g1);
+                    if (partial) {
+                        const uint4 k = lds128(ranges + (x + y) * 8);
+                        v0 = key >= (int)k.x && key < (int)k.y ? v0 : 0.0f;
+                        v1 = key >= (int)k.z && key < (int)k.w ? v1 : 0.0f;
+                    }
+                    o[y / 2] = pack2<T>(v0, v1);
+                    w[x + y] = CAP ? v0 * g0 : v0;
+                    w[x + y + 1] = CAP ? v1 * g1 : v1;
+                }
+                tmem_st16(s_at + x / 2, o);
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_p);
+            if (!mbar_wait_bounded(bar_dp, e & 1, p.err)) { ok = false; break; }
+            tc_fence_after();
+#pragma unroll
+            for (int x = 0; x < 64; x += 32) {
+                float d[32];
+                uint32_t o[16];
+                tmem_ld32(d_at + x, d);
+                tmem_wait_ld();
+#pragma unroll
+                for (int y = 0; y < 32; y += 2) {
+                    const uint4 q = lds128(stats + (x + y) * 8);
+                    float u0 = d[y] - __uint_as_float(q.y), u1 = d[y + 1] - __uint_as_float(q.w);
+                    if (kScaled) { u0 *= sigma; u1 *= sigma; }
+                    o[y / 2] = pack2<T>(w[x + y] * u0, w[x + y + 1] * u1);
+                }
+                tmem_st16(d_at + x / 2, o);
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_ds);
+        }
+        if (ok && n > 0) ok = mbar_wait_bounded(bar_done, 0, p.err);
+        if (ok) {
+            tc_fence_after();
+            const float back = p.sm_scale / sigma;
+            bool fine = true;
+            // the first half of the threads has dv, the second dk
+            T* out = key < p.Lk ? (half ? row_of<T>(p.dk, p.sdk, b, hk, key) : row_of<T>(p.dv, p.sdv, b, hk, key)) : nullptr;
+#pragma unroll
+            for (int x = 0; x < HD; x += 32) {
+                float o[32];
+                if (n > 0) {
+                    tmem_ld32(tmem + 256 + half * 128 + x + lanes, o);
+                    tmem_wait_ld();
+                }
+                if (key < p.Lk) {
+#pragma unroll
+                    for (int y = 0; y < 32; y += 8) {
+                        float v[8];
+#pragma unroll
+                        for (int z = 0; z < 8; ++z) {
+                            v[z] = n > 0 ? (half ? o[y + z] * back : o[y + z]) : 0.0f;
+                            fine = fine && fabsf(v[z]) <= 3.0e38f;
+                        }
+                        if (x + y < p.D) stg128(out + x + y, pack16(v, (T*)nullptr));
+                    }
+                }
+            }
+            const unsigned bad = __ballot_sync(0xffffffffu, key < p.Lk && !fine);
+            if (lane == 0) s_bad[warp] = bad;
+        } else if (lane == 0) s_bad[warp] = 0;
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 9) tmem_free(tmem, 512);
+    if (n > 0 && warp < 4) {
+        unsigned bad = s_bad[warp] | s_bad[warp + 4];
+        while (bad) {
+            const int at = __ffs(bad) - 1;
+            bad &= bad - 1;
+            exact_row_dkdv<T>(p, b, hk, k0 + warp * 32 + at);
+        }
+    }
+}
+
+}  // namespace dsdpa

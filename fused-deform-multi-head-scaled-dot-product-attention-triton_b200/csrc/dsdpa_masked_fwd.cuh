@@ -108,77 +108,79 @@ masked_fwd_kernel(const __grid_constant__ MaskedParams p, const __grid_constant_
     const int jb = end[0] == 0 ? first[1] : end[1] == 0 ? first[0] : min(first[0], first[1]), je = max(end[0], end[1]);
     auto used = [&](int t, int j) { return j >= first[t] && j < end[t]; };
 
-    if (warp >= 8) regs_release<80>();
-    else regs_claim<208>();
-    if (warp == 8) {
-        if (elect_one()) {
-            mbar_expect_tx(bar_q, 2 * L::kTileBytes);
+    if (warp >= 8) {
+        regs_release<80>();
+        if (warp == 8) {
+            if (elect_one()) {
+                mbar_expect_tx(bar_q, 2 * L::kTileBytes);
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int x = 0; x < HD / kPanel; ++x)
-                    tma_load_4d(sm_q + t * L::kTileBytes + x * 128 * 128, &mq, x * kPanel, q0 + t * kTileQ, h, b, bar_q);
-            int st = 0, ph = 1;      // the ring starts empty
-            bool ok = true;
-            for (int j = jb; j < je && ok; ++j) {
-                if (!used(0, j) && !used(1, j)) continue;
-#pragma unroll
-                for (int kv = 0; kv < 2; ++kv) {
-                    if (!mbar_wait_bounded(bar_empty + 8 * st, ph, p.err)) { ok = false; break; }
-                    const uint32_t dst = sm_ring + st * L::kTileBytes, full = bar_full + 8 * st;
-                    mbar_expect_tx(full, L::kTileBytes);
+                for (int t = 0; t < 2; ++t)
 #pragma unroll
                     for (int x = 0; x < HD / kPanel; ++x)
-                        tma_load_4d(dst + x * 128 * 128, kv ? &mv : &mk, x * kPanel, j * kTileK, hk, b, full);
-                    if (++st == L::kStages) { st = 0; ph ^= 1; }
-                }
-            }
-        }
-    } else if (warp == 9) {
-        if (elect_one()) {
-            const uint32_t id_s = mma_desc<T>(kTileK, false, negate != 0), id_o = mma_desc<T>(HD, true);
-            bool ok = mbar_wait_bounded(bar_q, 0, p.err), pending[2] = { false, false }, begun[2] = { false, false };
-            int st = 0, ph = 0, vst = 0, pp[2] = { 0, 0 };
-            // j == je: the products that are still to be done
-            for (int j = jb; j <= je && ok; ++j) {
-                const bool any = j < je && (used(0, j) || used(1, j));
-                if (j < je && !any) continue;
-                const bool had = pending[0] || pending[1];
-                int kst = 0;
-                if (had) {
-                    vst = st;
-                    if (!mbar_wait_bounded(bar_full + 8 * vst, ph, p.err)) { ok = false; break; }
-                    if (++st == L::kStages) { st = 0; ph ^= 1; }
-                }
-                if (any) {
-                    kst = st;
-                    if (!mbar_wait_bounded(bar_full + 8 * kst, ph, p.err)) { ok = false; break; }
-                    if (++st == L::kStages) { st = 0; ph ^= 1; }
-                }
+                        tma_load_4d(sm_q + t * L::kTileBytes + x * 128 * 128, &mq, x * kPanel, q0 + t * kTileQ, h, b, bar_q);
+                int st = 0, ph = 1;      // the ring starts empty
+                bool ok = true;
+                for (int j = jb; j < je && ok; ++j) {
+                    if (!used(0, j) && !used(1, j)) continue;
 #pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    const uint32_t s_at = tmem + t * kTileK, o_at = tmem + 2 * kTileK + t * HD;
-                    if (pending[t]) {
-                        if (!mbar_wait_bounded(bar_p + 8 * t, pp[t], p.err)) { ok = false; break; }
-                        pp[t] ^= 1;
-                        tc_fence_after();
-                        mma_weights<kTileK>(o_at, s_at, sm_ring + vst * L::kTileBytes, id_o, begun[t]);
-                        begun[t] = true;
-                        mma_commit(bar_o + 8 * t);
-                        pending[t] = false;
-                    }
-                    if (any && used(t, j)) {
-                        mma_rows<HD>(s_at, sm_q + t * L::kTileBytes, sm_ring + kst * L::kTileBytes, kTileK, id_s);
-                        mma_commit(bar_s + 8 * t);
-                        pending[t] = true;
+                    for (int kv = 0; kv < 2; ++kv) {
+                        if (!mbar_wait_bounded(bar_empty + 8 * st, ph, p.err)) { ok = false; break; }
+                        const uint32_t dst = sm_ring + st * L::kTileBytes, full = bar_full + 8 * st;
+                        mbar_expect_tx(full, L::kTileBytes);
+#pragma unroll
+                        for (int x = 0; x < HD / kPanel; ++x)
+                            tma_load_4d(dst + x * 128 * 128, kv ? &mv : &mk, x * kPanel, j * kTileK, hk, b, full);
+                        if (++st == L::kStages) { st = 0; ph ^= 1; }
                     }
                 }
-                if (!ok) break;
-                if (had) mma_commit(bar_empty + 8 * vst);
-                if (any) mma_commit(bar_empty + 8 * kst);
+            }
+        } else if (warp == 9) {
+            if (elect_one()) {
+                const uint32_t id_s = mma_desc<T>(kTileK, false, negate != 0), id_o = mma_desc<T>(HD, true);
+                bool ok = mbar_wait_bounded(bar_q, 0, p.err), pending[2] = { false, false }, begun[2] = { false, false };
+                int st = 0, ph = 0, vst = 0, pp[2] = { 0, 0 };
+                // j == je: the products that are still to be done
+                for (int j = jb; j <= je && ok; ++j) {
+                    const bool any = j < je && (used(0, j) || used(1, j));
+                    if (j < je && !any) continue;
+                    const bool had = pending[0] || pending[1];
+                    int kst = 0;
+                    if (had) {
+                        vst = st;
+                        if (!mbar_wait_bounded(bar_full + 8 * vst, ph, p.err)) { ok = false; break; }
+                        if (++st == L::kStages) { st = 0; ph ^= 1; }
+                    }
+                    if (any) {
+                        kst = st;
+                        if (!mbar_wait_bounded(bar_full + 8 * kst, ph, p.err)) { ok = false; break; }
+                        if (++st == L::kStages) { st = 0; ph ^= 1; }
+                    }
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        const uint32_t s_at = tmem + t * kTileK, o_at = tmem + 2 * kTileK + t * HD;
+                        if (pending[t]) {
+                            if (!mbar_wait_bounded(bar_p + 8 * t, pp[t], p.err)) { ok = false; break; }
+                            pp[t] ^= 1;
+                            tc_fence_after();
+                            mma_weights<kTileK>(o_at, s_at, sm_ring + vst * L::kTileBytes, id_o, begun[t]);
+                            begun[t] = true;
+                            mma_commit(bar_o + 8 * t);
+                            pending[t] = false;
+                        }
+                        if (any && used(t, j)) {
+                            mma_rows<HD>(s_at, sm_q + t * L::kTileBytes, sm_ring + kst * L::kTileBytes, kTileK, id_s);
+                            mma_commit(bar_s + 8 * t);
+                            pending[t] = true;
+                        }
+                    }
+                    if (!ok) break;
+                    if (had) mma_commit(bar_empty + 8 * vst);
+                    if (any) mma_commit(bar_empty + 8 * kst);
+                }
             }
         }
-    } else if (warp < 8) {
+    } else {
+        regs_claim<208>();
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;        // 32 lanes a warp, in the address's upper half
         const uint32_t s_at = tmem + tile * kTileK + lanes, o_at = tmem + 2 * kTileK + tile * HD + lanes;
         ScoreConsts c;

@@ -13,5 +13,26 @@ namespace dsdpa {
 cudaError_t tensor_map_16(CUtensorMap* map, int dtype, const void* base, int D, int rows, int L, int H, int B, const long long (&stride)[3]);
 
 template <typename T> cudaError_t launch_masked_fwd_tc(const MaskedParams& p, cudaStream_t s);
+// workspace: masked_bwd_space().bytes, p.delta pointing to its start; p.Lq > 0 and p.Lk > 0
+template <typename T> cudaError_t launch_masked_bwd_tc(const MaskedParams& p, void* workspace, cudaStream_t s);
+
+// Byte offsets in the backward's workspace: delta at 0, then what the tensor-core kernels pass on.
+struct MaskedBwdSpace {
+    size_t stats, ranges, tiles, amax, bytes;
+    int n;          // tiles of 128 queries
+    bool scaled;
+};
+inline MaskedBwdSpace masked_bwd_space(int dtype, int B, int Hq, int Hkv, int Lq) {
+    auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
+    MaskedBwdSpace w{};
+    w.n = (Lq + 127) / 128;
+    w.scaled = dtype == DSDPA_F16;
+    w.stats = up((size_t)B * Hq * Lq * 4);
+    w.ranges = w.stats + up((size_t)B * Hq * w.n * 128 * 8);
+    w.tiles = w.ranges + up((size_t)B * w.n * 128 * 8);
+    w.amax = w.tiles + up((size_t)B * w.n * 16);
+    w.bytes = w.amax + up((size_t)B * Hkv * 4);
+    return w;
+}
 
 }  // namespace dsdpa
