@@ -1,6 +1,7 @@
 // C ABI of the paged cache's operators: argument checks and launches.  Declarations are in include/dsdpa.h.
 #include <math.h>
 
+#include "dsdpa_cache_launch.h"
 #include "dsdpa_evict.cuh"
 #include "dsdpa_host.h"
 
@@ -63,11 +64,15 @@ int check(const dsdpa_cache_problem* p) {
         if (p->stride_k[i] < 0 || p->stride_v[i] < 0 || p->stride_k[i] * e % 16 || p->stride_v[i] * e % 16) return DSDPA_ERR_MISALIGNED;
     return DSDPA_OK;
 }
+// The tensor-core kernels take 16-bit storage with up to 128 elements a row; the row kernels the rest.
+bool on_tensor_cores(const dsdpa_cache_problem& p) { return p.dtype != DSDPA_F32 && p.D <= 128; }
+
 int check_tokens(const dsdpa_cache_problem* p) {
     const int st = check(p);
     if (st != DSDPA_OK) return st;
     if (p->Hq <= 0 || p->Hq % p->Hkv || (long long)p->B * p->Hq >= (1ll << 24) || p->T <= 0) return DSDPA_ERR_BAD_SHAPE;
     if (p->T > kTreeMax) return DSDPA_ERR_TOO_LARGE;
+    if (on_tensor_cores(*p) && plan_tree(*p).items == 0) return DSDPA_ERR_TOO_LARGE;
     if (!isfinite(p->sm_scale) || !isfinite(p->softcap)) return DSDPA_ERR_BAD_SHAPE;
     const int e = p->dtype == DSDPA_F32 ? 4 : 2;
     for (int i = 0; i < 3; ++i)
@@ -94,7 +99,9 @@ CacheParams params(const dsdpa_cache_problem& p, const dsdpa_cache_tree* t, cons
 }
 
 template <typename T>
-cudaError_t tree_forward(const CacheParams& p, cudaStream_t s) {
+cudaError_t tree_forward(const dsdpa_cache_problem& problem, const CacheParams& p, void* workspace, cudaStream_t s) {
+    if constexpr (DtypeOf<T>::value != DSDPA_F32)
+        if (on_tensor_cores(problem)) return launch_tree_tc<T>(p, plan_tree(problem), workspace, s);
     const long long rows = (long long)p.B * p.Hq * p.T;
     tree_rows_kernel<T><<<(unsigned)((rows + kRowWarps - 1) / kRowWarps), kRowWarps * 32, 0, s>>>(p);
     count_launches(1);
@@ -116,8 +123,7 @@ using namespace dsdpa;
 extern "C" {
 
 size_t dsdpa_tree_workspace_bytes(const dsdpa_cache_problem* p) {
-    (void)p;
-    return 0;
+    return check_tokens(p) == DSDPA_OK && on_tensor_cores(*p) ? plan_tree(*p).bytes : 0;
 }
 
 int dsdpa_tree_forward(const dsdpa_cache_problem* p, const dsdpa_cache_tree* tree, const void* q, const void* k_pages,
@@ -141,9 +147,9 @@ int dsdpa_tree_forward(const dsdpa_cache_problem* p, const dsdpa_cache_tree* tre
     c.out = out;
     c.lse = lse;
     switch (p->dtype) {
-        case DSDPA_F32: e = tree_forward<float>(c, (cudaStream_t)stream); break;
-        case DSDPA_BF16: e = tree_forward<__nv_bfloat16>(c, (cudaStream_t)stream); break;
-        default: e = tree_forward<__half>(c, (cudaStream_t)stream); break;
+        case DSDPA_F32: e = tree_forward<float>(*p, c, workspace, (cudaStream_t)stream); break;
+        case DSDPA_BF16: e = tree_forward<__nv_bfloat16>(*p, c, workspace, (cudaStream_t)stream); break;
+        default: e = tree_forward<__half>(*p, c, workspace, (cudaStream_t)stream); break;
     }
     return e == cudaSuccess ? DSDPA_OK : report_cuda_failure(e);
 }

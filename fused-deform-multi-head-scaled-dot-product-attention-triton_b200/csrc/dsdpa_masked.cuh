@@ -64,6 +64,12 @@ template <> __device__ __forceinline__ void store8<float>(float* p, const float 
     stg128(p, pack16(a, (float*)nullptr));
     stg128(p + 4, pack16(b, (float*)nullptr));
 }
+template <typename T> __device__ __forceinline__ void store4(T* p, const float (&f)[4]) {
+    const float g[8] = { f[0], f[1], f[2], f[3], 0.0f, 0.0f, 0.0f, 0.0f };
+    const uint4 r = pack16(g, (T*)nullptr);
+    *reinterpret_cast<uint2*>(p) = make_uint2(r.x, r.y);
+}
+template <> __device__ __forceinline__ void store4<float>(float* p, const float (&f)[4]) { stg128(p, pack16(f, (float*)nullptr)); }
 __device__ __forceinline__ float dot8(const float (&a)[8], const float (&b)[8]) {
     float s = 0.0f;
 #pragma unroll

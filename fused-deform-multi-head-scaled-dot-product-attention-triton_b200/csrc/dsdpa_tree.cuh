@@ -1,0 +1,467 @@
+// Attention of drafted tokens over a paged cache on the tensor cores: 16-bit storage, head dimensions up
+// to 128.
+//
+// The queries that share a key/value head -- tokens times the group's heads, up to 128 a tile -- are one operand,
+// so that the cache is read once for all of them.  Keys are split over blocks in chunks, whose results
+// tree_combine_kernel joins; a block stays and takes one item (sequence, head, query tile, chunk) after the
+// other, its loads running ahead of its arithmetic across items, so that the memory never waits.
+// Inside an item key tiles of 128 go in turn to two streams, each with its own running maximum, sum and
+// accumulator (tensor memory holds both), joined at the item's end: one stream's softmax runs while the
+// other's products do, which matters when a handful of rows leaves a single warp with all of the softmax.
+// Bound by DRAM for few rows (the cache is read once), by exp2 beyond about a hundred.
+// Roles: warps 0-3 and 4-7 the streams' softmax, 8-11 copy rows (cp.async: any page size and stride, rows
+// that are not there read as zero), 12 issues the matrix instructions.
+#pragma once
+
+#include "dsdpa_cache.cuh"
+#include "dsdpa_masked_fwd.cuh"
+
+namespace dsdpa {
+
+constexpr int kTreeThreads = 512;   // launched with 128 registers: 256 x 176 + 128 x 80 + 128 x 72 = 64512 of 65536
+constexpr int kTreeRows = 128, kTreeKeys = 128, kInfo = 16;
+
+struct TreeSplit {
+    int chunk;        // keys of an item, a multiple of 2 * kTreeKeys
+    int chunks;       // of the longest sequence that the table can hold
+    int row_tiles;
+    int items;
+    float* part;      // [B * Hq * T][chunks][D], normalised
+    float* part_lse;  // [B * Hq * T][chunks]
+};
+
+template <int HD>
+struct TreeLayout {
+    static constexpr int kTileBytes = 128 * HD * 2;
+    static constexpr int kStages = HD == 128 ? 4 : 8;
+    // Entries issued behind the one that a producer waits for: with it, three times 32 KB in flight cover the
+    // latency, and the ring's other entries are the products' to work on.
+    static constexpr int kAhead = HD == 128 ? 2 : 5;
+    static constexpr int kSmem = 2 * kTileBytes + kStages * kTileBytes + 1024 + 512;
+};
+
+struct TreeItem {
+    int b, hk, row0, rows, chunk, n, real, key0, tiles;
+};
+__device__ __forceinline__ TreeItem tree_item(const CacheParams& p, const TreeSplit& s, int at) {
+    TreeItem it;
+    it.chunk = at % s.chunks; at /= s.chunks;
+    it.row0 = at % s.row_tiles * kTreeRows; at /= s.row_tiles;
+    it.hk = at % p.Hkv;
+    it.b = at / p.Hkv;
+    it.rows = min(kTreeRows, p.T * p.group - it.row0);
+    it.n = cached_keys(p, it.b);
+    it.real = drafted_tokens(p, it.b);
+    it.key0 = it.chunk * s.chunk;
+    const int keys = it.real > 0 ? it.n + it.real : 0;
+    it.tiles = max(0, min(s.chunk, keys - it.key0) + kTreeKeys - 1) / kTreeKeys;
+    if (keys <= it.key0) it.tiles = 0;
+    return it;
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, unsigned bytes) {   // the rest of 16 is zero
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" :: "n"(N) : "memory"); }
+__device__ __forceinline__ void pair_barrier(int id) { asm volatile("bar.sync %0, 64;" :: "r"(id) : "memory"); }
+
+// The 32 rows whose addresses the warp's lanes hold (null: zeros) into rows 32w .. 32w+31 of a tile, swizzled.
+template <int HD>
+__device__ __forceinline__ void copy_rows(uint32_t tile, int w, int lane, const char* row, const char* any, int D) {
+    constexpr int kPer = HD / 8, kAt = 32 / kPer;          // 16-byte pieces of a row, rows of an instruction
+    const int c = lane % kPer;
+#pragma unroll
+    for (int i = 0; i < 32 / kAt; ++i) {
+        const int l = i * kAt + lane / kPer, r = w * 32 + l;
+        const char* src = (const char*)__shfl_sync(0xffffffffu, (unsigned long long)row, l);
+        const bool there = src != nullptr && c * 8 < D;
+        cp_async16(tile + (c >> 3) * 128 * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4), there ? src + c * 16 : any, there ? 16u : 0u);
+    }
+}
+
+template <typename T, int HD, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(kTreeThreads, 1)
+tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeSplit sp, int negate) {
+    using L = TreeLayout<HD>;
+    extern __shared__ char smem_raw[];
+    const uint32_t smem = (smem_addr(smem_raw) + 1023u) & ~1023u;
+    const uint32_t sm_q = smem, sm_ring = smem + 2 * L::kTileBytes, bars = sm_ring + L::kStages * L::kTileBytes;
+    const uint32_t bar_s = bars, bar_p = bars + 16, bar_o = bars + 32, bar_qe = bars + 48, bar_full = bars + 64,
+                   bar_empty = bar_full + 8 * L::kStages, slot = bar_empty + 8 * L::kStages;
+    __shared__ unsigned s_valid[kInfo][4];                 // keys of a tile that are there
+    __shared__ float s_at[BIAS ? kInfo : 1][kTreeKeys];    // their positions
+    __shared__ float s_o[4][32][33];                       // the second stream's accumulator, 32 columns at a time
+    __shared__ float s_m[kTreeRows], s_l[kTreeRows];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (tid == 0) {
+        for (int t = 0; t < 2; ++t) {
+            mbar_init(bar_s + 8 * t, 1);
+            mbar_init(bar_p + 8 * t, 4);
+            mbar_init(bar_o + 8 * t, 1);
+            mbar_init(bar_qe + 8 * t, 1);
+        }
+        for (int i = 0; i < L::kStages; ++i) { mbar_init(bar_full + 8 * i, 4); mbar_init(bar_empty + 8 * i, 1); }
+        fence_mbar_init();
+    }
+    if (warp == 12) tmem_alloc(slot, 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    uint32_t tmem;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(slot));
+
+    // Ring entries of an item with n tiles, in the order in which the products take them:
+    // K0 K1 V0 K2 V1 .. K(n-1) V(n-2) V(n-1); the query tile comes with K0.
+    if (warp >= 12) {
+        regs_release<72>();
+        if (warp == 12 && elect_one()) {
+            const uint32_t id_s = mma_desc<T>(kTreeKeys, false, negate != 0), id_o = mma_desc<T>(HD, true);
+            int st = 0, ph = 0, pp[2] = { 0, 0 }, item = 0;
+            bool ok = true;
+            auto take = [&]() {
+                const int at = st;
+                if (!mbar_wait_bounded(bar_full + 8 * st, ph, p.err)) { ok = false; return 0; }
+                tc_fence_after();
+                if (++st == L::kStages) { st = 0; ph ^= 1; }
+                return at;
+            };
+            for (int at = blockIdx.x; at < sp.items && ok; at += gridDim.x) {
+                const TreeItem it = tree_item(p, sp, at);
+                if (it.tiles == 0) continue;
+                auto score = [&](int i) {
+                    const int e = take();
+                    if (!ok) return;
+                    mma_rows<HD>(tmem + (i & 1) * kTreeKeys, sm_q + (item & 1) * L::kTileBytes, sm_ring + e * L::kTileBytes, kTreeKeys, id_s);
+                    mma_commit(bar_s + 8 * (i & 1));
+                    mma_commit(bar_empty + 8 * e);
+                    if (i + 1 == it.tiles) mma_commit(bar_qe + 8 * (item & 1));
+                };
+                score(0);
+                if (it.tiles > 1 && ok) score(1);
+                for (int i = 0; i < it.tiles && ok; ++i) {
+                    const int t = i & 1, e = take();
+                    if (!ok || !(ok = mbar_wait_bounded(bar_p + 8 * t, pp[t], p.err))) break;
+                    pp[t] ^= 1;
+                    tc_fence_after();
+                    mma_weights<kTreeKeys>(tmem + 256 + t * HD, tmem + t * kTreeKeys, sm_ring + e * L::kTileBytes, id_o, i >= 2);
+                    mma_commit(bar_o + 8 * t);
+                    mma_commit(bar_empty + 8 * e);
+                    if (i + 2 < it.tiles) score(i + 2);
+                }
+                ++item;
+            }
+        }
+    } else if (warp >= 8) {
+        regs_release<80>();
+        const int w = warp - 8;
+        int st = 0, ph = 1, item = 0, entries = 0, handed = 0, info = 0;
+        bool ok = true;
+        // an entry is handed over when its copies are there: kAhead entries after they were issued, or at once
+        // where the products may need it before the next one can be issued
+        auto hand_over = [&](int up_to) {
+            fence_proxy_async();
+            __syncwarp();
+            for (; handed < up_to; ++handed)
+                if (lane == 0) mbar_arrive(bar_full + 8 * (handed % L::kStages));
+        };
+        for (int at = blockIdx.x; at < sp.items && ok; at += gridDim.x) {
+            const TreeItem it = tree_item(p, sp, at);
+            if (it.tiles == 0) continue;
+            auto entry = [&](int i, bool is_v) {
+                if (!mbar_wait_bounded(bar_empty + 8 * st, ph, p.err)) { ok = false; return; }
+                if (i == 0 && !is_v) {
+                    // this item's queries, where the last item's but one were: its products may still have to be begun
+                    if (!__all_sync(0xffffffffu, mbar_try_wait(bar_qe + 8 * (item & 1), ((item >> 1) & 1) ^ 1))) {
+                        cp_async_wait<0>();
+                        hand_over(entries);
+                    }
+                    if (!mbar_wait_bounded(bar_qe + 8 * (item & 1), ((item >> 1) & 1) ^ 1, p.err)) { ok = false; return; }
+                    const int r = it.row0 + w * 32 + lane;
+                    const char* src = nullptr;
+                    if (w * 32 + lane < it.rows)
+                        src = (const char*)row_of<T>(p.q, p.sq, it.b, it.hk * p.group + r % p.group, r / p.group);
+                    copy_rows<HD>(sm_q + (item & 1) * L::kTileBytes, w, lane, src, (const char*)p.q, p.D);
+                }
+                const int j = it.key0 + i * kTreeKeys + w * 32 + lane, index = j / p.page_size;
+                const char* src = nullptr;
+                if (j < it.n + it.real) {
+                    const int page = page_of(p.table, p.width, p.pages, p.err, it.b, index);
+                    if (page >= 0)
+                        src = is_v ? (const char*)(row_of<T>(p.v, p.sv, 0, it.hk, j - index * p.page_size) + page * p.sv[0])
+                                   : (const char*)(row_of<T>(p.k, p.sk, 0, it.hk, j - index * p.page_size) + page * p.sk[0]);
+                }
+                if (!is_v) {
+                    const unsigned valid = __ballot_sync(0xffffffffu, src != nullptr);
+                    if (lane == 0) s_valid[info][w] = valid;
+                    if (BIAS) {
+                        int pos = j;
+                        if (src != nullptr) {
+                            if (j >= it.n) pos = first_position(p, it.b, it.n) + depth_of(tokens_above(p, it.b, j - it.n));
+                            else if (p.positions) pos = __ldg(p.positions + ((long long)it.b * p.Hkv + it.hk) * p.slots + j);
+                        }
+                        s_at[info][w * 32 + lane] = (float)pos;
+                    }
+                    info = (info + 1) % kInfo;
+                }
+                copy_rows<HD>(sm_ring + st * L::kTileBytes, w, lane, src, is_v ? (const char*)p.v : (const char*)p.k, p.D);
+                cp_async_commit();
+                if (++st == L::kStages) { st = 0; ph ^= 1; }
+                if (++entries - handed > L::kAhead) {
+                    cp_async_wait<L::kAhead>();
+                    hand_over(entries - L::kAhead);
+                }
+            };
+            entry(0, false);
+            if (it.tiles > 1 && ok) entry(1, false);
+            for (int i = 0; i < it.tiles && ok; ++i) {
+                entry(i, true);
+                if (i + 2 < it.tiles && ok) entry(i + 2, false);
+            }
+            ++item;
+        }
+        cp_async_wait<0>();
+        if (ok) hand_over(entries);
+    } else {
+        regs_claim<176>();
+        const int tile = warp >> 2, quad = warp & 3, in_tile = quad * 32 + lane;
+        const uint32_t lanes = (uint32_t)quad << 21, s_col = tmem + tile * kTreeKeys + lanes, o_col = tmem + 256 + tile * HD + lanes;
+        ScoreConsts c;
+        c.scale2 = fabsf(p.sm_scale) * kLog2e;
+        c.cap_in = CAP ? 2.0f * c.scale2 / p.cap : 0.0f;
+        c.cap_out = CAP ? p.cap * kLog2e : 0.0f;
+        int done = 0, info = 0;           // key tiles of this stream, of the block, so far
+        bool ok = true;
+        for (int at = blockIdx.x; at < sp.items && ok; at += gridDim.x) {
+            const TreeItem it = tree_item(p, sp, at);
+            if (it.tiles == 0 && it.chunk > 0) continue;
+            const bool busy = quad * 32 < it.rows;        // this warp has rows
+            const int gr = it.row0 + in_tile, t = gr / p.group, h = it.hk * p.group + gr % p.group;
+            const bool valid = in_tile < it.rows, real = valid && t < it.real;
+            unsigned long long above = real ? tokens_above(p, it.b, t) : 0ull;
+            const float slope2 = BIAS && valid ? __ldg(p.slopes + h) * kLog2e : 0.0f;
+            const float pos = BIAS && real ? (float)(first_position(p, it.b, it.n) + depth_of(above)) : 0.0f;
+            float m = kNegInf, l = 0.0f;
+            int mine = 0;
+            for (int i = tile; i < it.tiles; i += 2, ++mine) {
+                if (!mbar_wait_bounded(bar_s + 8 * tile, (done + mine) & 1, p.err)) { ok = false; break; }
+                tc_fence_after();
+                if (busy) {
+                    float s[kTreeKeys];
+#pragma unroll
+                    for (int x = 0; x < kTreeKeys; x += 32) tmem_ld32(s_col + x, s + x);
+                    tmem_wait_ld();
+                    const int slot_i = (info + i) % kInfo, k0 = it.key0 + i * kTreeKeys;
+                    unsigned see[4], all = ~0u;
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        const int left = it.n - (k0 + w * 32);       // cached keys from this word on
+                        const unsigned cached = left >= 32 ? ~0u : left > 0 ? (1u << left) - 1 : 0u;
+                        const unsigned tree = left >= 32 ? 0u : left > 0 ? (unsigned)(above << left) : left > -64 ? (unsigned)(above >> -left) : 0u;
+                        see[w] = real ? (cached | tree) & s_valid[slot_i][w] : 0u;
+                        all &= see[w];
+                    }
+                    if (CAP || BIAS) {
+#pragma unroll
+                        for (int x = 0; x < kTreeKeys; ++x) {
+                            float v = CAP ? capped_score2(s[x], c) : s[x] * c.scale2;
+                            if (BIAS) v = fmaf(-slope2, fabsf(pos - s_at[slot_i][x]), v);
+                            s[x] = v;
+                        }
+                    }
+                    if (!__all_sync(0xffffffffu, all == ~0u)) {
+#pragma unroll
+                        for (int x = 0; x < kTreeKeys; ++x) s[x] = see[x >> 5] >> (x & 31) & 1u ? s[x] : kNegInf;
+                    }
+                    float mx[4] = { s[0], s[1], s[2], s[3] };
+#pragma unroll
+                    for (int x = 4; x < kTreeKeys; ++x) mx[x & 3] = fmaxf(mx[x & 3], s[x]);
+                    float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                    if (!(CAP || BIAS)) top *= c.scale2;
+                    const bool move = top > m + 8.0f || (m == kNegInf && top > kNegInf);
+                    if (__any_sync(0xffffffffu, move)) {
+                        const float f = move ? (m == kNegInf ? 0.0f : fast_exp2(m - top)) : 1.0f;
+                        if (move) m = top;
+                        l *= f;
+                        if (mine > 0) {
+                            if (!mbar_wait_bounded(bar_o + 8 * tile, (done + mine - 1) & 1, p.err)) { ok = false; break; }
+                            tc_fence_after();
+#pragma unroll
+                            for (int x = 0; x < HD; x += 16) {
+                                float o[16];
+                                tmem_ld16(o_col + x, o);
+                                tmem_wait_ld();
+#pragma unroll
+                                for (int y = 0; y < 16; ++y) o[y] *= f;
+                                tmem_st16(o_col + x, reinterpret_cast<const uint32_t*>(o));
+                            }
+                        }
+                    }
+                    const float m0 = m == kNegInf ? 0.0f : m;
+                    float sum[4] = { 0.0f, 0.0f, 0.0f, 0.0f };
+#pragma unroll
+                    for (int x = 0; x < kTreeKeys; x += 32) {
+                        uint32_t w[16];
+#pragma unroll
+                        for (int y = 0; y < 32; y += 2) {
+                            const float a = (CAP || BIAS) ? s[x + y] - m0 : fmaf(s[x + y], c.scale2, -m0);
+                            const float e = (CAP || BIAS) ? s[x + y + 1] - m0 : fmaf(s[x + y + 1], c.scale2, -m0);
+                            const float pa = fast_exp2(a), pe = fast_exp2(e);
+                            sum[(y >> 1) & 1] += pa;
+                            sum[2 + ((y >> 1) & 1)] += pe;
+                            w[y / 2] = pack2<T>(pa, pe);
+                        }
+                        tmem_st16(s_col + x / 2, w);
+                    }
+                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    tmem_wait_st();
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar_p + 8 * tile);
+            }
+            if (!ok) break;
+            done += mine;
+            info = (info + it.tiles) % kInfo;
+            if (mine > 0 && !(ok = mbar_wait_bounded(bar_o + 8 * tile, (done - 1) & 1, p.err))) break;
+            if (!busy) continue;                           // the same for a warp and its partner of the other stream
+            tc_fence_after();
+            if (tile == 1) { s_m[in_tile] = m; s_l[in_tile] = l; }
+            pair_barrier(1 + quad);
+            // results of both streams to the larger of the two reference points
+            float f0 = 0.0f, f1 = 0.0f, inv = 0.0f, lse = kNegInf;
+            if (tile == 0) {
+                const float m1 = s_m[in_tile], l1 = s_l[in_tile], top = fmaxf(m, m1), t0 = top == kNegInf ? 0.0f : top;
+                f0 = fast_exp2(m - t0);
+                f1 = fast_exp2(m1 - t0);
+                const float sum = l * f0 + l1 * f1;
+                inv = sum != 0.0f ? 1.0f / sum : 0.0f;
+                lse = sum != 0.0f ? t0 + log2f(sum) : kNegInf;
+            }
+            pair_barrier(1 + quad);
+            const bool other = it.tiles > 1;               // the second stream has something
+            const long long row = ((long long)it.b * p.Hq + h) * p.T + t;
+            bool fine = lse == lse;
+#pragma unroll
+            for (int x = 0; x < HD; x += 32) {
+                if (tile == 1 && other) {
+                    float o[32];
+                    tmem_ld32(o_col + x, o);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int y = 0; y < 32; ++y) s_o[quad][lane][y] = o[y];
+                }
+                if (other) pair_barrier(1 + quad);
+                if (tile == 0) {
+                    float o[32];
+                    if (it.tiles > 0) {
+                        tmem_ld32(o_col + x, o);
+                        tmem_wait_ld();
+                    }
+                    const bool some = it.tiles > 0 && inv != 0.0f;
+#pragma unroll
+                    for (int y = 0; y < 32; ++y) {
+                        float v = some ? o[y] * f0 : 0.0f;
+                        if (some && other) v = fmaf(s_o[quad][lane][y], f1, v);
+                        o[y] = v * inv;
+                        fine = fine && fabsf(o[y]) <= 3.0e38f;
+                    }
+                    if (valid) {
+                        if (sp.chunks == 1) {
+                            T* out = (T*)p.out + row * p.D + x;
+#pragma unroll
+                            for (int y = 0; y < 32; y += 8)
+                                if (x + y < p.D) store8<T>(out + y, *reinterpret_cast<const float(*)[8]>(o + y));
+                        } else {
+                            float* out = sp.part + (row * sp.chunks + it.chunk) * p.D + x;
+#pragma unroll
+                            for (int y = 0; y < 32; y += 8)
+                                if (x + y < p.D) store8<float>(out + y, *reinterpret_cast<const float(*)[8]>(o + y));
+                        }
+                    }
+                }
+                if (other) pair_barrier(1 + quad);
+            }
+            if (tile == 0) {
+                if (valid) {
+                    if (sp.chunks == 1) p.lse[row] = lse;
+                    else sp.part_lse[row * sp.chunks + it.chunk] = lse;
+                }
+                __syncwarp();
+                // rows that something non-finite reached: once more, from the keys they see alone
+                unsigned bad = sp.chunks == 1 ? __ballot_sync(0xffffffffu, valid && !fine) : 0u;
+                while (bad) {
+                    const int r = __ffs(bad) - 1;
+                    bad &= bad - 1;
+                    const int g = gr - lane + r;
+                    exact_row_tree<T>(p, it.b, it.hk * p.group + g % p.group, g / p.group);
+                }
+            }
+            tc_fence_before();
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 12) tmem_free(tmem, 512);
+}
+
+// Joins the chunks of a row: out = sum_c 2^(lse_c - lse) part_c.  One warp a row.
+constexpr int kCombineWarps = 4;
+template <typename T>
+__global__ void __launch_bounds__(kCombineWarps * 32) tree_combine_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeSplit sp) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const long long row = (long long)blockIdx.x * kCombineWarps + threadIdx.x / 32;
+    if (row >= (long long)p.B * p.Hq * p.T) return;
+    const int lane = threadIdx.x & 31, t = (int)(row % p.T), h = (int)(row / p.T % p.Hq), b = (int)(row / p.T / p.Hq);
+    const int n = cached_keys(p, b), real = drafted_tokens(p, b);
+    const int used = t < real ? (n + real + sp.chunk - 1) / sp.chunk : 0;
+    const float* lses = sp.part_lse + row * sp.chunks;
+    float m = kNegInf;
+    bool nan = false;
+    for (int c = lane; c < used; c += 32) {
+        const float x = lses[c];
+        nan = nan || x != x;
+        m = fmaxf(m, x);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    nan = __any_sync(0xffffffffu, nan);
+    const float m0 = m == kNegInf ? 0.0f : m;
+    float sum = 0.0f, acc[2][4] = {};
+    const float* part = sp.part + row * sp.chunks * p.D + lane * 4;
+    for (int c = 0; c < used; ++c) {
+        const float f = exp2f(lses[c] - m0);
+        sum += f;
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+            if (k * 128 + lane * 4 < p.D) {
+                const float4 v = *reinterpret_cast<const float4*>(part + (long long)c * p.D + k * 128);
+                acc[k][0] = fmaf(f, v.x, acc[k][0]);
+                acc[k][1] = fmaf(f, v.y, acc[k][1]);
+                acc[k][2] = fmaf(f, v.z, acc[k][2]);
+                acc[k][3] = fmaf(f, v.w, acc[k][3]);
+            }
+    }
+    const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
+    bool fine = !nan;
+    T* out = (T*)p.out + row * p.D + lane * 4;
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+        if (k * 128 + lane * 4 < p.D) {
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                v[e] = acc[k][e] * inv;
+                fine = fine && fabsf(v[e]) <= 3.0e38f;
+            }
+            store4(out + k * 128, v);
+        }
+    if (lane == 0) p.lse[row] = sum != 0.0f ? m0 + log2f(sum) : kNegInf;
+    __syncwarp();
+    if (__any_sync(0xffffffffu, !fine)) exact_row_tree<T>(p, b, h, t);
+}
+
+}  // namespace dsdpa
