@@ -72,7 +72,6 @@ int check_tokens(const dsdpa_cache_problem* p) {
     if (st != DSDPA_OK) return st;
     if (p->Hq <= 0 || p->Hq % p->Hkv || (long long)p->B * p->Hq >= (1ll << 24) || p->T <= 0) return DSDPA_ERR_BAD_SHAPE;
     if (p->T > kTreeMax) return DSDPA_ERR_TOO_LARGE;
-    if (on_tensor_cores(*p) && plan_tree(*p).items == 0) return DSDPA_ERR_TOO_LARGE;
     if (!isfinite(p->sm_scale) || !isfinite(p->softcap)) return DSDPA_ERR_BAD_SHAPE;
     const int e = p->dtype == DSDPA_F32 ? 4 : 2;
     for (int i = 0; i < 3; ++i)

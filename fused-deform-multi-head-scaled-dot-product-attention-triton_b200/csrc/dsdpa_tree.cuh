@@ -1,13 +1,15 @@
 // Attention of drafted tokens over a paged cache on the tensor cores: 16-bit storage, head dimensions up
 // to 128.
 //
-// The queries that share a key/value head -- tokens times the group's heads, up to 128 a tile -- are one operand,
-// so that the cache is read once for all of them.  Keys are split over blocks in chunks, whose results
-// tree_combine_kernel joins; a block stays and takes one item (sequence, head, query tile, chunk) after the
-// other, its loads running ahead of its arithmetic across items, so that the memory never waits.
-// Inside an item key tiles of 128 go in turn to two streams, each with its own running maximum, sum and
-// accumulator (tensor memory holds both), joined at the item's end: one stream's softmax runs while the
-// other's products do, which matters when a handful of rows leaves a single warp with all of the softmax.
+// The queries that share a key/value head -- tokens times the group's heads, up to 128 a tile: a unit -- are one
+// operand, so that the cache is read once for all of them.  The key tiles of all units lie one behind the
+// other, and every block takes an equal share of that line, whatever the lengths are (they are known on the
+// device only): whole units, and at the ends of its share parts of units, whose results
+// tree_combine_kernel joins.  So all blocks end together, and no more than two parts a block have to be
+// written and read again.  A block's loads run ahead of its arithmetic, from one unit into the next.
+// Inside a unit key tiles of 128 go in turn to two streams, each with its own running maximum, sum and
+// accumulator (tensor memory holds both), joined at the end: one stream's softmax runs while the other's
+// products do, which matters when a handful of rows leaves a single warp with all of the softmax.
 // Bound by DRAM for few rows (the cache is read once), by exp2 beyond about a hundred.
 // Roles: warps 0-3 and 4-7 the streams' softmax, 8-11 copy rows (cp.async: any page size and stride, rows
 // that are not there read as zero), 12 issues the matrix instructions.
@@ -18,18 +20,19 @@
 
 namespace dsdpa {
 
-constexpr int kTreeThreads = 512;   // launched with 128 registers: 256 x 176 + 128 x 80 + 128 x 72 = 64512 of 65536
+constexpr int kTreeThreads = 416;
 constexpr int kTreeRows = 128, kTreeKeys = 128, kInfo = 16;
 
-struct TreeSplit {
-    int chunk;        // keys of an item, a multiple of 2 * kTreeKeys
-    int chunks;       // of the longest sequence that the table can hold
-    int row_tiles;
-    int items;
-    float* part;      // [B * Hq * T][chunks][D], normalised
-    float* part_lse;  // [B * Hq * T][chunks]
-};
+constexpr int kTreeMinShare = 2;    // key tiles: one for each stream
 
+struct TreeSplit {
+    int whole;            // units are not cut: no parts, no tree_combine_kernel
+    int row_tiles;
+    int part_rows;        // rows of a part
+    long long* start;     // [B + 1]: key tiles of a head's query tile in the sequences before, and [B + 1]: a block's share
+    float* part;          // [blocks * 2][part_rows][D], normalised
+    float* part_lse;      // [blocks * 2][part_rows]
+};
 template <int HD>
 struct TreeLayout {
     static constexpr int kTileBytes = 128 * HD * 2;
@@ -40,24 +43,58 @@ struct TreeLayout {
     static constexpr int kSmem = 2 * kTileBytes + kStages * kTileBytes + 1024 + 512;
 };
 
-struct TreeItem {
-    int b, hk, row0, rows, chunk, n, real, key0, tiles;
-};
-__device__ __forceinline__ TreeItem tree_item(const CacheParams& p, const TreeSplit& s, int at) {
-    TreeItem it;
-    it.chunk = at % s.chunks; at /= s.chunks;
-    it.row0 = at % s.row_tiles * kTreeRows; at /= s.row_tiles;
-    it.hk = at % p.Hkv;
-    it.b = at / p.Hkv;
-    it.rows = min(kTreeRows, p.T * p.group - it.row0);
-    it.n = cached_keys(p, it.b);
-    it.real = drafted_tokens(p, it.b);
-    it.key0 = it.chunk * s.chunk;
-    const int keys = it.real > 0 ? it.n + it.real : 0;
-    it.tiles = max(0, min(s.chunk, keys - it.key0) + kTreeKeys - 1) / kTreeKeys;
-    if (keys <= it.key0) it.tiles = 0;
-    return it;
+// Key tiles of a sequence: the same for all of its heads.
+__device__ __forceinline__ int tree_tiles(const CacheParams& p, int b) {
+    const int real = drafted_tokens(p, b);
+    return real > 0 ? (cached_keys(p, b) + real + kTreeKeys - 1) / kTreeKeys : 0;
 }
+
+// A unit, or the part of one that lies in a block's share.
+struct TreeItem {
+    int b, hk, row0, rows, n, real, key0, tiles;
+    int part;             // where its result goes: -1 to out and lse, else the number of the part
+};
+// Goes through the items of a block; every role has its own.
+struct TreeWalk {
+    int b, unit, tile;    // unit: of the sequence's heads * row_tiles
+    long long left;       // key tiles of the share; whole units: number of the next unit
+    bool first;
+    __device__ __forceinline__ bool next(const CacheParams& p, const TreeSplit& s, TreeItem& it) {
+        const int units = p.Hkv * s.row_tiles;
+        if (s.whole) {
+            if (left >= (long long)p.B * units) return false;
+            b = (int)(left / units);
+            unit = (int)(left % units);
+            tile = 0;
+            it.tiles = tree_tiles(p, b);
+            it.part = -1;
+            left += gridDim.x;
+        } else {
+            int nt = 0;
+            while (left > 0) {
+                nt = tree_tiles(p, b);
+                if (unit < units && nt > 0) break;
+                ++b;
+                unit = 0;
+            }
+            if (left <= 0) return false;
+            it.tiles = (int)min((long long)(nt - tile), left);
+            it.part = it.tiles == nt ? -1 : (int)blockIdx.x * 2 + (first ? 0 : 1);
+            left -= it.tiles;
+        }
+        first = false;
+        it.b = b;
+        it.hk = unit / s.row_tiles;
+        it.row0 = unit % s.row_tiles * kTreeRows;
+        it.rows = min(kTreeRows, p.T * p.group - it.row0);
+        it.n = cached_keys(p, b);
+        it.real = drafted_tokens(p, b);
+        it.key0 = tile * kTreeKeys;
+        ++unit;
+        tile = 0;
+        return true;
+    }
+};
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, unsigned bytes) {   // the rest of 16 is zero
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -93,6 +130,8 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
     __shared__ float s_at[BIAS ? kInfo : 1][kTreeKeys];    // their positions
     __shared__ float s_o[4][32][33];                       // the second stream's accumulator, 32 columns at a time
     __shared__ float s_m[kTreeRows], s_l[kTreeRows];
+    __shared__ long long s_sum[kTreeThreads / 32], s_left;
+    __shared__ int s_b, s_unit, s_tile;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -107,16 +146,60 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
         fence_mbar_init();
     }
     if (warp == 12) tmem_alloc(slot, 512);
+    if (sp.whole) {
+        if (tid == 0) { s_left = blockIdx.x; s_b = s_unit = s_tile = 0; }
+    } else {
+        // where this block's share begins: a thread has the key tiles of a few sequences
+        const int per = (p.B + kTreeThreads - 1) / kTreeThreads, b0 = min(p.B, tid * per), b1 = min(p.B, b0 + per);
+        long long mine = 0;
+        for (int b = b0; b < b1; ++b) mine += tree_tiles(p, b);
+        long long upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long t = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += t;
+        }
+        if (lane == 31) s_sum[warp] = upto;
+        if (tid == 0) { s_left = 0; s_b = s_unit = s_tile = 0; }
+        __syncthreads();
+        long long before = upto - mine, total = 0;
+        for (int w = 0; w < kTreeThreads / 32; ++w) {
+            if (w < warp) before += s_sum[w];
+            total += s_sum[w];
+        }
+        const int units = p.Hkv * sp.row_tiles;
+        const long long line = total * units, share = max((long long)kTreeMinShare, (line + gridDim.x - 1) / gridDim.x);
+        const long long from = share * blockIdx.x;
+        if (blockIdx.x == 0) {
+            long long at = before;
+            for (int b = b0; b < b1; ++b) { sp.start[b] = at; at += tree_tiles(p, b); }
+            if (tid == 0) { sp.start[p.B] = total; sp.start[p.B + 1] = share; }
+        }
+        if (from < line && from >= before * units && from < (before + mine) * units) {
+            long long at = before * units;
+            int b = b0;
+            for (;; ++b) {
+                const long long span = (long long)tree_tiles(p, b) * units;
+                if (from < at + span) break;
+                at += span;
+            }
+            const int nt = tree_tiles(p, b);
+            s_b = b;
+            s_unit = (int)((from - at) / nt);
+            s_tile = (int)((from - at) % nt);
+            s_left = min(share, line - from);
+        }
+    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     uint32_t tmem;
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(slot));
+    TreeWalk walk{ s_b, s_unit, s_tile, s_left, true };
 
     // Ring entries of an item with n tiles, in the order in which the products take them:
     // K0 K1 V0 K2 V1 .. K(n-1) V(n-2) V(n-1); the query tile comes with K0.
     if (warp >= 12) {
-        regs_release<72>();
         if (warp == 12 && elect_one()) {
             const uint32_t id_s = mma_desc<T>(kTreeKeys, false, negate != 0), id_o = mma_desc<T>(HD, true);
             int st = 0, ph = 0, pp[2] = { 0, 0 }, item = 0;
@@ -128,8 +211,8 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
                 if (++st == L::kStages) { st = 0; ph ^= 1; }
                 return at;
             };
-            for (int at = blockIdx.x; at < sp.items && ok; at += gridDim.x) {
-                const TreeItem it = tree_item(p, sp, at);
+            TreeItem it;
+            while (ok && walk.next(p, sp, it)) {
                 if (it.tiles == 0) continue;
                 auto score = [&](int i) {
                     const int e = take();
@@ -155,7 +238,6 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
             }
         }
     } else if (warp >= 8) {
-        regs_release<80>();
         const int w = warp - 8;
         int st = 0, ph = 1, item = 0, entries = 0, handed = 0, info = 0;
         bool ok = true;
@@ -167,10 +249,30 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
             for (; handed < up_to; ++handed)
                 if (lane == 0) mbar_arrive(bar_full + 8 * (handed % L::kStages));
         };
-        for (int at = blockIdx.x; at < sp.items && ok; at += gridDim.x) {
-            const TreeItem it = tree_item(p, sp, at);
-            if (it.tiles == 0) continue;
-            auto entry = [&](int i, bool is_v) {
+        // Page numbers are asked for ahead of the rows they lead to: a tile's three tiles before, the next item's
+        // first ones while this item's rows are copied.
+        auto next_item = [&](TreeItem& it) {
+            do {
+                if (!walk.next(p, sp, it)) it.tiles = -1;
+            } while (it.tiles == 0);
+        };
+        auto lookup = [&](const TreeItem& it, int i) {          // -1: no row
+            const int j = it.key0 + i * kTreeKeys + w * 32 + lane;
+            return i < it.tiles && j < it.n + it.real ? page_of(p.table, p.width, p.pages, p.err, it.b, j / p.page_size) : -1;
+        };
+        TreeItem it;
+        next_item(it);
+        int page[3] = { lookup(it, 0), lookup(it, 1), lookup(it, 2) };
+        while (it.tiles > 0 && ok) {
+            TreeItem then;
+            next_item(then);
+            const int after[3] = { lookup(then, 0), lookup(then, 1), lookup(then, 2) };
+            auto entry = [&](int i, bool is_v, int pg) {
+                const int j = it.key0 + i * kTreeKeys + w * 32 + lane, key = j - j / p.page_size * p.page_size;
+                const char* src = nullptr;
+                if (pg >= 0)
+                    src = is_v ? (const char*)(row_of<T>(p.v, p.sv, 0, it.hk, key) + pg * p.sv[0])
+                               : (const char*)(row_of<T>(p.k, p.sk, 0, it.hk, key) + pg * p.sk[0]);
                 if (!mbar_wait_bounded(bar_empty + 8 * st, ph, p.err)) { ok = false; return; }
                 if (i == 0 && !is_v) {
                     // this item's queries, where the last item's but one were: its products may still have to be begun
@@ -180,18 +282,10 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
                     }
                     if (!mbar_wait_bounded(bar_qe + 8 * (item & 1), ((item >> 1) & 1) ^ 1, p.err)) { ok = false; return; }
                     const int r = it.row0 + w * 32 + lane;
-                    const char* src = nullptr;
+                    const char* from = nullptr;
                     if (w * 32 + lane < it.rows)
-                        src = (const char*)row_of<T>(p.q, p.sq, it.b, it.hk * p.group + r % p.group, r / p.group);
-                    copy_rows<HD>(sm_q + (item & 1) * L::kTileBytes, w, lane, src, (const char*)p.q, p.D);
-                }
-                const int j = it.key0 + i * kTreeKeys + w * 32 + lane, index = j / p.page_size;
-                const char* src = nullptr;
-                if (j < it.n + it.real) {
-                    const int page = page_of(p.table, p.width, p.pages, p.err, it.b, index);
-                    if (page >= 0)
-                        src = is_v ? (const char*)(row_of<T>(p.v, p.sv, 0, it.hk, j - index * p.page_size) + page * p.sv[0])
-                                   : (const char*)(row_of<T>(p.k, p.sk, 0, it.hk, j - index * p.page_size) + page * p.sk[0]);
+                        from = (const char*)row_of<T>(p.q, p.sq, it.b, it.hk * p.group + r % p.group, r / p.group);
+                    copy_rows<HD>(sm_q + (item & 1) * L::kTileBytes, w, lane, from, (const char*)p.q, p.D);
                 }
                 if (!is_v) {
                     const unsigned valid = __ballot_sync(0xffffffffu, src != nullptr);
@@ -214,18 +308,25 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
                     hand_over(entries - L::kAhead);
                 }
             };
-            entry(0, false);
-            if (it.tiles > 1 && ok) entry(1, false);
+            entry(0, false, page[0]);
+            if (it.tiles > 1 && ok) entry(1, false, page[1]);
             for (int i = 0; i < it.tiles && ok; ++i) {
-                entry(i, true);
-                if (i + 2 < it.tiles && ok) entry(i + 2, false);
+                const int more = lookup(it, i + 3);
+                entry(i, true, page[0]);
+                if (i + 2 < it.tiles && ok) entry(i + 2, false, page[2]);
+                page[0] = page[1];
+                page[1] = page[2];
+                page[2] = more;
             }
             ++item;
+            it = then;
+            page[0] = after[0];
+            page[1] = after[1];
+            page[2] = after[2];
         }
         cp_async_wait<0>();
         if (ok) hand_over(entries);
     } else {
-        regs_claim<176>();
         const int tile = warp >> 2, quad = warp & 3, in_tile = quad * 32 + lane;
         const uint32_t lanes = (uint32_t)quad << 21, s_col = tmem + tile * kTreeKeys + lanes, o_col = tmem + 256 + tile * HD + lanes;
         ScoreConsts c;
@@ -234,9 +335,8 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
         c.cap_out = CAP ? p.cap * kLog2e : 0.0f;
         int done = 0, info = 0;           // key tiles of this stream, of the block, so far
         bool ok = true;
-        for (int at = blockIdx.x; at < sp.items && ok; at += gridDim.x) {
-            const TreeItem it = tree_item(p, sp, at);
-            if (it.tiles == 0 && it.chunk > 0) continue;
+        TreeItem it;
+        while (ok && walk.next(p, sp, it)) {
             const bool busy = quad * 32 < it.rows;        // this warp has rows
             const int gr = it.row0 + in_tile, t = gr / p.group, h = it.hk * p.group + gr % p.group;
             const bool valid = in_tile < it.rows, real = valid && t < it.real;
@@ -249,10 +349,7 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
                 if (!mbar_wait_bounded(bar_s + 8 * tile, (done + mine) & 1, p.err)) { ok = false; break; }
                 tc_fence_after();
                 if (busy) {
-                    float s[kTreeKeys];
-#pragma unroll
-                    for (int x = 0; x < kTreeKeys; x += 32) tmem_ld32(s_col + x, s + x);
-                    tmem_wait_ld();
+                    // 32 columns at a time, twice (for the maximum, for the weights): few registers and little code
                     const int slot_i = (info + i) % kInfo, k0 = it.key0 + i * kTreeKeys;
                     unsigned see[4], all = ~0u;
 #pragma unroll
@@ -263,22 +360,33 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
                         see[w] = real ? (cached | tree) & s_valid[slot_i][w] : 0u;
                         all &= see[w];
                     }
-                    if (CAP || BIAS) {
+                    const bool whole = __all_sync(0xffffffffu, all == ~0u);
+                    float top = kNegInf;
+#pragma unroll 1
+                    for (int w = 0; w < 4; ++w) {
+                        float s[32];
+                        tmem_ld32(s_col + w * 32, s);
+                        tmem_wait_ld();
+                        if (CAP || BIAS) {
 #pragma unroll
-                        for (int x = 0; x < kTreeKeys; ++x) {
-                            float v = CAP ? capped_score2(s[x], c) : s[x] * c.scale2;
-                            if (BIAS) v = fmaf(-slope2, fabsf(pos - s_at[slot_i][x]), v);
-                            s[x] = v;
+                            for (int x = 0; x < 32; ++x) {
+                                float v = CAP ? capped_score2(s[x], c) : s[x] * c.scale2;
+                                if (BIAS) v = fmaf(-slope2, fabsf(pos - s_at[slot_i][w * 32 + x]), v);
+                                s[x] = v;
+                            }
                         }
-                    }
-                    if (!__all_sync(0xffffffffu, all == ~0u)) {
+                        if (!whole) {
+                            const unsigned bits = w == 0 ? see[0] : w == 1 ? see[1] : w == 2 ? see[2] : see[3];
 #pragma unroll
-                        for (int x = 0; x < kTreeKeys; ++x) s[x] = see[x >> 5] >> (x & 31) & 1u ? s[x] : kNegInf;
-                    }
-                    float mx[4] = { s[0], s[1], s[2], s[3] };
+                            for (int x = 0; x < 32; ++x) s[x] = bits >> x & 1u ? s[x] : kNegInf;
+                        }
+                        if (CAP || BIAS || !whole) tmem_st32(s_col + w * 32, reinterpret_cast<const uint32_t*>(s));
+                        float mx[4] = { s[0], s[1], s[2], s[3] };
 #pragma unroll
-                    for (int x = 4; x < kTreeKeys; ++x) mx[x & 3] = fmaxf(mx[x & 3], s[x]);
-                    float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                        for (int x = 4; x < 32; ++x) mx[x & 3] = fmaxf(mx[x & 3], s[x]);
+                        top = fmaxf(top, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+                    }
+                    if (CAP || BIAS || !whole) tmem_wait_st();
                     if (!(CAP || BIAS)) top *= c.scale2;
                     const bool move = top > m + 8.0f || (m == kNegInf && top > kNegInf);
                     if (__any_sync(0xffffffffu, move)) {
@@ -288,32 +396,35 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
                         if (mine > 0) {
                             if (!mbar_wait_bounded(bar_o + 8 * tile, (done + mine - 1) & 1, p.err)) { ok = false; break; }
                             tc_fence_after();
-#pragma unroll
-                            for (int x = 0; x < HD; x += 16) {
-                                float o[16];
-                                tmem_ld16(o_col + x, o);
+#pragma unroll 1
+                            for (int x = 0; x < HD; x += 32) {
+                                float o[32];
+                                tmem_ld32(o_col + x, o);
                                 tmem_wait_ld();
 #pragma unroll
-                                for (int y = 0; y < 16; ++y) o[y] *= f;
-                                tmem_st16(o_col + x, reinterpret_cast<const uint32_t*>(o));
+                                for (int y = 0; y < 32; ++y) o[y] *= f;
+                                tmem_st32(o_col + x, reinterpret_cast<const uint32_t*>(o));
                             }
                         }
                     }
                     const float m0 = m == kNegInf ? 0.0f : m;
                     float sum[4] = { 0.0f, 0.0f, 0.0f, 0.0f };
-#pragma unroll
-                    for (int x = 0; x < kTreeKeys; x += 32) {
-                        uint32_t w[16];
+#pragma unroll 1
+                    for (int w = 0; w < 4; ++w) {
+                        float s[32];
+                        uint32_t u[16];
+                        tmem_ld32(s_col + w * 32, s);
+                        tmem_wait_ld();
 #pragma unroll
                         for (int y = 0; y < 32; y += 2) {
-                            const float a = (CAP || BIAS) ? s[x + y] - m0 : fmaf(s[x + y], c.scale2, -m0);
-                            const float e = (CAP || BIAS) ? s[x + y + 1] - m0 : fmaf(s[x + y + 1], c.scale2, -m0);
+                            const float a = (CAP || BIAS) ? s[y] - m0 : fmaf(s[y], c.scale2, -m0);
+                            const float e = (CAP || BIAS) ? s[y + 1] - m0 : fmaf(s[y + 1], c.scale2, -m0);
                             const float pa = fast_exp2(a), pe = fast_exp2(e);
                             sum[(y >> 1) & 1] += pa;
                             sum[2 + ((y >> 1) & 1)] += pe;
-                            w[y / 2] = pack2<T>(pa, pe);
+                            u[y / 2] = pack2<T>(pa, pe);
                         }
-                        tmem_st16(s_col + x / 2, w);
+                        tmem_st16(s_col + w * 16, u);     // behind what has been read
                     }
                     l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                     tmem_wait_st();
@@ -331,67 +442,73 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
             if (tile == 1) { s_m[in_tile] = m; s_l[in_tile] = l; }
             pair_barrier(1 + quad);
             // results of both streams to the larger of the two reference points
-            float f0 = 0.0f, f1 = 0.0f, inv = 0.0f, lse = kNegInf;
+            float g0 = 0.0f, g1 = 0.0f, inv = 0.0f, lse = kNegInf;
             if (tile == 0) {
                 const float m1 = s_m[in_tile], l1 = s_l[in_tile], top = fmaxf(m, m1), t0 = top == kNegInf ? 0.0f : top;
-                f0 = fast_exp2(m - t0);
-                f1 = fast_exp2(m1 - t0);
-                const float sum = l * f0 + l1 * f1;
+                const float f0 = fast_exp2(m - t0), f1 = fast_exp2(m1 - t0), sum = l * f0 + l1 * f1;
                 inv = sum != 0.0f ? 1.0f / sum : 0.0f;
                 lse = sum != 0.0f ? t0 + log2f(sum) : kNegInf;
+                g0 = f0 * inv;
+                g1 = f1 * inv;
             }
             pair_barrier(1 + quad);
             const bool other = it.tiles > 1;               // the second stream has something
-            const long long row = ((long long)it.b * p.Hq + h) * p.T + t;
-            bool fine = lse == lse;
-#pragma unroll
+            const long long row = ((long long)it.b * p.Hq + h) * p.T + t, part = (long long)it.part * sp.part_rows + in_tile;
+            // a sum of 0 x over the results is NaN where one is not finite
+            float nan0 = 0.0f * l, nan1 = 0.0f;
+#pragma unroll 1
             for (int x = 0; x < HD; x += 32) {
-                if (tile == 1 && other) {
-                    float o[32];
+                float o[32] = {};
+                if (it.tiles > tile) {
                     tmem_ld32(o_col + x, o);
                     tmem_wait_ld();
-#pragma unroll
-                    for (int y = 0; y < 32; ++y) s_o[quad][lane][y] = o[y];
                 }
-                if (other) pair_barrier(1 + quad);
-                if (tile == 0) {
-                    float o[32];
-                    if (it.tiles > 0) {
-                        tmem_ld32(o_col + x, o);
-                        tmem_wait_ld();
-                    }
-                    const bool some = it.tiles > 0 && inv != 0.0f;
+                if (other) {
+                    if (tile == 1) {
 #pragma unroll
-                    for (int y = 0; y < 32; ++y) {
-                        float v = some ? o[y] * f0 : 0.0f;
-                        if (some && other) v = fmaf(s_o[quad][lane][y], f1, v);
-                        o[y] = v * inv;
-                        fine = fine && fabsf(o[y]) <= 3.0e38f;
+                        for (int y = 0; y < 32; ++y) s_o[quad][lane][y] = o[y];
+                    }
+                    pair_barrier(1 + quad);
+                }
+                if (tile == 0) {
+                    if (inv == 0.0f) {
+#pragma unroll
+                        for (int y = 0; y < 32; ++y) o[y] = 0.0f;
+                    } else if (other) {
+#pragma unroll
+                        for (int y = 0; y < 32; ++y) o[y] = fmaf(o[y], g0, s_o[quad][lane][y] * g1);
+                    } else {
+#pragma unroll
+                        for (int y = 0; y < 32; ++y) o[y] *= g0;
+                    }
+#pragma unroll
+                    for (int y = 0; y < 32; y += 2) {
+                        nan0 = fmaf(o[y], 0.0f, nan0);
+                        nan1 = fmaf(o[y + 1], 0.0f, nan1);
                     }
                     if (valid) {
-                        if (sp.chunks == 1) {
-                            T* out = (T*)p.out + row * p.D + x;
 #pragma unroll
-                            for (int y = 0; y < 32; y += 8)
-                                if (x + y < p.D) store8<T>(out + y, *reinterpret_cast<const float(*)[8]>(o + y));
-                        } else {
-                            float* out = sp.part + (row * sp.chunks + it.chunk) * p.D + x;
+                        for (int y = 0; y < 32; y += 8)
+                            if (x + y < p.D) {
+                                float v[8];
 #pragma unroll
-                            for (int y = 0; y < 32; y += 8)
-                                if (x + y < p.D) store8<float>(out + y, *reinterpret_cast<const float(*)[8]>(o + y));
-                        }
+                                for (int z = 0; z < 8; ++z) v[z] = o[y + z];
+                                if (it.part < 0) store8<T>((T*)p.out + row * p.D + x + y, v);
+                                else store8<float>(sp.part + part * p.D + x + y, v);
+                            }
                     }
                 }
                 if (other) pair_barrier(1 + quad);
             }
             if (tile == 0) {
                 if (valid) {
-                    if (sp.chunks == 1) p.lse[row] = lse;
-                    else sp.part_lse[row * sp.chunks + it.chunk] = lse;
+                    if (it.part < 0) p.lse[row] = lse;
+                    else sp.part_lse[part] = lse;
                 }
                 __syncwarp();
                 // rows that something non-finite reached: once more, from the keys they see alone
-                unsigned bad = sp.chunks == 1 ? __ballot_sync(0xffffffffu, valid && !fine) : 0u;
+                const float nan = nan0 + nan1;
+                unsigned bad = it.part < 0 ? __ballot_sync(0xffffffffu, valid && nan != nan) : 0u;
                 while (bad) {
                     const int r = __ffs(bad) - 1;
                     bad &= bad - 1;
@@ -408,7 +525,7 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
     if (warp == 12) tmem_free(tmem, 512);
 }
 
-// Joins the chunks of a row: out = sum_c 2^(lse_c - lse) part_c.  One warp a row.
+// Joins the parts of a row: out = sum_c 2^(lse_c - lse) part_c; rows that see no key get their zeros.  One warp a row.
 constexpr int kCombineWarps = 4;
 template <typename T>
 __global__ void __launch_bounds__(kCombineWarps * 32) tree_combine_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeSplit sp) {
@@ -416,13 +533,20 @@ __global__ void __launch_bounds__(kCombineWarps * 32) tree_combine_kernel(const 
     const long long row = (long long)blockIdx.x * kCombineWarps + threadIdx.x / 32;
     if (row >= (long long)p.B * p.Hq * p.T) return;
     const int lane = threadIdx.x & 31, t = (int)(row % p.T), h = (int)(row / p.T % p.Hq), b = (int)(row / p.T / p.Hq);
-    const int n = cached_keys(p, b), real = drafted_tokens(p, b);
-    const int used = t < real ? (n + real + sp.chunk - 1) / sp.chunk : 0;
-    const float* lses = sp.part_lse + row * sp.chunks;
+    // the blocks whose shares the row's unit lies in
+    const int gr = t * p.group + h % p.group, nt = tree_tiles(p, b);
+    const long long share = sp.start[p.B + 1];
+    const long long from = sp.start[b] * p.Hkv * sp.row_tiles + (long long)(h / p.group * sp.row_tiles + gr / kTreeRows) * nt;
+    const int c0 = (int)(from / share), c1 = nt > 0 ? (int)((from + nt - 1) / share) : c0 - 1;
+    if (c0 == c1) return;                                // written by the block itself
+    const int used = c1 - c0 + 1;                        // 0: a query that sees no key
+    auto place = [&](int c) {                            // a block's first part, or its second
+        return ((long long)(c0 + c) * 2 + ((c0 + c) * share >= from ? 0 : 1)) * sp.part_rows + gr % kTreeRows;
+    };
     float m = kNegInf;
     bool nan = false;
     for (int c = lane; c < used; c += 32) {
-        const float x = lses[c];
+        const float x = sp.part_lse[place(c)];
         nan = nan || x != x;
         m = fmaxf(m, x);
     }
@@ -431,14 +555,15 @@ __global__ void __launch_bounds__(kCombineWarps * 32) tree_combine_kernel(const 
     nan = __any_sync(0xffffffffu, nan);
     const float m0 = m == kNegInf ? 0.0f : m;
     float sum = 0.0f, acc[2][4] = {};
-    const float* part = sp.part + row * sp.chunks * p.D + lane * 4;
+    const float* part = sp.part + lane * 4;
     for (int c = 0; c < used; ++c) {
-        const float f = exp2f(lses[c] - m0);
+        const long long at = place(c);
+        const float f = exp2f(sp.part_lse[at] - m0);
         sum += f;
 #pragma unroll
         for (int k = 0; k < 2; ++k)
             if (k * 128 + lane * 4 < p.D) {
-                const float4 v = *reinterpret_cast<const float4*>(part + (long long)c * p.D + k * 128);
+                const float4 v = *reinterpret_cast<const float4*>(part + at * p.D + k * 128);
                 acc[k][0] = fmaf(f, v.x, acc[k][0]);
                 acc[k][1] = fmaf(f, v.y, acc[k][1]);
                 acc[k][2] = fmaf(f, v.z, acc[k][2]);
