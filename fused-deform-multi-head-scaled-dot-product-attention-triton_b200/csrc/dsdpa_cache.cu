@@ -107,7 +107,9 @@ cudaError_t tree_forward(const dsdpa_cache_problem& problem, const CacheParams& 
     return cudaGetLastError();
 }
 template <typename T>
-cudaError_t weights_add(const CacheParams& p, cudaStream_t s) {
+cudaError_t weights_add(const dsdpa_cache_problem& problem, const CacheParams& p, cudaStream_t s) {
+    if constexpr (DtypeOf<T>::value != DSDPA_F32)
+        if (on_tensor_cores(problem)) return launch_weights_tc<T>(p, s);
     const long long rows = (long long)p.B * p.Hkv * p.width * p.page_size;
     weights_rows_kernel<T><<<(unsigned)((rows + kRowWarps - 1) / kRowWarps), kRowWarps * 32, 0, s>>>(p);
     count_launches(1);
@@ -172,9 +174,9 @@ int dsdpa_cache_weights(const dsdpa_cache_problem* p, const dsdpa_cache_tree* tr
     c.take = take;
     c.weights = weights;
     switch (p->dtype) {
-        case DSDPA_F32: e = weights_add<float>(c, (cudaStream_t)stream); break;
-        case DSDPA_BF16: e = weights_add<__nv_bfloat16>(c, (cudaStream_t)stream); break;
-        default: e = weights_add<__half>(c, (cudaStream_t)stream); break;
+        case DSDPA_F32: e = weights_add<float>(*p, c, (cudaStream_t)stream); break;
+        case DSDPA_BF16: e = weights_add<__nv_bfloat16>(*p, c, (cudaStream_t)stream); break;
+        default: e = weights_add<__half>(*p, c, (cudaStream_t)stream); break;
     }
     return e == cudaSuccess ? DSDPA_OK : report_cuda_failure(e);
 }

@@ -34,5 +34,6 @@ inline TreePlan plan_tree(const dsdpa_cache_problem& p) {
 }
 
 template <typename T> cudaError_t launch_tree_tc(const CacheParams& p, const TreePlan& t, void* workspace, cudaStream_t s);
+template <typename T> cudaError_t launch_weights_tc(const CacheParams& p, cudaStream_t s);
 
 }  // namespace dsdpa

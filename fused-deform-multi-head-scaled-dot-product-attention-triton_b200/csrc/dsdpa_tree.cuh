@@ -29,7 +29,7 @@ struct TreeSplit {
     int whole;            // units are not cut: no parts, no tree_combine_kernel
     int row_tiles;
     int part_rows;        // rows of a part
-    long long* start;     // [B + 1]: key tiles of a head's query tile in the sequences before, and [B + 1]: a block's share
+    long long* start;     // null, or [B + 1]: key tiles of a head's query tile in the sequences before, and [B + 1]: a block's share
     float* part;          // [blocks * 2][part_rows][D], normalised
     float* part_lse;      // [blocks * 2][part_rows]
 };
@@ -96,6 +96,59 @@ struct TreeWalk {
     }
 };
 
+// Where this block's share of the line begins, by all of its threads; the caller waits for them before it looks.
+struct TreeShare {
+    long long sum[kTreeThreads / 32], left;
+    int b, unit, tile;
+};
+__device__ __forceinline__ void find_share(const CacheParams& p, const TreeSplit& sp, TreeShare& out) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (sp.whole) {
+        if (tid == 0) { out.left = blockIdx.x; out.b = out.unit = out.tile = 0; }
+    } else {
+        // where this block's share begins: a thread has the key tiles of a few sequences
+        const int per = (p.B + kTreeThreads - 1) / kTreeThreads, b0 = min(p.B, tid * per), b1 = min(p.B, b0 + per);
+        long long mine = 0;
+        for (int b = b0; b < b1; ++b) mine += tree_tiles(p, b);
+        long long upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long t = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += t;
+        }
+        if (lane == 31) out.sum[warp] = upto;
+        if (tid == 0) { out.left = 0; out.b = out.unit = out.tile = 0; }
+        __syncthreads();
+        long long before = upto - mine, total = 0;
+        for (int w = 0; w < kTreeThreads / 32; ++w) {
+            if (w < warp) before += out.sum[w];
+            total += out.sum[w];
+        }
+        const int units = p.Hkv * sp.row_tiles;
+        const long long line = total * units, share = max((long long)kTreeMinShare, (line + gridDim.x - 1) / gridDim.x);
+        const long long from = share * blockIdx.x;
+        if (blockIdx.x == 0 && sp.start) {
+            long long at = before;
+            for (int b = b0; b < b1; ++b) { sp.start[b] = at; at += tree_tiles(p, b); }
+            if (tid == 0) { sp.start[p.B] = total; sp.start[p.B + 1] = share; }
+        }
+        if (from < line && from >= before * units && from < (before + mine) * units) {
+            long long at = before * units;
+            int b = b0;
+            for (;; ++b) {
+                const long long span = (long long)tree_tiles(p, b) * units;
+                if (from < at + span) break;
+                at += span;
+            }
+            const int nt = tree_tiles(p, b);
+            out.b = b;
+            out.unit = (int)((from - at) / nt);
+            out.tile = (int)((from - at) % nt);
+            out.left = min(share, line - from);
+        }
+    }
+}
+
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, unsigned bytes) {   // the rest of 16 is zero
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(dst), "l"(src), "r"(bytes) : "memory");
 }
@@ -130,8 +183,7 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
     __shared__ float s_at[BIAS ? kInfo : 1][kTreeKeys];    // their positions
     __shared__ float s_o[4][32][33];                       // the second stream's accumulator, 32 columns at a time
     __shared__ float s_m[kTreeRows], s_l[kTreeRows];
-    __shared__ long long s_sum[kTreeThreads / 32], s_left;
-    __shared__ int s_b, s_unit, s_tile;
+    __shared__ TreeShare share;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -146,56 +198,13 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
         fence_mbar_init();
     }
     if (warp == 12) tmem_alloc(slot, 512);
-    if (sp.whole) {
-        if (tid == 0) { s_left = blockIdx.x; s_b = s_unit = s_tile = 0; }
-    } else {
-        // where this block's share begins: a thread has the key tiles of a few sequences
-        const int per = (p.B + kTreeThreads - 1) / kTreeThreads, b0 = min(p.B, tid * per), b1 = min(p.B, b0 + per);
-        long long mine = 0;
-        for (int b = b0; b < b1; ++b) mine += tree_tiles(p, b);
-        long long upto = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long t = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += t;
-        }
-        if (lane == 31) s_sum[warp] = upto;
-        if (tid == 0) { s_left = 0; s_b = s_unit = s_tile = 0; }
-        __syncthreads();
-        long long before = upto - mine, total = 0;
-        for (int w = 0; w < kTreeThreads / 32; ++w) {
-            if (w < warp) before += s_sum[w];
-            total += s_sum[w];
-        }
-        const int units = p.Hkv * sp.row_tiles;
-        const long long line = total * units, share = max((long long)kTreeMinShare, (line + gridDim.x - 1) / gridDim.x);
-        const long long from = share * blockIdx.x;
-        if (blockIdx.x == 0) {
-            long long at = before;
-            for (int b = b0; b < b1; ++b) { sp.start[b] = at; at += tree_tiles(p, b); }
-            if (tid == 0) { sp.start[p.B] = total; sp.start[p.B + 1] = share; }
-        }
-        if (from < line && from >= before * units && from < (before + mine) * units) {
-            long long at = before * units;
-            int b = b0;
-            for (;; ++b) {
-                const long long span = (long long)tree_tiles(p, b) * units;
-                if (from < at + span) break;
-                at += span;
-            }
-            const int nt = tree_tiles(p, b);
-            s_b = b;
-            s_unit = (int)((from - at) / nt);
-            s_tile = (int)((from - at) % nt);
-            s_left = min(share, line - from);
-        }
-    }
+    find_share(p, sp, share);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     uint32_t tmem;
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(slot));
-    TreeWalk walk{ s_b, s_unit, s_tile, s_left, true };
+    TreeWalk walk{ share.b, share.unit, share.tile, share.left, true };
 
     // Ring entries of an item with n tiles, in the order in which the products take them:
     // K0 K1 V0 K2 V1 .. K(n-1) V(n-2) V(n-1); the query tile comes with K0.
