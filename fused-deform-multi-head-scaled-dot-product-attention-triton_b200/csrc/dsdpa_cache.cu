@@ -215,11 +215,28 @@ int dsdpa_cache_evict(const dsdpa_cache_problem* p, void* k_pages, void* v_pages
     for (int i = 0; i < 3; ++i) { v.sk[i] = p->stride_k[i] * es; v.sv[i] = p->stride_v[i] * es; }
     v.err = err;
     cudaStream_t s = (cudaStream_t)stream;
-    evict_select_kernel<<<(unsigned)(p->B * p->Hkv), kSelectThreads, 0, s>>>(v);
+    set_division(v);
+    // up to 32768 ranks (128 KB) beside the histograms
+    const int room = p->table_width * p->page_size;
+    v.held = room < 32768 ? room : 32768;
+    if ((e = cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 32768 * 4)) != cudaSuccess)
+        return report_cuda_failure(e);
+    evict_select_kernel<<<(unsigned)(p->B * p->Hkv), kSelectThreads, (size_t)v.held * 4, s>>>(v);
     if ((e = cudaGetLastError()) != cudaSuccess) return report_cuda_failure(e);
-    const unsigned slices = (unsigned)((v.row_bytes + 63) / 64);
-    evict_move_kernel<<<(unsigned)(p->B * p->Hkv) * 2 * slices, kMoveThreads, 0, s>>>(v);
-    if ((e = cudaGetLastError()) != cudaSuccess) return report_cuda_failure(e);
+    // whole rows where that gives every SM its blocks, narrower pieces (64 bytes at least, two sectors) where not
+    int width = 1, slices = 1;
+    while (width * 16 < v.row_bytes) width *= 2;
+    while (width > 4 && (long long)p->B * p->Hkv * 2 * slices < kSMs * kMoveBlocks) width /= 2, slices = (v.row_bytes + width * 16 - 1) / (width * 16);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(p->B * p->Hkv * 2 * slices));
+    cfg.blockDim = dim3(kMoveThreads);
+    cfg.stream = s;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if ((e = cudaLaunchKernelEx(&cfg, evict_move_kernel, v, width, slices)) != cudaSuccess) return report_cuda_failure(e);
     count_launches(2);
     return DSDPA_OK;
 }
