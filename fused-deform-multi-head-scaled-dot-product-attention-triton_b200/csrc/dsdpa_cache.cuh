@@ -46,6 +46,12 @@ __device__ __forceinline__ int page_of(const int* table, int width, int pages, i
     return page;
 }
 
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, unsigned bytes) {   // the rest of 16 is zero
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" :: "n"(N) : "memory"); }
+
 // The tokens that token t sees (bit u: token u), itself among them, from its chain of parents; its
 // depth is their number less one.  Every step goes to an earlier token, so the walk ends.
 __device__ __forceinline__ unsigned long long tokens_above(const CacheParams& p, int b, int t) {

@@ -145,17 +145,31 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __gr
         int more0 = __reduce_add_sync(0xffffffffu, lane < warp ? s_more[lane] : 0);
         int same0 = __reduce_add_sync(0xffffffffu, lane < warp ? s_same[lane] : 0);
         const unsigned below = (1u << lane) - 1;
-#pragma unroll 4
-        for (int i0 = lo; i0 < hi; i0 += 32) {
-            const int i = i0 + lane;
-            const unsigned u = i < hi ? rank(i) : 0u;
-            const unsigned bm = __ballot_sync(0xffffffffu, i < hi && u > prefix);
-            const unsigned bs = __ballot_sync(0xffffffffu, i < hi && u == prefix);
-            const int my_more = more0 + __popc(bm & below), my_same = same0 + __popc(bs & below);
-            const bool is_more = bm >> lane & 1, is_same = bs >> lane & 1;
-            if (is_more || (is_same && my_same < (int)need)) put(p.sinks + my_more + min(my_same, (int)need), first + i);
-            more0 += __popc(bm);
-            same0 += __popc(bs);
+        constexpr int kBatch = 8;                         // places first, then the loads that they need, then the stores
+        for (int i0 = lo; i0 < hi; i0 += 32 * kBatch) {
+            int to[kBatch];
+            float val[kBatch];
+#pragma unroll
+            for (int e = 0; e < kBatch; ++e) {
+                const int i = i0 + e * 32 + lane;
+                const unsigned u = i < hi ? rank(i) : 0u;
+                const unsigned bm = __ballot_sync(0xffffffffu, i < hi && u > prefix);
+                const unsigned bs = __ballot_sync(0xffffffffu, i < hi && u == prefix);
+                const int my_more = more0 + __popc(bm & below), my_same = same0 + __popc(bs & below);
+                const bool stays = (bm >> lane & 1) || ((bs >> lane & 1) && my_same < (int)need);
+                to[e] = stays ? p.sinks + my_more + min(my_same, (int)need) : -1;
+                val[e] = stays ? __ldg(w + first + i) : 0.0f;
+                more0 += __popc(bm);
+                same0 += __popc(bs);
+            }
+#pragma unroll
+            for (int e = 0; e < kBatch; ++e)
+                if (to[e] >= 0) {
+                    const int i = first + i0 + e * 32 + lane;
+                    kept[to[e]] = i;
+                    nw[to[e]] = val[e];
+                    if (np) np[to[e]] = pos ? __ldg(pos + i) : i;
+                }
         }
     }
     for (int i = left + tid; i < p.keep; i += kSelectThreads) kept[i] = -1;

@@ -149,11 +149,6 @@ __device__ __forceinline__ void find_share(const CacheParams& p, const TreeSplit
     }
 }
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, unsigned bytes) {   // the rest of 16 is zero
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" :: "n"(N) : "memory"); }
 __device__ __forceinline__ void pair_barrier(int id) { asm volatile("bar.sync %0, 64;" :: "r"(id) : "memory"); }
 
 // The 32 rows whose addresses the warp's lanes hold (null: zeros) into rows 32w .. 32w+31 of a tile, swizzled.
