@@ -31,32 +31,6 @@ cudaError_t tensor_map_16(CUtensorMap* map, int dtype, const void* base, int D, 
 
 namespace {
 
-constexpr int kRowWarps = 8;   // rows of a block of the row kernels, one warp each
-
-template <typename T>
-__global__ void __launch_bounds__(kRowWarps * 32) masked_rows_forward(const MaskedParams p) {
-    const long long n = (long long)p.B * p.Hq * p.Lq;
-    for (long long r = (long long)blockIdx.x * kRowWarps + threadIdx.x / 32; r < n; r += (long long)gridDim.x * kRowWarps)
-        exact_row_forward<T>(p, (int)(r / p.Lq / p.Hq), (int)(r / p.Lq % p.Hq), (int)(r % p.Lq));
-}
-template <typename T>
-__global__ void __launch_bounds__(kRowWarps * 32) masked_rows_dq(const MaskedParams p) {
-    const long long n = (long long)p.B * p.Hq * p.Lq;
-    for (long long r = (long long)blockIdx.x * kRowWarps + threadIdx.x / 32; r < n; r += (long long)gridDim.x * kRowWarps)
-        exact_row_dq<T>(p, (int)(r / p.Lq / p.Hq), (int)(r / p.Lq % p.Hq), (int)(r % p.Lq));
-}
-template <typename T>
-__global__ void __launch_bounds__(kRowWarps * 32) masked_rows_dkdv(const MaskedParams p) {
-    const long long n = (long long)p.B * p.Hkv * p.Lk;
-    for (long long r = (long long)blockIdx.x * kRowWarps + threadIdx.x / 32; r < n; r += (long long)gridDim.x * kRowWarps)
-        exact_row_dkdv<T>(p, (int)(r / p.Lk / p.Hkv), (int)(r / p.Lk % p.Hkv), (int)(r % p.Lk));
-}
-
-unsigned row_blocks(long long rows) {
-    const long long b = (rows + kRowWarps - 1) / kRowWarps;
-    return (unsigned)(b < (1ll << 30) ? b : (1ll << 30));
-}
-
 int check(const dsdpa_masked_problem* p) {
     if (!p) return DSDPA_ERR_NULL_POINTER;
     if (p->dtype != DSDPA_F32 && p->dtype != DSDPA_BF16 && p->dtype != DSDPA_F16) return DSDPA_ERR_BAD_DTYPE;
@@ -99,7 +73,7 @@ MaskedParams params(const dsdpa_masked_problem& p, const void* q, const void* k,
     return m;
 }
 
-// The tensor-core kernels take 16-bit storage with up to 128 elements a row; the row kernels the rest.
+// The tensor-core kernels take 16-bit storage with up to 128 elements a row; fp32 arithmetic the rest.
 template <typename T>
 bool on_tensor_cores(const MaskedParams& p) {
     return DtypeOf<T>::value != DSDPA_F32 && p.D <= 128 && p.Lq > 0 && p.Lk > 0;
@@ -108,28 +82,15 @@ bool on_tensor_cores(const MaskedParams& p) {
 template <typename T>
 cudaError_t forward(const MaskedParams& p, cudaStream_t s) {
     if constexpr (DtypeOf<T>::value != DSDPA_F32)
-        if (on_tensor_cores<T>(p)) {
-            count_launches(1);
-            return launch_masked_fwd_tc<T>(p, s);
-        }
-    masked_rows_forward<T><<<row_blocks((long long)p.B * p.Hq * p.Lq), kRowWarps * 32, 0, s>>>(p);
-    count_launches(1);
-    return cudaGetLastError();
+        if (on_tensor_cores<T>(p)) return launch_masked_fwd_tc<T>(p, s);
+    return launch_masked_fwd_simt<T>(p, s);
 }
 
 template <typename T>
 cudaError_t backward(const MaskedParams& p, void* workspace, cudaStream_t s) {
     if constexpr (DtypeOf<T>::value != DSDPA_F32)
         if (on_tensor_cores<T>(p)) return launch_masked_bwd_tc<T>(p, workspace, s);
-    if (p.Lq > 0) {
-        masked_rows_dq<T><<<row_blocks((long long)p.B * p.Hq * p.Lq), kRowWarps * 32, 0, s>>>(p);
-        count_launches(1);
-    }
-    if (p.Lk > 0) {
-        masked_rows_dkdv<T><<<row_blocks((long long)p.B * p.Hkv * p.Lk), kRowWarps * 32, 0, s>>>(p);
-        count_launches(1);
-    }
-    return cudaGetLastError();
+    return launch_masked_bwd_simt<T>(p, s);
 }
 
 size_t backward_bytes(const dsdpa_masked_problem& p) {

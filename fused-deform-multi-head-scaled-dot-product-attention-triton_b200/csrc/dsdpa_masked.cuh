@@ -70,6 +70,17 @@ template <typename T> __device__ __forceinline__ void store4(T* p, const float (
     *reinterpret_cast<uint2*>(p) = make_uint2(r.x, r.y);
 }
 template <> __device__ __forceinline__ void store4<float>(float* p, const float (&f)[4]) { stg128(p, pack16(f, (float*)nullptr)); }
+template <typename T> __device__ __forceinline__ void store2(T* p, float a, float b) {
+    const float g[8] = { a, b, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f };
+    *reinterpret_cast<uint32_t*>(p) = pack16(g, (T*)nullptr).x;
+}
+template <> __device__ __forceinline__ void store2<float>(float* p, float a, float b) { *reinterpret_cast<float2*>(p) = make_float2(a, b); }
+// Two packed 16-bit elements as fp32.
+template <typename T> __device__ __forceinline__ float2 to_float2(uint32_t u) {
+    float f[8];
+    unpack16(make_uint4(u, 0, 0, 0), f, (T*)nullptr);
+    return make_float2(f[0], f[1]);
+}
 __device__ __forceinline__ float dot8(const float (&a)[8], const float (&b)[8]) {
     float s = 0.0f;
 #pragma unroll

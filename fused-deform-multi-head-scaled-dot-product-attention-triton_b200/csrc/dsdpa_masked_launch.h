@@ -1,4 +1,4 @@
-// Host side of the tensor-core kernels of masked attention: tensor maps and launches.
+// Host side of masked attention's kernels: tensor maps and launches.
 #pragma once
 
 #include <cuda.h>
@@ -15,6 +15,10 @@ cudaError_t tensor_map_16(CUtensorMap* map, int dtype, const void* base, int D, 
 template <typename T> cudaError_t launch_masked_fwd_tc(const MaskedParams& p, cudaStream_t s);
 // workspace: masked_bwd_space().bytes, p.delta pointing to its start; p.Lq > 0 and p.Lk > 0
 template <typename T> cudaError_t launch_masked_bwd_tc(const MaskedParams& p, void* workspace, cudaStream_t s);
+
+// fp32 arithmetic; p.Lq or p.Lk may be 0, p.delta is the backward's workspace
+template <typename T> cudaError_t launch_masked_fwd_simt(const MaskedParams& p, cudaStream_t s);
+template <typename T> cudaError_t launch_masked_bwd_simt(const MaskedParams& p, cudaStream_t s);
 
 // Byte offsets in the backward's workspace: delta at 0, then what the tensor-core kernels pass on.
 struct MaskedBwdSpace {
