@@ -8,50 +8,6 @@
 namespace dsdpa {
 namespace {
 
-constexpr int kRowWarps = 8;
-
-template <typename T>
-__global__ void __launch_bounds__(kRowWarps * 32) tree_rows_kernel(const CacheParams p) {
-    const long long r = (long long)blockIdx.x * kRowWarps + threadIdx.x / 32;
-    if (r < (long long)p.B * p.Hq * p.T) exact_row_tree<T>(p, (int)(r / p.T / p.Hq), (int)(r / p.T % p.Hq), (int)(r % p.T));
-}
-
-// One warp sums one key's weights over the tokens and heads.
-template <typename T>
-__global__ void __launch_bounds__(kRowWarps * 32) weights_rows_kernel(const CacheParams p) {
-    const int lane = threadIdx.x & 31;
-    const long long per = (long long)p.width * p.page_size;
-    const long long r = (long long)blockIdx.x * kRowWarps + threadIdx.x / 32;
-    if (r >= (long long)p.B * p.Hkv * per) return;
-    const int j = (int)(r % per), hk = (int)(r / per % p.Hkv), b = (int)(r / per / p.Hkv);
-    const int n = cached_keys(p, b), real = drafted_tokens(p, b);
-    if (j >= n + real) return;
-    const int index = j / p.page_size, page = page_of(p.table, p.width, p.pages, p.err, b, index);
-    if (page < 0) return;
-    float k[8], sum = 0.0f;
-    load_row<T>(row_of<T>(p.k, p.sk, 0, hk, j - index * p.page_size) + page * p.sk[0], p.D, lane, k);
-    const int base = first_position(p, b, n);
-    int at = j;
-    if (j >= n) at = base + depth_of(tokens_above(p, b, j - n));
-    else if (p.positions) at = __ldg(p.positions + ((long long)b * p.Hkv + hk) * p.slots + j);
-    for (int t = 0; t < real; ++t) {
-        if (p.take && !p.take[(long long)b * p.T + t]) continue;
-        const unsigned long long above = tokens_above(p, b, t);
-        if (j >= n && !(above >> (j - n) & 1)) continue;
-        const int pos = base + depth_of(above);
-        for (int g = 0; g < p.group; ++g) {
-            const int h = hk * p.group + g;
-            float q[8];
-            load_row<T>(row_of<T>(p.q, p.sq, b, h, t), p.D, lane, q);
-            float s = soft_cap(p.sm_scale * warp_sum(dot8(q, k)), p.cap);
-            if (p.slopes) s -= __ldg(p.slopes + h) * fabsf((float)(pos - at));
-            const float lse = p.lse[((long long)b * p.Hq + h) * p.T + t];
-            if (lse != kNegInf) sum += exp2f(s * kLog2e - lse);
-        }
-    }
-    if (lane == 0) p.weights[((long long)b * p.Hkv + hk) * p.slots + j] += sum;
-}
-
 int check(const dsdpa_cache_problem* p) {
     if (!p) return DSDPA_ERR_NULL_POINTER;
     if (p->dtype != DSDPA_F32 && p->dtype != DSDPA_BF16 && p->dtype != DSDPA_F16) return DSDPA_ERR_BAD_DTYPE;
@@ -64,9 +20,6 @@ int check(const dsdpa_cache_problem* p) {
         if (p->stride_k[i] < 0 || p->stride_v[i] < 0 || p->stride_k[i] * e % 16 || p->stride_v[i] * e % 16) return DSDPA_ERR_MISALIGNED;
     return DSDPA_OK;
 }
-// The tensor-core kernels take 16-bit storage with up to 128 elements a row; the row kernels the rest.
-bool on_tensor_cores(const dsdpa_cache_problem& p) { return p.dtype != DSDPA_F32 && p.D <= 128; }
-
 int check_tokens(const dsdpa_cache_problem* p) {
     const int st = check(p);
     if (st != DSDPA_OK) return st;
@@ -99,21 +52,17 @@ CacheParams params(const dsdpa_cache_problem& p, const dsdpa_cache_tree* t, cons
 
 template <typename T>
 cudaError_t tree_forward(const dsdpa_cache_problem& problem, const CacheParams& p, void* workspace, cudaStream_t s) {
+    const TreePlan t = plan_tree(problem);
     if constexpr (DtypeOf<T>::value != DSDPA_F32)
-        if (on_tensor_cores(problem)) return launch_tree_tc<T>(p, plan_tree(problem), workspace, s);
-    const long long rows = (long long)p.B * p.Hq * p.T;
-    tree_rows_kernel<T><<<(unsigned)((rows + kRowWarps - 1) / kRowWarps), kRowWarps * 32, 0, s>>>(p);
-    count_launches(1);
-    return cudaGetLastError();
+        if (cache_on_tensor_cores(problem)) return launch_tree_tc<T>(p, t, workspace, s);
+    return launch_tree_simt<T>(p, t, workspace, s);
 }
 template <typename T>
 cudaError_t weights_add(const dsdpa_cache_problem& problem, const CacheParams& p, cudaStream_t s) {
+    const TreePlan t = plan_tree(problem);
     if constexpr (DtypeOf<T>::value != DSDPA_F32)
-        if (on_tensor_cores(problem)) return launch_weights_tc<T>(p, s);
-    const long long rows = (long long)p.B * p.Hkv * p.width * p.page_size;
-    weights_rows_kernel<T><<<(unsigned)((rows + kRowWarps - 1) / kRowWarps), kRowWarps * 32, 0, s>>>(p);
-    count_launches(1);
-    return cudaGetLastError();
+        if (cache_on_tensor_cores(problem)) return launch_weights_tc<T>(p, t, s);
+    return launch_weights_simt<T>(p, t, s);
 }
 
 }  // namespace
@@ -124,7 +73,7 @@ using namespace dsdpa;
 extern "C" {
 
 size_t dsdpa_tree_workspace_bytes(const dsdpa_cache_problem* p) {
-    return check_tokens(p) == DSDPA_OK && on_tensor_cores(*p) ? plan_tree(*p).bytes : 0;
+    return check_tokens(p) == DSDPA_OK ? plan_tree(*p).bytes : 0;
 }
 
 int dsdpa_tree_forward(const dsdpa_cache_problem* p, const dsdpa_cache_tree* tree, const void* q, const void* k_pages,

@@ -11,9 +11,9 @@
 namespace dsdpa {
 
 constexpr int kSimtThreads = 256, kSimtKeys = 64;
-template <int HD> struct SimtShape {
-    static constexpr int BM = HD == 256 ? 32 : 64;     // queries of a tile
-    static constexpr int RM = BM / 16;
+template <int HD, int ROWS = HD == 256 ? 2 : 4> struct SimtShape {
+    static constexpr int RM = ROWS;                    // rows of a thread
+    static constexpr int BM = 16 * RM;                 // queries of a tile
     static constexpr int S = HD + 4;                   // floats of a row: rows start 16 bytes further in the banks
     static constexpr int W = kSimtKeys + 4;            // floats of a row of weights
     static constexpr int NJ = HD >= 64 ? HD / 64 : 1;  // pieces of a row of sums that a thread has
@@ -52,9 +52,9 @@ __device__ __forceinline__ void simt_load(float* dst, const T* base, long long s
 __device__ __forceinline__ void simt_wait() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
 
 // s[r][c] = row (ty RM + r) of a . row (tx + 16 c) of b
-template <int HD>
-__device__ __forceinline__ void simt_dot(const float* a, const float* b, float (&s)[SimtShape<HD>::RM][4]) {
-    using L = SimtShape<HD>;
+template <int HD, int RM>
+__device__ __forceinline__ void simt_dot(const float* a, const float* b, float (&s)[RM][4]) {
+    using L = SimtShape<HD, RM>;
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
     float2 acc[L::RM][4] = {};
     const float* pa = a + ty * L::RM * L::S;
@@ -95,9 +95,9 @@ __device__ __forceinline__ void simt_piece(const float* row, int j, float2 (&v)[
 }
 
 // acc[r] += sum_k w[ty RM + r][k] b[k]: w has rows of queries, b keys
-template <int HD>
-__device__ __forceinline__ void simt_rows(const float* w, const float* b, float2 (&acc)[SimtShape<HD>::RM][SimtShape<HD>::NJ][2]) {
-    using L = SimtShape<HD>;
+template <int HD, int RM>
+__device__ __forceinline__ void simt_rows(const float* w, const float* b, float2 (&acc)[RM][SimtShape<HD>::NJ][2]) {
+    using L = SimtShape<HD, RM>;
     const int ty = threadIdx.x >> 4;
 #pragma unroll 2
     for (int k = 0; k < kSimtKeys; k += 4) {

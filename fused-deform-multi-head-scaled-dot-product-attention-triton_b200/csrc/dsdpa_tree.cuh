@@ -1,12 +1,8 @@
 // Attention of drafted tokens over a paged cache on the tensor cores: 16-bit storage, head dimensions up
 // to 128.
 //
-// The queries that share a key/value head -- tokens times the group's heads, up to 128 a tile: a unit -- are one
-// operand, so that the cache is read once for all of them.  The key tiles of all units lie one behind the
-// other, and every block takes an equal share of that line, whatever the lengths are (they are known on the
-// device only): whole units, and at the ends of its share parts of units, whose results
-// tree_combine_kernel joins.  So all blocks end together, and no more than two parts a block have to be
-// written and read again.  A block's loads run ahead of its arithmetic, from one unit into the next.
+// A unit's queries (up to 128 rows, dsdpa_share.cuh) are one operand, so that the cache is read once for all of them.
+// A block's loads run ahead of its arithmetic, from one unit into the next.
 // Inside a unit key tiles of 128 go in turn to two streams, each with its own running maximum, sum and
 // accumulator (tensor memory holds both), joined at the end: one stream's softmax runs while the other's
 // products do, which matters when a handful of rows leaves a single warp with all of the softmax.
@@ -15,24 +11,15 @@
 // that are not there read as zero), 12 issues the matrix instructions.
 #pragma once
 
-#include "dsdpa_cache.cuh"
 #include "dsdpa_masked_fwd.cuh"
+#include "dsdpa_share.cuh"
 
 namespace dsdpa {
 
 constexpr int kTreeThreads = 416;
 constexpr int kTreeRows = 128, kTreeKeys = 128, kInfo = 16;
+using TreeTile = ShareTile<kTreeRows, kTreeKeys>;
 
-constexpr int kTreeMinShare = 2;    // key tiles: one for each stream
-
-struct TreeSplit {
-    int whole;            // units are not cut: no parts, no tree_combine_kernel
-    int row_tiles;
-    int part_rows;        // rows of a part
-    long long* start;     // null, or [B + 1]: key tiles of a head's query tile in the sequences before, and [B + 1]: a block's share
-    float* part;          // [blocks * 2][part_rows][D], normalised
-    float* part_lse;      // [blocks * 2][part_rows]
-};
 template <int HD>
 struct TreeLayout {
     static constexpr int kTileBytes = 128 * HD * 2;
@@ -42,112 +29,6 @@ struct TreeLayout {
     static constexpr int kAhead = HD == 128 ? 2 : 5;
     static constexpr int kSmem = 2 * kTileBytes + kStages * kTileBytes + 1024 + 512;
 };
-
-// Key tiles of a sequence: the same for all of its heads.
-__device__ __forceinline__ int tree_tiles(const CacheParams& p, int b) {
-    const int real = drafted_tokens(p, b);
-    return real > 0 ? (cached_keys(p, b) + real + kTreeKeys - 1) / kTreeKeys : 0;
-}
-
-// A unit, or the part of one that lies in a block's share.
-struct TreeItem {
-    int b, hk, row0, rows, n, real, key0, tiles;
-    int part;             // where its result goes: -1 to out and lse, else the number of the part
-};
-// Goes through the items of a block; every role has its own.
-struct TreeWalk {
-    int b, unit, tile;    // unit: of the sequence's heads * row_tiles
-    long long left;       // key tiles of the share; whole units: number of the next unit
-    bool first;
-    __device__ __forceinline__ bool next(const CacheParams& p, const TreeSplit& s, TreeItem& it) {
-        const int units = p.Hkv * s.row_tiles;
-        if (s.whole) {
-            if (left >= (long long)p.B * units) return false;
-            b = (int)(left / units);
-            unit = (int)(left % units);
-            tile = 0;
-            it.tiles = tree_tiles(p, b);
-            it.part = -1;
-            left += gridDim.x;
-        } else {
-            int nt = 0;
-            while (left > 0) {
-                nt = tree_tiles(p, b);
-                if (unit < units && nt > 0) break;
-                ++b;
-                unit = 0;
-            }
-            if (left <= 0) return false;
-            it.tiles = (int)min((long long)(nt - tile), left);
-            it.part = it.tiles == nt ? -1 : (int)blockIdx.x * 2 + (first ? 0 : 1);
-            left -= it.tiles;
-        }
-        first = false;
-        it.b = b;
-        it.hk = unit / s.row_tiles;
-        it.row0 = unit % s.row_tiles * kTreeRows;
-        it.rows = min(kTreeRows, p.T * p.group - it.row0);
-        it.n = cached_keys(p, b);
-        it.real = drafted_tokens(p, b);
-        it.key0 = tile * kTreeKeys;
-        ++unit;
-        tile = 0;
-        return true;
-    }
-};
-
-// Where this block's share of the line begins, by all of its threads; the caller waits for them before it looks.
-struct TreeShare {
-    long long sum[kTreeThreads / 32], left;
-    int b, unit, tile;
-};
-__device__ __forceinline__ void find_share(const CacheParams& p, const TreeSplit& sp, TreeShare& out) {
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    if (sp.whole) {
-        if (tid == 0) { out.left = blockIdx.x; out.b = out.unit = out.tile = 0; }
-    } else {
-        // where this block's share begins: a thread has the key tiles of a few sequences
-        const int per = (p.B + kTreeThreads - 1) / kTreeThreads, b0 = min(p.B, tid * per), b1 = min(p.B, b0 + per);
-        long long mine = 0;
-        for (int b = b0; b < b1; ++b) mine += tree_tiles(p, b);
-        long long upto = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long t = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += t;
-        }
-        if (lane == 31) out.sum[warp] = upto;
-        if (tid == 0) { out.left = 0; out.b = out.unit = out.tile = 0; }
-        __syncthreads();
-        long long before = upto - mine, total = 0;
-        for (int w = 0; w < kTreeThreads / 32; ++w) {
-            if (w < warp) before += out.sum[w];
-            total += out.sum[w];
-        }
-        const int units = p.Hkv * sp.row_tiles;
-        const long long line = total * units, share = max((long long)kTreeMinShare, (line + gridDim.x - 1) / gridDim.x);
-        const long long from = share * blockIdx.x;
-        if (blockIdx.x == 0 && sp.start) {
-            long long at = before;
-            for (int b = b0; b < b1; ++b) { sp.start[b] = at; at += tree_tiles(p, b); }
-            if (tid == 0) { sp.start[p.B] = total; sp.start[p.B + 1] = share; }
-        }
-        if (from < line && from >= before * units && from < (before + mine) * units) {
-            long long at = before * units;
-            int b = b0;
-            for (;; ++b) {
-                const long long span = (long long)tree_tiles(p, b) * units;
-                if (from < at + span) break;
-                at += span;
-            }
-            const int nt = tree_tiles(p, b);
-            out.b = b;
-            out.unit = (int)((from - at) / nt);
-            out.tile = (int)((from - at) % nt);
-            out.left = min(share, line - from);
-        }
-    }
-}
 
 __device__ __forceinline__ void pair_barrier(int id) { asm volatile("bar.sync %0, 64;" :: "r"(id) : "memory"); }
 
@@ -178,7 +59,7 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
     __shared__ float s_at[BIAS ? kInfo : 1][kTreeKeys];    // their positions
     __shared__ float s_o[4][32][33];                       // the second stream's accumulator, 32 columns at a time
     __shared__ float s_m[kTreeRows], s_l[kTreeRows];
-    __shared__ TreeShare share;
+    __shared__ TreeShare<kTreeThreads> share;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -193,13 +74,13 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
         fence_mbar_init();
     }
     if (warp == 12) tmem_alloc(slot, 512);
-    find_share(p, sp, share);
+    find_share<TreeTile>(p, sp, share);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     uint32_t tmem;
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(slot));
-    TreeWalk walk{ share.b, share.unit, share.tile, share.left, true };
+    TreeWalk<TreeTile> walk{ share.b, share.unit, share.tile, share.left, true };
 
     // Ring entries of an item with n tiles, in the order in which the products take them:
     // K0 K1 V0 K2 V1 .. K(n-1) V(n-2) V(n-1); the query tile comes with K0.
@@ -527,70 +408,6 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
     tc_fence_before();
     __syncthreads();
     if (warp == 12) tmem_free(tmem, 512);
-}
-
-// Joins the parts of a row: out = sum_c 2^(lse_c - lse) part_c; rows that see no key get their zeros.  One warp a row.
-constexpr int kCombineWarps = 4;
-template <typename T>
-__global__ void __launch_bounds__(kCombineWarps * 32) tree_combine_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeSplit sp) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const long long row = (long long)blockIdx.x * kCombineWarps + threadIdx.x / 32;
-    if (row >= (long long)p.B * p.Hq * p.T) return;
-    const int lane = threadIdx.x & 31, t = (int)(row % p.T), h = (int)(row / p.T % p.Hq), b = (int)(row / p.T / p.Hq);
-    // the blocks whose shares the row's unit lies in
-    const int gr = t * p.group + h % p.group, nt = tree_tiles(p, b);
-    const long long share = sp.start[p.B + 1];
-    const long long from = sp.start[b] * p.Hkv * sp.row_tiles + (long long)(h / p.group * sp.row_tiles + gr / kTreeRows) * nt;
-    const int c0 = (int)(from / share), c1 = nt > 0 ? (int)((from + nt - 1) / share) : c0 - 1;
-    if (c0 == c1) return;                                // written by the block itself
-    const int used = c1 - c0 + 1;                        // 0: a query that sees no key
-    auto place = [&](int c) {                            // a block's first part, or its second
-        return ((long long)(c0 + c) * 2 + ((c0 + c) * share >= from ? 0 : 1)) * sp.part_rows + gr % kTreeRows;
-    };
-    float m = kNegInf;
-    bool nan = false;
-    for (int c = lane; c < used; c += 32) {
-        const float x = sp.part_lse[place(c)];
-        nan = nan || x != x;
-        m = fmaxf(m, x);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    nan = __any_sync(0xffffffffu, nan);
-    const float m0 = m == kNegInf ? 0.0f : m;
-    float sum = 0.0f, acc[2][4] = {};
-    const float* part = sp.part + lane * 4;
-    for (int c = 0; c < used; ++c) {
-        const long long at = place(c);
-        const float f = exp2f(sp.part_lse[at] - m0);
-        sum += f;
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-            if (k * 128 + lane * 4 < p.D) {
-                const float4 v = *reinterpret_cast<const float4*>(part + at * p.D + k * 128);
-                acc[k][0] = fmaf(f, v.x, acc[k][0]);
-                acc[k][1] = fmaf(f, v.y, acc[k][1]);
-                acc[k][2] = fmaf(f, v.z, acc[k][2]);
-                acc[k][3] = fmaf(f, v.w, acc[k][3]);
-            }
-    }
-    const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
-    bool fine = !nan;
-    T* out = (T*)p.out + row * p.D + lane * 4;
-#pragma unroll
-    for (int k = 0; k < 2; ++k)
-        if (k * 128 + lane * 4 < p.D) {
-            float v[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                v[e] = acc[k][e] * inv;
-                fine = fine && fabsf(v[e]) <= 3.0e38f;
-            }
-            store4(out + k * 128, v);
-        }
-    if (lane == 0) p.lse[row] = sum != 0.0f ? m0 + log2f(sum) : kNegInf;
-    __syncwarp();
-    if (__any_sync(0xffffffffu, !fine)) exact_row_tree<T>(p, b, h, t);
 }
 
 }  // namespace dsdpa

@@ -25,7 +25,7 @@ weights_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ Tr
     __shared__ unsigned s_valid[kInfo][4];
     __shared__ float s_lse[2][kTreeRows], s_pos[2][BIAS ? kTreeRows : 1], s_slope[2][BIAS ? kTreeRows : 1];
     __shared__ unsigned long long s_above[2][kTreeRows];
-    __shared__ TreeShare share;
+    __shared__ TreeShare<kTreeThreads> share;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rows = p.T * p.group, passes = (rows + kTreeRows - 1) / kTreeRows;
 
@@ -37,13 +37,13 @@ weights_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ Tr
         fence_mbar_init();
     }
     if (warp == 12) tmem_alloc(slot, 512);
-    find_share(p, sp, share);
+    find_share<TreeTile>(p, sp, share);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     uint32_t tmem;
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(slot));
-    TreeWalk walk{ share.b, share.unit, share.tile, share.left, true };
+    TreeWalk<TreeTile> walk{ share.b, share.unit, share.tile, share.left, true };
     // an item's passes over its rows; pass numbers run on over the items
     int pass = 0;
 
