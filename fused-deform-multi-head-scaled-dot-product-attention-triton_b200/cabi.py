@@ -173,7 +173,9 @@ def lib() -> ctypes.CDLL:
     L.dsdpa_build_is_checked.restype = ci
     L.dsdpa_describe_plan.argtypes = [pp, ctypes.c_char_p, ctypes.c_size_t]
     L.dsdpa_describe_plan.restype = ci
-    mp, cp, tp, sz = ctypes.POINTER(MaskedProblem), ctypes.POINTER(CacheProblem), ctypes.POINTER(CacheTree), ctypes.c_size_t
+    # the problem structs of these go as void pointers: byref of the mirrors above, or their bytes
+    mp = cp = tp = vp
+    sz = ctypes.c_size_t
     for name, restype, argtypes in (
             ("dsdpa_masked_forward", ci, [mp] + [vp] * 7 + [ci, vp]),
             ("dsdpa_masked_backward_workspace_bytes", sz, [mp]),

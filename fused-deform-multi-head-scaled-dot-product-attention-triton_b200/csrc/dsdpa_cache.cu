@@ -168,7 +168,8 @@ int dsdpa_cache_evict(const dsdpa_cache_problem* p, void* k_pages, void* v_pages
     // up to 32768 ranks (128 KB) beside the histograms
     const int room = p->table_width * p->page_size;
     v.held = room < 32768 ? room : 32768;
-    if ((e = cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 32768 * 4)) != cudaSuccess)
+    static SmemOnce once;
+    if ((e = allow_smem(evict_select_kernel, 32768 * 4, once)) != cudaSuccess)
         return report_cuda_failure(e);
     evict_select_kernel<<<(unsigned)(p->B * p->Hkv), kSelectThreads, (size_t)v.held * 4, s>>>(v);
     if ((e = cudaGetLastError()) != cudaSuccess) return report_cuda_failure(e);

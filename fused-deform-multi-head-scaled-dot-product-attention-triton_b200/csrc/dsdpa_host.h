@@ -3,6 +3,7 @@
 
 #include <cuda_runtime.h>
 #include <stdint.h>
+#include <atomic>
 
 #include "../../include/dsdpa.h"
 
@@ -29,5 +30,20 @@ struct DeviceGuard {
         if (prev >= 0 && cudaGetDevice(&cur) == cudaSuccess && cur != prev) (void)cudaSetDevice(prev);
     }
 };
+
+// Lets a kernel have `bytes` of dynamic shared memory, once per device; `done` is the calling instantiation's own.
+struct SmemOnce {
+    std::atomic<bool> done[64] = {};
+};
+template <typename K>
+inline cudaError_t allow_smem(K kern, int bytes, SmemOnce& once) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev >= 0 && dev < 64 && once.done[dev].load(std::memory_order_relaxed)) return cudaSuccess;
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && dev >= 0 && dev < 64) once.done[dev].store(true, std::memory_order_relaxed);
+    return e;
+}
 
 }  // namespace dsdpa

@@ -6,8 +6,8 @@ The device work is libdeform_sdpa.so's, through the C ABI of ``include/dsdpa.h``
 """
 from __future__ import annotations
 
-import ctypes
 import math
+import struct
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -15,21 +15,26 @@ from torch.autograd.function import once_differentiable
 from . import cabi, op
 
 
+_raw_stream = torch._C._cuda_getCurrentRawStream     # of a device index; torch.cuda.current_stream makes an object first
+_PROBLEM = struct.Struct("=6i2fiI25q")                # struct dsdpa_masked_problem, packed: a call spends its time in the host
+
+
 def _usable(t):
     """Rows contiguous and 16-byte aligned, no dimension broadcast: what the kernels read as it lies."""
+    if t.data_ptr() % 16:
+        return False
+    if t.is_contiguous():
+        return t.shape[-1] * t.element_size() % 16 == 0
     e = t.element_size()
-    return (t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and
-            all(st > 0 and st * e % 16 == 0 for st, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1) and
-            all(st * e % 16 == 0 and st >= 0 for st in t.stride()[:-1]))
+    return (t.stride(-1) == 1 and
+            all(n < 2 or (st > 0 and st * e % 16 == 0) for st, n in zip(t.stride()[:-1], t.shape[:-1])))
 
 
 def _as_rows(t):
-    t = t.detach()
-    if not _usable(t):
-        t = t.contiguous()
-        if t.data_ptr() % 16:
-            t = t.clone()
-    return t
+    if _usable(t):
+        return t
+    t = t.detach().contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
 
 
 def _check_inputs(q, k, v, sm_scale, softcap, visible, slopes, name):
@@ -76,72 +81,103 @@ def _check_slopes(slopes, heads, device, name):
         raise ValueError(f"{name}: slopes must be fp32 [{heads}] on {device}")
 
 
-def _mask_args(q, visible, slopes):
+def _mask_args(visible, slopes):
     """visible and slopes as the library takes them, and the batch stride of visible."""
-    stride = 0
-    if visible is not None:
-        if visible.dim() == 2:
-            visible = visible.unsqueeze(0)
-        if visible.shape[0] == 1 or visible.stride(0) == 0:
-            visible = visible[:1]
-        visible = visible.contiguous()
-        if visible.data_ptr() % 8:
-            visible = visible.clone()
-        stride = 0 if visible.shape[0] == 1 else visible.stride(0)
-    return visible, slopes.contiguous() if slopes is not None else None, stride
+    if slopes is not None:
+        slopes = slopes.contiguous()
+    if visible is None:
+        return None, slopes, 0
+    if visible.dim() == 2:
+        visible = visible.unsqueeze(0)
+    if visible.shape[0] == 1 or visible.stride(0) == 0:
+        visible = visible[:1]
+    visible = visible.contiguous()
+    if visible.data_ptr() % 8:
+        visible = visible.clone()
+    return visible, slopes, 0 if visible.shape[0] == 1 else visible.stride(0)
 
 
-def _problem(q, k, sm_scale, softcap, causal, stride_visible, /, **rows):
-    prob = cabi.MaskedProblem(q.shape[0], q.shape[1], k.shape[1], q.shape[2], k.shape[2], q.shape[3], float(sm_scale),
-                              float(softcap), op._DTYPES[q.dtype], cabi.MASKED_CAUSAL if causal else 0)
-    for name, t in rows.items():
-        setattr(prob, "stride_" + name, (ctypes.c_longlong * 3)(*t.stride()[:3]))
-    prob.stride_visible = stride_visible
-    return prob
+def _plain(q, k, v, visible, slopes):
+    """The usual arguments, seen at a glance; whatever else comes is looked at by _check_inputs."""
+    dev, dt = q.get_device(), q.dtype
+    if dev < 0 or k.get_device() != dev or v.get_device() != dev or k.dtype is not dt or v.dtype is not dt or dt not in op._DTYPES:
+        return False
+    qs, ks = q.shape, k.shape
+    if len(qs) != 4 or len(ks) != 4 or v.shape != ks or qs[0] != ks[0] or qs[3] != ks[3] or ks[1] == 0 or qs[1] % ks[1] or \
+            qs[3] % 8 or not 8 <= qs[3] <= 256:
+        return False
+    if visible is not None and (visible.dtype is not torch.int32 or visible.shape != (qs[0], qs[2], 2) or visible.get_device() != dev):
+        return False
+    return slopes is None or (slopes.dtype is torch.float32 and slopes.shape == (qs[1],) and slopes.get_device() == dev and
+                              not slopes.requires_grad)
+
+
+def _numbers(q, sm_scale, softcap):
+    sm_scale = q.shape[-1] ** -0.5 if sm_scale is None else float(sm_scale)
+    softcap = float(softcap)
+    if not (math.isfinite(sm_scale) and 0.0 <= softcap < math.inf):
+        _check_numbers(sm_scale, softcap, "masked_sdpa")
+    return sm_scale, softcap
 
 
 def masked_forward_raw(q, k, v, sm_scale=None, *, causal=False, visible=None, softcap=0.0, slopes=None):
     """Forward through the C ABI.  Returns ``(out, lse)``, lse fp32 [B, heads, Lq] in base 2; no autograd.
 
     Arguments as for ``masked_sdpa``."""
-    sm_scale = q.shape[-1] ** -0.5 if sm_scale is None else float(sm_scale)
-    _check_inputs(q, k, v, sm_scale, softcap, visible, slopes, "masked_sdpa")
+    sm_scale, softcap = _numbers(q, sm_scale, softcap)
+    if not _plain(q, k, v, visible, slopes):
+        _check_inputs(q, k, v, sm_scale, softcap, visible, slopes, "masked_sdpa")
     q, k, v = _as_rows(q), _as_rows(k), _as_rows(v)
+    B, Hq, Lq, D = q.shape
     out = torch.empty_like(q)
-    lse = torch.empty(q.shape[:3], device=q.device, dtype=torch.float32)
-    if lse.numel() == 0:
+    lse = torch.empty((B, Hq, Lq), device=q.device, dtype=torch.float32)
+    if not B * Hq * Lq:
         return out, lse
-    visible, slopes, stride = _mask_args(q, visible, slopes)
-    prob = _problem(q, k, sm_scale, softcap, causal, stride, q=q, k=k, v=v, out=out)
-    stream = torch.cuda.current_stream(q.device).cuda_stream
-    p = op._ptr
-    cabi.check(cabi.lib().dsdpa_masked_forward(ctypes.byref(prob), p(q), p(k), p(v), p(visible), p(slopes), p(out), p(lse),
-                                               q.device.index, ctypes.c_void_p(stream)))
+    visible, slopes, stride = _mask_args(visible, slopes)
+    qt, kt, vt, ot = q.stride(), k.stride(), v.stride(), out.stride()
+    prob = _PROBLEM.pack(B, Hq, k.shape[1], Lq, k.shape[2], D, sm_scale, softcap, op._DTYPES[q.dtype], cabi.MASKED_CAUSAL if causal else 0,
+                         qt[0], qt[1], qt[2], kt[0], kt[1], kt[2], vt[0], vt[1], vt[2], ot[0], ot[1], ot[2],
+                         0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, stride)
+    dev = q.get_device()
+    st = cabi.lib().dsdpa_masked_forward(prob, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                                         None if visible is None else visible.data_ptr(), None if slopes is None else slopes.data_ptr(),
+                                         out.data_ptr(), lse.data_ptr(), dev, _raw_stream(dev))
+    if st:
+        cabi.check(st)
     return out, lse
 
 
 def masked_backward_raw(q, k, v, out, lse, dout, sm_scale=None, *, causal=False, visible=None, softcap=0.0, slopes=None):
     """Backward through the C ABI.  Returns ``(dq, dk, dv)``; ``out`` and ``lse`` are the forward's."""
-    sm_scale = q.shape[-1] ** -0.5 if sm_scale is None else float(sm_scale)
-    _check_inputs(q, k, v, sm_scale, softcap, visible, slopes, "masked_sdpa")
+    sm_scale, softcap = _numbers(q, sm_scale, softcap)
+    if not _plain(q, k, v, visible, slopes):
+        _check_inputs(q, k, v, sm_scale, softcap, visible, slopes, "masked_sdpa")
+    dev = q.get_device()
     if out.shape != q.shape or dout.shape != q.shape or lse.shape != q.shape[:3]:
         raise ValueError("masked_sdpa: out, dout and lse must have the shapes of the forward's results")
-    if out.dtype != q.dtype or lse.dtype != torch.float32 or not (out.device == lse.device == dout.device == q.device):
+    if out.dtype != q.dtype or lse.dtype != torch.float32 or out.get_device() != dev or lse.get_device() != dev or dout.get_device() != dev:
         raise ValueError("masked_sdpa: out and lse must be the forward's results")
-    q, k, v, out, dout = _as_rows(q), _as_rows(k), _as_rows(v), _as_rows(out), _as_rows(dout.to(q.dtype))
-    lse = lse.contiguous()
+    if dout.dtype != q.dtype:
+        dout = dout.to(q.dtype)
+    q, k, v, out, dout, lse = _as_rows(q), _as_rows(k), _as_rows(v), _as_rows(out), _as_rows(dout), lse.contiguous()
     dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
-    if q.shape[0] == 0 or q.shape[1] == 0 or (q.shape[2] == 0 and k.shape[2] == 0):
+    B, Hq, Lq, D = q.shape
+    Hkv, Lk = k.shape[1], k.shape[2]
+    if not B * Hq or not (Lq or Lk):
         return dq, dk, dv
-    visible, slopes, stride = _mask_args(q, visible, slopes)
-    prob = _problem(q, k, sm_scale, softcap, causal, stride, q=q, k=k, v=v, out=out, dout=dout, dq=dq, dk=dk, dv=dv)
+    visible, slopes, stride = _mask_args(visible, slopes)
+    rows = []
+    for t in (q, k, v, out, dout, dq, dk, dv):
+        rows += t.stride()[:3]
+    prob = _PROBLEM.pack(B, Hq, Hkv, Lq, Lk, D, sm_scale, softcap, op._DTYPES[q.dtype], cabi.MASKED_CAUSAL if causal else 0, *rows, stride)
     L = cabi.lib()
-    n = int(L.dsdpa_masked_backward_workspace_bytes(ctypes.byref(prob)))
+    n = L.dsdpa_masked_backward_workspace_bytes(prob)
     ws = torch.empty(n, device=q.device, dtype=torch.uint8) if n else None
-    stream = torch.cuda.current_stream(q.device).cuda_stream
-    p = op._ptr
-    cabi.check(L.dsdpa_masked_backward(ctypes.byref(prob), p(q), p(k), p(v), p(visible), p(slopes), p(out), p(lse), p(dout),
-                                       p(dq), p(dk), p(dv), p(ws), n, q.device.index, ctypes.c_void_p(stream)))
+    st = L.dsdpa_masked_backward(prob, q.data_ptr(), k.data_ptr(), v.data_ptr(), None if visible is None else visible.data_ptr(),
+                                 None if slopes is None else slopes.data_ptr(), out.data_ptr(), lse.data_ptr(), dout.data_ptr(),
+                                 dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), None if ws is None else ws.data_ptr(), n, dev, _raw_stream(dev))
+    if st:
+        cabi.check(st)
     return dq, dk, dv
 
 

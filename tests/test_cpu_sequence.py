@@ -35,6 +35,20 @@ def test_structs_match_the_header(name, mirror, size):
     assert ctypes.sizeof(mirror) == size
 
 
+def test_packed_problems_are_the_structs():
+    """The front end packs the structs instead of filling their mirrors."""
+    n = [f[0] for f in cabi.MaskedProblem._fields_]
+    got = cabi.MaskedProblem.from_buffer_copy(be.masked._PROBLEM.pack(*range(1, 11), *range(100, 125)))
+    assert be.masked._PROBLEM.size == ctypes.sizeof(cabi.MaskedProblem)
+    assert [getattr(got, x) for x in n[:10]] == list(range(1, 11))
+    assert [v for x in n[10:18] for v in getattr(got, x)] + [got.stride_visible] == list(range(100, 125))
+    n = [f[0] for f in cabi.CacheProblem._fields_]
+    got = cabi.CacheProblem.from_buffer_copy(be.cache._PROBLEM.pack(*range(1, 14), *range(100, 109)))
+    assert be.cache._PROBLEM.size == ctypes.sizeof(cabi.CacheProblem)
+    assert [getattr(got, x) for x in n[:13]] == list(range(1, 14))
+    assert [v for x in n[13:] for v in getattr(got, x)] == list(range(100, 109))
+
+
 def masked_problem(**kw):
     base = dict(B=1, Hq=4, Hkv=2, Lq=10, Lk=12, D=64, sm_scale=0.125, softcap=0.0, dtype=cabi.BF16, flags=0)
     base.update(kw)
