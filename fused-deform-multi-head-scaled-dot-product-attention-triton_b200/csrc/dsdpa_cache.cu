@@ -8,6 +8,8 @@
 namespace dsdpa {
 namespace {
 
+bool bad_v(const dsdpa_cache_problem* p) { return bad_stride(p->stride_v, p->dtype, p->pages, p->Hkv, p->page_size); }
+
 int check(const dsdpa_cache_problem* p) {
     if (!p) return DSDPA_ERR_NULL_POINTER;
     if (p->dtype != DSDPA_F32 && p->dtype != DSDPA_BF16 && p->dtype != DSDPA_F16) return DSDPA_ERR_BAD_DTYPE;
@@ -15,10 +17,7 @@ int check(const dsdpa_cache_problem* p) {
     if (p->B <= 0 || p->Hkv <= 0 || p->pages <= 0 || p->page_size <= 0 || p->table_width <= 0) return DSDPA_ERR_BAD_SHAPE;
     if ((long long)p->table_width * p->page_size > (1ll << 30) || (long long)p->B * p->Hkv >= (1ll << 20)) return DSDPA_ERR_BAD_SHAPE;
     if (p->flags) return DSDPA_ERR_BAD_FLAGS;
-    const int e = p->dtype == DSDPA_F32 ? 4 : 2;
-    for (int i = 0; i < 3; ++i)
-        if (p->stride_k[i] < 0 || p->stride_v[i] < 0 || p->stride_k[i] * e % 16 || p->stride_v[i] * e % 16) return DSDPA_ERR_MISALIGNED;
-    return DSDPA_OK;
+    return bad_stride(p->stride_k, p->dtype, p->pages, p->Hkv, p->page_size) ? DSDPA_ERR_MISALIGNED : DSDPA_OK;
 }
 int check_tokens(const dsdpa_cache_problem* p) {
     const int st = check(p);
@@ -26,10 +25,7 @@ int check_tokens(const dsdpa_cache_problem* p) {
     if (p->Hq <= 0 || p->Hq % p->Hkv || (long long)p->B * p->Hq >= (1ll << 24) || p->T <= 0) return DSDPA_ERR_BAD_SHAPE;
     if (p->T > kTreeMax) return DSDPA_ERR_TOO_LARGE;
     if (!isfinite(p->sm_scale) || !isfinite(p->softcap)) return DSDPA_ERR_BAD_SHAPE;
-    const int e = p->dtype == DSDPA_F32 ? 4 : 2;
-    for (int i = 0; i < 3; ++i)
-        if (p->stride_q[i] < 0 || p->stride_q[i] * e % 16) return DSDPA_ERR_MISALIGNED;
-    return DSDPA_OK;
+    return bad_stride(p->stride_q, p->dtype, p->B, p->Hq, p->T) ? DSDPA_ERR_MISALIGNED : DSDPA_OK;
 }
 bool odd4(const void* p) { return ((uintptr_t)p & 3) != 0; }
 bool odd_tree(const dsdpa_cache_tree* t) {
@@ -47,6 +43,7 @@ CacheParams params(const dsdpa_cache_problem& p, const dsdpa_cache_tree* t, cons
     c.cap = p.softcap > 0.0f ? p.softcap : 0.0f;
     for (int i = 0; i < 3; ++i) { c.sq[i] = p.stride_q[i]; c.sk[i] = p.stride_k[i]; c.sv[i] = p.stride_v[i]; }
     c.err = err;
+    c.div = page_division(p.page_size);
     return c;
 }
 
@@ -83,7 +80,7 @@ int dsdpa_tree_forward(const dsdpa_cache_problem* p, const dsdpa_cache_tree* tre
     if (st != DSDPA_OK) return st;
     if (!q || !k_pages || !v_pages || !page_table || !lens || !out || !lse) return DSDPA_ERR_NULL_POINTER;
     if (misaligned(q) || misaligned(k_pages) || misaligned(v_pages) || misaligned(out) || misaligned(workspace) ||
-        odd4(page_table) || odd4(lens) || odd4(lse) || odd_tree(tree))
+        odd4(page_table) || odd4(lens) || odd4(lse) || odd_tree(tree) || bad_v(p))
         return DSDPA_ERR_MISALIGNED;
     if (tree && tree->positions && p->slots < p->table_width * p->page_size) return DSDPA_ERR_BAD_SHAPE;
     const size_t need = dsdpa_tree_workspace_bytes(p);
@@ -140,7 +137,7 @@ int dsdpa_cache_evict(const dsdpa_cache_problem* p, void* k_pages, void* v_pages
         return DSDPA_ERR_NULL_POINTER;
     if (new_weights == weights || (new_positions && new_positions == positions)) return DSDPA_ERR_BAD_SHAPE;
     if (misaligned(k_pages) || misaligned(v_pages) || odd4(page_table) || odd4(lens) || odd4(weights) || odd4(positions) ||
-        odd4(out_table) || odd4(kept) || odd4(new_lens) || odd4(new_weights) || odd4(new_positions))
+        odd4(out_table) || odd4(kept) || odd4(new_lens) || odd4(new_weights) || odd4(new_positions) || bad_v(p))
         return DSDPA_ERR_MISALIGNED;
     if (p->slots < p->table_width * p->page_size || keep <= 0 || sinks < 0 || recent < 0 || sinks > keep || recent > keep - sinks)
         return DSDPA_ERR_BAD_SHAPE;
@@ -164,7 +161,7 @@ int dsdpa_cache_evict(const dsdpa_cache_problem* p, void* k_pages, void* v_pages
     for (int i = 0; i < 3; ++i) { v.sk[i] = p->stride_k[i] * es; v.sv[i] = p->stride_v[i] * es; }
     v.err = err;
     cudaStream_t s = (cudaStream_t)stream;
-    set_division(v);
+    v.div = page_division(p->page_size);
     // up to 32768 ranks (128 KB) beside the histograms
     const int room = p->table_width * p->page_size;
     v.held = room < 32768 ? room : 32768;

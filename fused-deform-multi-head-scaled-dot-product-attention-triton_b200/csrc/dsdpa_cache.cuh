@@ -9,6 +9,20 @@ namespace dsdpa {
 
 constexpr int kTreeMax = DSDPA_TREE_MAX;
 
+// n / page_size = n mul >> shift for 0 <= n < 2^30.  With l = ceil(log2 d), k = 30 + l and m = floor(2^k / d) + 1: m d =
+// 2^k + e with 0 < e <= d <= 2^l, so n m / 2^k is n / d plus less than 2^30 / 2^k = 2^-l <= 1 / d, which cannot reach the
+// next whole number.
+struct PageDivision {
+    unsigned long long mul;
+    int shift;
+};
+inline PageDivision page_division(int page_size) {
+    int l = 0;
+    while ((1ll << l) < page_size) ++l;
+    return { (1ull << (30 + l)) / (unsigned)page_size + 1, 30 + l };
+}
+__device__ __forceinline__ int page_index(const PageDivision& d, int n) { return (int)(((unsigned)n * d.mul) >> d.shift); }
+
 struct CacheParams {
     const void *q, *k, *v;
     const int *table, *lens, *parents, *drafted, *positions, *start;
@@ -20,6 +34,7 @@ struct CacheParams {
     float sm_scale, cap;
     long long sq[3], sk[3], sv[3];
     int* err;
+    PageDivision div;
     // weights
     const unsigned char* take;
     float* weights;
@@ -35,15 +50,19 @@ __device__ __forceinline__ int cached_keys(const CacheParams& p, int b) {
 __device__ __forceinline__ int drafted_tokens(const CacheParams& p, int b) {
     return p.drafted ? max(0, min(__ldg(p.drafted + b), p.T)) : p.T;
 }
-// The page of key number n of sequence b; -1 (and a report) where the table has no valid one.
+// Entry `index` of sequence b's row of the table, as it stands there; -1 behind the row's end.
+__device__ __forceinline__ int table_entry(const int* table, int width, int b, int index) {
+    return index < width ? __ldg(table + (long long)b * width + index) : -1;
+}
+// The page, or -1 (and a report) where it is none.  (Apart from table_entry, so that a kernel can ask for an entry long
+// before it has to look at it.)
+__device__ __forceinline__ int checked_page(int page, int pages, int* err) {
+    if ((unsigned)page < (unsigned)pages) return page;
+    atomicCAS(err, 0, kErrBounds);
+    return -1;
+}
 __device__ __forceinline__ int page_of(const int* table, int width, int pages, int* err, int b, int index) {
-    int page = -1;
-    if (index < width) page = __ldg(table + (long long)b * width + index);
-    if ((unsigned)page >= (unsigned)pages) {
-        atomicCAS(err, 0, kErrBounds);
-        return -1;
-    }
-    return page;
+    return checked_page(table_entry(table, width, b, index), pages, err);
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, unsigned bytes) {   // the rest of 16 is zero

@@ -16,19 +16,9 @@ struct EvictParams {
     int row_bytes;
     long long sk[3], sv[3];   // bytes: page, head, slot
     int held;                 // ranks that evict_select_kernel has room for in shared memory
-    unsigned long long div_mul;   // n / page_size = n div_mul >> div_shift for n < 2^30
-    int div_shift;
+    PageDivision div;
     int* err;
 };
-// With l = ceil(log2 d), k = 30 + l and m = floor(2^k / d) + 1: m d = 2^k + e with 0 < e <= d <= 2^l, so n m / 2^k is
-// n / d plus less than 2^30 / 2^k = 2^-l <= 1 / d, which cannot reach the next whole number.
-inline void set_division(EvictParams& p) {
-    int l = 0;
-    while ((1ll << l) < p.page_size) ++l;
-    p.div_shift = 30 + l;
-    p.div_mul = (1ull << p.div_shift) / (unsigned)p.page_size + 1;
-}
-__device__ __forceinline__ int page_index(const EvictParams& p, int n) { return (int)(((unsigned)n * p.div_mul) >> p.div_shift); }
 
 constexpr int kSelectThreads = 1024;
 
@@ -209,7 +199,7 @@ __global__ void __launch_bounds__(kMoveThreads, kMoveBlocks) evict_move_kernel(c
             const int i = i0 + u * per + mine;
             to[u] = nullptr;
             if (key[u] < 0) continue;
-            const int si = page_index(p, key[u]), di = page_index(p, i);
+            const int si = page_index(p.div, key[u]), di = page_index(p.div, i);
             const int from_page = page_of(p.table, p.width, p.pages, p.err, b, si);
             const int to_page = page_of(p.out_table, p.out_width, p.pages, p.err, b, di);
             if (from_page < 0 || to_page < 0) continue;

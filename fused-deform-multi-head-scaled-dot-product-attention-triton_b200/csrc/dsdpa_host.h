@@ -18,6 +18,14 @@ void count_launches(int n);
 
 inline bool misaligned(const void* p) { return ((uintptr_t)p & 15u) != 0; }
 
+// Strides of dimensions that have one element do not matter.
+inline bool bad_stride(const long long (&st)[3], int dtype, int B, int H, int L) {
+    const int n[3] = { B, H, L };
+    for (int i = 0; i < 3; ++i)
+        if (n[i] > 1 && (st[i] <= 0 || (st[i] * (dtype == DSDPA_F32 ? 4 : 2)) % 16)) return true;
+    return false;
+}
+
 struct DeviceGuard {
     int prev = -1;
     cudaError_t err = cudaSuccess;

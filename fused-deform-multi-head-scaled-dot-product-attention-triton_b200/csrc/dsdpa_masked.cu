@@ -43,13 +43,6 @@ int check(const dsdpa_masked_problem* p) {
     return DSDPA_OK;
 }
 
-// Strides of dimensions that have one element do not matter.
-bool bad_stride(const long long (&st)[3], int dtype, int B, int H, int L) {
-    const int n[3] = { B, H, L };
-    for (int i = 0; i < 3; ++i)
-        if (n[i] > 1 && (st[i] <= 0 || (st[i] * (dtype == DSDPA_F32 ? 4 : 2)) % 16)) return true;
-    return false;
-}
 bool bad_q(const long long (&st)[3], const dsdpa_masked_problem* p) { return bad_stride(st, p->dtype, p->B, p->Hq, p->Lq); }
 bool bad_k(const long long (&st)[3], const dsdpa_masked_problem* p) { return bad_stride(st, p->dtype, p->B, p->Hkv, p->Lk); }
 

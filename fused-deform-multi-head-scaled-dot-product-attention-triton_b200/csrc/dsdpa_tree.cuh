@@ -37,12 +37,15 @@ template <int HD>
 __device__ __forceinline__ void copy_rows(uint32_t tile, int w, int lane, const char* row, const char* any, int D) {
     constexpr int kPer = HD / 8, kAt = 32 / kPer;          // 16-byte pieces of a row, rows of an instruction
     const int c = lane % kPer;
+    // all exchanges first: the copies keep their order, and would have every one of them wait for an exchange
+    const char* src[32 / kAt];
+#pragma unroll
+    for (int i = 0; i < 32 / kAt; ++i) src[i] = (const char*)__shfl_sync(0xffffffffu, (unsigned long long)row, i * kAt + lane / kPer);
+    const uint32_t dst = tile + (c >> 3) * 128 * 128 + w * 32 * 128 + (lane / kPer) * 128;
 #pragma unroll
     for (int i = 0; i < 32 / kAt; ++i) {
-        const int l = i * kAt + lane / kPer, r = w * 32 + l;
-        const char* src = (const char*)__shfl_sync(0xffffffffu, (unsigned long long)row, l);
-        const bool there = src != nullptr && c * 8 < D;
-        cp_async16(tile + (c >> 3) * 128 * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4), there ? src + c * 16 : any, there ? 16u : 0u);
+        const bool there = src[i] != nullptr && c * 8 < D;
+        cp_async16(dst + i * kAt * 128 + (((c & 7) ^ ((i * kAt + lane / kPer) & 7)) << 4), there ? src[i] + c * 16 : any, there ? 16u : 0u);
     }
 }
 
@@ -141,9 +144,9 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
                 if (!walk.next(p, sp, it)) it.tiles = -1;
             } while (it.tiles == 0);
         };
-        auto lookup = [&](const TreeItem& it, int i) {          // -1: no row
+        auto lookup = [&](const TreeItem& it, int i) {          // not looked at yet: nothing waits for it here
             const int j = it.key0 + i * kTreeKeys + w * 32 + lane;
-            return i < it.tiles && j < it.n + it.real ? page_of(p.table, p.width, p.pages, p.err, it.b, j / p.page_size) : -1;
+            return i < it.tiles && j < it.n + it.real ? table_entry(p.table, p.width, it.b, page_index(p.div, j)) : 0;
         };
         TreeItem it;
         next_item(it);
@@ -153,9 +156,9 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
             next_item(then);
             const int after[3] = { lookup(then, 0), lookup(then, 1), lookup(then, 2) };
             auto entry = [&](int i, bool is_v, int pg) {
-                const int j = it.key0 + i * kTreeKeys + w * 32 + lane, key = j - j / p.page_size * p.page_size;
+                const int j = it.key0 + i * kTreeKeys + w * 32 + lane, key = j - page_index(p.div, j) * p.page_size;
                 const char* src = nullptr;
-                if (pg >= 0)
+                if (j < it.n + it.real && (pg = checked_page(pg, p.pages, p.err)) >= 0)
                     src = is_v ? (const char*)(row_of<T>(p.v, p.sv, 0, it.hk, key) + pg * p.sv[0])
                                : (const char*)(row_of<T>(p.k, p.sk, 0, it.hk, key) + pg * p.sk[0]);
                 if (!mbar_wait_bounded(bar_empty + 8 * st, ph, p.err)) { ok = false; return; }

@@ -80,9 +80,9 @@ weights_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ Tr
             for (; handed < up_to; ++handed)
                 if (lane == 0) mbar_arrive(bar_full + 8 * (handed % L::kStages));
         };
-        auto lookup = [&](const TreeItem& it, int i) {
+        auto lookup = [&](const TreeItem& it, int i) {          // not looked at yet: nothing waits for it here
             const int j = it.key0 + i * kTreeKeys + w * 32 + lane;
-            return i < it.tiles && j < it.n + it.real ? page_of(p.table, p.width, p.pages, p.err, it.b, j / p.page_size) : -1;
+            return i < it.tiles && j < it.n + it.real ? table_entry(p.table, p.width, it.b, page_index(p.div, j)) : 0;
         };
         TreeItem it;
         while (ok && walk.next(p, sp, it))
@@ -114,9 +114,11 @@ weights_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ Tr
                     s_slope[buf][col] = valid ? __ldg(p.slopes + h) * kLog2e : 0.0f;
                 }
                 for (int i = 0; i < it.tiles; ++i) {
-                    const int j = it.key0 + i * kTreeKeys + w * 32 + lane, key = j - j / p.page_size * p.page_size;
+                    const int j = it.key0 + i * kTreeKeys + w * 32 + lane, key = j - page_index(p.div, j) * p.page_size;
                     const int more = lookup(it, i + 1);
-                    const char* src = page >= 0 ? (const char*)(row_of<T>(p.k, p.sk, 0, it.hk, key) + page * p.sk[0]) : nullptr;
+                    const char* src = nullptr;
+                    if (j < it.n + it.real && (page = checked_page(page, p.pages, p.err)) >= 0)
+                        src = (const char*)(row_of<T>(p.k, p.sk, 0, it.hk, key) + page * p.sk[0]);
                     if (!(ok = mbar_wait_bounded(bar_empty + 8 * st, ph, p.err))) break;
                     const unsigned there = __ballot_sync(0xffffffffu, src != nullptr);
                     if (lane == 0) s_valid[entries % kInfo][w] = there;
