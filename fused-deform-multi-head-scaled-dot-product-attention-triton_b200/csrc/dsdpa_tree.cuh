@@ -60,8 +60,8 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
                    bar_empty = bar_full + 8 * L::kStages, slot = bar_empty + 8 * L::kStages;
     __shared__ unsigned s_valid[kInfo][4];                 // keys of a tile that are there
     __shared__ float s_at[BIAS ? kInfo : 1][kTreeKeys];    // their positions
-    __shared__ float s_o[4][32][33];                       // the second stream's accumulator, 32 columns at a time
-    __shared__ float s_m[kTreeRows], s_l[kTreeRows];
+    __shared__ float s_m[2][kTreeRows], s_l[2][kTreeRows]; // what the streams tell one another
+    __shared__ unsigned s_odd[4][2];
     __shared__ TreeShare<kTreeThreads> share;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
@@ -237,7 +237,7 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
                 if (!mbar_wait_bounded(bar_s + 8 * tile, (done + mine) & 1, p.err)) { ok = false; break; }
                 tc_fence_after();
                 if (busy) {
-                    // 32 columns at a time, twice (for the maximum, for the weights): few registers and little code
+                    // 64 columns at a time, twice (for the maximum, for the weights): few registers, little code
                     const int slot_i = (info + i) % kInfo, k0 = it.key0 + i * kTreeKeys;
                     unsigned see[4], all = ~0u;
 #pragma unroll
@@ -251,28 +251,34 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
                     const bool whole = __all_sync(0xffffffffu, all == ~0u);
                     float top = kNegInf;
 #pragma unroll 1
-                    for (int w = 0; w < 4; ++w) {
-                        float s[32];
-                        tmem_ld32(s_col + w * 32, s);
+                    for (int w = 0; w < 2; ++w) {
+                        float s[64];
+                        tmem_ld32(s_col + w * 64, s);
+                        tmem_ld32(s_col + w * 64 + 32, s + 32);
                         tmem_wait_ld();
                         if (CAP || BIAS) {
 #pragma unroll
-                            for (int x = 0; x < 32; ++x) {
+                            for (int x = 0; x < 64; ++x) {
                                 float v = CAP ? capped_score2(s[x], c) : s[x] * c.scale2;
-                                if (BIAS) v = fmaf(-slope2, fabsf(pos - s_at[slot_i][w * 32 + x]), v);
+                                if (BIAS) v = fmaf(-slope2, fabsf(pos - s_at[slot_i][w * 64 + x]), v);
                                 s[x] = v;
                             }
                         }
                         if (!whole) {
-                            const unsigned bits = w == 0 ? see[0] : w == 1 ? see[1] : w == 2 ? see[2] : see[3];
+                            const unsigned lo = w ? see[2] : see[0], hi = w ? see[3] : see[1];
 #pragma unroll
-                            for (int x = 0; x < 32; ++x) s[x] = bits >> x & 1u ? s[x] : kNegInf;
+                            for (int x = 0; x < 64; ++x) s[x] = (x < 32 ? lo : hi) >> (x & 31) & 1u ? s[x] : kNegInf;
                         }
-                        if (CAP || BIAS || !whole) tmem_st32(s_col + w * 32, reinterpret_cast<const uint32_t*>(s));
-                        float mx[4] = { s[0], s[1], s[2], s[3] };
+                        if (CAP || BIAS || !whole) {
+                            tmem_st32(s_col + w * 64, reinterpret_cast<const uint32_t*>(s));
+                            tmem_st32(s_col + w * 64 + 32, reinterpret_cast<const uint32_t*>(s + 32));
+                        }
+                        float mx[8];
 #pragma unroll
-                        for (int x = 4; x < 32; ++x) mx[x & 3] = fmaxf(mx[x & 3], s[x]);
-                        top = fmaxf(top, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+                        for (int x = 0; x < 8; ++x) mx[x] = s[x];
+#pragma unroll
+                        for (int x = 8; x < 64; ++x) mx[x & 7] = fmaxf(mx[x & 7], s[x]);
+                        top = fmaxf(top, fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7]))));
                     }
                     if (CAP || BIAS || !whole) tmem_wait_st();
                     if (!(CAP || BIAS)) top *= c.scale2;
@@ -298,13 +304,14 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
                     const float m0 = m == kNegInf ? 0.0f : m;
                     float sum[4] = { 0.0f, 0.0f, 0.0f, 0.0f };
 #pragma unroll 1
-                    for (int w = 0; w < 4; ++w) {
-                        float s[32];
-                        uint32_t u[16];
-                        tmem_ld32(s_col + w * 32, s);
+                    for (int w = 0; w < 2; ++w) {
+                        float s[64];
+                        uint32_t u[32];
+                        tmem_ld32(s_col + w * 64, s);
+                        tmem_ld32(s_col + w * 64 + 32, s + 32);
                         tmem_wait_ld();
 #pragma unroll
-                        for (int y = 0; y < 32; y += 2) {
+                        for (int y = 0; y < 64; y += 2) {
                             const float a = (CAP || BIAS) ? s[y] - m0 : fmaf(s[y], c.scale2, -m0);
                             const float e = (CAP || BIAS) ? s[y + 1] - m0 : fmaf(s[y + 1], c.scale2, -m0);
                             const float pa = fast_exp2(a), pe = fast_exp2(e);
@@ -312,7 +319,7 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
                             sum[2 + ((y >> 1) & 1)] += pe;
                             u[y / 2] = pack2<T>(pa, pe);
                         }
-                        tmem_st16(s_col + w * 16, u);     // behind what has been read
+                        tmem_st32(s_col + w * 32, u);     // behind what has been read
                     }
                     l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                     tmem_wait_st();
@@ -327,76 +334,71 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
             if (mine > 0 && !(ok = mbar_wait_bounded(bar_o + 8 * tile, (done - 1) & 1, p.err))) break;
             if (!busy) continue;                           // the same for a warp and its partner of the other stream
             tc_fence_after();
-            if (tile == 1) { s_m[in_tile] = m; s_l[in_tile] = l; }
+            // Both streams' results to the larger of the two reference points: the pair of warps that has the same rows
+            // exchanges these, and takes a half of the columns each -- tensor memory has both accumulators.
+            s_m[tile][in_tile] = m;
+            s_l[tile][in_tile] = l;
+            tc_fence_before();
             pair_barrier(1 + quad);
-            // results of both streams to the larger of the two reference points
-            float g0 = 0.0f, g1 = 0.0f, inv = 0.0f, lse = kNegInf;
-            if (tile == 0) {
-                const float m1 = s_m[in_tile], l1 = s_l[in_tile], top = fmaxf(m, m1), t0 = top == kNegInf ? 0.0f : top;
-                const float f0 = fast_exp2(m - t0), f1 = fast_exp2(m1 - t0), sum = l * f0 + l1 * f1;
-                inv = sum != 0.0f ? 1.0f / sum : 0.0f;
-                lse = sum != 0.0f ? t0 + log2f(sum) : kNegInf;
-                g0 = f0 * inv;
-                g1 = f1 * inv;
-            }
-            pair_barrier(1 + quad);
-            const bool other = it.tiles > 1;               // the second stream has something
+            tc_fence_after();
+            const float m1 = s_m[tile ^ 1][in_tile], l1 = s_l[tile ^ 1][in_tile], top = fmaxf(m, m1), t0 = top == kNegInf ? 0.0f : top;
+            const float f0 = fast_exp2(m - t0), f1 = fast_exp2(m1 - t0);
+            // (in the order of the streams, so that both warps get the same)
+            const float total = tile == 0 ? l * f0 + l1 * f1 : l1 * f1 + l * f0, inv = total != 0.0f ? 1.0f / total : 0.0f;
+            const float lse = total != 0.0f ? t0 + log2f(total) : kNegInf;
+            const float g0 = (tile == 0 ? f0 : f1) * inv, g1 = (tile == 0 ? f1 : f0) * inv;
             const long long row = ((long long)it.b * p.Hq + h) * p.T + t, part = (long long)it.part * sp.part_rows + in_tile;
             // a sum of 0 x over the results is NaN where one is not finite
-            float nan0 = 0.0f * l, nan1 = 0.0f;
+            float nan0 = 0.0f * total, nan1 = 0.0f;
 #pragma unroll 1
-            for (int x = 0; x < HD; x += 32) {
+            for (int x = tile * (HD / 2); x < (tile + 1) * (HD / 2); x += 32) {
                 float o[32] = {};
-                if (it.tiles > tile) {
-                    tmem_ld32(o_col + x, o);
+                if (it.tiles > 1) {
+                    float z[32];
+                    tmem_ld32(tmem + 256 + x + lanes, o);
+                    tmem_ld32(tmem + 256 + HD + x + lanes, z);
                     tmem_wait_ld();
+#pragma unroll
+                    for (int y = 0; y < 32; ++y) o[y] = fmaf(o[y], g0, z[y] * g1);
+                } else if (it.tiles > 0) {
+                    tmem_ld32(tmem + 256 + x + lanes, o);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int y = 0; y < 32; ++y) o[y] *= g0;
                 }
-                if (other) {
-                    if (tile == 1) {
+                if (inv == 0.0f) {
 #pragma unroll
-                        for (int y = 0; y < 32; ++y) s_o[quad][lane][y] = o[y];
-                    }
-                    pair_barrier(1 + quad);
+                    for (int y = 0; y < 32; ++y) o[y] = 0.0f;
                 }
-                if (tile == 0) {
-                    if (inv == 0.0f) {
 #pragma unroll
-                        for (int y = 0; y < 32; ++y) o[y] = 0.0f;
-                    } else if (other) {
-#pragma unroll
-                        for (int y = 0; y < 32; ++y) o[y] = fmaf(o[y], g0, s_o[quad][lane][y] * g1);
-                    } else {
-#pragma unroll
-                        for (int y = 0; y < 32; ++y) o[y] *= g0;
-                    }
-#pragma unroll
-                    for (int y = 0; y < 32; y += 2) {
-                        nan0 = fmaf(o[y], 0.0f, nan0);
-                        nan1 = fmaf(o[y + 1], 0.0f, nan1);
-                    }
-                    if (valid) {
-#pragma unroll
-                        for (int y = 0; y < 32; y += 8)
-                            if (x + y < p.D) {
-                                float v[8];
-#pragma unroll
-                                for (int z = 0; z < 8; ++z) v[z] = o[y + z];
-                                if (it.part < 0) store8<T>((T*)p.out + row * p.D + x + y, v);
-                                else store8<float>(sp.part + part * p.D + x + y, v);
-                            }
-                    }
+                for (int y = 0; y < 32; y += 2) {
+                    nan0 = fmaf(o[y], 0.0f, nan0);
+                    nan1 = fmaf(o[y + 1], 0.0f, nan1);
                 }
-                if (other) pair_barrier(1 + quad);
-            }
-            if (tile == 0) {
                 if (valid) {
-                    if (it.part < 0) p.lse[row] = lse;
-                    else sp.part_lse[part] = lse;
+#pragma unroll
+                    for (int y = 0; y < 32; y += 8)
+                        if (x + y < p.D) {
+                            float v[8];
+#pragma unroll
+                            for (int z = 0; z < 8; ++z) v[z] = o[y + z];
+                            if (it.part < 0) store8<T>((T*)p.out + row * p.D + x + y, v);
+                            else store8<float>(sp.part + part * p.D + x + y, v);
+                        }
                 }
-                __syncwarp();
-                // rows that something non-finite reached: once more, from the keys they see alone
-                const float nan = nan0 + nan1;
-                unsigned bad = it.part < 0 ? __ballot_sync(0xffffffffu, valid && nan != nan) : 0u;
+            }
+            if (tile == 0 && valid) {
+                if (it.part < 0) p.lse[row] = lse;
+                else sp.part_lse[part] = lse;
+            }
+            // rows that something non-finite reached: once more, from the keys they see alone
+            const float nan = nan0 + nan1;
+            const unsigned odd = it.part < 0 ? __ballot_sync(0xffffffffu, valid && nan != nan) : 0u;
+            if (lane == 0) s_odd[quad][tile] = odd;
+            tc_fence_before();
+            pair_barrier(1 + quad);                       // both have read the accumulators; then the next products may write them
+            if (tile == 0) {
+                unsigned bad = s_odd[quad][0] | s_odd[quad][1];
                 while (bad) {
                     const int r = __ffs(bad) - 1;
                     bad &= bad - 1;
@@ -404,7 +406,6 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
                     exact_row_tree<T>(p, it.b, it.hk * p.group + g % p.group, g / p.group);
                 }
             }
-            tc_fence_before();
         }
     }
     __syncwarp();
