@@ -51,14 +51,15 @@ template <typename T>
 cudaError_t tree_forward(const dsdpa_cache_problem& problem, const CacheParams& p, void* workspace, cudaStream_t s) {
     const TreePlan t = plan_tree(problem);
     if constexpr (DtypeOf<T>::value != DSDPA_F32)
-        if (cache_on_tensor_cores(problem)) return launch_tree_tc<T>(p, t, workspace, s);
+        if (cache_on_tensor_cores(problem))
+            return cache_few_rows(problem) ? launch_tree_few<T>(p, t, workspace, s) : launch_tree_tc<T>(p, t, workspace, s);
     return launch_tree_simt<T>(p, t, workspace, s);
 }
 template <typename T>
 cudaError_t weights_add(const dsdpa_cache_problem& problem, const CacheParams& p, cudaStream_t s) {
     const TreePlan t = plan_tree(problem);
     if constexpr (DtypeOf<T>::value != DSDPA_F32)
-        if (cache_on_tensor_cores(problem)) return launch_weights_tc<T>(p, t, s);
+        if (cache_on_tensor_cores(problem)) return cache_few_rows(problem) ? launch_weights_few<T>(p, t, s) : launch_weights_tc<T>(p, t, s);
     return launch_weights_simt<T>(p, t, s);
 }
 

@@ -8,6 +8,15 @@ namespace dsdpa {
 
 // The tensor-core kernels take 16-bit storage with up to 128 elements a row; fp32 arithmetic the rest.
 inline bool cache_on_tensor_cores(const dsdpa_cache_problem& p) { return p.dtype != DSDPA_F32 && p.D <= 128; }
+// ... and of these a warp's own matrix instructions those with up to 16 rows to a key/value head.
+inline bool cache_few_rows(const dsdpa_cache_problem& p) { return cache_on_tensor_cores(p) && p.T * (p.Hq / p.Hkv) <= 16; }
+
+// Blocks of four warps that the few-row kernels are compiled to have on an SM: with 128 elements a row tree attention needs
+// more than 128 registers a thread.
+constexpr int few_blocks(int hd, int rows, bool weights) {
+    if (rows > 8) return weights ? 3 : 2;
+    return weights || hd == 64 ? 4 : 3;
+}
 
 // A call's work, as far as the host can know it (the lengths are on the device).
 struct TreePlan {
@@ -17,30 +26,34 @@ struct TreePlan {
 };
 inline TreePlan plan_tree(const dsdpa_cache_problem& p) {
     TreePlan t{};
-    const bool tc = cache_on_tensor_cores(p);
+    const bool tc = cache_on_tensor_cores(p), few = cache_few_rows(p);
     const long long room = (long long)p.table_width * p.page_size;
-    const int rows = p.T * (p.Hq / p.Hkv), keys = tc ? 128 : 64;
-    t.row_unit = tc ? 128 : rows <= 16 ? 16 : p.D <= 128 ? 64 : 32;
+    const int hd = p.D <= 64 ? 64 : 128, rows = p.T * (p.Hq / p.Hkv), keys = few ? 32 : tc ? 128 : 64, workers = few ? 4 : 1;   // a block's
+    t.row_unit = few ? 16 : tc ? 128 : rows <= 16 ? 16 : p.D <= 128 ? 64 : 32;
     t.row_tiles = (rows + t.row_unit - 1) / t.row_unit;
     t.part_rows = rows < t.row_unit ? rows : t.row_unit;
     const long long units = (long long)p.B * p.Hkv * t.row_tiles, tiles = (room + keys - 1) / keys;
-    // A cache of up to four key tiles is not worth a second kernel: a block goes through it while the launch
-    // of one would take.
-    t.whole = tiles <= 4;
+    // A cache of up to 512 keys (256 in fp32 arithmetic) is not worth a second kernel: a block goes through it while the
+    // launch of one would take.
+    t.whole = room <= (tc ? 512 : 256);
     // as many blocks as stay on the SMs at once, but no share below two key tiles
-    const long long stay = tc ? kSMs : p.D <= 64 ? 3 * kSMs : p.D <= 128 ? 2 * kSMs : kSMs;
-    const long long most = t.whole ? units : (units * tiles + 1) / 2, most_weights = ((long long)p.B * p.Hkv * tiles + 1) / 2;
-    t.blocks = (int)(most < stay ? most : stay);
-    t.weight_blocks = (int)(most_weights < stay ? most_weights : stay);
+    const long long stay = few ? few_blocks(hd, rows, false) * kSMs : tc ? kSMs : p.D <= 64 ? 3 * kSMs : p.D <= 128 ? 2 * kSMs : kSMs;
+    const long long stay_weights = few ? few_blocks(hd, rows, true) * kSMs : stay, least = 2 * workers;
+    const long long most = t.whole ? units : (units * tiles + least - 1) / least, most_weights = ((long long)p.B * p.Hkv * tiles + least - 1) / least;
+    t.blocks = (int)(most < stay || t.whole ? (most < 65536 ? most : 65536) : stay);
+    t.weight_blocks = (int)(most_weights < stay_weights ? most_weights : stay_weights);
+    const size_t parts = (size_t)t.blocks * workers * 2;
     if (!t.whole) {
         auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
         t.part_lse = up(((size_t)p.B + 2) * 8);
-        t.part = t.part_lse + up((size_t)t.blocks * 2 * t.part_rows * 4);
-        t.bytes = t.part + (size_t)t.blocks * 2 * t.part_rows * p.D * 4;
+        t.part = t.part_lse + up(parts * t.part_rows * 4);
+        t.bytes = t.part + parts * t.part_rows * p.D * 4;
     }
     return t;
 }
 
+template <typename T> cudaError_t launch_tree_few(const CacheParams& p, const TreePlan& t, void* workspace, cudaStream_t s);
+template <typename T> cudaError_t launch_weights_few(const CacheParams& p, const TreePlan& t, cudaStream_t s);
 template <typename T> cudaError_t launch_tree_tc(const CacheParams& p, const TreePlan& t, void* workspace, cudaStream_t s);
 template <typename T> cudaError_t launch_tree_simt(const CacheParams& p, const TreePlan& t, void* workspace, cudaStream_t s);
 template <typename T> cudaError_t launch_weights_tc(const CacheParams& p, const TreePlan& t, cudaStream_t s);

@@ -70,7 +70,7 @@ tree_simt_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     find_share<Tile>(p, sp, share);
     __syncthreads();
-    TreeWalk<Tile> walk{ share.b, share.unit, share.tile, share.left, true };
+    TreeWalk<Tile> walk = share.template walk<Tile>();
     TreeItem it;
     while (walk.next(p, sp, it)) {
         __syncthreads();                                        // the last item's tiles are read
@@ -181,7 +181,7 @@ weights_simt_kernel(const __grid_constant__ CacheParams p, const __grid_constant
     const int rows = p.T * p.group, passes = (rows + L::BM - 1) / L::BM;
     find_share<Tile>(p, sp, share);
     __syncthreads();
-    TreeWalk<Tile> walk{ share.b, share.unit, share.tile, share.left, true };
+    TreeWalk<Tile> walk = share.template walk<Tile>();
     TreeItem it;
     while (walk.next(p, sp, it)) {
         float* out = p.weights + ((long long)it.b * p.Hkv + it.hk) * p.slots;

@@ -75,6 +75,9 @@ template <typename T> __device__ __forceinline__ void store2(T* p, float a, floa
     *reinterpret_cast<uint32_t*>(p) = pack16(g, (T*)nullptr).x;
 }
 template <> __device__ __forceinline__ void store2<float>(float* p, float a, float b) { *reinterpret_cast<float2*>(p) = make_float2(a, b); }
+template <typename T> __device__ __forceinline__ T from_float(float x);
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+template <> __device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
 // Two packed 16-bit elements as fp32.
 template <typename T> __device__ __forceinline__ float2 to_float2(uint32_t u) {
     float f[8];

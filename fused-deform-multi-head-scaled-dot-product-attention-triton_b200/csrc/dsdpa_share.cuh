@@ -1,30 +1,29 @@
 // How a call's work over a paged cache is shared out.
 //
 // The queries that share a key/value head -- tokens times the group's heads, so many a tile: a unit -- meet the same keys.
-// The key tiles of all units lie one behind the other, and every block takes an equal share of that line,
-// whatever the lengths are (they are known on the device only): whole units, and at the ends of its share
-// parts of units, whose results tree_combine_kernel joins.  So all blocks end together, and no more than
-// two parts a block have to be written and read again.
+// The key tiles of all units lie one behind the other, and every worker -- a block, or a warp -- takes an equal share
+// of that line, whatever the lengths are (they are known on the device only): whole units, and at the ends
+// of its share parts of units, whose results tree_combine_kernel joins.  So all workers end together, and no
+// more than two parts a worker have to be written and read again.
 #pragma once
 
 #include "dsdpa_cache.cuh"
 
 namespace dsdpa {
 
-constexpr int kTreeMinShare = 2;    // key tiles
-
-template <int ROWS, int KEYS>
+// Rows of a unit's tile, keys of a key tile, key tiles of the smallest share, workers of a block.
+template <int ROWS, int KEYS, int LEAST = 2, int WORKERS = 1>
 struct ShareTile {
-    static constexpr int kRows = ROWS, kKeys = KEYS;
+    static constexpr int kRows = ROWS, kKeys = KEYS, kLeast = LEAST, kWorkers = WORKERS;
 };
 
 struct TreeSplit {
     int whole;            // units are not cut: no parts, no tree_combine_kernel
     int row_tiles;
     int part_rows;        // rows of a part
-    long long* start;     // null, or [B + 1]: key tiles of a head's query tile in the sequences before, and [B + 1]: a block's share
-    float* part;          // [blocks * 2][part_rows][D], normalised
-    float* part_lse;      // [blocks * 2][part_rows]
+    long long* start;     // null, or [B + 1]: key tiles of a head's query tile in the sequences before, and [B + 1]: a worker's share
+    float* part;          // [workers * 2][part_rows][D], normalised
+    float* part_lse;      // [workers * 2][part_rows]
 };
 // Key tiles of a sequence: the same for all of its heads.
 template <typename Tile>
@@ -33,17 +32,18 @@ __device__ __forceinline__ int tree_tiles(const CacheParams& p, int b) {
     return real > 0 ? (cached_keys(p, b) + real + Tile::kKeys - 1) / Tile::kKeys : 0;
 }
 
-// A unit, or the part of one that lies in a block's share.
+// A unit, or the part of one that lies in a worker's share.
 struct TreeItem {
     int b, hk, row0, rows, n, real, key0, tiles;
     int part;             // where its result goes: -1 to out and lse, else the number of the part
 };
-// Goes through the items of a block; every role has its own.
+// Goes through the items of a worker; every role of a block has its own.
 template <typename Tile>
 struct TreeWalk {
     int b, unit, tile;    // unit: of the sequence's heads * row_tiles
     long long left;       // key tiles of the share; whole units: number of the next unit
     bool first;
+    int worker;
     __device__ __forceinline__ bool next(const CacheParams& p, const TreeSplit& s, TreeItem& it) {
         const int units = p.Hkv * s.row_tiles;
         if (s.whole) {
@@ -64,7 +64,7 @@ struct TreeWalk {
             }
             if (left <= 0) return false;
             it.tiles = (int)min((long long)(nt - tile), left);
-            it.part = it.tiles == nt ? -1 : (int)blockIdx.x * 2 + (first ? 0 : 1);
+            it.part = it.tiles == nt ? -1 : worker * 2 + (first ? 0 : 1);
             left -= it.tiles;
         }
         first = false;
@@ -81,17 +81,21 @@ struct TreeWalk {
     }
 };
 
-// Where this block's share of the line begins, by all of its threads; the caller waits for them before it looks.
-template <int THREADS>
+// Where the shares of this block's workers begin, by all of its threads; the caller waits for them before it looks.
+template <int THREADS, int WORKERS = 1>
 struct TreeShare {
-    long long sum[THREADS / 32], left;
-    int b, unit, tile;
+    long long sum[THREADS / 32], left[WORKERS];
+    int b[WORKERS], unit[WORKERS], tile[WORKERS];
+    template <typename Tile>
+    __device__ __forceinline__ TreeWalk<Tile> walk(int w = 0) const {
+        return TreeWalk<Tile>{ b[w], unit[w], tile[w], left[w], true, (int)blockIdx.x * WORKERS + w };
+    }
 };
 template <typename Tile, int THREADS>
-__device__ __forceinline__ void find_share(const CacheParams& p, const TreeSplit& sp, TreeShare<THREADS>& out) {
+__device__ __forceinline__ void find_share(const CacheParams& p, const TreeSplit& sp, TreeShare<THREADS, Tile::kWorkers>& out) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (sp.whole) {
-        if (tid == 0) { out.left = blockIdx.x; out.b = out.unit = out.tile = 0; }
+        if (tid < Tile::kWorkers) { out.left[tid] = blockIdx.x; out.b[tid] = out.unit[tid] = out.tile[tid] = 0; }
     } else {
         // where this block's share begins: a thread has the key tiles of a few sequences
         const int per = (p.B + THREADS - 1) / THREADS, b0 = min(p.B, tid * per), b1 = min(p.B, b0 + per);
@@ -104,7 +108,7 @@ __device__ __forceinline__ void find_share(const CacheParams& p, const TreeSplit
             if (lane >= o) upto += t;
         }
         if (lane == 31) out.sum[warp] = upto;
-        if (tid == 0) { out.left = 0; out.b = out.unit = out.tile = 0; }
+        if (tid < Tile::kWorkers) { out.left[tid] = 0; out.b[tid] = out.unit[tid] = out.tile[tid] = 0; }
         __syncthreads();
         long long before = upto - mine, total = 0;
         for (int w = 0; w < THREADS / 32; ++w) {
@@ -112,14 +116,16 @@ __device__ __forceinline__ void find_share(const CacheParams& p, const TreeSplit
             total += out.sum[w];
         }
         const int units = p.Hkv * sp.row_tiles;
-        const long long line = total * units, share = max((long long)kTreeMinShare, (line + gridDim.x - 1) / gridDim.x);
-        const long long from = share * blockIdx.x;
+        const long long line = total * units, workers = (long long)gridDim.x * Tile::kWorkers;
+        const long long share = max((long long)Tile::kLeast, (line + workers - 1) / workers);
         if (blockIdx.x == 0 && sp.start) {
             long long at = before;
             for (int b = b0; b < b1; ++b) { sp.start[b] = at; at += tree_tiles<Tile>(p, b); }
             if (tid == 0) { sp.start[p.B] = total; sp.start[p.B + 1] = share; }
         }
-        if (from < line && from >= before * units && from < (before + mine) * units) {
+        for (int k = 0; k < Tile::kWorkers; ++k) {
+            const long long from = share * ((long long)blockIdx.x * Tile::kWorkers + k);
+            if (from >= line || from < before * units || from >= (before + mine) * units) continue;
             long long at = before * units;
             int b = b0;
             for (;; ++b) {
@@ -128,10 +134,10 @@ __device__ __forceinline__ void find_share(const CacheParams& p, const TreeSplit
                 at += span;
             }
             const int nt = tree_tiles<Tile>(p, b);
-            out.b = b;
-            out.unit = (int)((from - at) / nt);
-            out.tile = (int)((from - at) % nt);
-            out.left = min(share, line - from);
+            out.b[k] = b;
+            out.unit[k] = (int)((from - at) / nt);
+            out.tile[k] = (int)((from - at) % nt);
+            out.left[k] = min(share, line - from);
         }
     }
 }
@@ -144,14 +150,14 @@ __global__ void __launch_bounds__(kCombineWarps * 32) tree_combine_kernel(const 
     const long long row = (long long)blockIdx.x * kCombineWarps + threadIdx.x / 32;
     if (row >= (long long)p.B * p.Hq * p.T) return;
     const int lane = threadIdx.x & 31, t = (int)(row % p.T), h = (int)(row / p.T % p.Hq), b = (int)(row / p.T / p.Hq);
-    // the blocks whose shares the row's unit lies in
+    // the workers whose shares the row's unit lies in
     const int gr = t * p.group + h % p.group, nt = tree_tiles<Tile>(p, b);
     const long long share = sp.start[p.B + 1];
     const long long from = sp.start[b] * p.Hkv * sp.row_tiles + (long long)(h / p.group * sp.row_tiles + gr / Tile::kRows) * nt;
     const int c0 = (int)(from / share), c1 = nt > 0 ? (int)((from + nt - 1) / share) : c0 - 1;
-    if (c0 == c1) return;                                // written by the block itself
+    if (c0 == c1) return;                                // written by the worker itself
     const int used = c1 - c0 + 1;                        // 0: a query that sees no key
-    auto place = [&](int c) {                            // a block's first part, or its second
+    auto place = [&](int c) {                            // a worker's first part, or its second
         return ((long long)(c0 + c) * 2 + ((c0 + c) * share >= from ? 0 : 1)) * sp.part_rows + gr % Tile::kRows;
     };
     float m = kNegInf;

@@ -83,7 +83,7 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
     tc_fence_after();
     uint32_t tmem;
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(slot));
-    TreeWalk<TreeTile> walk{ share.b, share.unit, share.tile, share.left, true };
+    TreeWalk<TreeTile> walk = share.walk<TreeTile>();
 
     // Ring entries of an item with n tiles, in the order in which the products take them:
     // K0 K1 V0 K2 V1 .. K(n-1) V(n-2) V(n-1); the query tile comes with K0.

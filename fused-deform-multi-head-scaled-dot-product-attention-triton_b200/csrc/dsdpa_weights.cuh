@@ -43,7 +43,7 @@ weights_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ Tr
     tc_fence_after();
     uint32_t tmem;
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(slot));
-    TreeWalk<TreeTile> walk{ share.b, share.unit, share.tile, share.left, true };
+    TreeWalk<TreeTile> walk = share.walk<TreeTile>();
     // an item's passes over its rows; pass numbers run on over the items
     int pass = 0;
 
