@@ -23,9 +23,20 @@ cudaError_t tensor_map_16(CUtensorMap* map, int dtype, const void* base, int D, 
     const cuuint64_t strides[3] = { L > 1 ? (cuuint64_t)stride[2] * 2 : 16, H > 1 ? (cuuint64_t)stride[1] * 2 : 16,
                                     B > 1 ? (cuuint64_t)stride[0] * 2 : 16 };
     const cuuint32_t box[4] = { 64, (cuuint32_t)rows, 1, 1 }, step[4] = { 1, 1, 1, 1 };
-    const CUresult r = encode(map, dtype == DSDPA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
-                              const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    auto call = [&]() {
+        return encode(map, dtype == DSDPA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base),
+                      dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    };
+    CUresult r = call();
+    if (r != CUDA_SUCCESS) {
+        // a driver call wants the device's context bound to the thread, which the runtime does only when it has to: a
+        // thread that an autograd engine has just started may come here first
+        int device = 0;
+        cudaError_t e;
+        if ((e = cudaGetDevice(&device)) != cudaSuccess || (e = cudaSetDevice(device)) != cudaSuccess) return e;
+        r = call();
+    }
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
@@ -87,7 +98,7 @@ cudaError_t backward(const MaskedParams& p, void* workspace, cudaStream_t s) {
 }
 
 size_t backward_bytes(const dsdpa_masked_problem& p) {
-    const MaskedBwdSpace w = masked_bwd_space(p.dtype, p.B, p.Hq, p.Hkv, p.Lq);
+    const MaskedBwdSpace w = masked_bwd_space(p.dtype, p.B, p.Hq, p.Lq);
     return p.dtype != DSDPA_F32 && p.D <= 128 ? w.bytes : w.stats;
 }
 

@@ -26,7 +26,7 @@ struct BwdStats {
     float2* stats;    // [B, Hq, tiles * 128]: lse (+inf: no weight) and delta
     int2* ranges;     // [B, tiles * 128]: visible keys
     int4* tiles;      // [B, tiles]: least lo, largest hi over rows that see something; largest lo, least hi over all rows
-    unsigned* amax;   // [B, Hkv]: exponent field of the largest |dout| (fp16)
+    unsigned* amax;   // [B, Hq, tiles]: exponent field of the largest |dout| (fp16)
     int n;            // tiles of a sequence
 };
 
@@ -73,6 +73,7 @@ masked_dq_kernel(const __grid_constant__ MaskedParams p, const __grid_constant__
     const uint32_t bar_q = bars, bar_s = bars + 8, bar_dp = bars + 24, bar_ds = bars + 32, bar_done = bars + 40, bar_full = bars + 48,
                    bar_empty = bar_full + 8 * L::kStages, slot = bar_empty + 8 * L::kStages;
     __shared__ int s_lo, s_hi, s_lomax, s_himin;
+    __shared__ unsigned s_top;
     __shared__ float s_part[2][kTileQ];
     __shared__ unsigned char s_big[2][kTileQ];
     __shared__ unsigned s_bad[8];
@@ -81,7 +82,7 @@ masked_dq_kernel(const __grid_constant__ MaskedParams p, const __grid_constant__
     const int qt = st.n - 1 - (int)(blockIdx.x / (p.B * p.Hq)), q0 = qt * kTileQ;
 
     if (tid == 0) {
-        s_lo = 0x7fffffff; s_hi = 0; s_lomax = -1; s_himin = 0x7fffffff;
+        s_lo = 0x7fffffff; s_hi = 0; s_lomax = -1; s_himin = 0x7fffffff; s_top = 0;
         mbar_init(bar_q, 1);
         mbar_init(bar_s, 1);
         mbar_init(bar_s + 8, 1);
@@ -218,7 +219,7 @@ masked_dq_kernel(const __grid_constant__ MaskedParams p, const __grid_constant__
             if (row < p.Lq) p.delta[at] = delta;
             if (kScaled) {
                 const unsigned top = __reduce_max_sync(0xffffffffu, big);
-                if (lane == 0) atomicMax(st.amax + b * p.Hkv + hk, top);
+                if (lane == 0) atomicMax(&s_top, top);
             }
         }
         const float ndelta = -delta * sigma;
@@ -301,6 +302,7 @@ masked_dq_kernel(const __grid_constant__ MaskedParams p, const __grid_constant__
     tc_fence_before();
     __syncthreads();
     if (warp == 9) tmem_free(tmem, 512);
+    if (kScaled && tid == 0) st.amax[(long long)bh * st.n + qt] = s_top;
     // rows that something non-finite reached: once more, from the keys they see alone
     if (n > 0 && warp < 4) {
         unsigned bad = s_bad[warp] | s_bad[warp + 4];
@@ -334,7 +336,7 @@ masked_dkdv_kernel(const __grid_constant__ MaskedParams p, const __grid_constant
     const uint32_t bar_kv = bars, bar_qf = bars + 8, bar_qe = bars + 24, bar_of = bars + 40, bar_oe = bars + 56, bar_s = bars + 72,
                    bar_dp = bars + 80, bar_p = bars + 88, bar_ds = bars + 96, bar_done = bars + 104, slot = bars + 112;
     __shared__ int s_first, s_end;
-    __shared__ unsigned s_bad[8];
+    __shared__ unsigned s_bad[8], s_top;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int bh = blockIdx.x % (p.B * p.Hkv), b = bh / p.Hkv, hk = bh % p.Hkv;
     const int k0 = (int)(blockIdx.x / (p.B * p.Hkv)) * kTileK;       // first keys first: with a causal mask most queries see them
@@ -343,7 +345,7 @@ masked_dkdv_kernel(const __grid_constant__ MaskedParams p, const __grid_constant
     auto tile_rows = [&](int e) { return sm_rows + (uint32_t)(e & 1) * 2 * L::kRowBytes; };
 
     if (tid == 0) {
-        s_first = 0x7fffffff; s_end = 0;
+        s_first = 0x7fffffff; s_end = 0; s_top = 0;
         mbar_init(bar_kv, 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(bar_qf + 8 * i, 1);
@@ -369,6 +371,14 @@ masked_dkdv_kernel(const __grid_constant__ MaskedParams p, const __grid_constant
     lo = warp_min(lo);
     hi = warp_max(hi);
     if (lane == 0) { atomicMin(&s_first, lo); atomicMax(&s_end, hi); }
+    if (kScaled) {
+        // the largest |dout| of the group's heads
+        const unsigned* from = st.amax + (long long)(b * p.Hq + hk * p.group) * st.n;
+        unsigned top = 0;
+        for (int i = tid; i < p.group * st.n; i += kBwdThreads) top = max(top, from[i]);
+        top = __reduce_max_sync(0xffffffffu, top);
+        if (lane == 0) atomicMax(&s_top, top);
+    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -440,7 +450,7 @@ masked_dkdv_kernel(const __grid_constant__ MaskedParams p, const __grid_constant
         c.scale2 = fabsf(p.sm_scale) * kLog2e;
         c.cap_in = CAP ? 2.0f * c.scale2 / p.cap : 0.0f;
         c.cap_out = CAP ? p.cap * kLog2e : 0.0f;
-        const float sigma = kScaled ? scale_down(st.amax[bh]) : 1.0f;
+        const float sigma = kScaled ? scale_down(s_top) : 1.0f;
         const uint32_t s_at = tmem + half * 64 + lanes, d_at = s_at + 128;
         bool ok = true;
         for (int e = 0; e < n; ++e) {

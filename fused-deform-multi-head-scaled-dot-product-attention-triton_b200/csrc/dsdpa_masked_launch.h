@@ -26,7 +26,7 @@ struct MaskedBwdSpace {
     int n;          // tiles of 128 queries
     bool scaled;
 };
-inline MaskedBwdSpace masked_bwd_space(int dtype, int B, int Hq, int Hkv, int Lq) {
+inline MaskedBwdSpace masked_bwd_space(int dtype, int B, int Hq, int Lq) {
     auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
     MaskedBwdSpace w{};
     w.n = (Lq + 127) / 128;
@@ -35,7 +35,7 @@ inline MaskedBwdSpace masked_bwd_space(int dtype, int B, int Hq, int Hkv, int Lq
     w.ranges = w.stats + up((size_t)B * Hq * w.n * 128 * 8);
     w.tiles = w.ranges + up((size_t)B * w.n * 128 * 8);
     w.amax = w.tiles + up((size_t)B * w.n * 16);
-    w.bytes = w.amax + up((size_t)B * Hkv * 4);
+    w.bytes = w.amax + up((size_t)B * Hq * w.n * 4);
     return w;
 }
 

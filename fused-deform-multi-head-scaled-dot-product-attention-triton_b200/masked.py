@@ -181,6 +181,18 @@ def masked_backward_raw(q, k, v, out, lse, dout, sm_scale=None, *, causal=False,
     return dq, dk, dv
 
 
+def _grads(ctx, dout):
+    q, k, v, out, lse, visible, slopes = ctx.saved_tensors
+    dq, dk, dv = masked_backward_raw(q, k, v, out, lse, dout, ctx.sm_scale, causal=ctx.causal, visible=visible,
+                                     softcap=ctx.softcap, slopes=slopes)
+    if op.check_device_errors:
+        cabi.check(cabi.lib().dsdpa_device_error(q.device.index))
+    return dq, dk, dv, None, None, None, None, None
+
+
+_grads_once = once_differentiable(_grads)
+
+
 class _MaskedSDPA(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, sm_scale, causal, visible, softcap, slopes):
@@ -190,14 +202,9 @@ class _MaskedSDPA(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dout):
-        q, k, v, out, lse, visible, slopes = ctx.saved_tensors
-        dq, dk, dv = masked_backward_raw(q, k, v, out, lse, dout, ctx.sm_scale, causal=ctx.causal, visible=visible,
-                                         softcap=ctx.softcap, slopes=slopes)
-        if op.check_device_errors:
-            cabi.check(cabi.lib().dsdpa_device_error(q.device.index))
-        return dq, dk, dv, None, None, None, None, None
+        # gradients of gradients are refused where somebody asks for them
+        return _grads_once(ctx, dout) if torch.is_grad_enabled() else _grads(ctx, dout)
 
 
 def masked_sdpa(q, k, v, sm_scale=None, *, causal=False, visible=None, softcap=0.0, slopes=None):

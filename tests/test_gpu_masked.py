@@ -272,3 +272,32 @@ def test_long_rows_keep_their_precision():
     k[:, :, -1] *= 4
     check(q, k, v, do, 0.5, slopes=torch.tensor([0.01], device="cuda"))
     check(q, k, v, do, 0.5, causal=True)
+
+
+def test_threads_of_their_own():
+    """A thread whose first CUDA call this is (an autograd engine starts such threads), all memory coming from the cache."""
+    import threading
+    q, k, v, do = make(1, 2, 1, 200, 200, 64, torch.float16, seed=17)
+    want = be.masked_forward_raw(q, k, v, 0.125, causal=True)
+    grads = be.masked_backward_raw(q, k, v, *want, do, 0.125, causal=True)
+    for _ in range(3):
+        [t.clone() for t in (q, k, v, do, *want)]
+    torch.cuda.synchronize()
+    got = []
+
+    def work():
+        try:
+            out = be.masked_forward_raw(q, k, v, 0.125, causal=True)
+            got.append((out, be.masked_backward_raw(q, k, v, *out, do, 0.125, causal=True)))
+        except Exception as e:
+            got.append(e)
+    threads = [threading.Thread(target=work) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert len(got) == 4
+    for g in got:
+        assert not isinstance(g, Exception), g
+        assert all(torch.equal(a, b) for a, b in zip(g[0] + g[1], want + grads))
