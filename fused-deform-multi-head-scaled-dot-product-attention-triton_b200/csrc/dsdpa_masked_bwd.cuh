@@ -78,6 +78,7 @@ masked_dq_kernel(const __grid_constant__ MaskedParams p, const __grid_constant__
     __shared__ unsigned char s_big[2][kTileQ];
     __shared__ unsigned s_bad[8];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int bh = blockIdx.x % (p.B * p.Hq), b = bh / p.Hq, h = bh % p.Hq, hk = h / p.group;
     const int qt = st.n - 1 - (int)(blockIdx.x / (p.B * p.Hq)), q0 = qt * kTileQ;
 
@@ -94,6 +95,14 @@ masked_dq_kernel(const __grid_constant__ MaskedParams p, const __grid_constant__
     }
     if (warp == 9) tmem_alloc(slot, 512);
     __syncthreads();
+    if (warp == 8 && elect_one()) {
+        mbar_expect_tx(bar_q, 2 * L::kTileBytes);
+#pragma unroll
+        for (int x = 0; x < HD / kPanel; ++x) {
+            tma_load_4d(sm_q + x * 128 * 128, &mq, x * kPanel, q0, h, b, bar_q);
+            tma_load_4d(sm_do + x * 128 * 128, &mdo, x * kPanel, q0, h, b, bar_q);
+        }
+    }
     const int half = warp >> 2, in_tile = (warp & 3) * 32 + lane, row = q0 + in_tile;
     int2 r = make_int2(0, 0);
     int lo_most = -1, hi_least = 0x7fffffff;
@@ -113,29 +122,6 @@ masked_dq_kernel(const __grid_constant__ MaskedParams p, const __grid_constant__
             atomicMax(&s_lomax, lo_most);
             atomicMin(&s_himin, hi_least);
         }
-        // delta = out.dout: each half of the threads has half of the row
-        float part = 0.0f;
-        unsigned big = 0;
-        if (r.x < r.y) {
-            const T* o = row_of<T>(p.out_in, p.so, b, h, row);
-            const T* g = row_of<T>(p.dout, p.sdo, b, h, row);
-#pragma unroll
-            for (int x = 0; x < HD / 2; x += 8) {
-                const int d = half * (HD / 2) + x;
-                if (d < p.D) {
-                    float a[8], e[8];
-                    load8<T>(o + d, a);
-                    load8<T>(g + d, e);
-                    part += dot8(a, e);
-                    if (kScaled) {
-#pragma unroll
-                        for (int y = 0; y < 8; ++y) big = max(big, __float_as_uint(e[y]) & 0x7fffffffu);
-                    }
-                }
-            }
-        }
-        s_part[half][in_tile] = part;
-        s_big[half][in_tile] = (unsigned char)(big >> 23);
     }
     tc_fence_before();
     __syncthreads();
@@ -147,12 +133,6 @@ masked_dq_kernel(const __grid_constant__ MaskedParams p, const __grid_constant__
 
     if (warp == 8) {
         if (elect_one() && n > 0) {
-            mbar_expect_tx(bar_q, 2 * L::kTileBytes);
-#pragma unroll
-            for (int x = 0; x < HD / kPanel; ++x) {
-                tma_load_4d(sm_q + x * 128 * 128, &mq, x * kPanel, q0, h, b, bar_q);
-                tma_load_4d(sm_do + x * 128 * 128, &mdo, x * kPanel, q0, h, b, bar_q);
-            }
             int at = 0, ph = 1;
             bool ok = true;
             for (int i = 0; i < n && ok; ++i)
@@ -168,11 +148,12 @@ masked_dq_kernel(const __grid_constant__ MaskedParams p, const __grid_constant__
                 }
         }
     } else if (warp == 9) {
-        if (elect_one() && n > 0) {
+        // (a block without keys waits for its queries too: it must not end before they are there)
+        if (elect_one()) {
             // columns: S of even and of odd key blocks (dS in their place), dP, dq
             const uint32_t id_s = mma_desc<T>(kTileK, false, negate != 0), id_dp = mma_desc<T>(kTileK, false), id_dq = mma_desc<T>(HD, true);
             const uint32_t t_dp = tmem + 256, t_dq = tmem + 384;
-            bool ok = mbar_wait_bounded(bar_q, 0, p.err);
+            bool ok = mbar_wait_bounded(bar_q, 0, p.err) && n > 0;
             auto tile = [&](int e) { return sm_ring + (uint32_t)(e % L::kStages) * L::kTileBytes; };     // entry e: k of block e/2, or v
             auto arrived = [&](int e) { return mbar_wait_bounded(bar_full + 8 * (e % L::kStages), (e / L::kStages) & 1, p.err); };
             auto score = [&](int i) {
@@ -207,6 +188,30 @@ masked_dq_kernel(const __grid_constant__ MaskedParams p, const __grid_constant__
         c.cap_out = CAP ? p.cap * kLog2e : 0.0f;
         const float slope2 = BIAS ? __ldg(p.slopes + h) * kLog2e : 0.0f;
         const bool sees = r.x < r.y;
+        // delta = out.dout, while the first products are made: each half of the threads has half of the row
+        float sum = 0.0f;
+        unsigned most = 0;
+        if (sees) {
+            const T* o = row_of<T>(p.out_in, p.so, b, h, row);
+            const T* g = row_of<T>(p.dout, p.sdo, b, h, row);
+#pragma unroll
+            for (int x = 0; x < HD / 2; x += 8) {
+                const int d = half * (HD / 2) + x;
+                if (d < p.D) {
+                    float a[8], e[8];
+                    load8<T>(o + d, a);
+                    load8<T>(g + d, e);
+                    sum += dot8(a, e);
+                    if (kScaled) {
+#pragma unroll
+                        for (int y = 0; y < 8; ++y) most = max(most, __float_as_uint(e[y]) & 0x7fffffffu);
+                    }
+                }
+            }
+        }
+        s_part[half][in_tile] = sum;
+        s_big[half][in_tile] = (unsigned char)(most >> 23);
+        asm volatile("bar.sync 1, 256;" ::: "memory");
         const float delta = s_part[0][in_tile] + s_part[1][in_tile];
         const unsigned big = max((unsigned)s_big[0][in_tile], (unsigned)s_big[1][in_tile]);
         const float sigma = kScaled ? scale_down(big) : 1.0f;
@@ -362,6 +367,15 @@ masked_dkdv_kernel(const __grid_constant__ MaskedParams p, const __grid_constant
     }
     if (warp == 9) tmem_alloc(slot, 512);
     __syncthreads();
+    if (warp == 8 && elect_one()) {
+        mbar_expect_tx(bar_kv, 2 * L::kTileBytes);
+#pragma unroll
+        for (int x = 0; x < HD / kPanel; ++x) {
+            tma_load_4d(sm_k + x * 128 * 128, &mk, x * kPanel, k0, hk, b, bar_kv);
+            tma_load_4d(sm_v + x * 128 * 128, &mv, x * kPanel, k0, hk, b, bar_kv);
+        }
+    }
+    asm volatile("griddepcontrol.wait;" ::: "memory");      // masked_dq_kernel's results from here on
     // the query tiles between the first and the last that see any of these keys
     int lo = 0x7fffffff, hi = 0;
     for (int i = tid; i < st.n; i += kBwdThreads) {
@@ -388,12 +402,6 @@ masked_dkdv_kernel(const __grid_constant__ MaskedParams p, const __grid_constant
 
     if (warp == 8) {
         if (elect_one() && n > 0) {
-            mbar_expect_tx(bar_kv, 2 * L::kTileBytes);
-#pragma unroll
-            for (int x = 0; x < HD / kPanel; ++x) {
-                tma_load_4d(sm_k + x * 128 * 128, &mk, x * kPanel, k0, hk, b, bar_kv);
-                tma_load_4d(sm_v + x * 128 * 128, &mv, x * kPanel, k0, hk, b, bar_kv);
-            }
             bool ok = true;
             for (int e = 0; e < n && ok; ++e) {
                 const int h = hk * p.group + e / span, q0 = (first + e % span) * kTileQ;
@@ -411,11 +419,11 @@ masked_dkdv_kernel(const __grid_constant__ MaskedParams p, const __grid_constant
             }
         }
     } else if (warp == 9) {
-        if (elect_one() && n > 0) {
+        if (elect_one()) {
             // columns: S^T (P^T in its place), dP^T (dS^T in its place), dv, dk
             const uint32_t id_s = mma_desc<T>(kTileQ, false, negate != 0), id_dp = mma_desc<T>(kTileQ, false), id_g = mma_desc<T>(HD, true);
             const uint32_t t_dp = tmem + 128, t_dv = tmem + 256, t_dk = tmem + 384;
-            bool ok = mbar_wait_bounded(bar_kv, 0, p.err);
+            bool ok = mbar_wait_bounded(bar_kv, 0, p.err) && n > 0;
             auto score = [&](int e) {
                 if (!mbar_wait_bounded(bar_qf + 8 * (e & 1), (e >> 1) & 1, p.err)) return false;
                 mma_rows<HD>(tmem, sm_k, tile_q(e), kTileQ, id_s);

@@ -78,6 +78,14 @@ masked_fwd_kernel(const __grid_constant__ MaskedParams p, const __grid_constant_
     }
     if (warp == 9) tmem_alloc(slot, 512);
     __syncthreads();
+    if (warp == 8 && elect_one()) {
+        mbar_expect_tx(bar_q, 2 * L::kTileBytes);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int x = 0; x < HD / kPanel; ++x)
+                tma_load_4d(sm_q + t * L::kTileBytes + x * 128 * 128, &mq, x * kPanel, q0 + t * kTileQ, h, b, bar_q);
+    }
     int2 r = make_int2(0, 0);
     int lo_most = -1, hi_least = 0x7fffffff;     // over the warp's rows: keys inside need no mask
     const int tile = warp >> 2, row = q0 + tile * kTileQ + (warp & 3) * 32 + lane;
@@ -112,12 +120,6 @@ masked_fwd_kernel(const __grid_constant__ MaskedParams p, const __grid_constant_
         regs_release<80>();
         if (warp == 8) {
             if (elect_one()) {
-                mbar_expect_tx(bar_q, 2 * L::kTileBytes);
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int x = 0; x < HD / kPanel; ++x)
-                        tma_load_4d(sm_q + t * L::kTileBytes + x * 128 * 128, &mq, x * kPanel, q0 + t * kTileQ, h, b, bar_q);
                 int st = 0, ph = 1;      // the ring starts empty
                 bool ok = true;
                 for (int j = jb; j < je && ok; ++j) {
