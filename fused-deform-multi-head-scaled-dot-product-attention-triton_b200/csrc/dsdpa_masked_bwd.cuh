@@ -21,9 +21,18 @@ namespace dsdpa {
 
 constexpr int kBwdThreads = 320;
 
+struct Yes { static constexpr bool value = true; };
+struct No { static constexpr bool value = false; };
+
+__device__ __forceinline__ float4 lds_float4(uint32_t at) {
+    float4 f;
+    asm("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w) : "r"(at) : "memory");
+    return f;
+}
+
 // What masked_dq_kernel leaves for masked_dkdv_kernel, in whole tiles of 128 queries.
 struct BwdStats {
-    float2* stats;    // [B, Hq, tiles * 128]: lse (+inf: no weight) and delta
+    float* stats;     // [B, Hq, tiles][2][128]: -lse (-inf: no weight), and -delta
     int2* ranges;     // [B, tiles * 128]: visible keys
     int4* tiles;      // [B, tiles]: least lo, largest hi over rows that see something; largest lo, least hi over all rows
     unsigned* amax;   // [B, Hq, tiles]: exponent field of the largest |dout| (fp16)
@@ -35,20 +44,21 @@ __device__ __forceinline__ float scale_down(unsigned e) {
     return e == 0 || e >= 254 ? 1.0f : __uint_as_float((unsigned)(254 - e) << 23);
 }
 
-// The weight of one pair from its product qk; `slope` gets the factor that the cap's derivative puts on ds.
+// The weights of two pairs from their products qk; `slope` gets the factors that the cap's derivative puts on ds.
 template <bool CAP, bool BIAS>
-__device__ __forceinline__ float pair_weight(float qk, const ScoreConsts& c, float slope2, float dist, float lse, float& slope) {
-    float s;
+__device__ __forceinline__ float2 pair_weights(float2 qk, const ScoreConsts& c, float slope2, float d0, float d1, float2 neg_lse, float2& slope) {
+    float2 s;
     if (CAP) {
-        const float r = rcp_approx(1.0f + fast_exp2(qk * c.cap_in));
-        s = fmaf(-2.0f * c.cap_out, r, c.cap_out) - lse;
-        slope = 4.0f * fmaf(-r, r, r);              // 1 - tanh^2
+        const float2 r = make_float2(rcp_approx(1.0f + fast_exp2(qk.x * c.cap_in)), rcp_approx(1.0f + fast_exp2(qk.y * c.cap_in)));
+        s = add2(fma2(make_float2(-2.0f * c.cap_out, -2.0f * c.cap_out), r, make_float2(c.cap_out, c.cap_out)), neg_lse);
+        const float2 r2 = fma2(make_float2(-r.x, -r.y), r, r);
+        slope = make_float2(4.0f * r2.x, 4.0f * r2.y);              // 1 - tanh^2
     } else {
-        s = fmaf(qk, c.scale2, -lse);
-        slope = 1.0f;
+        s = fma2(qk, make_float2(c.scale2, c.scale2), neg_lse);
+        slope = make_float2(1.0f, 1.0f);
     }
-    if (BIAS) s = fmaf(-slope2, fabsf(dist), s);
-    return fast_exp2(s);
+    if (BIAS) s = make_float2(fmaf(-slope2, fabsf(d0), s.x), fmaf(-slope2, fabsf(d1), s.y));
+    return make_float2(fast_exp2(s.x), fast_exp2(s.y));
 }
 
 // d[128 x HD] (+)= w[128 x 128] b[128 x HD]; w's halves lie in columns 0 .. 31 and 64 .. 95 of its region, each
@@ -219,7 +229,9 @@ masked_dq_kernel(const __grid_constant__ MaskedParams p, const __grid_constant__
         float lse = sees ? p.lse[at] : kNegInf;
         if (lse == kNegInf) lse = -kNegInf;                 // weight exp2(s - inf) = 0
         if (half == 0) {
-            st.stats[(long long)bh * st.n * kTileQ + row] = make_float2(lse, delta);
+            float* stats = st.stats + ((long long)bh * st.n + qt) * 2 * kTileQ + in_tile;
+            stats[0] = -lse;
+            stats[kTileQ] = -delta;
             if (h == 0) st.ranges[(long long)b * st.n * kTileQ + row] = r;
             if (row < p.Lq) p.delta[at] = delta;
             if (kScaled) {
@@ -243,9 +255,12 @@ masked_dq_kernel(const __grid_constant__ MaskedParams p, const __grid_constant__
             const bool partial = lo_most > n0 || hi_least < n0 + 64;
             const int a = r.x - n0, e = r.y - n0;
 #pragma unroll
-            for (int x = 0; x < 64; ++x) {
-                float slope, v = pair_weight<CAP, BIAS>(w[x], c, slope2, d0 - (float)x, lse, slope);
-                w[x] = CAP ? v * slope : v;
+            for (int x = 0; x < 64; x += 2) {
+                float2 slope, v = pair_weights<CAP, BIAS>(make_float2(w[x], w[x + 1]), c, slope2, d0 - (float)x, d0 - (float)(x + 1),
+                                                          make_float2(-lse, -lse), slope);
+                if (CAP) v = mul2(v, slope);
+                w[x] = v.x;
+                w[x + 1] = v.y;
             }
             if (partial) {
 #pragma unroll
@@ -261,9 +276,10 @@ masked_dq_kernel(const __grid_constant__ MaskedParams p, const __grid_constant__
                 tmem_wait_ld();
 #pragma unroll
                 for (int y = 0; y < 32; y += 2) {
-                    const float u0 = kScaled ? fmaf(d[y], sigma, ndelta) : d[y] + ndelta;
-                    const float u1 = kScaled ? fmaf(d[y + 1], sigma, ndelta) : d[y + 1] + ndelta;
-                    o[y / 2] = pack2<T>(w[x + y] * u0, w[x + y + 1] * u1);
+                    const float2 dp = make_float2(d[y], d[y + 1]), nd = make_float2(ndelta, ndelta);
+                    const float2 u = kScaled ? fma2(dp, make_float2(sigma, sigma), nd) : add2(dp, nd);
+                    const float2 ds = mul2(make_float2(w[x + y], w[x + y + 1]), u);
+                    o[y / 2] = pack2<T>(ds.x, ds.y);
                 }
                 tmem_st16(s_at + x / 2, o);
             }
@@ -410,7 +426,7 @@ masked_dkdv_kernel(const __grid_constant__ MaskedParams p, const __grid_constant
                 mbar_expect_tx(full, L::kTileBytes + 2 * L::kRowBytes);
 #pragma unroll
                 for (int x = 0; x < HD / kPanel; ++x) tma_load_4d(tile_q(e) + x * 128 * 128, &mq, x * kPanel, q0, h, b, full);
-                bulk_g2s(tile_rows(e), st.stats + ((long long)b * p.Hq + h) * st.n * kTileQ + q0, L::kRowBytes, full);
+                bulk_g2s(tile_rows(e), st.stats + (((long long)b * p.Hq + h) * st.n * kTileQ + q0) * 2, L::kRowBytes, full);
                 bulk_g2s(tile_rows(e) + L::kRowBytes, st.ranges + (long long)b * st.n * kTileQ + q0, L::kRowBytes, full);
                 if (!(ok = mbar_wait_bounded(bar_oe + 8 * (e & 1), ph, p.err))) break;
                 mbar_expect_tx(dfull, L::kTileBytes);
@@ -466,7 +482,8 @@ masked_dkdv_kernel(const __grid_constant__ MaskedParams p, const __grid_constant
             const float slope2 = BIAS ? __ldg(p.slopes + hk * p.group + e / span) * kLog2e : 0.0f;
             const int4 t = __ldg(st.tiles + (long long)b * st.n + qt);
             const bool partial = t.z > k0 || t.w < k0 + kTileK;
-            const uint32_t stats = tile_rows(e) + half * 64 * 8, ranges = stats + L::kRowBytes;
+            const uint32_t neg_lse = tile_rows(e) + half * 64 * 4, neg_delta = neg_lse + kTileQ * 4;
+            const uint32_t ranges = tile_rows(e) + L::kRowBytes + half * 64 * 8;
             const float d0 = (float)(q0 + (p.Lk - p.Lq) - key);
             float w[64];
             if (!mbar_wait_bounded(bar_qf + 8 * (e & 1), (e >> 1) & 1, p.err) || !mbar_wait_bounded(bar_s, e & 1, p.err)) { ok = false; break; }
@@ -474,26 +491,34 @@ masked_dkdv_kernel(const __grid_constant__ MaskedParams p, const __grid_constant
             tmem_ld32(s_at, w);
             tmem_ld32(s_at + 32, w + 32);
             tmem_wait_ld();
+            auto weights = [&](auto masked) {
 #pragma unroll
-            for (int x = 0; x < 64; x += 32) {
-                uint32_t o[16];
+                for (int x = 0; x < 64; x += 32) {
+                    uint32_t o[16];
 #pragma unroll
-                for (int y = 0; y < 32; y += 2) {
-                    const uint4 q = lds128(stats + (x + y) * 8);       // lse, delta of two queries
-                    float g0, g1;
-                    float v0 = pair_weight<CAP, BIAS>(w[x + y], c, slope2, d0 + (float)(x + y), __uint_as_float(q.x), g0);
-                    float v1 = pair_weight<CAP, BIAS>(w[x + y + 1], c, slope2, d0 + (float)(x + y + 1), __uint_as_float(q.z), g1);
-                    if (partial) {
-                        const uint4 k = lds128(ranges + (x + y) * 8);
-                        v0 = key >= (int)k.x && key < (int)k.y ? v0 : 0.0f;
-                        v1 = key >= (int)k.z && key < (int)k.w ? v1 : 0.0f;
+                    for (int y = 0; y < 32; y += 4) {
+                        const float4 nl = lds_float4(neg_lse + (x + y) * 4);
+#pragma unroll
+                        for (int z = 0; z < 4; z += 2) {
+                            const int at = x + y + z;
+                            float2 slope, v = pair_weights<CAP, BIAS>(make_float2(w[at], w[at + 1]), c, slope2, d0 + (float)at, d0 + (float)(at + 1),
+                                                                      z ? make_float2(nl.z, nl.w) : make_float2(nl.x, nl.y), slope);
+                            if (decltype(masked)::value) {
+                                const uint4 k = lds128(ranges + at * 8);
+                                v.x = key >= (int)k.x && key < (int)k.y ? v.x : 0.0f;
+                                v.y = key >= (int)k.z && key < (int)k.w ? v.y : 0.0f;
+                            }
+                            o[(y + z) / 2] = pack2<T>(v.x, v.y);
+                            if (CAP) v = mul2(v, slope);
+                            w[at] = v.x;
+                            w[at + 1] = v.y;
+                        }
                     }
-                    o[y / 2] = pack2<T>(v0, v1);
-                    w[x + y] = CAP ? v0 * g0 : v0;
-                    w[x + y + 1] = CAP ? v1 * g1 : v1;
+                    tmem_st16(s_at + x / 2, o);
                 }
-                tmem_st16(s_at + x / 2, o);
-            }
+            };
+            if (partial) weights(Yes{});
+            else weights(No{});
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
@@ -507,11 +532,15 @@ masked_dkdv_kernel(const __grid_constant__ MaskedParams p, const __grid_constant
                 tmem_ld32(d_at + x, d);
                 tmem_wait_ld();
 #pragma unroll
-                for (int y = 0; y < 32; y += 2) {
-                    const uint4 q = lds128(stats + (x + y) * 8);
-                    float u0 = d[y] - __uint_as_float(q.y), u1 = d[y + 1] - __uint_as_float(q.w);
-                    if (kScaled) { u0 *= sigma; u1 *= sigma; }
-                    o[y / 2] = pack2<T>(w[x + y] * u0, w[x + y + 1] * u1);
+                for (int y = 0; y < 32; y += 4) {
+                    const float4 nd = lds_float4(neg_delta + (x + y) * 4);
+#pragma unroll
+                    for (int z = 0; z < 4; z += 2) {
+                        float2 u = add2(make_float2(d[y + z], d[y + z + 1]), z ? make_float2(nd.z, nd.w) : make_float2(nd.x, nd.y));
+                        if (kScaled) u = mul2(u, make_float2(sigma, sigma));
+                        const float2 ds = mul2(make_float2(w[x + y + z], w[x + y + z + 1]), u);
+                        o[(y + z) / 2] = pack2<T>(ds.x, ds.y);
+                    }
                 }
                 tmem_st16(d_at + x / 2, o);
             }

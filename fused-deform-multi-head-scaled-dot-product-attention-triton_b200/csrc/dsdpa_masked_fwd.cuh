@@ -242,22 +242,21 @@ masked_fwd_kernel(const __grid_constant__ MaskedParams p, const __grid_constant_
                 }
             }
             const float m0 = m == kNegInf ? 0.0f : m;
-            float sum[4] = { 0.0f, 0.0f, 0.0f, 0.0f };
+            float2 sum[2] = { make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f) };
+            const float2 scale = make_float2(c.scale2, c.scale2), to = make_float2(-m0, -m0);
 #pragma unroll
             for (int x = 0; x < kTileK; x += 32) {
                 uint32_t w[16];
 #pragma unroll
                 for (int y = 0; y < 32; y += 2) {
-                    const float a = (CAP || BIAS) ? s[x + y] - m0 : fmaf(s[x + y], c.scale2, -m0);
-                    const float e = (CAP || BIAS) ? s[x + y + 1] - m0 : fmaf(s[x + y + 1], c.scale2, -m0);
-                    const float pa = weight_exp2(a), pe = weight_exp2(e);
-                    sum[(y >> 1) & 1] += pa;
-                    sum[2 + ((y >> 1) & 1)] += pe;
-                    w[y / 2] = pack2<T>(pa, pe);
+                    const float2 v = make_float2(s[x + y], s[x + y + 1]), a = (CAP || BIAS) ? add2(v, to) : fma2(v, scale, to);
+                    const float2 e = make_float2(weight_exp2(a.x), weight_exp2(a.y));
+                    sum[(y >> 1) & 1] = add2(sum[(y >> 1) & 1], e);
+                    w[y / 2] = pack2<T>(e.x, e.y);
                 }
                 tmem_st16(s_at + x / 2, w);
             }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();

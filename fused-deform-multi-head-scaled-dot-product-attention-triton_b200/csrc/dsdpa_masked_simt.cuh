@@ -22,10 +22,7 @@ template <int HD, int ROWS = HD == 256 ? 2 : 4> struct SimtShape {
     static constexpr int kSmemBwd = (2 * BM * S + 2 * kSimtKeys * S + BM * W) * 4;
 };
 
-__device__ __forceinline__ void fma2(float2& d, float2 a, float2 b) {
-    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%0, %1};\n\t"
-        "fma.rn.f32x2 z, x, y, z;\n\tmov.b64 {%0, %1}, z;\n\t}" : "+f"(d.x), "+f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-}
+__device__ __forceinline__ void add_fma2(float2& d, float2 a, float2 b) { d = fma2(a, b, d); }
 
 // Rows [row0, row0 + N) of one head into shared memory as fp32; rows and elements that do not exist are zero.
 template <typename T, int HD, int N>
@@ -70,8 +67,8 @@ __device__ __forceinline__ void simt_dot(const float* a, const float* b, float (
         for (int r = 0; r < L::RM; ++r)
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                fma2(acc[r][c], make_float2(x[r].x, x[r].y), make_float2(y[c].x, y[c].y));
-                fma2(acc[r][c], make_float2(x[r].z, x[r].w), make_float2(y[c].z, y[c].w));
+                add_fma2(acc[r][c], make_float2(x[r].x, x[r].y), make_float2(y[c].x, y[c].y));
+                add_fma2(acc[r][c], make_float2(x[r].z, x[r].w), make_float2(y[c].z, y[c].w));
             }
     }
 #pragma unroll
@@ -114,7 +111,7 @@ __device__ __forceinline__ void simt_rows(const float* w, const float* b, float2
                 for (int r = 0; r < L::RM; ++r) {
                     const float f = e == 0 ? x[r].x : e == 1 ? x[r].y : e == 2 ? x[r].z : x[r].w;
 #pragma unroll
-                    for (int q = 0; q < L::CW / 2; ++q) fma2(acc[r][j][q], make_float2(f, f), v[q]);
+                    for (int q = 0; q < L::CW / 2; ++q) add_fma2(acc[r][j][q], make_float2(f, f), v[q]);
                 }
             }
     }
@@ -133,10 +130,10 @@ __device__ __forceinline__ void simt_columns(const float* w, const float* b, flo
             simt_piece<HD>(b + q * L::S, j, v);
 #pragma unroll
             for (int z = 0; z < L::CW / 2; ++z) {
-                fma2(acc[0][j][z], make_float2(x.x, x.x), v[z]);
-                fma2(acc[1][j][z], make_float2(x.y, x.y), v[z]);
-                fma2(acc[2][j][z], make_float2(x.z, x.z), v[z]);
-                fma2(acc[3][j][z], make_float2(x.w, x.w), v[z]);
+                add_fma2(acc[0][j][z], make_float2(x.x, x.x), v[z]);
+                add_fma2(acc[1][j][z], make_float2(x.y, x.y), v[z]);
+                add_fma2(acc[2][j][z], make_float2(x.z, x.z), v[z]);
+                add_fma2(acc[3][j][z], make_float2(x.w, x.w), v[z]);
             }
         }
     }
