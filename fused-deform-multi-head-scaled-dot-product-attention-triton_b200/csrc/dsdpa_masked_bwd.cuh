@@ -44,19 +44,12 @@ __device__ __forceinline__ float scale_down(unsigned e) {
     return e == 0 || e >= 254 ? 1.0f : __uint_as_float((unsigned)(254 - e) << 23);
 }
 
-// The weights of two pairs from their products qk; `slope` gets the factors that the cap's derivative puts on ds.
+// The weights of two pairs from what cap_scores left (or the products); `slope` gets the factors that the cap's derivative
+// puts on ds: 1 - tanh^2.
 template <bool CAP, bool BIAS>
-__device__ __forceinline__ float2 pair_weights(float2 qk, const ScoreConsts& c, float slope2, float d0, float d1, float2 neg_lse, float2& slope) {
-    float2 s;
-    if (CAP) {
-        const float2 r = make_float2(rcp_approx(1.0f + fast_exp2(qk.x * c.cap_in)), rcp_approx(1.0f + fast_exp2(qk.y * c.cap_in)));
-        s = add2(fma2(make_float2(-2.0f * c.cap_out, -2.0f * c.cap_out), r, make_float2(c.cap_out, c.cap_out)), neg_lse);
-        const float2 r2 = fma2(make_float2(-r.x, -r.y), r, r);
-        slope = make_float2(4.0f * r2.x, 4.0f * r2.y);              // 1 - tanh^2
-    } else {
-        s = fma2(qk, make_float2(c.scale2, c.scale2), neg_lse);
-        slope = make_float2(1.0f, 1.0f);
-    }
+__device__ __forceinline__ float2 pair_weights(float2 t, float unit, float slope2, float d0, float d1, float2 neg_lse, float2& slope) {
+    float2 s = fma2(t, make_float2(unit, unit), neg_lse);
+    if (CAP) slope = fma2(make_float2(-t.x, -t.y), t, make_float2(1.0f, 1.0f));
     if (BIAS) s = make_float2(fmaf(-slope2, fabsf(d0), s.x), fmaf(-slope2, fabsf(d1), s.y));
     return make_float2(fast_exp2(s.x), fast_exp2(s.y));
 }
@@ -194,8 +187,9 @@ masked_dq_kernel(const __grid_constant__ MaskedParams p, const __grid_constant__
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;
         ScoreConsts c;
         c.scale2 = fabsf(p.sm_scale) * kLog2e;
-        c.cap_in = CAP ? 2.0f * c.scale2 / p.cap : 0.0f;
+        c.cap_in = CAP ? 2.0f * fabsf(p.sm_scale) / p.cap : 0.0f;
         c.cap_out = CAP ? p.cap * kLog2e : 0.0f;
+        const float unit = CAP ? c.cap_out : c.scale2;
         const float slope2 = BIAS ? __ldg(p.slopes + h) * kLog2e : 0.0f;
         const bool sees = r.x < r.y;
         // delta = out.dout, while the first products are made: each half of the threads has half of the row
@@ -254,9 +248,10 @@ masked_dq_kernel(const __grid_constant__ MaskedParams p, const __grid_constant__
             const float d0 = (float)(pos - n0);
             const bool partial = lo_most > n0 || hi_least < n0 + 64;
             const int a = r.x - n0, e = r.y - n0;
+            if (CAP) cap_scores(w, c);
 #pragma unroll
             for (int x = 0; x < 64; x += 2) {
-                float2 slope, v = pair_weights<CAP, BIAS>(make_float2(w[x], w[x + 1]), c, slope2, d0 - (float)x, d0 - (float)(x + 1),
+                float2 slope, v = pair_weights<CAP, BIAS>(make_float2(w[x], w[x + 1]), unit, slope2, d0 - (float)x, d0 - (float)(x + 1),
                                                           make_float2(-lse, -lse), slope);
                 if (CAP) v = mul2(v, slope);
                 w[x] = v.x;
@@ -472,8 +467,9 @@ masked_dkdv_kernel(const __grid_constant__ MaskedParams p, const __grid_constant
         const int half = warp >> 2, in_tile = (warp & 3) * 32 + lane, key = k0 + in_tile;
         ScoreConsts c;
         c.scale2 = fabsf(p.sm_scale) * kLog2e;
-        c.cap_in = CAP ? 2.0f * c.scale2 / p.cap : 0.0f;
+        c.cap_in = CAP ? 2.0f * fabsf(p.sm_scale) / p.cap : 0.0f;
         c.cap_out = CAP ? p.cap * kLog2e : 0.0f;
+        const float unit = CAP ? c.cap_out : c.scale2;
         const float sigma = kScaled ? scale_down(s_top) : 1.0f;
         const uint32_t s_at = tmem + half * 64 + lanes, d_at = s_at + 128;
         bool ok = true;
@@ -491,6 +487,7 @@ masked_dkdv_kernel(const __grid_constant__ MaskedParams p, const __grid_constant
             tmem_ld32(s_at, w);
             tmem_ld32(s_at + 32, w + 32);
             tmem_wait_ld();
+            if (CAP) cap_scores(w, c);
             auto weights = [&](auto masked) {
 #pragma unroll
                 for (int x = 0; x < 64; x += 32) {
@@ -501,7 +498,7 @@ masked_dkdv_kernel(const __grid_constant__ MaskedParams p, const __grid_constant
 #pragma unroll
                         for (int z = 0; z < 4; z += 2) {
                             const int at = x + y + z;
-                            float2 slope, v = pair_weights<CAP, BIAS>(make_float2(w[at], w[at + 1]), c, slope2, d0 + (float)at, d0 + (float)(at + 1),
+                            float2 slope, v = pair_weights<CAP, BIAS>(make_float2(w[at], w[at + 1]), unit, slope2, d0 + (float)at, d0 + (float)(at + 1),
                                                                       z ? make_float2(nl.z, nl.w) : make_float2(nl.x, nl.y), slope);
                             if (decltype(masked)::value) {
                                 const uint4 k = lds128(ranges + at * 8);

@@ -219,8 +219,9 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
         const uint32_t lanes = (uint32_t)quad << 21, s_col = tmem + tile * kTreeKeys + lanes, o_col = tmem + 256 + tile * HD + lanes;
         ScoreConsts c;
         c.scale2 = fabsf(p.sm_scale) * kLog2e;
-        c.cap_in = CAP ? 2.0f * c.scale2 / p.cap : 0.0f;
+        c.cap_in = CAP ? 2.0f * fabsf(p.sm_scale) / p.cap : 0.0f;
         c.cap_out = CAP ? p.cap * kLog2e : 0.0f;
+        const float unit = CAP ? c.cap_out : c.scale2;    // of what cap_scores, or the product, left: scores in base 2
         int done = 0, info = 0;           // key tiles of this stream, of the block, so far
         bool ok = true;
         TreeItem it;
@@ -256,13 +257,10 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
                         tmem_ld32(s_col + w * 64, s);
                         tmem_ld32(s_col + w * 64 + 32, s + 32);
                         tmem_wait_ld();
-                        if (CAP || BIAS) {
+                        if (CAP) cap_scores(s, c);
+                        if (BIAS) {
 #pragma unroll
-                            for (int x = 0; x < 64; ++x) {
-                                float v = CAP ? capped_score2(s[x], c) : s[x] * c.scale2;
-                                if (BIAS) v = fmaf(-slope2, fabsf(pos - s_at[slot_i][w * 64 + x]), v);
-                                s[x] = v;
-                            }
+                            for (int x = 0; x < 64; ++x) s[x] = fmaf(-slope2, fabsf(pos - s_at[slot_i][w * 64 + x]), s[x] * unit);
                         }
                         if (!whole) {
                             const unsigned lo = w ? see[2] : see[0], hi = w ? see[3] : see[1];
@@ -281,7 +279,7 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
                         top = fmaxf(top, fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7]))));
                     }
                     if (CAP || BIAS || !whole) tmem_wait_st();
-                    if (!(CAP || BIAS)) top *= c.scale2;
+                    if (!BIAS) top *= unit;
                     const bool move = top > m + 8.0f || (m == kNegInf && top > kNegInf);
                     if (__any_sync(0xffffffffu, move)) {
                         const float f = move ? (m == kNegInf ? 0.0f : fast_exp2(m - top)) : 1.0f;
@@ -302,7 +300,8 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
                         }
                     }
                     const float m0 = m == kNegInf ? 0.0f : m;
-                    float sum[4] = { 0.0f, 0.0f, 0.0f, 0.0f };
+                    float2 sum[2] = { make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f) };
+                    const float2 scale = make_float2(unit, unit), to = make_float2(-m0, -m0);
 #pragma unroll 1
                     for (int w = 0; w < 2; ++w) {
                         float s[64];
@@ -312,16 +311,14 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
                         tmem_wait_ld();
 #pragma unroll
                         for (int y = 0; y < 64; y += 2) {
-                            const float a = (CAP || BIAS) ? s[y] - m0 : fmaf(s[y], c.scale2, -m0);
-                            const float e = (CAP || BIAS) ? s[y + 1] - m0 : fmaf(s[y + 1], c.scale2, -m0);
-                            const float pa = fast_exp2(a), pe = fast_exp2(e);
-                            sum[(y >> 1) & 1] += pa;
-                            sum[2 + ((y >> 1) & 1)] += pe;
-                            u[y / 2] = pack2<T>(pa, pe);
+                            const float2 v = make_float2(s[y], s[y + 1]), a = BIAS ? add2(v, to) : fma2(v, scale, to);
+                            const float2 e = make_float2(fast_exp2(a.x), fast_exp2(a.y));
+                            sum[(y >> 1) & 1] = add2(sum[(y >> 1) & 1], e);
+                            u[y / 2] = pack2<T>(e.x, e.y);
                         }
                         tmem_st32(s_col + w * 32, u);     // behind what has been read
                     }
-                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                     tmem_wait_st();
                 }
                 tc_fence_before();

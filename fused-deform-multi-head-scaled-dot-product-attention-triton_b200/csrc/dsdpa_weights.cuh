@@ -139,8 +139,9 @@ weights_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ Tr
         const uint32_t lanes = (uint32_t)quad << 21;
         ScoreConsts c;
         c.scale2 = fabsf(p.sm_scale) * kLog2e;
-        c.cap_in = CAP ? 2.0f * c.scale2 / p.cap : 0.0f;
+        c.cap_in = CAP ? 2.0f * fabsf(p.sm_scale) / p.cap : 0.0f;
         c.cap_out = CAP ? p.cap * kLog2e : 0.0f;
+        const float unit = CAP ? c.cap_out : c.scale2;
         int n = 0, m = 0;          // key tiles of the block, and of this side
         bool ok = true;
         TreeItem it;
@@ -170,10 +171,11 @@ weights_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ Tr
                         float s[16], part[4] = { 0.0f, 0.0f, 0.0f, 0.0f };
                         tmem_ld16(tmem + buffer * kTreeRows + x + lanes, s);
                         tmem_wait_ld();
+                        if (CAP) cap_scores(s, c);
 #pragma unroll
                         for (int y = 0; y < 16; ++y) {
                             const float lse = s_lse[buf][x + y];
-                            float v = CAP ? capped_score2(s[y], c) - lse : fmaf(s[y], c.scale2, -lse);
+                            float v = fmaf(s[y], unit, -lse);
                             if (BIAS) v = fmaf(-s_slope[buf][x + y], fabsf(s_pos[buf][x + y] - at), v);
                             s[y] = fast_exp2(v);
                         }
