@@ -78,7 +78,7 @@ tree_simt_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ 
             const int gr = it.row0 + r;
             return r < it.rows ? row_of<T>(p.q, p.sq, it.b, it.hk * p.group + gr % p.group, gr / p.group) : nullptr;
         });
-        float m[RM], l[RM], slope[RM], pos[RM];
+        float m[RM], l[RM], slope2[RM], pos[RM];
         unsigned long long above[RM];
         bool real[RM];
         float2 acc[RM][L::NJ][2] = {};
@@ -87,7 +87,7 @@ tree_simt_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ 
             const int in_tile = ty * RM + r, gr = it.row0 + in_tile, t = gr / p.group, h = it.hk * p.group + gr % p.group;
             real[r] = in_tile < it.rows && t < it.real;
             above[r] = real[r] ? tokens_above(p, it.b, t) : 0ull;
-            slope[r] = p.slopes && real[r] ? __ldg(p.slopes + h) : 0.0f;
+            slope2[r] = p.slopes && real[r] ? __ldg(p.slopes + h) * kLog2e : 0.0f;
             pos[r] = p.slopes && real[r] ? (float)(first_position(p, it.b, it.n) + depth_of(above[r])) : 0.0f;
             m[r] = kNegInf;
             l[r] = 0.0f;
@@ -111,24 +111,25 @@ tree_simt_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ 
             simt_gather<T, HD, kSimtKeys>(sv, p.D, p.v, rows_of(p.v, p.sv, k0, s_page[cur]));
             float s[RM][4];
             simt_dot<HD, RM>(sq, sk, s);
+            const float unit = simt_cap(s, p.sm_scale, p.cap);
 #pragma unroll
             for (int r = 0; r < RM; ++r) {
                 float top = kNegInf;
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     const int key = k0 + tx + 16 * c, draft = key - it.n;
-                    float x = soft_cap(p.sm_scale * s[r][c], p.cap);
-                    if (p.slopes) x -= slope[r] * fabsf(pos[r] - (float)s_at[cur][tx + 16 * c]);
+                    float x = s[r][c] * unit;
+                    if (p.slopes) x = fmaf(-slope2[r], fabsf(pos[r] - (float)s_at[cur][tx + 16 * c]), x);
                     const bool sees = real[r] && s_page[cur][tx + 16 * c] >= 0 && (draft < 0 || (above[r] >> (draft & 63) & 1u));
-                    s[r][c] = sees ? x * kLog2e : kNegInf;
+                    s[r][c] = sees ? x : kNegInf;
                     top = fmaxf(top, s[r][c]);
                 }
                 top = fmaxf(m[r], half_warp_max(top));
-                const float t0 = top == kNegInf ? 0.0f : top, f = exp2f(m[r] - t0);
+                const float t0 = top == kNegInf ? 0.0f : top, f = fast_exp2(m[r] - t0);
                 float sum = 0.0f;
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    const float w = exp2f(s[r][c] - t0);
+                    const float w = fast_exp2(s[r][c] - t0);
                     sw[(ty * RM + r) * L::W + tx + 16 * c] = w;
                     sum += w;
                 }
@@ -185,7 +186,7 @@ weights_simt_kernel(const __grid_constant__ CacheParams p, const __grid_constant
     TreeItem it;
     while (walk.next(p, sp, it)) {
         float* out = p.weights + ((long long)it.b * p.Hkv + it.hk) * p.slots;
-        float slope[RM], pos[RM], lse[RM];
+        float slope2[RM], pos[RM], lse[RM];
         unsigned long long above[RM];
         // the rows of a pass; a row that does not count has an infinite lse
         auto take_rows = [&](int pass) {
@@ -198,13 +199,13 @@ weights_simt_kernel(const __grid_constant__ CacheParams p, const __grid_constant
                 const int gr = pass * L::BM + ty * RM + r, t = gr / p.group, h = it.hk * p.group + gr % p.group;
                 lse[r] = -kNegInf;
                 above[r] = 0;
-                slope[r] = pos[r] = 0.0f;
+                slope2[r] = pos[r] = 0.0f;
                 if (gr < rows && t < it.real && !(p.take && !p.take[(long long)it.b * p.T + t])) {
                     const float x = p.lse[((long long)it.b * p.Hq + h) * p.T + t];
                     lse[r] = x == kNegInf ? -kNegInf : x;
                     above[r] = tokens_above(p, it.b, t);
                     if (p.slopes) {
-                        slope[r] = __ldg(p.slopes + h);
+                        slope2[r] = __ldg(p.slopes + h) * kLog2e;
                         pos[r] = (float)(first_position(p, it.b, it.n) + depth_of(above[r]));
                     }
                 }
@@ -229,15 +230,16 @@ weights_simt_kernel(const __grid_constant__ CacheParams p, const __grid_constant
                 __syncthreads();
                 float s[RM][4];
                 simt_dot<HD, RM>(sq, sk, s);
+                const float unit = simt_cap(s, p.sm_scale, p.cap);
 #pragma unroll
                 for (int r = 0; r < RM; ++r)
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
                         const int draft = k0 + tx + 16 * c - it.n;
-                        float x = soft_cap(p.sm_scale * s[r][c], p.cap);
-                        if (p.slopes) x -= slope[r] * fabsf(pos[r] - (float)s_at[tx + 16 * c]);
+                        float x = s[r][c] * unit;
+                        if (p.slopes) x = fmaf(-slope2[r], fabsf(pos[r] - (float)s_at[tx + 16 * c]), x);
                         const bool sees = lse[r] != -kNegInf && (draft < 0 || (above[r] >> (draft & 63) & 1u));
-                        sum[c] += sees ? exp2f(x * kLog2e - lse[r]) : 0.0f;
+                        sum[c] += sees ? fast_exp2(x - lse[r]) : 0.0f;
                     }
             }
 #pragma unroll

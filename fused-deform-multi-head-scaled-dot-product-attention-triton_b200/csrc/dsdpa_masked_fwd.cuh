@@ -35,33 +35,6 @@ struct ScoreConsts {
     float cap_in;       // 2 |sm_scale| / cap
     float cap_out;      // cap log2(e)
 };
-__device__ __forceinline__ float rcp_approx(float x) {
-    float y;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-// tanh(a / 2), the cap's argument being a = 2 x / cap.  For |a| < 2 (scores below the cap) an odd polynomial, fitted to
-// the least largest relative error (5e-8; evaluated in fp32 1.5e-7): ten fma-pipe operations for two values where
-// the general form, 1 - 2 / (1 + e^a), takes four of the special-function unit, which is what these kernels run
-// out of: the capped backward over 28x28 image tokens and text (D = 64) takes 245 us with that form alone.
-__device__ __forceinline__ float2 half_tanh_small(float2 a) {
-    constexpr float k[7] = { 4.999999702e-01f, -4.166604951e-02f, 4.164126236e-03f, -4.176330403e-04f, 3.962886694e-05f, -3.028993660e-06f, 1.270779535e-07f };
-    const float2 u = mul2(a, a);
-    float2 r = make_float2(k[6], k[6]);
-#pragma unroll
-    for (int i = 5; i >= 0; --i) r = fma2(r, u, make_float2(k[i], k[i]));
-    return mul2(r, a);
-}
-__device__ __forceinline__ float half_tanh(float a) { return fmaf(-2.0f, rcp_approx(1.0f + fast_exp2(a * kLog2e)), 1.0f); }
-// Whether all of a warp's values are below 2 in magnitude: their top exponent bit says so (for NaN too).
-template <int N>
-__device__ __forceinline__ bool all_small(const float (&a)[N]) {
-    unsigned any = 0;
-#pragma unroll
-    for (int i = 0; i < N; i += 2) any |= __float_as_uint(a[i]) | __float_as_uint(a[i + 1]);
-    return !__any_sync(0xffffffffu, any & 0x40000000u);
-}
 // Products q.k of one thread to tanh(x / cap); y = cap of it.
 template <int N>
 __device__ __forceinline__ void cap_scores(float (&s)[N], const ScoreConsts& c) {

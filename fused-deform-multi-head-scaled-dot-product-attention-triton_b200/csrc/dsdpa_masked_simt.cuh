@@ -162,6 +162,34 @@ __device__ __forceinline__ float simt_store(T* row, const float2 (&acc)[SimtShap
     }
     return nan;
 }
+// Products q.k to scores in base 2 without bias: s times the result.  With a cap s becomes tanh(x / cap), as a polynomial
+// where that is enough, by CUDA's tanhf where not (fp32 storage shows more than the short form's error).
+template <int RM>
+__device__ __forceinline__ float simt_cap(float (&s)[RM][4], float sm_scale, float cap) {
+    if (!(cap > 0.0f)) return sm_scale * kLog2e;
+    const float in = 2.0f * sm_scale / cap;
+    float a[4 * RM];
+#pragma unroll
+    for (int i = 0; i < 4 * RM; ++i) a[i] = s[i / 4][i % 4] * in;
+    if (all_small(a)) {
+#pragma unroll
+        for (int i = 0; i < 4 * RM; i += 2) {
+            const float2 t = half_tanh_small(make_float2(a[i], a[i + 1]));
+            s[i / 4][i % 4] = t.x;
+            s[i / 4][i % 4 + 1] = t.y;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4 * RM; ++i) s[i / 4][i % 4] = tanhf(0.5f * a[i]);
+    }
+    return cap * kLog2e;
+}
+// What simt_cap left to a weight, and dp to d(loss) / d(sm_scale q.k).
+__device__ __forceinline__ void simt_grad(float t, float unit, bool capped, float bias, float dp, float lse, float delta, float& w, float& ds) {
+    w = fast_exp2(fmaf(t, unit, -bias) - lse);
+    ds = w * (dp - delta);
+    if (capped) ds *= fmaf(-t, t, 1.0f);
+}
 __device__ __forceinline__ float half_warp_max(float x) {
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
@@ -216,7 +244,7 @@ masked_simt_fwd_kernel(const __grid_constant__ MaskedParams p, int qtiles) {
     __syncthreads();
     const int first = s_hi > 0 ? s_lo / kSimtKeys : 0, end = s_hi > 0 ? (s_hi + kSimtKeys - 1) / kSimtKeys : 0;
     const T *kb = row_of<T>(p.k, p.sk, b, hk, 0), *vb = row_of<T>(p.v, p.sv, b, hk, 0);
-    const float slope = p.slopes ? __ldg(p.slopes + h) : 0.0f;
+    const float slope2 = p.slopes ? __ldg(p.slopes + h) * kLog2e : 0.0f;
     float m[L::RM], l[L::RM];
     float2 acc[L::RM][L::NJ][2] = {};
 #pragma unroll
@@ -232,6 +260,7 @@ masked_simt_fwd_kernel(const __grid_constant__ MaskedParams p, int qtiles) {
         simt_load<T, HD, kSimtKeys>(sv, vb, p.sv[2], n0, p.Lk, p.D);
         float s[L::RM][4];
         simt_dot<HD>(sq, sk, s);
+        const float unit = simt_cap(s, p.sm_scale, p.cap);
 #pragma unroll
         for (int r = 0; r < L::RM; ++r) {
             const int pos = q0 + ty * L::RM + r + (p.Lk - p.Lq);
@@ -239,17 +268,17 @@ masked_simt_fwd_kernel(const __grid_constant__ MaskedParams p, int qtiles) {
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 const int key = n0 + tx + 16 * c;
-                float x = soft_cap(p.sm_scale * s[r][c], p.cap);
-                if (p.slopes) x -= slope * fabsf((float)(pos - key));
-                s[r][c] = key >= rg[r].x && key < rg[r].y ? x * kLog2e : kNegInf;
+                float x = s[r][c] * unit;
+                if (p.slopes) x = fmaf(-slope2, fabsf((float)(pos - key)), x);
+                s[r][c] = key >= rg[r].x && key < rg[r].y ? x : kNegInf;
                 top = fmaxf(top, s[r][c]);
             }
             top = fmaxf(m[r], half_warp_max(top));
-            const float t0 = top == kNegInf ? 0.0f : top, f = exp2f(m[r] - t0);
+            const float t0 = top == kNegInf ? 0.0f : top, f = fast_exp2(m[r] - t0);
             float sum = 0.0f;
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                const float w = exp2f(s[r][c] - t0);
+                const float w = fast_exp2(s[r][c] - t0);
                 sw[(ty * L::RM + r) * L::W + tx + 16 * c] = w;
                 sum += w;
             }
@@ -304,6 +333,7 @@ masked_simt_dq_kernel(const __grid_constant__ MaskedParams p, int qtiles) {
         else { lo = min(lo, rg[r].x); hi = max(hi, rg[r].y); }
         const bool sees = rg[r].x < rg[r].y;
         lse[r] = sees ? p.lse[(long long)bh * p.Lq + i] : kNegInf;
+        if (lse[r] == kNegInf) lse[r] = -kNegInf;                // weight exp2(s - inf) = 0
         // delta = out.dout, the row's 16 threads together
         float part = 0.0f;
         if (sees) {
@@ -324,7 +354,7 @@ masked_simt_dq_kernel(const __grid_constant__ MaskedParams p, int qtiles) {
     __syncthreads();
     const int first = s_hi > 0 ? s_lo / kSimtKeys : 0, end = s_hi > 0 ? (s_hi + kSimtKeys - 1) / kSimtKeys : 0;
     const T *kb = row_of<T>(p.k, p.sk, b, hk, 0), *vb = row_of<T>(p.v, p.sv, b, hk, 0);
-    const float slope = p.slopes ? __ldg(p.slopes + h) : 0.0f;
+    const float slope2 = p.slopes ? __ldg(p.slopes + h) * kLog2e : 0.0f;
     float2 acc[L::RM][L::NJ][2] = {};
     if (first < end) {
         simt_load<T, HD, L::BM>(sq, row_of<T>(p.q, p.sq, b, h, 0), p.sq[2], q0, p.Lq, p.D);
@@ -339,14 +369,16 @@ masked_simt_dq_kernel(const __grid_constant__ MaskedParams p, int qtiles) {
         float s[L::RM][4], dp[L::RM][4];
         simt_dot<HD>(sq, sk, s);
         simt_dot<HD>(sg, sv, dp);
+        const float unit = simt_cap(s, p.sm_scale, p.cap);
 #pragma unroll
         for (int r = 0; r < L::RM; ++r) {
             const int pos = q0 + ty * L::RM + r + (p.Lk - p.Lq);
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 const int key = n0 + tx + 16 * c;
-                float w = 0.0f, ds = 0.0f;
-                if (key >= rg[r].x && key < rg[r].y) pair_grad(p, s[r][c], dp[r][c], lse[r], delta[r], slope, pos - key, w, ds);
+                float w, ds;
+                simt_grad(s[r][c], unit, p.cap > 0.0f, p.slopes ? slope2 * fabsf((float)(pos - key)) : 0.0f, dp[r][c], lse[r], delta[r], w, ds);
+                if (!(key >= rg[r].x && key < rg[r].y)) ds = 0.0f;
                 sw[(ty * L::RM + r) * L::W + tx + 16 * c] = ds;
             }
         }
@@ -398,7 +430,7 @@ masked_simt_dkdv_kernel(const __grid_constant__ MaskedParams p) {
     float2 ak[4][L::NJ][2] = {}, av[4][L::NJ][2] = {};
     for (int g = 0; g < p.group; ++g) {
         const int h = hk * p.group + g;
-        const float slope = p.slopes ? __ldg(p.slopes + h) : 0.0f;
+        const float slope2 = p.slopes ? __ldg(p.slopes + h) * kLog2e : 0.0f;
         for (int t = first; t < end; ++t) {
             const int q0 = t * L::BM;
             simt_load<T, HD, L::BM>(sq, row_of<T>(p.q, p.sq, b, h, 0), p.sq[2], q0, p.Lq, p.D);
@@ -408,6 +440,7 @@ masked_simt_dkdv_kernel(const __grid_constant__ MaskedParams p) {
             float s[L::RM][4], dp[L::RM][4];
             simt_dot<HD>(sq, sk, s);
             simt_dot<HD>(sg, sv, dp);
+            const float unit = simt_cap(s, p.sm_scale, p.cap);
 #pragma unroll
             for (int r = 0; r < L::RM; ++r) {
                 const int i = q0 + ty * L::RM + r, pos = i + (p.Lk - p.Lq);
@@ -417,13 +450,15 @@ masked_simt_dkdv_kernel(const __grid_constant__ MaskedParams p) {
                     rg = key_range(p, b, i);
                     const long long row = ((long long)b * p.Hq + h) * p.Lq + i;
                     lse = p.lse[row];
+                    if (lse == kNegInf) lse = -kNegInf;
                     delta = p.delta[row];
                 }
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     const int key = k0 + tx + 16 * c;
-                    float w = 0.0f, ds = 0.0f;
-                    if (key >= rg.x && key < rg.y) pair_grad(p, s[r][c], dp[r][c], lse, delta, slope, pos - key, w, ds);
+                    float w, ds;
+                    simt_grad(s[r][c], unit, p.cap > 0.0f, p.slopes ? slope2 * fabsf((float)(pos - key)) : 0.0f, dp[r][c], lse, delta, w, ds);
+                    if (!(key >= rg.x && key < rg.y)) w = ds = 0.0f;
                     sw[(ty * L::RM + r) * L::W + tx + 16 * c] = w;
                     s[r][c] = ds;
                 }
