@@ -47,10 +47,10 @@ __device__ __forceinline__ float scale_down(unsigned e) {
 // The weights of two pairs from what cap_scores left (or the products); `slope` gets the factors that the cap's derivative
 // puts on ds: 1 - tanh^2.
 template <bool CAP, bool BIAS>
-__device__ __forceinline__ float2 pair_weights(float2 t, float unit, float slope2, float d0, float d1, float2 neg_lse, float2& slope) {
+__device__ __forceinline__ float2 pair_weights(float2 t, float unit, float slope2, float2 dist, float2 neg_lse, float2& slope) {
     float2 s = fma2(t, make_float2(unit, unit), neg_lse);
     if (CAP) slope = fma2(make_float2(-t.x, -t.y), t, make_float2(1.0f, 1.0f));
-    if (BIAS) s = make_float2(fmaf(-slope2, fabsf(d0), s.x), fmaf(-slope2, fabsf(d1), s.y));
+    if (BIAS) s = fma2(make_float2(-slope2, -slope2), make_float2(fabsf(dist.x), fabsf(dist.y)), s);
     return make_float2(fast_exp2(s.x), fast_exp2(s.y));
 }
 
@@ -251,7 +251,8 @@ masked_dq_kernel(const __grid_constant__ MaskedParams p, const __grid_constant__
             if (CAP) cap_scores(w, c);
 #pragma unroll
             for (int x = 0; x < 64; x += 2) {
-                float2 slope, v = pair_weights<CAP, BIAS>(make_float2(w[x], w[x + 1]), unit, slope2, d0 - (float)x, d0 - (float)(x + 1),
+                float2 slope, v = pair_weights<CAP, BIAS>(make_float2(w[x], w[x + 1]), unit, slope2,
+                                                          add2(make_float2(d0, d0), make_float2(-(float)x, -(float)(x + 1))),
                                                           make_float2(-lse, -lse), slope);
                 if (CAP) v = mul2(v, slope);
                 w[x] = v.x;
@@ -498,7 +499,8 @@ masked_dkdv_kernel(const __grid_constant__ MaskedParams p, const __grid_constant
 #pragma unroll
                         for (int z = 0; z < 4; z += 2) {
                             const int at = x + y + z;
-                            float2 slope, v = pair_weights<CAP, BIAS>(make_float2(w[at], w[at + 1]), unit, slope2, d0 + (float)at, d0 + (float)(at + 1),
+                            float2 slope, v = pair_weights<CAP, BIAS>(make_float2(w[at], w[at + 1]), unit, slope2,
+                                                                      add2(make_float2(d0, d0), make_float2((float)at, (float)(at + 1))),
                                                                       z ? make_float2(nl.z, nl.w) : make_float2(nl.x, nl.y), slope);
                             if (decltype(masked)::value) {
                                 const uint4 k = lds128(ranges + at * 8);

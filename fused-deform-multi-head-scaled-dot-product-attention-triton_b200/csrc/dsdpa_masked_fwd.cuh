@@ -57,6 +57,25 @@ __device__ __forceinline__ void cap_scores(float (&s)[N], const ScoreConsts& c) 
     }
 }
 
+// s unit - slope2 |d0 - x| for keys x = 0, 1, ...; `past`: none of them lies behind the query (the usual case, in which the
+// distance needs no magnitude and the bias is linear in x).
+template <int N>
+__device__ __forceinline__ void add_bias(float (&s)[N], float unit, float slope2, float d0, bool past) {
+    const float2 u = make_float2(unit, unit);
+    if (__all_sync(0xffffffffu, past)) {
+        const float2 k = make_float2(slope2, slope2), b = make_float2(-slope2 * d0, -slope2 * d0);
+#pragma unroll
+        for (int x = 0; x < N; x += 2) {
+            const float2 v = fma2(make_float2(s[x], s[x + 1]), u, fma2(k, make_float2((float)x, (float)(x + 1)), b));
+            s[x] = v.x;
+            s[x + 1] = v.y;
+        }
+    } else {
+#pragma unroll
+        for (int x = 0; x < N; ++x) s[x] = fmaf(-slope2, fabsf(d0 - (float)x), s[x] * unit);
+    }
+}
+
 __device__ __forceinline__ int warp_min(int x) { return __reduce_min_sync(0xffffffffu, x); }
 __device__ __forceinline__ int warp_max(int x) { return __reduce_max_sync(0xffffffffu, x); }
 
@@ -215,11 +234,7 @@ masked_fwd_kernel(const __grid_constant__ MaskedParams p, const __grid_constant_
             tmem_wait_ld();
             const int n0 = j * kTileK;
             if (CAP) cap_scores(s, c);
-            if (BIAS) {
-                const float d0 = (float)(pos - n0);
-#pragma unroll
-                for (int x = 0; x < kTileK; ++x) s[x] = fmaf(-slope2, fabsf(d0 - (float)x), s[x] * unit);
-            }
+            if (BIAS) add_bias(s, unit, slope2, (float)(pos - n0), pos - n0 >= kTileK - 1);
             if (lo_most > n0 || hi_least < n0 + kTileK) {
                 const int a = r.x - n0, e = r.y - n0;
 #pragma unroll

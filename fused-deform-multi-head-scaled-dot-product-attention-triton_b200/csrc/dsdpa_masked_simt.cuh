@@ -19,6 +19,7 @@ template <int HD, int ROWS = HD == 256 ? 2 : 4> struct SimtShape {
     static constexpr int NJ = HD >= 64 ? HD / 64 : 1;  // pieces of a row of sums that a thread has
     static constexpr int CW = HD >= 64 ? 4 : HD / 16;  // floats of a piece
     static constexpr int kSmemFwd = (BM * S + 2 * kSimtKeys * S + BM * W) * 4;
+    static constexpr int kBlocks = HD <= 64 ? 2 : 1;   // of an SM, by shared memory and by registers
     static constexpr int kSmemBwd = (2 * BM * S + 2 * kSimtKeys * S + BM * W) * 4;
 };
 
@@ -219,7 +220,7 @@ __device__ __forceinline__ void simt_redo(unsigned bad, F f) {
 }
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(kSimtThreads)
+__global__ void __launch_bounds__(kSimtThreads, SimtShape<HD>::kBlocks)
 masked_simt_fwd_kernel(const __grid_constant__ MaskedParams p, int qtiles) {
     using L = SimtShape<HD>;
     extern __shared__ float4 simt_smem[];
@@ -310,7 +311,7 @@ masked_simt_fwd_kernel(const __grid_constant__ MaskedParams p, int qtiles) {
 }
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(kSimtThreads)
+__global__ void __launch_bounds__(kSimtThreads, SimtShape<HD>::kBlocks)
 masked_simt_dq_kernel(const __grid_constant__ MaskedParams p, int qtiles) {
     using L = SimtShape<HD>;
     extern __shared__ float4 simt_smem[];
@@ -398,7 +399,7 @@ masked_simt_dq_kernel(const __grid_constant__ MaskedParams p, int qtiles) {
 }
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(kSimtThreads)
+__global__ void __launch_bounds__(kSimtThreads, SimtShape<HD>::kBlocks)
 masked_simt_dkdv_kernel(const __grid_constant__ MaskedParams p) {
     using L = SimtShape<HD>;
     extern __shared__ float4 simt_smem[];

@@ -259,8 +259,13 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
                         tmem_wait_ld();
                         if (CAP) cap_scores(s, c);
                         if (BIAS) {
+                            // cached keys at their own numbers lie before every query that starts behind them
+                            if (!p.positions && !p.start && k0 + kTreeKeys <= it.n) {
+                                add_bias(s, unit, slope2, pos - (float)(k0 + w * 64), true);
+                            } else {
 #pragma unroll
-                            for (int x = 0; x < 64; ++x) s[x] = fmaf(-slope2, fabsf(pos - s_at[slot_i][w * 64 + x]), s[x] * unit);
+                                for (int x = 0; x < 64; ++x) s[x] = fmaf(-slope2, fabsf(pos - s_at[slot_i][w * 64 + x]), s[x] * unit);
+                            }
                         }
                         if (!whole) {
                             const unsigned lo = w ? see[2] : see[0], hi = w ? see[3] : see[1];
