@@ -145,6 +145,9 @@ masked_fwd_kernel(const __grid_constant__ MaskedParams p, const __grid_constant_
     }
     const int jb = end[0] == 0 ? first[1] : end[1] == 0 ? first[0] : min(first[0], first[1]), je = max(end[0], end[1]);
     auto used = [&](int t, int j) { return j >= first[t] && j < end[t]; };
+    // With a bias the nearest keys, which lie last, come first: they have the large scores, and a row's reference point
+    // is found once instead of moving with every tile.
+    auto turn = [](int j, int from, int to) { return BIAS ? from + to - 1 - j : j; };
 
     if (warp >= 8) {
         regs_release<80>();
@@ -152,7 +155,8 @@ masked_fwd_kernel(const __grid_constant__ MaskedParams p, const __grid_constant_
             if (elect_one()) {
                 int st = 0, ph = 1;      // the ring starts empty
                 bool ok = true;
-                for (int j = jb; j < je && ok; ++j) {
+                for (int i = jb; i < je && ok; ++i) {
+                    const int j = turn(i, jb, je);
                     if (!used(0, j) && !used(1, j)) continue;
 #pragma unroll
                     for (int kv = 0; kv < 2; ++kv) {
@@ -171,10 +175,11 @@ masked_fwd_kernel(const __grid_constant__ MaskedParams p, const __grid_constant_
                 const uint32_t id_s = mma_desc<T>(kTileK, false, negate != 0), id_o = mma_desc<T>(HD, true);
                 bool ok = mbar_wait_bounded(bar_q, 0, p.err), pending[2] = { false, false }, begun[2] = { false, false };
                 int st = 0, ph = 0, vst = 0, pp[2] = { 0, 0 };
-                // j == je: the products that are still to be done
-                for (int j = jb; j <= je && ok; ++j) {
-                    const bool any = j < je && (used(0, j) || used(1, j));
-                    if (j < je && !any) continue;
+                // i == je: the products that are still to be done
+                for (int i = jb; i <= je && ok; ++i) {
+                    const int j = turn(i, jb, je);
+                    const bool any = i < je && (used(0, j) || used(1, j));
+                    if (i < je && !any) continue;
                     const bool had = pending[0] || pending[1];
                     int kst = 0;
                     if (had) {
@@ -225,14 +230,14 @@ masked_fwd_kernel(const __grid_constant__ MaskedParams p, const __grid_constant_
         float m = kNegInf, l = 0.0f;
         int n = 0;
         bool ok = true;
-        for (int j = first[tile]; j < end[tile]; ++j, ++n) {
+        for (int i = first[tile]; i < end[tile]; ++i, ++n) {
             if (!mbar_wait_bounded(bar_s + 8 * tile, n & 1, p.err)) { ok = false; break; }
             tc_fence_after();
             float s[kTileK];
 #pragma unroll
             for (int x = 0; x < kTileK; x += 32) tmem_ld32(s_at + x, s + x);
             tmem_wait_ld();
-            const int n0 = j * kTileK;
+            const int n0 = turn(i, first[tile], end[tile]) * kTileK;
             if (CAP) cap_scores(s, c);
             if (BIAS) add_bias(s, unit, slope2, (float)(pos - n0), pos - n0 >= kTileK - 1);
             if (lo_most > n0 || hi_least < n0 + kTileK) {

@@ -16,7 +16,9 @@
 
 namespace dsdpa {
 
-constexpr int kTreeThreads = 416;
+constexpr int kTreeThreads = 512;              // warps 13-15 idle: registers are split by groups of four warps
+// The launch gives 128 registers a thread; a softmax thread holds 64 scores twice, the warpgroup with the matrix
+// instructions hardly any: 256 x 176 + 128 x 96 + 128 x 64 = 65536.
 constexpr int kTreeRows = 128, kTreeKeys = 128, kInfo = 16;
 using TreeTile = ShareTile<kTreeRows, kTreeKeys>;
 
@@ -85,9 +87,13 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(slot));
     TreeWalk<TreeTile> walk = share.walk<TreeTile>();
 
+    // With a bias the nearest keys, which lie last, come first: they have the large scores, and a row's reference point is
+    // found once instead of moving with every tile.
+    auto first_key = [](const TreeItem& it, int i) { return it.key0 + (BIAS ? it.tiles - 1 - i : i) * kTreeKeys; };
     // Ring entries of an item with n tiles, in the order in which the products take them:
     // K0 K1 V0 K2 V1 .. K(n-1) V(n-2) V(n-1); the query tile comes with K0.
     if (warp >= 12) {
+        regs_release<64>();
         if (warp == 12 && elect_one()) {
             const uint32_t id_s = mma_desc<T>(kTreeKeys, false, negate != 0), id_o = mma_desc<T>(HD, true);
             int st = 0, ph = 0, pp[2] = { 0, 0 }, item = 0;
@@ -126,6 +132,7 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
             }
         }
     } else if (warp >= 8) {
+        regs_release<96>();
         const int w = warp - 8;
         int st = 0, ph = 1, item = 0, entries = 0, handed = 0, info = 0;
         bool ok = true;
@@ -145,7 +152,7 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
             } while (it.tiles == 0);
         };
         auto lookup = [&](const TreeItem& it, int i) {          // not looked at yet: nothing waits for it here
-            const int j = it.key0 + i * kTreeKeys + w * 32 + lane;
+            const int j = first_key(it, i) + w * 32 + lane;
             return i < it.tiles && j < it.n + it.real ? table_entry(p.table, p.width, it.b, page_index(p.div, j)) : 0;
         };
         TreeItem it;
@@ -156,7 +163,7 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
             next_item(then);
             const int after[3] = { lookup(then, 0), lookup(then, 1), lookup(then, 2) };
             auto entry = [&](int i, bool is_v, int pg) {
-                const int j = it.key0 + i * kTreeKeys + w * 32 + lane, key = j - page_index(p.div, j) * p.page_size;
+                const int j = first_key(it, i) + w * 32 + lane, key = j - page_index(p.div, j) * p.page_size;
                 const char* src = nullptr;
                 if (j < it.n + it.real && (pg = checked_page(pg, p.pages, p.err)) >= 0)
                     src = is_v ? (const char*)(row_of<T>(p.v, p.sv, 0, it.hk, key) + pg * p.sv[0])
@@ -215,6 +222,7 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
         cp_async_wait<0>();
         if (ok) hand_over(entries);
     } else {
+        regs_claim<176>();
         const int tile = warp >> 2, quad = warp & 3, in_tile = quad * 32 + lane;
         const uint32_t lanes = (uint32_t)quad << 21, s_col = tmem + tile * kTreeKeys + lanes, o_col = tmem + 256 + tile * HD + lanes;
         ScoreConsts c;
@@ -239,7 +247,7 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
                 tc_fence_after();
                 if (busy) {
                     // 64 columns at a time, twice (for the maximum, for the weights): few registers, little code
-                    const int slot_i = (info + i) % kInfo, k0 = it.key0 + i * kTreeKeys;
+                    const int slot_i = (info + i) % kInfo, k0 = first_key(it, i);
                     unsigned see[4], all = ~0u;
 #pragma unroll
                     for (int w = 0; w < 4; ++w) {
@@ -250,10 +258,9 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
                         all &= see[w];
                     }
                     const bool whole = __all_sync(0xffffffffu, all == ~0u);
-                    float top = kNegInf;
+                    float top = kNegInf, s[64];
 #pragma unroll 1
-                    for (int w = 0; w < 2; ++w) {
-                        float s[64];
+                    for (int w = 1; w >= 0; --w) {
                         tmem_ld32(s_col + w * 64, s);
                         tmem_ld32(s_col + w * 64 + 32, s + 32);
                         tmem_wait_ld();
@@ -272,7 +279,7 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
 #pragma unroll
                             for (int x = 0; x < 64; ++x) s[x] = (x < 32 ? lo : hi) >> (x & 31) & 1u ? s[x] : kNegInf;
                         }
-                        if (CAP || BIAS || !whole) {
+                        if (w && (CAP || BIAS || !whole)) {
                             tmem_st32(s_col + w * 64, reinterpret_cast<const uint32_t*>(s));
                             tmem_st32(s_col + w * 64 + 32, reinterpret_cast<const uint32_t*>(s + 32));
                         }
@@ -309,11 +316,12 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
                     const float2 scale = make_float2(unit, unit), to = make_float2(-m0, -m0);
 #pragma unroll 1
                     for (int w = 0; w < 2; ++w) {
-                        float s[64];
                         uint32_t u[32];
-                        tmem_ld32(s_col + w * 64, s);
-                        tmem_ld32(s_col + w * 64 + 32, s + 32);
-                        tmem_wait_ld();
+                        if (w) {
+                            tmem_ld32(s_col + 64, s);
+                            tmem_ld32(s_col + 96, s + 32);
+                            tmem_wait_ld();
+                        }
 #pragma unroll
                         for (int y = 0; y < 64; y += 2) {
                             const float2 v = make_float2(s[y], s[y + 1]), a = BIAS ? add2(v, to) : fma2(v, scale, to);
