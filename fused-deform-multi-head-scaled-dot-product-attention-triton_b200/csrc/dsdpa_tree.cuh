@@ -16,9 +16,7 @@
 
 namespace dsdpa {
 
-constexpr int kTreeThreads = 512;              // warps 13-15 idle: registers are split by groups of four warps
-// The launch gives 128 registers a thread; a softmax thread holds 64 scores twice, the warpgroup with the matrix
-// instructions hardly any: 256 x 176 + 128 x 96 + 128 x 64 = 65536.
+constexpr int kTreeThreads = 416;
 constexpr int kTreeRows = 128, kTreeKeys = 128, kInfo = 16;
 using TreeTile = ShareTile<kTreeRows, kTreeKeys>;
 
@@ -93,7 +91,6 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
     // Ring entries of an item with n tiles, in the order in which the products take them:
     // K0 K1 V0 K2 V1 .. K(n-1) V(n-2) V(n-1); the query tile comes with K0.
     if (warp >= 12) {
-        regs_release<64>();
         if (warp == 12 && elect_one()) {
             const uint32_t id_s = mma_desc<T>(kTreeKeys, false, negate != 0), id_o = mma_desc<T>(HD, true);
             int st = 0, ph = 0, pp[2] = { 0, 0 }, item = 0;
@@ -132,7 +129,6 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
             }
         }
     } else if (warp >= 8) {
-        regs_release<96>();
         const int w = warp - 8;
         int st = 0, ph = 1, item = 0, entries = 0, handed = 0, info = 0;
         bool ok = true;
@@ -222,7 +218,6 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
         cp_async_wait<0>();
         if (ok) hand_over(entries);
     } else {
-        regs_claim<176>();
         const int tile = warp >> 2, quad = warp & 3, in_tile = quad * 32 + lane;
         const uint32_t lanes = (uint32_t)quad << 21, s_col = tmem + tile * kTreeKeys + lanes, o_col = tmem + 256 + tile * HD + lanes;
         ScoreConsts c;
@@ -246,51 +241,44 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
                 if (!mbar_wait_bounded(bar_s + 8 * tile, (done + mine) & 1, p.err)) { ok = false; break; }
                 tc_fence_after();
                 if (busy) {
-                    // 64 columns at a time, twice (for the maximum, for the weights): few registers, little code
+                    // 32 columns at a time, twice (for the maximum, for the weights): the code stays small, and with it the
+                    // time that the two streams' warps wait for instructions
                     const int slot_i = (info + i) % kInfo, k0 = first_key(it, i);
-                    unsigned see[4], all = ~0u;
-#pragma unroll
+                    const bool linear = BIAS && !p.positions && !p.start && k0 + kTreeKeys <= it.n;
+                    float top = kNegInf;
+#pragma unroll 1
                     for (int w = 0; w < 4; ++w) {
-                        const int left = it.n - (k0 + w * 32);       // cached keys from this word on
+                        float s[32];
+                        tmem_ld32(s_col + w * 32, s);
+                        const int left = it.n - (k0 + w * 32);       // cached keys from this column on
                         const unsigned cached = left >= 32 ? ~0u : left > 0 ? (1u << left) - 1 : 0u;
                         const unsigned tree = left >= 32 ? 0u : left > 0 ? (unsigned)(above << left) : left > -64 ? (unsigned)(above >> -left) : 0u;
-                        see[w] = real ? (cached | tree) & s_valid[slot_i][w] : 0u;
-                        all &= see[w];
-                    }
-                    const bool whole = __all_sync(0xffffffffu, all == ~0u);
-                    float top = kNegInf, s[64];
-#pragma unroll 1
-                    for (int w = 1; w >= 0; --w) {
-                        tmem_ld32(s_col + w * 64, s);
-                        tmem_ld32(s_col + w * 64 + 32, s + 32);
+                        const unsigned see = real ? (cached | tree) & s_valid[slot_i][w] : 0u;
+                        const bool whole = __all_sync(0xffffffffu, see == ~0u);
                         tmem_wait_ld();
                         if (CAP) cap_scores(s, c);
                         if (BIAS) {
                             // cached keys at their own numbers lie before every query that starts behind them
-                            if (!p.positions && !p.start && k0 + kTreeKeys <= it.n) {
-                                add_bias(s, unit, slope2, pos - (float)(k0 + w * 64), true);
+                            if (linear) {
+                                add_bias(s, unit, slope2, pos - (float)(k0 + w * 32), true);
                             } else {
 #pragma unroll
-                                for (int x = 0; x < 64; ++x) s[x] = fmaf(-slope2, fabsf(pos - s_at[slot_i][w * 64 + x]), s[x] * unit);
+                                for (int x = 0; x < 32; ++x) s[x] = fmaf(-slope2, fabsf(pos - s_at[slot_i][w * 32 + x]), s[x] * unit);
                             }
                         }
                         if (!whole) {
-                            const unsigned lo = w ? see[2] : see[0], hi = w ? see[3] : see[1];
 #pragma unroll
-                            for (int x = 0; x < 64; ++x) s[x] = (x < 32 ? lo : hi) >> (x & 31) & 1u ? s[x] : kNegInf;
+                            for (int x = 0; x < 32; ++x) s[x] = see >> x & 1u ? s[x] : kNegInf;
                         }
-                        if (w && (CAP || BIAS || !whole)) {
-                            tmem_st32(s_col + w * 64, reinterpret_cast<const uint32_t*>(s));
-                            tmem_st32(s_col + w * 64 + 32, reinterpret_cast<const uint32_t*>(s + 32));
-                        }
-                        float mx[8];
+                        if (CAP || BIAS || !whole) tmem_st32(s_col + w * 32, reinterpret_cast<const uint32_t*>(s));
+                        float mx[4];
 #pragma unroll
-                        for (int x = 0; x < 8; ++x) mx[x] = s[x];
+                        for (int x = 0; x < 4; ++x) mx[x] = s[x];
 #pragma unroll
-                        for (int x = 8; x < 64; ++x) mx[x & 7] = fmaxf(mx[x & 7], s[x]);
-                        top = fmaxf(top, fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7]))));
+                        for (int x = 4; x < 32; ++x) mx[x & 3] = fmaxf(mx[x & 3], s[x]);
+                        top = fmaxf(top, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
                     }
-                    if (CAP || BIAS || !whole) tmem_wait_st();
+                    tmem_wait_st();
                     if (!BIAS) top *= unit;
                     const bool move = top > m + 8.0f || (m == kNegInf && top > kNegInf);
                     if (__any_sync(0xffffffffu, move)) {
@@ -315,21 +303,19 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
                     float2 sum[2] = { make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f) };
                     const float2 scale = make_float2(unit, unit), to = make_float2(-m0, -m0);
 #pragma unroll 1
-                    for (int w = 0; w < 2; ++w) {
-                        uint32_t u[32];
-                        if (w) {
-                            tmem_ld32(s_col + 64, s);
-                            tmem_ld32(s_col + 96, s + 32);
-                            tmem_wait_ld();
-                        }
+                    for (int w = 0; w < 4; ++w) {
+                        float s[32];
+                        uint32_t u[16];
+                        tmem_ld32(s_col + w * 32, s);
+                        tmem_wait_ld();
 #pragma unroll
-                        for (int y = 0; y < 64; y += 2) {
+                        for (int y = 0; y < 32; y += 2) {
                             const float2 v = make_float2(s[y], s[y + 1]), a = BIAS ? add2(v, to) : fma2(v, scale, to);
                             const float2 e = make_float2(fast_exp2(a.x), fast_exp2(a.y));
                             sum[(y >> 1) & 1] = add2(sum[(y >> 1) & 1], e);
                             u[y / 2] = pack2<T>(e.x, e.y);
                         }
-                        tmem_st32(s_col + w * 32, u);     // behind what has been read
+                        tmem_st16(s_col + w * 16, u);     // behind what has been read
                     }
                     l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                     tmem_wait_st();

@@ -12,10 +12,8 @@
 
 namespace dsdpa {
 
-constexpr int kWeightsThreads = 416;
-
 template <typename T, int HD, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(kWeightsThreads, 1)
+__global__ void __launch_bounds__(kTreeThreads, 1)
 weights_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeSplit sp, int negate) {
     using L = TreeLayout<HD>;
     extern __shared__ char smem_raw[];
@@ -27,7 +25,7 @@ weights_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ Tr
     __shared__ unsigned s_valid[kInfo][4];
     __shared__ float s_lse[2][kTreeRows], s_pos[2][BIAS ? kTreeRows : 1], s_slope[2][BIAS ? kTreeRows : 1];
     __shared__ unsigned long long s_above[2][kTreeRows];
-    __shared__ TreeShare<kWeightsThreads> share;
+    __shared__ TreeShare<kTreeThreads> share;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rows = p.T * p.group, passes = (rows + kTreeRows - 1) / kTreeRows;
 
