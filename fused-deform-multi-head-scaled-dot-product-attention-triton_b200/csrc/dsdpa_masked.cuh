@@ -121,12 +121,16 @@ __device__ __forceinline__ float rcp_approx(float x) {
 // the least largest relative error (5e-8; evaluated in fp32 1.5e-7): ten fma-pipe operations for two values where
 // the general form, 1 - 2 / (1 + e^a), takes four of the special-function unit, which is what these kernels run
 // out of: the capped backward over 28x28 image tokens and text (D = 64) takes 245 us with that form alone.
+constexpr int kTanhTerms = 7;
+__device__ __forceinline__ float tanh_term(int i) {
+    constexpr float k[kTanhTerms] = { 4.999999702e-01f, -4.166604951e-02f, 4.164126236e-03f, -4.176330403e-04f, 3.962886694e-05f, -3.028993660e-06f, 1.270779535e-07f };
+    return k[i];
+}
 __device__ __forceinline__ float2 half_tanh_small(float2 a) {
-    constexpr float k[7] = { 4.999999702e-01f, -4.166604951e-02f, 4.164126236e-03f, -4.176330403e-04f, 3.962886694e-05f, -3.028993660e-06f, 1.270779535e-07f };
     const float2 u = mul2(a, a);
-    float2 r = make_float2(k[6], k[6]);
+    float2 r = make_float2(tanh_term(kTanhTerms - 1), tanh_term(kTanhTerms - 1));
 #pragma unroll
-    for (int i = 5; i >= 0; --i) r = fma2(r, u, make_float2(k[i], k[i]));
+    for (int i = kTanhTerms - 2; i >= 0; --i) r = fma2(r, u, make_float2(tanh_term(i), tanh_term(i)));
     return mul2(r, a);
 }
 __device__ __forceinline__ float half_tanh(float a) { return fmaf(-2.0f, rcp_approx(1.0f + fast_exp2(a * kLog2e)), 1.0f); }

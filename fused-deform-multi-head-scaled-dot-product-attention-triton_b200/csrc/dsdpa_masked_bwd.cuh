@@ -44,7 +44,14 @@ __device__ __forceinline__ float scale_down(unsigned e) {
     return e == 0 || e >= 254 ? 1.0f : __uint_as_float((unsigned)(254 - e) << 23);
 }
 
-// The weights of two pairs from what cap_scores left (or the products); `slope` gets the factors that the cap's derivative
+// Two products that scale_scores has been at to tanh(x / cap); as they are where there is no cap.  Done pair by pair with what
+// follows, so that the fma pipes and the special-function unit work at the same time.
+template <bool CAP, bool SMALL>
+__device__ __forceinline__ float2 capped_pair(float2 a) {
+    if (!CAP) return a;
+    return SMALL ? half_tanh_small(a) : make_float2(half_tanh(a.x), half_tanh(a.y));
+}
+// The weights of two pairs from what capped_pair left; `slope` gets the factors that the cap's derivative
 // puts on ds: 1 - tanh^2.
 template <bool CAP, bool BIAS>
 __device__ __forceinline__ float2 pair_weights(float2 t, float unit, float slope2, float2 dist, float2 neg_lse, float2& slope) {
@@ -248,16 +255,19 @@ masked_dq_kernel(const __grid_constant__ MaskedParams p, const __grid_constant__
             const float d0 = (float)(pos - n0);
             const bool partial = lo_most > n0 || hi_least < n0 + 64;
             const int a = r.x - n0, e = r.y - n0;
-            if (CAP) cap_scores(w, c);
+            auto weights = [&](auto small) {
 #pragma unroll
-            for (int x = 0; x < 64; x += 2) {
-                float2 slope, v = pair_weights<CAP, BIAS>(make_float2(w[x], w[x + 1]), unit, slope2,
-                                                          add2(make_float2(d0, d0), make_float2(-(float)x, -(float)(x + 1))),
-                                                          make_float2(-lse, -lse), slope);
-                if (CAP) v = mul2(v, slope);
-                w[x] = v.x;
-                w[x + 1] = v.y;
-            }
+                for (int x = 0; x < 64; x += 2) {
+                    const float2 y = capped_pair<CAP, decltype(small)::value>(make_float2(w[x], w[x + 1]));
+                    float2 slope, v = pair_weights<CAP, BIAS>(y, unit, slope2, add2(make_float2(d0, d0), make_float2(-(float)x, -(float)(x + 1))),
+                                                              make_float2(-lse, -lse), slope);
+                    if (CAP) v = mul2(v, slope);
+                    w[x] = v.x;
+                    w[x + 1] = v.y;
+                }
+            };
+            if (!CAP || scale_scores(w, c)) weights(Yes{});
+            else weights(No{});
             if (partial) {
 #pragma unroll
                 for (int x = 0; x < 64; ++x) w[x] = x >= a && x < e ? w[x] : 0.0f;
@@ -488,8 +498,8 @@ masked_dkdv_kernel(const __grid_constant__ MaskedParams p, const __grid_constant
             tmem_ld32(s_at, w);
             tmem_ld32(s_at + 32, w + 32);
             tmem_wait_ld();
-            if (CAP) cap_scores(w, c);
-            auto weights = [&](auto masked) {
+            const bool small = !CAP || scale_scores(w, c);
+            auto weights = [&](auto masked, auto is_small) {
 #pragma unroll
                 for (int x = 0; x < 64; x += 32) {
                     uint32_t o[16];
@@ -499,8 +509,8 @@ masked_dkdv_kernel(const __grid_constant__ MaskedParams p, const __grid_constant
 #pragma unroll
                         for (int z = 0; z < 4; z += 2) {
                             const int at = x + y + z;
-                            float2 slope, v = pair_weights<CAP, BIAS>(make_float2(w[at], w[at + 1]), unit, slope2,
-                                                                      add2(make_float2(d0, d0), make_float2((float)at, (float)(at + 1))),
+                            const float2 t = capped_pair<CAP, decltype(is_small)::value>(make_float2(w[at], w[at + 1]));
+                            float2 slope, v = pair_weights<CAP, BIAS>(t, unit, slope2, add2(make_float2(d0, d0), make_float2((float)at, (float)(at + 1))),
                                                                       z ? make_float2(nl.z, nl.w) : make_float2(nl.x, nl.y), slope);
                             if (decltype(masked)::value) {
                                 const uint4 k = lds128(ranges + at * 8);
@@ -516,8 +526,9 @@ masked_dkdv_kernel(const __grid_constant__ MaskedParams p, const __grid_constant
                     tmem_st16(s_at + x / 2, o);
                 }
             };
-            if (partial) weights(Yes{});
-            else weights(No{});
+            if (!small) weights(Yes{}, No{});
+            else if (partial) weights(Yes{}, Yes{});
+            else weights(No{}, Yes{});
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();

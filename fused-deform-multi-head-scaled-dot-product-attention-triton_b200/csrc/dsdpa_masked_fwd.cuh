@@ -35,16 +35,21 @@ struct ScoreConsts {
     float cap_in;       // 2 |sm_scale| / cap
     float cap_out;      // cap log2(e)
 };
-// Products q.k of one thread to tanh(x / cap); y = cap of it.
+// Products q.k of one thread to 2 x / cap; whether all of the warp's are in half_tanh_small's range.
 template <int N>
-__device__ __forceinline__ void cap_scores(float (&s)[N], const ScoreConsts& c) {
+__device__ __forceinline__ bool scale_scores(float (&s)[N], const ScoreConsts& c) {
 #pragma unroll
     for (int i = 0; i < N; i += 2) {
         const float2 a = mul2(make_float2(s[i], s[i + 1]), make_float2(c.cap_in, c.cap_in));
         s[i] = a.x;
         s[i + 1] = a.y;
     }
-    if (all_small(s)) {
+    return all_small(s);
+}
+// Products q.k of one thread to tanh(x / cap); y = cap of it.
+template <int N>
+__device__ __forceinline__ void cap_scores(float (&s)[N], const ScoreConsts& c) {
+    if (scale_scores(s, c)) {
 #pragma unroll
         for (int i = 0; i < N; i += 2) {
             const float2 t = half_tanh_small(make_float2(s[i], s[i + 1]));
@@ -227,6 +232,10 @@ masked_fwd_kernel(const __grid_constant__ MaskedParams p, const __grid_constant_
         const float unit = CAP ? c.cap_out : c.scale2;            // of what cap_scores, or the product, left: scores in base 2
         const float slope2 = BIAS ? __ldg(p.slopes + h) * kLog2e : 0.0f;
         const int pos = row + (p.Lk - p.Lq);
+        constexpr bool kLate = CAP && !BIAS;
+        float cap_term[kTanhTerms];
+#pragma unroll
+        for (int i = 0; i < kTanhTerms; ++i) cap_term[i] = kLate ? tanh_term(i) * c.cap_out : 0.0f;
         float m = kNegInf, l = 0.0f;
         int n = 0;
         bool ok = true;
@@ -238,18 +247,38 @@ masked_fwd_kernel(const __grid_constant__ MaskedParams p, const __grid_constant_
             for (int x = 0; x < kTileK; x += 32) tmem_ld32(s_at + x, s + x);
             tmem_wait_ld();
             const int n0 = turn(i, first[tile], end[tile]) * kTileK;
-            if (CAP) cap_scores(s, c);
-            if (BIAS) add_bias(s, unit, slope2, (float)(pos - n0), pos - n0 >= kTileK - 1);
-            if (lo_most > n0 || hi_least < n0 + kTileK) {
-                const int a = r.x - n0, e = r.y - n0;
+            const int a = r.x - n0, e = r.y - n0;
+            const bool partial = lo_most > n0 || hi_least < n0 + kTileK;
+            float top;
+            bool small = false;
+            auto largest = [&]() {
+                float mx[4] = { s[0], s[1], s[2], s[3] };
 #pragma unroll
-                for (int x = 0; x < kTileK; ++x) s[x] = x >= a && x < e ? s[x] : kNegInf;
+                for (int x = 4; x < kTileK; ++x) mx[x & 3] = fmaxf(mx[x & 3], s[x]);
+                return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+            };
+            if (kLate) {
+                // the cap keeps the order: the largest score is the largest product's, and the cap itself is done together with
+                // exp2, so that the fma pipes and the special-function unit work at the same time
+                small = scale_scores(s, c);
+                if (partial) {
+                    top = kNegInf;
+#pragma unroll
+                    for (int x = 0; x < kTileK; ++x) top = fmaxf(top, x >= a && x < e ? s[x] : kNegInf);
+                    if (max(a, 0) < min(e, kTileK)) top = half_tanh(top) * unit;
+                } else {
+                    top = half_tanh(largest()) * unit;
+                }
+            } else {
+                if (CAP) cap_scores(s, c);
+                if (BIAS) add_bias(s, unit, slope2, (float)(pos - n0), pos - n0 >= kTileK - 1);
+                if (partial) {
+#pragma unroll
+                    for (int x = 0; x < kTileK; ++x) s[x] = x >= a && x < e ? s[x] : kNegInf;
+                }
+                top = largest();
+                if (!BIAS) top *= unit;                           // not negative: the order stays
             }
-            float mx[4] = { s[0], s[1], s[2], s[3] };
-#pragma unroll
-            for (int x = 4; x < kTileK; ++x) mx[x & 3] = fmaxf(mx[x & 3], s[x]);
-            float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-            if (!BIAS) top *= unit;                               // not negative: the order stays
             // the reference point moves when a row's maximum is more than 8 above it (or it has none yet)
             const bool move = top > m + 8.0f || (m == kNegInf && top > kNegInf);
             if (__any_sync(0xffffffffu, move)) {
@@ -273,17 +302,38 @@ masked_fwd_kernel(const __grid_constant__ MaskedParams p, const __grid_constant_
             const float m0 = m == kNegInf ? 0.0f : m;
             float2 sum[2] = { make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f) };
             const float2 scale = make_float2(unit, unit), to = make_float2(-m0, -m0);
+            // weights from what `score` says of two columns, less the reference point
+            auto weigh = [&](auto score) {
 #pragma unroll
-            for (int x = 0; x < kTileK; x += 32) {
-                uint32_t w[16];
+                for (int x = 0; x < kTileK; x += 32) {
+                    uint32_t w[16];
 #pragma unroll
-                for (int y = 0; y < 32; y += 2) {
-                    const float2 v = make_float2(s[x + y], s[x + y + 1]), a = BIAS ? add2(v, to) : fma2(v, scale, to);
-                    const float2 e = make_float2(weight_exp2(a.x), weight_exp2(a.y));
-                    sum[(y >> 1) & 1] = add2(sum[(y >> 1) & 1], e);
-                    w[y / 2] = pack2<T>(e.x, e.y);
+                    for (int y = 0; y < 32; y += 2) {
+                        const float2 v = score(x + y), e = make_float2(weight_exp2(v.x), weight_exp2(v.y));
+                        sum[(y >> 1) & 1] = add2(sum[(y >> 1) & 1], e);
+                        w[y / 2] = pack2<T>(e.x, e.y);
+                    }
+                    tmem_st16(s_at + x / 2, w);
                 }
-                tmem_st16(s_at + x / 2, w);
+            };
+            if constexpr (kLate) {
+                auto seen = [&](int x, float2 v) { return make_float2(x >= a && x < e ? v.x : kNegInf, x + 1 >= a && x + 1 < e ? v.y : kNegInf); };
+                auto capped = [&](int x) {
+                    const float2 v = make_float2(s[x], s[x + 1]), u = mul2(v, v);
+                    float2 t = make_float2(cap_term[kTanhTerms - 1], cap_term[kTanhTerms - 1]);
+#pragma unroll
+                    for (int i = kTanhTerms - 2; i >= 0; --i) t = fma2(t, u, make_float2(cap_term[i], cap_term[i]));
+                    return fma2(t, v, to);
+                };
+                if (!small)
+                    weigh([&](int x) { return seen(x, fma2(make_float2(half_tanh(s[x]), half_tanh(s[x + 1])), scale, to)); });
+                else if (partial) weigh([&](int x) { return seen(x, capped(x)); });
+                else weigh(capped);
+            } else {
+                weigh([&](int x) {
+                    const float2 v = make_float2(s[x], s[x + 1]);
+                    return BIAS ? add2(v, to) : fma2(v, scale, to);
+                });
             }
             l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
             tmem_wait_st();
