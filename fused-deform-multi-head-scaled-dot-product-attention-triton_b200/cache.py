@@ -87,8 +87,8 @@ def _tokens(q, k_pages, page_table, sm_scale, softcap, parents, drafted, slopes,
     _check_int(start, (B,), dev, "start", name)
     if positions is not None:
         slots = page_table.shape[1] * k_pages.shape[2]
-        _check_int(positions, (B, Hkv, positions.shape[-1]), dev, "positions", name)
-        if positions.shape[2] < slots:
+        _check_int(positions, (B, Hkv, *positions.shape[2:3]), dev, "positions", name)
+        if positions.dim() != 3 or positions.shape[2] < slots:
             raise ValueError(f"{name}: positions must be int32 [B, kv_heads, {slots} or more]")
     held = [None if t is None else t.contiguous() for t in (parents, drafted, positions, start, slopes)]
     return struct.pack("=5Q", *(0 if t is None else t.data_ptr() for t in held)), held
@@ -186,8 +186,8 @@ def cache_evict(k_pages, v_pages, page_table, lens, weights, keep, *, sinks=0, r
         positions = positions.contiguous()
     B, Hkv = page_table.shape[0], k_pages.shape[1]
     if out_table is not None:
-        _check_int(out_table, (B, out_table.shape[-1]), dev, "out_table", name)
-        if out_table.shape[1] * k_pages.shape[2] < min(keep, page_table.shape[1] * k_pages.shape[2]):
+        _check_int(out_table, (B, *out_table.shape[1:2]), dev, "out_table", name)
+        if out_table.dim() != 2 or out_table.shape[1] * k_pages.shape[2] < min(keep, page_table.shape[1] * k_pages.shape[2]):
             raise ValueError(f"{name}: out_table has no room for {keep} keys")
     page_table, lens = page_table.contiguous(), lens.contiguous()
     out_table = page_table if out_table is None else out_table.contiguous()

@@ -2,6 +2,8 @@
 #include <cudaTypedefs.h>
 #include <math.h>
 
+#include <atomic>
+
 #include "dsdpa_host.h"
 #include "dsdpa_masked.cuh"
 #include "dsdpa_masked_launch.h"
@@ -10,7 +12,8 @@ namespace dsdpa {
 
 cudaError_t tensor_map_16(CUtensorMap* map, int dtype, const void* base, int D, int rows, int L, int H, int B, const long long (&stride)[3]) {
     // a driver call, reached through the runtime: the library links no driver library
-    static PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
+    static std::atomic<PFN_cuTensorMapEncodeTiled_v12000> known{ nullptr };
+    PFN_cuTensorMapEncodeTiled_v12000 encode = known.load(std::memory_order_relaxed);
     if (!encode) {
         void* fn = nullptr;
         cudaDriverEntryPointQueryResult found;
@@ -18,6 +21,7 @@ cudaError_t tensor_map_16(CUtensorMap* map, int dtype, const void* base, int D, 
         if (e != cudaSuccess) return e;
         if (!fn || found != cudaDriverEntryPointSuccess) return cudaErrorNotSupported;
         encode = (PFN_cuTensorMapEncodeTiled_v12000)fn;
+        known.store(encode, std::memory_order_relaxed);
     }
     const cuuint64_t dims[4] = { (cuuint64_t)D, (cuuint64_t)L, (cuuint64_t)H, (cuuint64_t)B };
     const cuuint64_t strides[3] = { L > 1 ? (cuuint64_t)stride[2] * 2 : 16, H > 1 ? (cuuint64_t)stride[1] * 2 : 16,

@@ -10,6 +10,7 @@ import math
 import struct
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import cabi, op
@@ -20,11 +21,12 @@ _PROBLEM = struct.Struct("=6i2fiI25q")                # struct dsdpa_masked_prob
 
 
 def _usable(t):
-    """Rows contiguous and 16-byte aligned, no dimension broadcast: what the kernels read as it lies."""
+    """Rows contiguous and 16-byte aligned, no dimension broadcast: what the kernels read as it lies.  Rows are known to
+    have a multiple of 8 elements."""
     if t.data_ptr() % 16:
         return False
     if t.is_contiguous():
-        return t.shape[-1] * t.element_size() % 16 == 0
+        return True
     e = t.element_size()
     return (t.stride(-1) == 1 and
             all(n < 2 or (st > 0 and st * e % 16 == 0) for st, n in zip(t.stride()[:-1], t.shape[:-1])))
@@ -164,7 +166,7 @@ def masked_backward_raw(q, k, v, out, lse, dout, sm_scale=None, *, causal=False,
     B, Hq, Lq, D = q.shape
     Hkv, Lk = k.shape[1], k.shape[2]
     if not B * Hq or not (Lq or Lk):
-        return dq, dk, dv
+        return dq, dk.zero_(), dv.zero_()
     visible, slopes, stride = _mask_args(visible, slopes)
     rows = []
     for t in (q, k, v, out, dout, dq, dk, dv):
@@ -217,6 +219,8 @@ def masked_sdpa(q, k, v, sm_scale=None, *, causal=False, visible=None, softcap=0
     Query heads in groups of ``heads // kv_heads`` share a key/value head.  D is a multiple of 8 up to 256.
     A query that sees no key gives zeros; keys it does not see have no part in its result, whatever they
     hold.  Gradients for q, k and v, bit-reproducible."""
+    if not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)) and forward_ad._current_level < 0:
+        return masked_forward_raw(q, k, v, sm_scale, causal=causal, visible=visible, softcap=softcap, slopes=slopes)[0]
     sm_scale = q.shape[-1] ** -0.5 if sm_scale is None else float(sm_scale)
     return _MaskedSDPA.apply(q, k, v, sm_scale, bool(causal), visible, float(softcap), slopes)
 

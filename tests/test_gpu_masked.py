@@ -301,3 +301,43 @@ def test_threads_of_their_own():
     for g in got:
         assert not isinstance(g, Exception), g
         assert all(torch.equal(a, b) for a, b in zip(g[0] + g[1], want + grads))
+
+
+def test_no_query_heads():
+    q, k, v, do = make(1, 0, 2, 5, 7, 64, torch.bfloat16)
+    out, lse = be.masked_forward_raw(q, k, v)
+    dq, dk, dv = be.masked_backward_raw(q, k, v, out, lse, do)
+    assert out.shape == dq.shape == q.shape and (dk == 0).all() and (dv == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_without_gradients_the_same_result(dtype):
+    q, k, v, _ = make(2, 4, 2, 130, 130, 32, dtype, seed=18)
+    out = be.masked_sdpa(q, k, v, causal=True, softcap=20.0)
+    assert not out.requires_grad
+    leaf = q.clone().requires_grad_()
+    with torch.no_grad():
+        quiet = be.masked_sdpa(leaf, k, v, causal=True, softcap=20.0)
+    loud = be.masked_sdpa(leaf, k, v, causal=True, softcap=20.0)
+    assert not quiet.requires_grad and loud.requires_grad
+    assert torch.equal(out, quiet) and torch.equal(out, loud)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("scale", [0.05, 3.0], ids=["below the cap", "above the cap"])
+@pytest.mark.parametrize("causal", [False, True])
+def test_caps_over_whole_and_cut_tiles(dtype, scale, causal):
+    """Scores on either side of the cap, over key tiles that every row of a query tile sees and over ones that some do not."""
+    q, k, v, do = make(1, 2, 1, 390, 650, 64, dtype, seed=19)
+    check(q, k, v, do, scale, causal=causal, softcap=4.0)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_steep_bias_over_many_tiles(dtype):
+    """Nearest keys first: every row's maximum is in its first tile, which a window may have taken away."""
+    q, k, v, do = make(1, 2, 1, 300, 1500, 64, dtype, seed=20)
+    slopes = torch.tensor([0.25, 0.002], device="cuda")
+    check(q, k, v, do, 0.125, causal=True, slopes=slopes)
+    i = torch.arange(300, device="cuda", dtype=torch.int32)
+    visible = torch.stack([torch.zeros_like(i), (i * 5 - 200).clamp(min=0)], -1)
+    check(q, k, v, do, 0.125, slopes=slopes, visible=visible, softcap=3.0)
