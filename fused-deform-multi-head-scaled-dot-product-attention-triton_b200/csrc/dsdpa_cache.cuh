@@ -73,17 +73,21 @@ template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile(
 
 // The tokens that token t sees (bit u: token u), itself among them, from its chain of parents; its
 // depth is their number less one.  Every step goes to an earlier token, so the walk ends.
-__device__ __forceinline__ unsigned long long tokens_above(const CacheParams& p, int b, int t) {
-    if (!p.parents) return t == 63 ? ~0ull : (1ull << (t + 1)) - 1;
+template <typename F>
+__device__ __forceinline__ unsigned long long walk_up(int t, int* err, F parent) {
     unsigned long long seen = 1ull << t;
     int at = t;
     while (true) {
-        const int up = __ldg(p.parents + (long long)b * p.T + at);
-        if (up < -1 || up >= at) atomicCAS(p.err, 0, kErrBounds);
+        const int up = parent(at);
+        if (up < -1 || up >= at) atomicCAS(err, 0, kErrBounds);
         if (up < 0 || up >= at) return seen;
         seen |= 1ull << up;
         at = up;
     }
+}
+__device__ __forceinline__ unsigned long long tokens_above(const CacheParams& p, int b, int t) {
+    if (!p.parents) return t == 63 ? ~0ull : (1ull << (t + 1)) - 1;
+    return walk_up(t, p.err, [&](int at) { return __ldg(p.parents + (long long)b * p.T + at); });
 }
 __device__ __forceinline__ int depth_of(unsigned long long above) { return __popcll(above) - 1; }
 __device__ __forceinline__ int first_position(const CacheParams& p, int b, int n) { return p.start ? __ldg(p.start + b) : n; }

@@ -29,7 +29,7 @@ inline TreePlan plan_tree(const dsdpa_cache_problem& p) {
     const bool tc = cache_on_tensor_cores(p), few = cache_few_rows(p);
     const long long room = (long long)p.table_width * p.page_size;
     const int hd = p.D <= 64 ? 64 : 128, rows = p.T * (p.Hq / p.Hkv), keys = few ? 32 : tc ? 128 : 64, workers = few ? 4 : 1;   // a block's
-    t.row_unit = few ? 16 : tc ? 128 : rows <= 16 ? 16 : p.D <= 128 ? 64 : 32;
+    t.row_unit = few ? 16 : tc ? 128 : rows <= 16 ? 16 : rows <= 32 || p.D > 128 ? 32 : 64;
     t.row_tiles = (rows + t.row_unit - 1) / t.row_unit;
     t.part_rows = rows < t.row_unit ? rows : t.row_unit;
     const long long units = (long long)p.B * p.Hkv * t.row_tiles, tiles = (room + keys - 1) / keys;

@@ -1,5 +1,5 @@
 // Tree attention and accumulated weights in fp32 arithmetic: fp32 storage, and 16-bit storage with more than 128
-// elements a row.  Units of 16 rows (decoding) or 64, keys 64 at a time, on the register tiles of
+// elements a row.  Units of 16, 32 or 64 rows, keys 64 at a time, on the register tiles of
 // dsdpa_masked_simt.cuh; work is shared out as in dsdpa_share.cuh.  Bound by DRAM for a few rows, by the fma pipe
 // for many.
 #pragma once
@@ -39,16 +39,27 @@ __device__ __forceinline__ void simt_gather(float* dst, int D, const void* any, 
     cp_async_commit();
 }
 
+// What the drafted tokens of a sequence see (tokens_above), for the whole block: the parents come from memory once, and the walks
+// up the tree, every step of which waits for the one before, go through shared memory.  All threads; the caller
+// waits before anybody reads, and before the next call.
+struct SimtTokens { int parent[kTreeMax]; unsigned long long above[kTreeMax]; };
+__device__ __forceinline__ void simt_tokens(const CacheParams& p, const TreeItem& it, SimtTokens& s) {
+    const int t = threadIdx.x;
+    if (t < it.real) s.parent[t] = p.parents ? __ldg(p.parents + (long long)it.b * p.T + t) : t - 1;
+    __syncthreads();
+    if (t < it.real) s.above[t] = walk_up(t, p.err, [&](int at) { return s.parent[at]; });
+}
+
 // What a tile's keys are, by threads 0 .. 63: their pages (-1: absent) and positions.
-__device__ __forceinline__ void simt_keys(const CacheParams& p, const TreeItem& it, int k0, int* s_page, int* s_at) {
+__device__ __forceinline__ void simt_keys(const CacheParams& p, const TreeItem& it, const SimtTokens& tokens, int k0, int* s_page, int* s_at) {
     const int t = threadIdx.x;
     if (t >= kSimtKeys) return;
     const int j = k0 + t;
     int page = -1, at = j;
     if (j < it.n + it.real) {
-        page = page_of(p.table, p.width, p.pages, p.err, it.b, j / p.page_size);
+        page = page_of(p.table, p.width, p.pages, p.err, it.b, page_index(p.div, j));
         if (p.slopes) {
-            if (j >= it.n) at = first_position(p, it.b, it.n) + depth_of(tokens_above(p, it.b, j - it.n));
+            if (j >= it.n) at = first_position(p, it.b, it.n) + depth_of(tokens.above[j - it.n]);
             else if (p.positions) at = __ldg(p.positions + ((long long)it.b * p.Hkv + it.hk) * p.slots + j);
         }
     }
@@ -66,6 +77,7 @@ tree_simt_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ 
     float *sq = reinterpret_cast<float*>(simt_smem), *sk = sq + L::BM * L::S, *sv = sk + kSimtKeys * L::S, *sw = sv + kSimtKeys * L::S;
     __shared__ int s_page[2][kSimtKeys], s_at[2][kSimtKeys];
     __shared__ TreeShare<kSimtThreads> share;
+    __shared__ SimtTokens tokens;
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     find_share<Tile>(p, sp, share);
@@ -74,10 +86,12 @@ tree_simt_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ 
     TreeItem it;
     while (walk.next(p, sp, it)) {
         __syncthreads();                                        // the last item's tiles are read
+        simt_tokens(p, it, tokens);
         simt_gather<T, HD, L::BM>(sq, p.D, p.q, [&](int r) -> const T* {
             const int gr = it.row0 + r;
             return r < it.rows ? row_of<T>(p.q, p.sq, it.b, it.hk * p.group + gr % p.group, gr / p.group) : nullptr;
         });
+        __syncthreads();
         float m[RM], l[RM], slope2[RM], pos[RM];
         unsigned long long above[RM];
         bool real[RM];
@@ -86,7 +100,7 @@ tree_simt_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ 
         for (int r = 0; r < RM; ++r) {
             const int in_tile = ty * RM + r, gr = it.row0 + in_tile, t = gr / p.group, h = it.hk * p.group + gr % p.group;
             real[r] = in_tile < it.rows && t < it.real;
-            above[r] = real[r] ? tokens_above(p, it.b, t) : 0ull;
+            above[r] = real[r] ? tokens.above[t] : 0ull;
             slope2[r] = p.slopes && real[r] ? __ldg(p.slopes + h) * kLog2e : 0.0f;
             pos[r] = p.slopes && real[r] ? (float)(first_position(p, it.b, it.n) + depth_of(above[r])) : 0.0f;
             m[r] = kNegInf;
@@ -95,17 +109,17 @@ tree_simt_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ 
         auto rows_of = [&](const void* base, const long long (&st)[3], int k0, const int* pages) {
             return [=, &st](int r) -> const T* {
                 const int page = pages[r], j = k0 + r;
-                return page < 0 ? nullptr : row_of<T>(base, st, 0, it.hk, j % p.page_size) + page * st[0];
+                return page < 0 ? nullptr : row_of<T>(base, st, 0, it.hk, j - page_index(p.div, j) * p.page_size) + page * st[0];
             };
         };
         if (it.tiles > 0) {
-            simt_keys(p, it, it.key0, s_page[0], s_at[0]);
+            simt_keys(p, it, tokens, it.key0, s_page[0], s_at[0]);
             __syncthreads();
             simt_gather<T, HD, kSimtKeys>(sk, p.D, p.k, rows_of(p.k, p.sk, it.key0, s_page[0]));
         }
         for (int i = 0; i < it.tiles; ++i) {
             const int k0 = it.key0 + i * kSimtKeys, cur = i & 1;
-            if (i + 1 < it.tiles) simt_keys(p, it, k0 + kSimtKeys, s_page[cur ^ 1], s_at[cur ^ 1]);
+            if (i + 1 < it.tiles) simt_keys(p, it, tokens, k0 + kSimtKeys, s_page[cur ^ 1], s_at[cur ^ 1]);
             cp_async_wait<0>();
             __syncthreads();                                    // q, k are there; the last tile's v and weights are read
             simt_gather<T, HD, kSimtKeys>(sv, p.D, p.v, rows_of(p.v, p.sv, k0, s_page[cur]));
@@ -178,6 +192,7 @@ weights_simt_kernel(const __grid_constant__ CacheParams p, const __grid_constant
     float *sq = reinterpret_cast<float*>(simt_smem), *sk = sq + L::BM * L::S, *part = sk + kSimtKeys * L::S;
     __shared__ int s_page[kSimtKeys], s_at[kSimtKeys];
     __shared__ TreeShare<kSimtThreads> share;
+    __shared__ SimtTokens tokens;
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
     const int rows = p.T * p.group, passes = (rows + L::BM - 1) / L::BM;
     find_share<Tile>(p, sp, share);
@@ -203,7 +218,7 @@ weights_simt_kernel(const __grid_constant__ CacheParams p, const __grid_constant
                 if (gr < rows && t < it.real && !(p.take && !p.take[(long long)it.b * p.T + t])) {
                     const float x = p.lse[((long long)it.b * p.Hq + h) * p.T + t];
                     lse[r] = x == kNegInf ? -kNegInf : x;
-                    above[r] = tokens_above(p, it.b, t);
+                    above[r] = tokens.above[t];
                     if (p.slopes) {
                         slope2[r] = __ldg(p.slopes + h) * kLog2e;
                         pos[r] = (float)(first_position(p, it.b, it.n) + depth_of(above[r]));
@@ -212,13 +227,16 @@ weights_simt_kernel(const __grid_constant__ CacheParams p, const __grid_constant
             }
         };
         __syncthreads();
+        simt_tokens(p, it, tokens);
+        __syncthreads();
         if (passes == 1) take_rows(0);
         for (int i = 0; i < it.tiles; ++i) {
             const int k0 = it.key0 + i * kSimtKeys;
-            simt_keys(p, it, k0, s_page, s_at);
+            simt_keys(p, it, tokens, k0, s_page, s_at);
             __syncthreads();
             simt_gather<T, HD, kSimtKeys>(sk, p.D, p.k, [&](int r) -> const T* {
-                return s_page[r] < 0 ? nullptr : row_of<T>(p.k, p.sk, 0, it.hk, (k0 + r) % p.page_size) + s_page[r] * p.sk[0];
+                const int j = k0 + r;
+                return s_page[r] < 0 ? nullptr : row_of<T>(p.k, p.sk, 0, it.hk, j - page_index(p.div, j) * p.page_size) + s_page[r] * p.sk[0];
             });
             float sum[4] = { 0.0f, 0.0f, 0.0f, 0.0f };
             for (int pass = 0; pass < passes; ++pass) {

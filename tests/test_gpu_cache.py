@@ -240,6 +240,18 @@ def test_bad_pages_and_parents_are_left_out_and_reported():
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T", [5, 9, 20])
+def test_parents_behind_the_last_token_are_not_looked_at(dtype, T):
+    c = Cache([40, 7, 90], T, 2, 64, 16, dtype, seed=31)
+    tree = random_tree(3, T, 32)
+    for row, real in zip(tree, (T, 3, 1)):
+        row[real:] = [-7] * (T - real)
+    be.cabi.check(be.cabi.lib().dsdpa_device_error(0))
+    check(c, c.q(4, T), 0.125, parents=tree, drafted=[T, 3, 1], slopes=torch.full((4,), 0.1, device="cuda"))
+    assert be.cabi.lib().dsdpa_device_error(0) == be.cabi.OK
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("in_place", [True, False])
 @pytest.mark.parametrize("keep,sinks,recent", [(1, 0, 0), (50, 4, 10), (50, 20, 30), (64, 0, 64), (300, 3, 7), (5000, 4, 4)])
 def test_evict(dtype, in_place, keep, sinks, recent):
