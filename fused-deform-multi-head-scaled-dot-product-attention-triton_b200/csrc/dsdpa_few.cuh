@@ -211,7 +211,8 @@ __device__ __forceinline__ void few_scores(const CacheParams& p, const TreeItem&
     }
 }
 
-// o[c][j]: rows lane / 4 (first two) and lane / 4 + 8, elements 64 c + 16 t + j and + 8.
+// o[c][j]: rows lane / 4 (first two) and lane / 4 + 8, elements 64 c + 16 t + j and + 8.  With up to 8 rows the other 8 of the
+// instruction take what rounding the weights to the storage type has left off: twice its bits, for nothing.
 template <typename T, int HD, int NR>
 struct FewState {
     float m[NR], l[NR];
@@ -247,7 +248,11 @@ struct FewState {
 #pragma unroll
                 for (int c = 0; c < HD / 64; ++c)
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) { o[c][j][2 * r] *= f; o[c][j][2 * r + 1] *= f; }
+                    for (int j = 0; j < 8; ++j) {
+                        o[c][j][2 * r] *= f;
+                        o[c][j][2 * r + 1] *= f;
+                        if (NR == 1) { o[c][j][2] *= f; o[c][j][3] *= f; }
+                    }
             }
         }
         uint32_t a[2][2] = {};
@@ -259,6 +264,10 @@ struct FewState {
                 const float x = fast_exp2(s[j][2 * r] - m0), y = fast_exp2(s[j][2 * r + 1] - m0);
                 l[r] += x + y;                            // this thread's part of the sum
                 a[j][r] = pack2<T>(x, y);
+                if (NR == 1) {
+                    const float2 hi = to_float2<T>(a[j][0]);
+                    a[j][1] = pack2<T>(x - hi.x, y - hi.y);
+                }
             }
         }
         const uint4 w = make_uint4(a[0][0], a[0][1], a[1][0], a[1][1]);
@@ -270,6 +279,13 @@ struct FewState {
                 mma16816<T>(o[c][j], w, __byte_perm(word_of(v[0][c], j >> 1), word_of(v[1][c], j >> 1), pick),
                             __byte_perm(word_of(v[2][c], j >> 1), word_of(v[3][c], j >> 1), pick));
             }
+    }
+    __device__ __forceinline__ void join() {
+        if (NR > 1) return;
+#pragma unroll
+        for (int c = 0; c < HD / 64; ++c)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) { o[c][j][0] += o[c][j][2]; o[c][j][1] += o[c][j][3]; }
     }
     // the keys of an item, 16 at a time: groups first, first + step, ...
     __device__ __forceinline__ void run(const CacheParams& p, const TreeItem& it, int lane, int first, int step, const uint4* q,
@@ -323,6 +339,7 @@ tree_few_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ T
         few_queries<T, HD, NR>(p, it, lane, q, row);
         st.clear();
         st.run(p, it, lane, sp.whole ? warp : 0, sp.whole ? kFewWarps : 1, q, row, scale2);
+        st.join();
         unsigned bad[NR] = {};
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
