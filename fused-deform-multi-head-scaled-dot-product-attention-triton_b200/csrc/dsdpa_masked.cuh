@@ -120,7 +120,8 @@ __device__ __forceinline__ float rcp_approx(float x) {
 // tanh(a / 2), the cap's argument being a = 2 x / cap.  For |a| < 2 (scores below the cap) an odd polynomial, fitted to
 // the least largest relative error (5e-8; evaluated in fp32 1.5e-7): ten fma-pipe operations for two values where
 // the general form, 1 - 2 / (1 + e^a), takes four of the special-function unit, which is what these kernels run
-// out of: the capped backward over 28x28 image tokens and text (D = 64) takes 245 us with that form alone.
+// out of: the capped backward over four sequences of 1571 image and text tokens (16 heads, D = 64) takes 245 us with
+// that form alone, 208 us with this one.
 constexpr int kTanhTerms = 7;
 __device__ __forceinline__ float tanh_term(int i) {
     constexpr float k[kTanhTerms] = { 4.999999702e-01f, -4.166604951e-02f, 4.164126236e-03f, -4.176330403e-04f, 3.962886694e-05f, -3.028993660e-06f, 1.270779535e-07f };
