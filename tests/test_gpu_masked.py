@@ -341,3 +341,27 @@ def test_steep_bias_over_many_tiles(dtype):
     i = torch.arange(300, device="cuda", dtype=torch.int32)
     visible = torch.stack([torch.zeros_like(i), (i * 5 - 200).clamp(min=0)], -1)
     check(q, k, v, do, 0.125, slopes=slopes, visible=visible, softcap=3.0)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_training_step_in_a_graph(dtype):
+    """Forward and backward through autograd, captured once and replayed with other inputs."""
+    q, k, v, do = make(1, 4, 2, 150, 150, 64, dtype, seed=21)
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+
+    def step():
+        out = be.masked_sdpa(*leaves, causal=True, softcap=10.0)
+        return (out.detach(), *torch.autograd.grad(out, leaves, do))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    with torch.no_grad():
+        for t in leaves:
+            t.mul_(0.5)
+    graph.replay()
+    assert all(torch.equal(a, b) for a, b in zip(got, step()))
