@@ -53,6 +53,8 @@ cudaError_t tree_forward(const dsdpa_cache_problem& problem, const CacheParams& 
     if constexpr (DtypeOf<T>::value != DSDPA_F32)
         if (cache_on_tensor_cores(problem))
             return cache_few_rows(problem) ? launch_tree_few<T>(p, t, workspace, s) : launch_tree_tc<T>(p, t, workspace, s);
+    if constexpr (DtypeOf<T>::value == DSDPA_F32)
+        if (cache_few_f32(problem)) return launch_tree_few_f32(p, t, workspace, s);
     return launch_tree_simt<T>(p, t, workspace, s);
 }
 template <typename T>
@@ -60,6 +62,8 @@ cudaError_t weights_add(const dsdpa_cache_problem& problem, const CacheParams& p
     const TreePlan t = plan_tree(problem);
     if constexpr (DtypeOf<T>::value != DSDPA_F32)
         if (cache_on_tensor_cores(problem)) return cache_few_rows(problem) ? launch_weights_few<T>(p, t, s) : launch_weights_tc<T>(p, t, s);
+    if constexpr (DtypeOf<T>::value == DSDPA_F32)
+        if (cache_few_f32(problem)) return launch_weights_few_f32(p, t, s);
     return launch_weights_simt<T>(p, t, s);
 }
 

@@ -11,6 +11,13 @@ inline bool cache_on_tensor_cores(const dsdpa_cache_problem& p) { return p.dtype
 // ... and of these a warp's own matrix instructions those with up to 16 rows to a key/value head.
 inline bool cache_few_rows(const dsdpa_cache_problem& p) { return cache_on_tensor_cores(p) && p.T * (p.Hq / p.Hkv) <= 16; }
 
+// fp32 with up to 8 rows has few-row kernels too, for caches that are worth a second kernel (plan_tree's `whole`).
+constexpr int kFewRowsF32 = 8, kWholeF32 = 256;
+inline bool cache_few_f32(const dsdpa_cache_problem& p) {
+    return p.dtype == DSDPA_F32 && p.D <= 128 && p.T * (p.Hq / p.Hkv) <= kFewRowsF32 && (long long)p.table_width * p.page_size > kWholeF32;
+}
+constexpr int few_f32_blocks(int chunks, bool weights) { return weights ? 4 : chunks == 1 ? 3 : 2; }   // by registers
+
 // Blocks of four warps that the few-row kernels are compiled to have on an SM: with 128 elements a row tree attention needs
 // more than 128 registers a thread.
 constexpr int few_blocks(int hd, int rows, bool weights) {
@@ -26,19 +33,19 @@ struct TreePlan {
 };
 inline TreePlan plan_tree(const dsdpa_cache_problem& p) {
     TreePlan t{};
-    const bool tc = cache_on_tensor_cores(p), few = cache_few_rows(p);
+    const bool tc = cache_on_tensor_cores(p), few = cache_few_rows(p), few32 = cache_few_f32(p);
     const long long room = (long long)p.table_width * p.page_size;
-    const int hd = p.D <= 64 ? 64 : 128, rows = p.T * (p.Hq / p.Hkv), keys = few ? 32 : tc ? 128 : 64, workers = few ? 4 : 1;   // a block's
-    t.row_unit = few ? 16 : tc ? 128 : rows <= 16 ? 16 : rows <= 32 || p.D > 128 ? 32 : 64;
+    const int hd = p.D <= 64 ? 64 : 128, rows = p.T * (p.Hq / p.Hkv), keys = few || few32 ? 32 : tc ? 128 : 64, workers = few || few32 ? 4 : 1;   // a block's
+    t.row_unit = few32 ? kFewRowsF32 : few ? 16 : tc ? 128 : rows <= 16 ? 16 : rows <= 32 || p.D > 128 ? 32 : 64;
     t.row_tiles = (rows + t.row_unit - 1) / t.row_unit;
     t.part_rows = rows < t.row_unit ? rows : t.row_unit;
     const long long units = (long long)p.B * p.Hkv * t.row_tiles, tiles = (room + keys - 1) / keys;
     // A cache of up to 512 keys (256 in fp32 arithmetic) is not worth a second kernel: a block goes through it while the
     // launch of one would take.
-    t.whole = room <= (tc ? 512 : 256);
+    t.whole = room <= (tc ? 512 : kWholeF32);
     // as many blocks as stay on the SMs at once, but no share below two key tiles
-    const long long stay = few ? few_blocks(hd, rows, false) * kSMs : tc ? kSMs : p.D <= 64 ? 3 * kSMs : p.D <= 128 ? 2 * kSMs : kSMs;
-    const long long stay_weights = few ? few_blocks(hd, rows, true) * kSMs : stay, least = 2 * workers;
+    const long long stay = few32 ? few_f32_blocks(rows <= 4 ? 1 : 2, false) * kSMs : few ? few_blocks(hd, rows, false) * kSMs : tc ? kSMs : p.D <= 64 ? 3 * kSMs : p.D <= 128 ? 2 * kSMs : kSMs;
+    const long long stay_weights = few32 ? few_f32_blocks(1, true) * kSMs : few ? few_blocks(hd, rows, true) * kSMs : stay, least = 2 * workers;
     const long long most = t.whole ? units : (units * tiles + least - 1) / least, most_weights = ((long long)p.B * p.Hkv * tiles + least - 1) / least;
     t.blocks = (int)(most < stay || t.whole ? (most < 65536 ? most : 65536) : stay);
     t.weight_blocks = (int)(most_weights < stay_weights ? most_weights : stay_weights);
@@ -54,6 +61,8 @@ inline TreePlan plan_tree(const dsdpa_cache_problem& p) {
 
 template <typename T> cudaError_t launch_tree_few(const CacheParams& p, const TreePlan& t, void* workspace, cudaStream_t s);
 template <typename T> cudaError_t launch_weights_few(const CacheParams& p, const TreePlan& t, cudaStream_t s);
+cudaError_t launch_tree_few_f32(const CacheParams& p, const TreePlan& t, void* workspace, cudaStream_t s);
+cudaError_t launch_weights_few_f32(const CacheParams& p, const TreePlan& t, cudaStream_t s);
 template <typename T> cudaError_t launch_tree_tc(const CacheParams& p, const TreePlan& t, void* workspace, cudaStream_t s);
 template <typename T> cudaError_t launch_tree_simt(const CacheParams& p, const TreePlan& t, void* workspace, cudaStream_t s);
 template <typename T> cudaError_t launch_weights_tc(const CacheParams& p, const TreePlan& t, cudaStream_t s);

@@ -402,3 +402,17 @@ def test_two_streams_at_once():
     for i in range(2):
         for out, lse in got[i]:
             assert torch.equal(out, want[i][0]) and torch.equal(lse, want[i][1])
+
+
+@pytest.mark.parametrize("D", [8, 32, 40, 64, 96, 128])
+@pytest.mark.parametrize("page,Hq,Hkv,T", [(16, 2, 2, 1), (7, 4, 1, 1), (64, 3, 1, 2), (1, 2, 1, 4), (48, 8, 1, 1)])
+def test_few_rows_in_fp32(D, page, Hq, Hkv, T):
+    """Up to eight rows over caches that are shared out between warps."""
+    c = Cache([700, 0, 31, 1025, 256, 5], T, Hkv, D, page, torch.float32, seed=D + page)
+    tree = random_tree(6, T, page) if T > 1 else None
+    check(c, c.q(Hq, T), D ** -0.5, parents=tree)
+    slopes = torch.linspace(0.3, 0.01, Hq, device="cuda")
+    positions = torch.sort(torch.randint(0, 3000, (6, Hkv, c.slots), generator=c.g, device="cuda"), -1).values.int()
+    take = torch.rand(6, T, generator=c.g, device="cuda") < 0.5
+    check(c, c.q(Hq, T), 2 * D ** -0.5, parents=tree, drafted=[T, 0, 1, T, 1, T], softcap=6.0, slopes=slopes, take=take)
+    check(c, c.q(Hq, T), -D ** -0.5, parents=tree, slopes=slopes, positions=positions, start=[3000, 1, 3001, 3005, 2999, 3000])
