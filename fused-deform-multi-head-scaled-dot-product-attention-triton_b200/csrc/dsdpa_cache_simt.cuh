@@ -1,8 +1,8 @@
 // Tree attention and accumulated weights in fp32 arithmetic: fp32 storage, and 16-bit storage with more than 128
 // elements a row.  Units of 16, 32 or 64 rows, keys 64 at a time, on the register tiles of
 // dsdpa_masked_simt.cuh; work is shared out as in dsdpa_share.cuh.  Bound by the fma pipe and, for
-// short caches, by latency: 17 tokens over three caches of 2000 keys (8 heads, D = 64, fp32) take 15 us; for 64 caches of
-// up to 8192 keys, 32 heads on 8, one token each (D = 128, fp32), 1.15 ms, 1.7 TB/s, with 4 of a tile's 16 rows in use.
+// short caches, by latency: 17 tokens over three caches of 2000 keys (8 heads, D = 64, fp32) take 15 us.  (Up to
+// eight rows of fp32 over longer caches have kernels of their own, dsdpa_few_f32.cuh.)
 #pragma once
 
 #include "dsdpa_masked_simt.cuh"

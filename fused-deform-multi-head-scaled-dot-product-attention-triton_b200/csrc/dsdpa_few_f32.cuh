@@ -8,7 +8,8 @@
 // would take 32 log2(lanes)) and of which a lane then has 32 / lanes: the scores.  Their weights go through
 // shared memory back to all lanes.  The register tiles of dsdpa_cache_simt.cuh spend 16 rows' fmas on whatever rows
 // there are: for 64 caches of up to 8192 keys, 32 heads on 8, one token each (D = 128) they take 1150 us and
-// 723 us (weights).  Bound by DRAM.
+// 723 us (weights), these kernels 320 us (6.2 TB/s of the 6.5 that a copy reaches) and 175 us (5.7).  Bound by DRAM;
+// with 8 rows (522 us) by the arithmetic between the loads, two blocks an SM.
 #pragma once
 
 #include "dsdpa_cache_launch.h"
@@ -70,16 +71,32 @@ struct F32Few {
         slot = j - page_index(p.div, j) * p.page_size;
         there = __ballot_sync(0xffffffffu, page >= 0);
     }
+    __device__ __forceinline__ static float4 row_part(const float* from) {
+        const uint4 u = ldg128_stream(from);
+        return make_float4(__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z), __uint_as_float(u.w));
+    }
     __device__ __forceinline__ void load(const CacheParams& p, const TreeItem& it, const void* base, const long long (&st)[3], float4 (&x)[8]) const {
         const float* from = row_of<float>(base, st, 0, it.hk, 0) + at * 4;
+        // the usual step: all keys there, every lane with elements (no load behind a condition: it would be waited for at once)
+        if (there == (kStep == 32 ? ~0u : (1u << kStep % 32) - 1) && p.D == HD) {
+            if (p.page_size % kStep == 0) {              // on one page
+                from += __shfl_sync(0xffffffffu, page, 0) * st[0] + (__shfl_sync(0xffffffffu, slot, 0) + group) * st[2];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = row_part(from + e * kGroups * st[2]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int key = key_of(e, group);
+                    x[e] = row_part(from + __shfl_sync(0xffffffffu, page, key) * st[0] + __shfl_sync(0xffffffffu, slot, key) * st[2]);
+                }
+            }
+            return;
+        }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const int key = key_of(e, group), pg = __shfl_sync(0xffffffffu, page, key), sl = __shfl_sync(0xffffffffu, slot, key);
             x[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (pg >= 0 && at * 4 < p.D) {
-                const uint4 u = ldg128_stream(from + pg * st[0] + sl * st[2]);
-                x[e] = make_float4(__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z), __uint_as_float(u.w));
-            }
+            if (pg >= 0 && at * 4 < p.D) x[e] = row_part(from + pg * st[0] + sl * st[2]);
         }
     }
     // Scores in base 2 of this lane's (key, row) pairs: numbers at * kHeld + v, key the number / 4, row 4 c + the number % 4.
