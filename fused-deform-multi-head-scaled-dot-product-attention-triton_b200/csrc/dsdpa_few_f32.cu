@@ -11,7 +11,7 @@ cudaError_t tree(const CacheParams& p, const TreePlan& t, const TreeSplit& sp, c
     tree_few_f32_kernel<HD, NC><<<t.blocks, kF32Warps * 32, 0, s>>>(p, sp);
     count_launches(1);
     const cudaError_t e = cudaGetLastError();
-    return e != cudaSuccess ? e : launch_combine<float, F32Tile>(p, sp, s);
+    return e != cudaSuccess ? e : launch_combine<float, F32Tile>(p, t, sp, s);
 }
 template <int HD, int NC>
 cudaError_t weights(const CacheParams& p, const TreePlan& t, cudaStream_t s) {

@@ -142,12 +142,15 @@ __device__ __forceinline__ void find_share(const CacheParams& p, const TreeSplit
     }
 }
 
-// Joins the parts of a row: out = sum_c 2^(lse_c - lse) part_c; rows that see no key get their zeros.  One warp a row.
-constexpr int kCombineWarps = 4;
-template <typename T, typename Tile>
+// Joins the parts of a row: out = sum_c 2^(lse_c - lse) part_c; rows that see no key get their zeros.  A row has WARPS warps of a
+// block of kCombineWarps: one where there are many rows, all where a few long caches leave many parts to each.
+constexpr int kCombineWarps = 8;
+template <typename T, typename Tile, int WARPS>
 __global__ void __launch_bounds__(kCombineWarps * 32) tree_combine_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeSplit sp) {
+    __shared__ float s_acc[WARPS > 1 ? kCombineWarps : 1][WARPS > 1 ? 256 : 1], s_sum[kCombineWarps];
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const long long row = (long long)blockIdx.x * kCombineWarps + threadIdx.x / 32;
+    const int warp = threadIdx.x / 32, mine = warp % WARPS;           // the same row for all threads, or no barrier below
+    const long long row = (long long)blockIdx.x * (kCombineWarps / WARPS) + warp / WARPS;
     if (row >= (long long)p.B * p.Hq * p.T) return;
     const int lane = threadIdx.x & 31, t = (int)(row % p.T), h = (int)(row / p.T % p.Hq), b = (int)(row / p.T / p.Hq);
     // the workers whose shares the row's unit lies in
@@ -173,19 +176,44 @@ __global__ void __launch_bounds__(kCombineWarps * 32) tree_combine_kernel(const 
     const float m0 = m == kNegInf ? 0.0f : m;
     float sum = 0.0f, acc[2][4] = {};
     const float* part = sp.part + lane * 4;
-    for (int c = 0; c < used; ++c) {
-        const long long at = place(c);
-        const float f = exp2f(sp.part_lse[at] - m0);
-        sum += f;
+    // a lane has a part's factor, so that the parts themselves are asked for several at a time
+    for (int first = mine * 32; first < used; first += WARPS * 32) {
+        const float own = first + lane < used ? exp2f(sp.part_lse[place(first + lane)] - m0) : 0.0f;
+        sum += own;
+        const int n = min(32, used - first);
+#pragma unroll 8
+        for (int c = 0; c < n; ++c) {
+            const long long at = place(first + c);
+            const float f = __shfl_sync(0xffffffffu, own, c);
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+                if (k * 128 + lane * 4 < p.D) {
+                    const float4 v = *reinterpret_cast<const float4*>(part + at * p.D + k * 128);
+                    acc[k][0] = fmaf(f, v.x, acc[k][0]);
+                    acc[k][1] = fmaf(f, v.y, acc[k][1]);
+                    acc[k][2] = fmaf(f, v.z, acc[k][2]);
+                    acc[k][3] = fmaf(f, v.w, acc[k][3]);
+                }
+        }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if constexpr (WARPS > 1) {
+        static_assert(WARPS == kCombineWarps, "a block has one row");
 #pragma unroll
         for (int k = 0; k < 2; ++k)
-            if (k * 128 + lane * 4 < p.D) {
-                const float4 v = *reinterpret_cast<const float4*>(part + at * p.D + k * 128);
-                acc[k][0] = fmaf(f, v.x, acc[k][0]);
-                acc[k][1] = fmaf(f, v.y, acc[k][1]);
-                acc[k][2] = fmaf(f, v.z, acc[k][2]);
-                acc[k][3] = fmaf(f, v.w, acc[k][3]);
-            }
+            if (k * 128 + lane * 4 < p.D) *reinterpret_cast<float4*>(&s_acc[warp][k * 128 + lane * 4]) = make_float4(acc[k][0], acc[k][1], acc[k][2], acc[k][3]);
+        if (lane == 0) s_sum[warp] = sum;
+        __syncthreads();
+        if (warp > 0) return;
+        for (int w = 1; w < WARPS; ++w) {
+            sum += s_sum[w];
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (k * 128 + lane * 4 < p.D) acc[k][e] += s_acc[w][k * 128 + lane * 4 + e];
+        }
     }
     const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
     bool fine = !nan;

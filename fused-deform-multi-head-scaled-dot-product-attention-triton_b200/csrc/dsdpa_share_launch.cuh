@@ -13,10 +13,12 @@ inline TreeSplit tree_split(const TreePlan& t, void* workspace) {
 
 // The second kernel's blocks are in place when the first one's end, and wait for its results there.
 template <typename T, typename Tile>
-cudaError_t launch_combine(const CacheParams& p, const TreeSplit& sp, cudaStream_t s) {
+cudaError_t launch_combine(const CacheParams& p, const TreePlan& t, const TreeSplit& sp, cudaStream_t s) {
     cudaLaunchConfig_t cfg{};
     const long long rows = (long long)p.B * p.Hq * p.T;
-    cfg.gridDim = dim3((unsigned)((rows + kCombineWarps - 1) / kCombineWarps));
+    // parts of a row on average, from the workers of the first kernel: above a warp's 32 a block takes them together
+    const bool spread = (long long)t.blocks * Tile::kWorkers > 32ll * p.B * p.Hkv * t.row_tiles;
+    cfg.gridDim = dim3((unsigned)(spread ? rows : (rows + kCombineWarps - 1) / kCombineWarps));
     cfg.blockDim = dim3(kCombineWarps * 32);
     cfg.stream = s;
     cudaLaunchAttribute attr{};
@@ -24,7 +26,7 @@ cudaError_t launch_combine(const CacheParams& p, const TreeSplit& sp, cudaStream
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, tree_combine_kernel<T, Tile>, p, sp);
+    const cudaError_t e = spread ? cudaLaunchKernelEx(&cfg, tree_combine_kernel<T, Tile, kCombineWarps>, p, sp) : cudaLaunchKernelEx(&cfg, tree_combine_kernel<T, Tile, 1>, p, sp);
     count_launches(1);
     return e;
 }
