@@ -110,15 +110,16 @@ def tree_sdpa(q, k_pages, v_pages, page_table, lens, sm_scale=None, *, parents=N
     dev = _check_pages(k_pages, v_pages, page_table, lens, name)
     tree, held = _tokens(q, k_pages, page_table, sm_scale, softcap, parents, drafted, slopes, positions, start, dev, name)
     q = masked._as_rows(q)
-    out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-    lse = torch.empty(q.shape[:3], device=q.device, dtype=torch.float32)
-    if 0 in q.shape:
+    B, Hq, T, _ = q.shape
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    lse = q.new_empty((B, Hq, T), dtype=torch.float32)
+    if not B * Hq * T:
         return out, lse
     page_table, lens = page_table.contiguous(), lens.contiguous()
     prob = _problem(q, k_pages, v_pages, page_table, sm_scale, softcap, positions.shape[2] if positions is not None else 0)
     L = cabi.lib()
     n = L.dsdpa_tree_workspace_bytes(prob)
-    ws = torch.empty(n, device=q.device, dtype=torch.uint8) if n else None
+    ws = q.new_empty(n, dtype=torch.uint8) if n else None
     st = L.dsdpa_tree_forward(prob, tree, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), lens.data_ptr(),
                               out.data_ptr(), lse.data_ptr(), None if ws is None else ws.data_ptr(), n, dev, masked._raw_stream(dev))
     if st:
@@ -191,7 +192,7 @@ def cache_evict(k_pages, v_pages, page_table, lens, weights, keep, *, sinks=0, r
             raise ValueError(f"{name}: out_table has no room for {keep} keys")
     page_table, lens = page_table.contiguous(), lens.contiguous()
     out_table = page_table if out_table is None else out_table.contiguous()
-    kept = torch.empty((B, Hkv, keep), device=k_pages.device, dtype=torch.int32)
+    kept = lens.new_empty((B, Hkv, keep))
     new_lens, new_weights = torch.empty_like(lens), torch.empty_like(weights)
     new_positions = torch.empty_like(positions) if positions is not None else None
     if B:

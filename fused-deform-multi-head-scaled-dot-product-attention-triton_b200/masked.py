@@ -132,7 +132,7 @@ def masked_forward_raw(q, k, v, sm_scale=None, *, causal=False, visible=None, so
     q, k, v = _as_rows(q), _as_rows(k), _as_rows(v)
     B, Hq, Lq, D = q.shape
     out = torch.empty_like(q)
-    lse = torch.empty((B, Hq, Lq), device=q.device, dtype=torch.float32)
+    lse = q.new_empty((B, Hq, Lq), dtype=torch.float32)
     if not B * Hq * Lq:
         return out, lse
     visible, slopes, stride = _mask_args(visible, slopes)
@@ -174,7 +174,7 @@ def masked_backward_raw(q, k, v, out, lse, dout, sm_scale=None, *, causal=False,
     prob = _PROBLEM.pack(B, Hq, Hkv, Lq, Lk, D, sm_scale, softcap, op._DTYPES[q.dtype], cabi.MASKED_CAUSAL if causal else 0, *rows, stride)
     L = cabi.lib()
     n = L.dsdpa_masked_backward_workspace_bytes(prob)
-    ws = torch.empty(n, device=q.device, dtype=torch.uint8) if n else None
+    ws = q.new_empty(n, dtype=torch.uint8) if n else None
     st = L.dsdpa_masked_backward(prob, q.data_ptr(), k.data_ptr(), v.data_ptr(), None if visible is None else visible.data_ptr(),
                                  None if slopes is None else slopes.data_ptr(), out.data_ptr(), lse.data_ptr(), dout.data_ptr(),
                                  dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), None if ws is None else ws.data_ptr(), n, dev, _raw_stream(dev))
