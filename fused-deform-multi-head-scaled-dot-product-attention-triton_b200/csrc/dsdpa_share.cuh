@@ -148,13 +148,13 @@ constexpr int kCombineWarps = 8;
 template <typename T, typename Tile, int WARPS>
 __global__ void __launch_bounds__(kCombineWarps * 32) tree_combine_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeSplit sp) {
     __shared__ __align__(16) float s_acc[WARPS > 1 ? kCombineWarps : 1][WARPS > 1 ? 256 : 1], s_sum[kCombineWarps];
-    asm volatile("griddepcontrol.wait;" ::: "memory");
     const int warp = threadIdx.x / 32, mine = warp % WARPS;           // the same row for all threads, or no barrier below
     const long long row = (long long)blockIdx.x * (kCombineWarps / WARPS) + warp / WARPS;
     if (row >= (long long)p.B * p.Hq * p.T) return;
     const int lane = threadIdx.x & 31, t = (int)(row % p.T), h = (int)(row / p.T % p.Hq), b = (int)(row / p.T / p.Hq);
     // the workers whose shares the row's unit lies in
     const int gr = t * p.group + h % p.group, nt = tree_tiles<Tile>(p, b);
+    asm volatile("griddepcontrol.wait;" ::: "memory");                // the first kernel's results from here on
     const long long share = sp.start[p.B + 1];
     const long long from = sp.start[b] * p.Hkv * sp.row_tiles + (long long)(h / p.group * sp.row_tiles + gr / Tile::kRows) * nt;
     const int c0 = (int)(from / share), c1 = nt > 0 ? (int)((from + nt - 1) / share) : c0 - 1;
@@ -163,10 +163,11 @@ __global__ void __launch_bounds__(kCombineWarps * 32) tree_combine_kernel(const 
     auto place = [&](int c) {                            // a worker's first part, or its second
         return ((long long)(c0 + c) * 2 + ((c0 + c) * share >= from ? 0 : 1)) * sp.part_rows + gr % Tile::kRows;
     };
-    float m = kNegInf;
+    float m = kNegInf, kept = kNegInf;                    // kept: of this warp's first 32 parts
     bool nan = false;
     for (int c = lane; c < used; c += 32) {
         const float x = sp.part_lse[place(c)];
+        if (c - lane == mine * 32) kept = x;
         nan = nan || x != x;
         m = fmaxf(m, x);
     }
@@ -175,25 +176,25 @@ __global__ void __launch_bounds__(kCombineWarps * 32) tree_combine_kernel(const 
     nan = __any_sync(0xffffffffu, nan);
     const float m0 = m == kNegInf ? 0.0f : m;
     float sum = 0.0f, acc[2][4] = {};
-    const float* part = sp.part + lane * 4;
-    // a lane has a part's factor, so that the parts themselves are asked for several at a time
+    // A lane has a part's factor, so that the parts themselves are asked for several at a time; lanes without elements read
+    // the first ones (a load behind a condition would be waited for at once).
+    const float *part0 = sp.part + (lane * 4 < p.D ? lane * 4 : 0), *part1 = sp.part + (128 + lane * 4 < p.D ? 128 + lane * 4 : 0);
+    auto add = [&](float (&to)[4], float f, const float* from) {
+        const float4 v = *reinterpret_cast<const float4*>(from);
+        to[0] = fmaf(f, v.x, to[0]);
+        to[1] = fmaf(f, v.y, to[1]);
+        to[2] = fmaf(f, v.z, to[2]);
+        to[3] = fmaf(f, v.w, to[3]);
+    };
     for (int first = mine * 32; first < used; first += WARPS * 32) {
-        const float own = first + lane < used ? exp2f(sp.part_lse[place(first + lane)] - m0) : 0.0f;
+        const float own = first + lane < used ? exp2f((first == mine * 32 ? kept : sp.part_lse[place(first + lane)]) - m0) : 0.0f;
         sum += own;
         const int n = min(32, used - first);
 #pragma unroll 8
-        for (int c = 0; c < n; ++c) {
-            const long long at = place(first + c);
-            const float f = __shfl_sync(0xffffffffu, own, c);
-#pragma unroll
-            for (int k = 0; k < 2; ++k)
-                if (k * 128 + lane * 4 < p.D) {
-                    const float4 v = *reinterpret_cast<const float4*>(part + at * p.D + k * 128);
-                    acc[k][0] = fmaf(f, v.x, acc[k][0]);
-                    acc[k][1] = fmaf(f, v.y, acc[k][1]);
-                    acc[k][2] = fmaf(f, v.z, acc[k][2]);
-                    acc[k][3] = fmaf(f, v.w, acc[k][3]);
-                }
+        for (int c = 0; c < n; ++c) add(acc[0], __shfl_sync(0xffffffffu, own, c), part0 + place(first + c) * p.D);
+        if (p.D > 128) {
+#pragma unroll 8
+            for (int c = 0; c < n; ++c) add(acc[1], __shfl_sync(0xffffffffu, own, c), part1 + place(first + c) * p.D);
         }
     }
 #pragma unroll
