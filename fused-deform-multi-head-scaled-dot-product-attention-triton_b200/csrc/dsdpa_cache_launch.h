@@ -40,9 +40,11 @@ inline TreePlan plan_tree(const dsdpa_cache_problem& p) {
     t.row_tiles = (rows + t.row_unit - 1) / t.row_unit;
     t.part_rows = rows < t.row_unit ? rows : t.row_unit;
     const long long units = (long long)p.B * p.Hkv * t.row_tiles, tiles = (room + keys - 1) / keys;
-    // A cache of up to 512 keys (256 in fp32 arithmetic) is not worth a second kernel: a block goes through it while the
-    // launch of one would take.
-    t.whole = room <= (tc ? 512 : kWholeF32);
+    // A short cache is not worth a second kernel: a block goes through it while the launch of one would take (few rows, one
+    // cache of 500 keys: 14 us whole, of 740 19 us whole and 17 us cut; fp32 arithmetic half of that).  With 32 rows a key
+    // tile costs less for each: one cache of 740 keys 16.2 us whole and 16.8 us cut, of 1000 19 and 17; and where the units
+    // fill half of the SMs by themselves 8 caches of 2000 keys 30 and 35 us, 64 of them 113 and 125 us.
+    t.whole = room <= (few ? 512 : !tc ? kWholeF32 : units >= 64 ? 2048 : 768);
     // as many blocks as stay on the SMs at once, but no share below two key tiles
     const long long stay = few32 ? few_f32_blocks(rows <= 4 ? 1 : 2, false) * kSMs : few ? few_blocks(hd, rows, false) * kSMs : tc ? kSMs : p.D <= 64 ? 3 * kSMs : p.D <= 128 ? 2 * kSMs : kSMs;
     const long long stay_weights = few32 ? few_f32_blocks(1, true) * kSMs : few ? few_blocks(hd, rows, true) * kSMs : stay, least = 2 * workers;
