@@ -416,3 +416,12 @@ def test_few_rows_in_fp32(D, page, Hq, Hkv, T):
     take = torch.rand(6, T, generator=c.g, device="cuda") < 0.5
     check(c, c.q(Hq, T), 2 * D ** -0.5, parents=tree, drafted=[T, 0, 1, T, 1, T], softcap=6.0, slopes=slopes, take=take)
     check(c, c.q(Hq, T), -D ** -0.5, parents=tree, slopes=slopes, positions=positions, start=[3000, 1, 3001, 3005, 2999, 3000])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("Hq,T", [(8, 1), (4, 4), (1, 13), (16, 1), (2, 9), (1, 64)])
+def test_short_caches_with_every_number_of_rows(dtype, D, Hq, T):
+    """One block goes through a short cache; its shared memory grows with the rows."""
+    c = Cache([300, 17, 0, 440], T, 1, D, 32, dtype, seed=D + T)
+    check(c, c.q(Hq, T), D ** -0.5, parents=random_tree(4, T, 5) if T > 1 else None)
