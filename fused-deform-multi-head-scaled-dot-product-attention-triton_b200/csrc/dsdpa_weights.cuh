@@ -153,7 +153,8 @@ weights_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ Tr
                 for (int i = 0; i < it.tiles; ++i, ++n) {
                     if ((i & 1) != side) continue;       // the same thread in every pass
                     const int j = it.key0 + i * kTreeKeys + quad * 32 + lane, draft = j - it.n;
-                    const bool exists = draft < it.real;
+                    // a drafted key that the table has no room for is behind the row of weights too
+                    const bool exists = draft < it.real && j < p.width * p.page_size;
                     const float old = exists ? out[j] : 0.0f;
                     float at = (float)j;
                     if (BIAS && exists) {

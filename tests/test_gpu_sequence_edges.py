@@ -1,0 +1,73 @@
+"""Calls of the sequence operators at the ends of what their documentation allows, on every kernel that can take them:
+rows from one to more than 128 to a key/value head, caches that one block goes through and caches that are cut."""
+import math
+
+import pytest
+import torch
+
+import ops
+import sequence_ref as ref
+from test_gpu_cache import Cache, as_int
+
+be = ops.backend
+cabi = be.cabi
+pytestmark = pytest.mark.gpu
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+# heads of a group and tokens: 1, 8, 12, 20, 64 and 160 rows
+ROWS = [(1, 1), (2, 4), (4, 3), (4, 5), (1, 64), (4, 40)]
+
+
+def present(c, b, n, T, table=None):
+    """Numbers of sequence b's cached and drafted keys that lie in a page of its table."""
+    table = c.table if table is None else table
+    room = table.shape[1] * c.page
+    return [j for j in range(min(n, room) + T) if j < room and 0 <= table[b, j // c.page].item() < c.k.shape[0]]
+
+
+def among(c, q, b, n, keys, sm, table=None):
+    """Results of sequence b's tokens (a chain) from those keys alone, the bounds, and p of [heads, T, keys]."""
+    table = c.table if table is None else table
+    n = min(n, table.shape[1] * c.page)
+    T, g = q.shape[2], q.shape[1] // c.k.shape[1]
+    at = torch.tensor(keys, dtype=torch.long, device="cuda")
+    page = table[b].long()[at // c.page]
+    k, v = (x[page, :, at % c.page].transpose(0, 1).repeat_interleave(g, 0)[None] for x in (c.k, c.v))
+    seen = at[None, :] <= n + torch.arange(T, device="cuda")[:, None]
+    res, tol = ref.attend(q[b][None], k, v, seen[None, None], (n + torch.arange(T, device="cuda")[:, None] - at).double()[None, None], sm)
+    s = sm * q[b].double() @ k[0].double().transpose(-1, -2)
+    p = torch.softmax(s.masked_fill(~seen, -math.inf), -1)
+    return {x: t[0] for x, t in res.items()}, {x: t[0] for x, t in tol.items()}, p, at
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("group,T", ROWS)
+@pytest.mark.parametrize("pages", [4, 200])
+def test_lengths_beyond_the_table(dtype, group, T, pages):
+    """Drafted keys that the table has no room for, or a length that it cannot hold, with rows of weights that end where the
+    table's room does: those keys are absent, the others are right, nobody else's weights change."""
+    page, Hkv = 16, 2
+    room = pages * page
+    few = min(40, room - T)
+    c = Cache([room - T, few, room - T], T, Hkv, 64, page, dtype, seed=T + pages)
+    assert c.slots == room
+    q = c.q(Hkv * group, T)
+    lens = [room - T + (T + 1) // 2, few, room + 1000]
+    out, lse = be.tree_sdpa(q, c.k, c.v, c.table, as_int(lens), 0.125)
+    assert cabi.lib().dsdpa_device_error(0) == cabi.ERR_DEVICE_BOUNDS
+    held = torch.rand(5, Hkv, room, generator=c.g, device="cuda")
+    before = held.clone()
+    be.cache_weights(held[1:4], q, lse, c.k, c.table, as_int(lens), 0.125)
+    assert cabi.lib().dsdpa_device_error(0) == cabi.ERR_DEVICE_BOUNDS
+    assert torch.equal(held[0], before[0]) and torch.equal(held[4], before[4])
+    for b, n in enumerate(lens):
+        keys = present(c, b, n, T)
+        res, tol, p, at = among(c, q, b, n, keys, 0.125)
+        ref.assert_within(out[b], res["out"], tol["out"], f"out of sequence {b}")
+        ref.assert_within(lse[b], res["lse"], tol["lse"], f"lse of sequence {b}")
+        add = p.view(Hkv, -1, *p.shape[-2:])
+        err = (add * (2 * tol["lse"].view(Hkv, -1, T, 1) + 2.0 ** -19)).sum((1, 2))
+        want = before[1 + b][:, at].double() + add.sum((1, 2))
+        ref.assert_within(held[1 + b][:, at], want, err + (group * T + 2) * ref.E32 * want.abs(), f"weights of sequence {b}")
+        other = torch.ones(room, dtype=torch.bool, device="cuda")
+        other[at] = False
+        assert torch.equal(held[1 + b][:, other], before[1 + b][:, other])
