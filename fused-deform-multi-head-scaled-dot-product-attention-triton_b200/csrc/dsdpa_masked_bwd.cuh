@@ -493,7 +493,7 @@ masked_dkdv_kernel(const __grid_constant__ MaskedParams p, const __grid_constant
         for (int e = 0; e < n; ++e) {
             const int qt = first + e % span, q0 = qt * kTileQ + half * 64;
             const float slope2 = BIAS ? __ldg(p.slopes + hk * p.group + e / span) * kLog2e : 0.0f;
-            const int4 t = __ldg(st.tiles + (long long)b * st.n + qt);
+            const int4 t = st.tiles[(long long)b * st.n + qt];          // written while this kernel was resident: not by the read-only path
             const bool partial = t.z > k0 || t.w < k0 + kTileK;
             const uint32_t neg_lse = tile_rows(e) + half * 64 * 4, neg_delta = neg_lse + kTileQ * 4;
             const uint32_t ranges = tile_rows(e) + L::kRowBytes + half * 64 * 8;
