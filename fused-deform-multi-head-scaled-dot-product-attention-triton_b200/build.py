@@ -43,11 +43,14 @@ def _nvcc() -> str:
 
 
 def _newest_source(src: Path, dep: Path) -> float:
-    """Newest of src and the repository's headers that nvcc found it to include (infinite while that is not known)."""
+    """Newest of src and the repository's headers that nvcc found it to include; infinite while that is not known, as in a
+    tree that was copied or moved with its objects, whose dependency files (absolute paths) name another one's headers."""
     if not dep.exists():
         return float("inf")
-    files = [Path(f) for f in dep.read_text().replace("\\\n", " ").split(":", 1)[1].split()]
-    own = [f for f in files if HERE.parent in f.resolve().parents] + [src]
+    files = [Path(f).resolve() for f in dep.read_text().replace("\\\n", " ").split(":", 1)[-1].split()]
+    if src.resolve() not in files:
+        return float("inf")
+    own = [f for f in files if HERE.parent in f.parents]
     return max(f.stat().st_mtime if f.exists() else float("inf") for f in own)
 
 
