@@ -229,7 +229,7 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
         c.cap_out = CAP ? p.cap * kLog2e : 0.0f;
         const float unit = CAP ? c.cap_out : c.scale2;    // of what cap_scores, or the product, left: scores in base 2
         int done = 0, info = 0;           // key tiles of this stream, of the block, so far
-        bool ok = true;
+        bool ok = true, again = false;
         TreeItem it;
         while (ok && walk.next(p, sp, it)) {
             const bool busy = quad * 32 < it.rows;        // this warp has rows
@@ -390,18 +390,30 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
                 if (it.part < 0) p.lse[row] = lse;
                 else sp.part_lse[part] = lse;
             }
-            // rows that something non-finite reached: once more, from the keys they see alone
+            // rows that something non-finite reached are marked by an lse of NaN, which no other row has, and done once more
+            // behind the loop: the other roles wait for this warp here, with limits
             const float nan = nan0 + nan1;
             const unsigned odd = it.part < 0 ? __ballot_sync(0xffffffffu, valid && nan != nan) : 0u;
             if (lane == 0) s_odd[quad][tile] = odd;
             tc_fence_before();
             pair_barrier(1 + quad);                       // both have read the accumulators; then the next products may write them
             if (tile == 0) {
-                unsigned bad = s_odd[quad][0] | s_odd[quad][1];
-                while (bad) {
-                    const int r = __ffs(bad) - 1;
+                const unsigned bad = s_odd[quad][0] | s_odd[quad][1];
+                again = again || bad != 0u;
+                if (bad >> lane & 1u) p.lse[row] = __int_as_float(0x7fffffff);
+            }
+        }
+        if (ok && again) {
+            walk = share.walk<TreeTile>();
+            while (walk.next(p, sp, it)) {
+                if (it.part >= 0) continue;               // tree_combine_kernel's
+                const int gr = it.row0 + in_tile, t = gr / p.group, h = it.hk * p.group + gr % p.group;
+                const bool valid = in_tile < it.rows;
+                const float lse = valid ? p.lse[((long long)it.b * p.Hq + h) * p.T + t] : 0.0f;
+                unsigned bad = __ballot_sync(0xffffffffu, lse != lse);
+                while (bad) {                             // from the keys that the row sees alone
+                    const int g = gr - lane + __ffs(bad) - 1;
                     bad &= bad - 1;
-                    const int g = gr - lane + r;
                     exact_row_tree<T>(p, it.b, it.hk * p.group + g % p.group, g / p.group);
                 }
             }

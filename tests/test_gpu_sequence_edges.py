@@ -1,5 +1,6 @@
 """Calls of the sequence operators at the ends of what their documentation allows, on every kernel that can take them:
 rows from one to more than 128 to a key/value head, caches that one block goes through and caches that are cut."""
+import copy
 import math
 
 import pytest
@@ -71,3 +72,41 @@ def test_lengths_beyond_the_table(dtype, group, T, pages):
         other = torch.ones(room, dtype=torch.bool, device="cuda")
         other[at] = False
         assert torch.equal(held[1 + b][:, other], before[1 + b][:, other])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("group,T", ROWS)
+@pytest.mark.parametrize("B,n", [(3, 50), (170, 150), (3, 5000), (70, 2500)])
+def test_non_finite_values_reach_the_rows_that_see_them_only(dtype, group, T, B, n):
+    """More sequences than blocks and caches that are cut: a NaN in the last token's value and in one sequence's first value,
+    and an infinity in a cached key's value of another sequence."""
+    D, sm = 64, 0.125
+    lens = [n + 7 * (b % 5) for b in range(B)]
+    c = Cache(lens, T, 1, D, 32, dtype, seed=T + n)
+    q = c.q(group, T)
+    for b, m in enumerate(lens):
+        if b % 3 != 2 or T == 1:
+            at = m + T - 1
+            c.v[c.table[b, at // 32].item(), :, at % 32] = math.nan
+    c.v[c.table[1, 0].item(), :, 0, 3] = math.nan
+    c.v[c.table[2, 1].item(), :, 1] = math.inf
+    out, lse = be.tree_sdpa(q, c.k, c.v, c.table, c.lens, sm)
+    for b, m in enumerate(lens):
+        if b in (1, 2):
+            bad = torch.zeros(D, dtype=torch.bool, device="cuda")
+            bad[3 if b == 1 else slice(None)] = True
+            assert not torch.isfinite(out[b, :, :, bad]).any()
+            assert torch.isfinite(out[b, :, :T - 1, ~bad]).all()
+        elif b % 3 != 2 or T == 1:
+            assert torch.isnan(out[b, :, T - 1]).all()
+    # the first sequences of the others, and the last one
+    others = [b for b in range(B) if b not in (1, 2)]
+    for b in others[:6] + others[-1:]:
+        res, tol, _, _ = among(c, q, b, lens[b], list(range(lens[b] + T)), sm)
+        ref.assert_within(lse[b], res["lse"], tol["lse"], f"lse of sequence {b}")
+        if T > 1:
+            rows = slice(0, T - 1) if b % 3 != 2 else slice(0, T)
+            clean = copy.copy(c)
+            clean.v = torch.nan_to_num(c.v, nan=0.0, posinf=0.0)
+            res, tol, _, _ = among(clean, q, b, lens[b], list(range(lens[b] + T)), sm)
+            ref.assert_within(out[b, :, rows], res["out"][:, rows], tol["out"][:, rows], f"out of sequence {b}")
