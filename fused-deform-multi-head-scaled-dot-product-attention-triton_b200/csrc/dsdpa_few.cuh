@@ -174,11 +174,15 @@ __device__ __forceinline__ void few_scores(const CacheParams& p, const TreeItem&
         }
     }
     if (p.cap > 0.0f) {
-        const float in = 2.0f * scale2 / p.cap, out = p.cap * kLog2e;
+        const float in = 2.0f * p.sm_scale / p.cap, out = p.cap * kLog2e;
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int c = 0; c < 2 * NR; ++c) s[j][c] = fmaf(-2.0f * out, rcp_approx(1.0f + fast_exp2(s[j][c] * in)), out);
+            for (int c = 0; c < 2 * NR; c += 2) {
+                const float2 t = half_tanh_any(mul2(make_float2(s[j][c], s[j][c + 1]), make_float2(in, in)));
+                s[j][c] = t.x * out;
+                s[j][c + 1] = t.y * out;
+            }
     } else {
 #pragma unroll
         for (int j = 0; j < 2; ++j)
@@ -229,21 +233,22 @@ struct FewState {
     }
     // 16 keys' weights, from their scores, and values
     __device__ __forceinline__ void add(float (&s)[2][4], const uint4 (&v)[4][HD / 64]) {
-        bool move = false;
+        bool move[NR], any = false;
         float top[NR];
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
             top[r] = fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1]));
             top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
             top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-            move = move || top[r] > m[r] + 8.0f || (m[r] == kNegInf && top[r] > kNegInf);
+            move[r] = top[r] > m[r] + 8.0f || (m[r] == kNegInf && top[r] > kNegInf);
+            any = any || move[r];
         }
-        // the reference points move when a row's maximum is more than 8 above its own
-        if (__any_sync(0xffffffffu, move)) {
+        // a row's reference point moves when its maximum is more than 8 above it, whatever the other rows' do
+        if (__any_sync(0xffffffffu, any)) {
 #pragma unroll
             for (int r = 0; r < NR; ++r) {
-                const float to = fmaxf(m[r], top[r]), f = to == kNegInf ? 1.0f : fast_exp2(m[r] - to);
-                m[r] = to;
+                const float f = move[r] ? fast_exp2(m[r] - top[r]) : 1.0f;
+                if (move[r]) m[r] = top[r];
                 l[r] *= f;
 #pragma unroll
                 for (int c = 0; c < HD / 64; ++c)

@@ -193,25 +193,25 @@ tree_few_f32_kernel(const __grid_constant__ CacheParams p, const __grid_constant
                 few.load(p, it, p.k, p.sk, k);
                 ahead = few.ask(p, it, k0 + 2 * F::kStep);
             }
-            // the reference points move when a row's maximum is more than 8 above its own
+            // a row's reference point moves when its maximum is more than 8 above it, whatever the other rows' do
             float top[NC][F::kHeld];
-            bool move = false;
+            bool move[NC][F::kHeld], any = false;
 #pragma unroll
             for (int c = 0; c < NC; ++c)
 #pragma unroll
                 for (int x = 0; x < F::kHeld; ++x) {
                     top[c][x] = few.over_keys(s[c][x], [](float a, float b) { return fmaxf(a, b); });
-                    move = move || top[c][x] > m[c][x] + 8.0f || (m[c][x] == kNegInf && top[c][x] > kNegInf);
+                    move[c][x] = top[c][x] > m[c][x] + 8.0f || (m[c][x] == kNegInf && top[c][x] > kNegInf);
+                    any = any || move[c][x];
                 }
-            if (__any_sync(0xffffffffu, move)) {
+            if (__any_sync(0xffffffffu, any)) {
 #pragma unroll
                 for (int c = 0; c < NC; ++c) {
                     float f[F::kHeld];
 #pragma unroll
                     for (int x = 0; x < F::kHeld; ++x) {
-                        const float to = fmaxf(m[c][x], top[c][x]);
-                        f[x] = to == kNegInf ? 1.0f : fast_exp2(m[c][x] - to);
-                        m[c][x] = to;
+                        f[x] = move[c][x] ? fast_exp2(m[c][x] - top[c][x]) : 1.0f;
+                        if (move[c][x]) m[c][x] = top[c][x];
                         l[c][x] *= f[x];
                     }
 #pragma unroll

@@ -135,7 +135,16 @@ __device__ __forceinline__ float2 half_tanh_small(float2 a) {
     return mul2(r, a);
 }
 __device__ __forceinline__ float half_tanh(float a) { return fmaf(-2.0f, rcp_approx(1.0f + fast_exp2(a * kLog2e)), 1.0f); }
-// Whether all of a warp's values are below 2 in magnitude: their top exponent bit says so (for NaN too).
+__device__ __forceinline__ bool is_small(float a) { return fabsf(a) < 2.0f; }
+// Any two values, each by the form that its own size asks for: what a score becomes does not depend on the others that a
+// warp happens to hold, hidden ones among them, and the general form, which is good to a step of 1, is not taken where
+// that is much of the result.  (Both forms for every value of a warp that has one above the cap: a forward all of whose
+// key tiles have some takes 224 us where the general form alone took 171, 4 x 16 heads of 2048, D = 64.)
+__device__ __forceinline__ float2 half_tanh_any(float2 a) {
+    const float2 t = half_tanh_small(a);
+    return make_float2(is_small(a.x) ? t.x : half_tanh(a.x), is_small(a.y) ? t.y : half_tanh(a.y));
+}
+// Whether all of a warp's values are small: their top exponent bit says so (NaN is not).
 template <int N>
 __device__ __forceinline__ bool all_small(const float (&a)[N]) {
     unsigned any = 0;

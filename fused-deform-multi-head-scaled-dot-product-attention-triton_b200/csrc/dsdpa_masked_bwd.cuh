@@ -55,7 +55,7 @@ __device__ __forceinline__ float scale_down(unsigned e) {
 template <bool CAP, bool SMALL>
 __device__ __forceinline__ float2 capped_pair(float2 a) {
     if (!CAP) return a;
-    return SMALL ? half_tanh_small(a) : make_float2(half_tanh(a.x), half_tanh(a.y));
+    return SMALL ? half_tanh_small(a) : half_tanh_any(a);
 }
 // The weights of two pairs from what capped_pair left; `slope` gets the factors that the cap's derivative
 // puts on ds: 1 - tanh^2.

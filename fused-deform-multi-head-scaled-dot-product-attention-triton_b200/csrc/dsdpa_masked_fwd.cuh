@@ -65,7 +65,11 @@ __device__ __forceinline__ void cap_scores(float (&s)[N], const ScoreConsts& c) 
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i) s[i] = half_tanh(s[i]);
+        for (int i = 0; i < N; i += 2) {
+            const float2 t = half_tanh_any(make_float2(s[i], s[i + 1]));
+            s[i] = t.x;
+            s[i + 1] = t.y;
+        }
     }
 }
 
@@ -332,8 +336,12 @@ masked_fwd_kernel(const __grid_constant__ MaskedParams p, const __grid_constant_
                     for (int i = kTanhTerms - 2; i >= 0; --i) t = fma2(t, u, make_float2(cap_term[i], cap_term[i]));
                     return fma2(t, v, to);
                 };
-                if (!small)
-                    weigh([&](int x) { return seen(x, fma2(make_float2(half_tanh(s[x]), half_tanh(s[x + 1])), scale, to)); });
+                // each by its own size, as half_tanh_any has it
+                auto any = [&](int x) {
+                    const float2 t = capped(x), g = fma2(make_float2(half_tanh(s[x]), half_tanh(s[x + 1])), scale, to);
+                    return make_float2(is_small(s[x]) ? t.x : g.x, is_small(s[x + 1]) ? t.y : g.y);
+                };
+                if (!small) weigh([&](int x) { return seen(x, any(x)); });
                 else if (partial) weigh([&](int x) { return seen(x, capped(x)); });
                 else weigh(capped);
             } else {

@@ -166,7 +166,8 @@ __device__ __forceinline__ float simt_store(T* row, const float2 (&acc)[SimtShap
     return nan;
 }
 // Products q.k to scores in base 2 without bias: s times the result.  With a cap s becomes tanh(x / cap), as a polynomial
-// where that is enough, by CUDA's tanhf where not (fp32 storage shows more than the short form's error).
+// where that is enough, by CUDA's tanhf where not (fp32 storage shows more than the short form's error): each score by its
+// own size, whatever the others are.
 template <int RM>
 __device__ __forceinline__ float simt_cap(float (&s)[RM][4], float sm_scale, float cap) {
     if (!(cap > 0.0f)) return sm_scale * kLog2e;
@@ -183,7 +184,11 @@ __device__ __forceinline__ float simt_cap(float (&s)[RM][4], float sm_scale, flo
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < 4 * RM; ++i) s[i / 4][i % 4] = tanhf(0.5f * a[i]);
+        for (int i = 0; i < 4 * RM; i += 2) {
+            const float2 t = half_tanh_small(make_float2(a[i], a[i + 1]));
+            s[i / 4][i % 4] = is_small(a[i]) ? t.x : tanhf(0.5f * a[i]);
+            s[i / 4][i % 4 + 1] = is_small(a[i + 1]) ? t.y : tanhf(0.5f * a[i + 1]);
+        }
     }
     return cap * kLog2e;
 }

@@ -110,3 +110,85 @@ def test_non_finite_values_reach_the_rows_that_see_them_only(dtype, group, T, B,
             clean.v = torch.nan_to_num(c.v, nan=0.0, posinf=0.0)
             res, tol, _, _ = among(clean, q, b, lens[b], list(range(lens[b] + T)), sm)
             ref.assert_within(out[b, :, rows], res["out"][:, rows], tol["out"][:, rows], f"out of sequence {b}")
+
+
+def capped_bounds(cap, uncapped):
+    """A capped form's results with bounds that have no term of the cap's own size: the scores' error is relative to them (the
+    polynomial is good to 3 units of 2^-24, the general form, taken from 0.76 cap on, to 4), which is 8 E32 |y| of the 16 that
+    the uncapped form's bound has.  For caps far above the scores the weights are the uncapped ones'."""
+    return cap[0], uncapped[1]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("softcap", [2.0 ** 14, 1e6, 1e12])
+@pytest.mark.parametrize("group,T", ROWS)
+@pytest.mark.parametrize("n", [150, 3000])
+def test_wide_caps_over_a_cache(dtype, softcap, group, T, n):
+    """A cap far above the scores leaves them as they are, to their own rounding."""
+    c = Cache([n, 40], T, 2, 64, 16, dtype, seed=T + n)
+    q, sm = c.q(2 * group, T), 0.3
+    out, lse = be.tree_sdpa(q, c.k, c.v, c.table, c.lens, sm, softcap=softcap)
+    w = torch.zeros(2, 2, c.slots, device="cuda")
+    be.cache_weights(w, q, lse, c.k, c.table, c.lens, sm, softcap=softcap)
+    for b, m in enumerate([n, 40]):
+        res, tol = capped_bounds(ref.tree_one(q[b], c.k, c.v, c.table[b], m, sm, softcap=softcap), ref.tree_one(q[b], c.k, c.v, c.table[b], m, sm))
+        ref.assert_within(out[b], res["out"], tol["out"], "out")
+        ref.assert_within(lse[b], res["lse"], tol["lse"], "lse")
+        p = among(c, q, b, m, list(range(m + T)), sm)[2].view(2, -1, T, m + T)      # uncapped: off by (x / cap)^2 x / 3 < 1e-7
+        want, err = p.sum((1, 2)), (p * (2 * tol["lse"].view(2, -1, T, 1) + 2.0 ** -19)).sum((1, 2))
+        ref.assert_within(w[b, :, :m + T], want, err + (group * T + 2) * ref.E32 * want, "weights")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D", [32, 64, 128, 256])
+@pytest.mark.parametrize("causal", [False, True])
+def test_one_score_above_a_wide_cap(dtype, D, causal):
+    """One query's scores above the cap, the others' far below it: these keep the precision of their own size."""
+    g = torch.Generator(device="cuda").manual_seed(D)
+    q, k, v = (torch.randn(1, 2, 200, D, generator=g, device="cuda").to(dtype) for _ in range(3))
+    q[:, :, 150] *= 4096
+    cap, sm = 4096.0, 2 * D ** -0.5
+    out, lse = be.masked_forward_raw(q, k, v, sm, causal=causal, softcap=cap)
+    keep = [i for i in range(200) if i != 150]
+    res, _ = ref.masked(q, k, v, sm, causal=causal, softcap=cap)
+    _, tol = ref.masked(q, k, v, sm, causal=causal)
+    for n, t in (("out", out), ("lse", lse)):
+        ref.assert_within(t[:, :, keep], res[n][:, :, keep], tol[n][:, :, keep], n)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D", [32, 64, 128, 256])
+@pytest.mark.parametrize("bias", [False, True])
+def test_hidden_scores_above_the_cap_change_no_bit(dtype, D, bias):
+    g = torch.Generator(device="cuda").manual_seed(D)
+    q, k, v, do = (torch.randn(1, 2, 190, D, generator=g, device="cuda").to(dtype) for _ in range(4))
+    kw = dict(causal=True, softcap=3.0, slopes=torch.tensor([0.1, 0.01], device="cuda") if bias else None)
+    q *= 0.1
+
+    def call():
+        out, lse = be.masked_forward_raw(q, k, v, 0.2, **kw)
+        return out, lse, be.masked_backward_raw(q, k, v, out, lse, do, 0.2, **kw)[0]
+    want = call()
+    for t in (q, k, v):
+        t[:, :, 189] = 300.0                # the last token's key, which nobody else sees, and its own row
+    for a, b in zip(call(), want):
+        assert torch.equal(a[:, :, :189], b[:, :, :189])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("group,T", ROWS[1:])
+@pytest.mark.parametrize("n", [70, 3000])
+def test_hidden_drafts_above_the_cap_change_no_bit(dtype, group, T, n):
+    c = Cache([n], T, 1, 64, 16, dtype, seed=T)
+    q = c.q(group, T) * 0.1
+    take = torch.ones(1, T, dtype=torch.bool, device="cuda")
+    take[:, -1] = False
+
+    def call():
+        out, lse = be.tree_sdpa(q, c.k, c.v, c.table, c.lens, 0.2, softcap=3.0)
+        w = be.cache_weights(torch.zeros(1, 1, c.slots, device="cuda"), q, lse, c.k, c.table, c.lens, 0.2, softcap=3.0, take=take)
+        return out[:, :, :-1], lse[:, :, :-1], w
+    want = call()
+    c.k[c.table[0, (n + T - 1) // 16].item(), :, (n + T - 1) % 16] = 300.0
+    q[:, :, -1] = 300.0
+    assert all(torch.equal(a, b) for a, b in zip(call(), want))
