@@ -92,52 +92,70 @@ __device__ __forceinline__ unsigned long long tokens_above(const CacheParams& p,
 __device__ __forceinline__ int depth_of(unsigned long long above) { return __popcll(above) - 1; }
 __device__ __forceinline__ int first_position(const CacheParams& p, int b, int n) { return p.start ? __ldg(p.start + b) : n; }
 
-// out and lse of one drafted token, by one warp.
+// out and lse of one drafted token, by one warp (as in dsdpa_masked.cuh).
 template <typename T>
 __device__ __noinline__ void exact_row_tree(const CacheParams& p, int b, int h, int t) {
-    const int lane = threadIdx.x & 31, hk = h / p.group;
+    constexpr int kSteps = 2;
+    const int lane = threadIdx.x & 31, hk = h / p.group, D = p.D;
+    const RowLanes rl(D, lane);
     const int n = cached_keys(p, b), real = drafted_tokens(p, b);
-    const float slope = p.slopes ? __ldg(p.slopes + h) : 0.0f;
-    float q[8], acc[8] = {}, m = kNegInf, l = 0.0f;
+    const float slope = p.slopes ? __ldg(p.slopes + h) : 0.0f, sm_scale = p.sm_scale, cap = p.cap;
+    float acc[8] = {};
+    RowSoftmax sum;
     if (t < real) {
         const unsigned long long above = tokens_above(p, b, t);
         const int base = first_position(p, b, n), pos = base + depth_of(above);
-        load_row<T>(row_of<T>(p.q, p.sq, b, h, t), p.D, lane, q);
-        int page = -1, page_index = -1;
-        for (int j = 0; j < n + real; ++j) {
-            if (j >= n && !(above >> (j - n) & 1)) continue;
-            const int index = j / p.page_size;
-            if (index != page_index) {
-                page_index = index;
-                page = page_of(p.table, p.width, p.pages, p.err, b, index);
-            }
-            if (page < 0) continue;
-            const int slot = j - index * p.page_size;
-            float k[8], v[8];
-            load_row<T>(row_of<T>(p.k, p.sk, 0, hk, slot) + page * p.sk[0], p.D, lane, k);
-            load_row<T>(row_of<T>(p.v, p.sv, 0, hk, slot) + page * p.sv[0], p.D, lane, v);
-            float s = soft_cap(p.sm_scale * warp_sum(dot8(q, k)), p.cap);
-            if (p.slopes) {
-                int at = j;
-                if (j >= n) at = base + depth_of(tokens_above(p, b, j - n));
-                else if (p.positions) at = __ldg(p.positions + ((long long)b * p.Hkv + hk) * p.slots + j);
-                s -= slope * fabsf((float)(pos - at));
-            }
-            s *= kLog2e;
-            if (s == kNegInf) continue;
-            const float m2 = fmaxf(m, s), c = exp2f(m - m2), w = exp2f(s - m2);
-            l = fmaf(l, c, w);
-            m = m2;
+        const T *k = row_of<T>(p.k, p.sk, 0, hk, 0), *v = row_of<T>(p.v, p.sv, 0, hk, 0);
+        float q[8];
+        load_piece<T>(row_of<T>(p.q, p.sq, b, h, t), rl.at, D, q);
+        for (int j0 = 0; j0 < n + real; j0 += kSteps * rl.places) {
+            RowPiece<T> kr[kSteps], vr[kSteps];
+            float s[kSteps], w[kSteps], f[8];
+            bool on[kSteps];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) acc[e] = fmaf(acc[e], c, w * v[e]);
+            for (int e = 0; e < kSteps; ++e) {
+                const int j = j0 + e * rl.places + rl.place, index = page_index(p.div, j);
+                int page = -1;
+                if (j < n + real && (j < n || (above >> (j - n) & 1))) page = page_of(p.table, p.width, p.pages, p.err, b, index);
+                on[e] = page >= 0;
+                const int slot = on[e] ? j - index * p.page_size : 0;
+                kr[e].load(k + max(page, 0) * p.sk[0] + slot * p.sk[2], rl.at, D);
+                vr[e].load(v + max(page, 0) * p.sv[0] + slot * p.sv[2], rl.at, D);
+            }
+#pragma unroll
+            for (int e = 0; e < kSteps; ++e) {
+                kr[e].get(rl.at, D, f);
+                s[e] = rl.row_sum(dot8(q, f));
+            }
+#pragma unroll
+            for (int e = 0; e < kSteps; ++e) {
+                const int j = j0 + e * rl.places + rl.place;
+                s[e] = soft_cap(sm_scale * s[e], cap);
+                if (p.slopes && on[e]) {
+                    int at = j;
+                    if (j >= n) at = base + depth_of(tokens_above(p, b, j - n));
+                    else if (p.positions) at = __ldg(p.positions + ((long long)b * p.Hkv + hk) * p.slots + j);
+                    s[e] -= slope * fabsf((float)(pos - at));
+                }
+                s[e] = on[e] ? s[e] * kLog2e : kNegInf;
+            }
+            const float c = sum.next(s, w);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[e] *= c;
+#pragma unroll
+            for (int e = 0; e < kSteps; ++e) {
+                vr[e].get(rl.at, D, f);
+                if (s[e] != kNegInf) add_piece(acc, w[e], f);
+            }
         }
     }
-    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+    sum.join(rl, acc);
+    const float inv = sum.l != 0.0f ? 1.0f / sum.l : 0.0f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) acc[e] *= inv;
     const long long row = ((long long)b * p.Hq + h) * p.T + t;
-    if (lane * 8 < p.D) store8<T>((T*)p.out + row * p.D + lane * 8, acc);
-    if (lane == 0) p.lse[row] = l != 0.0f ? m + log2f(l) : kNegInf;
+    if (rl.place == 0 && rl.at * 8 < D) store8<T>((T*)p.out + row * D + rl.at * 8, acc);
+    if (lane == 0) p.lse[row] = sum.l != 0.0f ? sum.m + log2f(sum.l) : kNegInf;
 }
 
 }  // namespace dsdpa

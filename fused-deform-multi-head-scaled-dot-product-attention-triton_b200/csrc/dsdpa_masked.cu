@@ -102,7 +102,7 @@ cudaError_t backward(const MaskedParams& p, void* workspace, cudaStream_t s) {
 }
 
 size_t backward_bytes(const dsdpa_masked_problem& p) {
-    const MaskedBwdSpace w = masked_bwd_space(p.dtype, p.B, p.Hq, p.Lq);
+    const MaskedBwdSpace w = masked_bwd_space(p.B, p.Hq, p.Lq);
     return p.dtype != DSDPA_F32 && p.D <= 128 ? w.bytes : w.stats;
 }
 

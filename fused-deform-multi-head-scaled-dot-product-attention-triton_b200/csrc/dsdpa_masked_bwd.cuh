@@ -36,12 +36,14 @@ __device__ __forceinline__ float4 lds_float4(uint32_t at) {
     return f;
 }
 
-// What masked_dq_kernel leaves for masked_dkdv_kernel, in whole tiles of 128 queries.
+// What masked_dq_kernel leaves for masked_dkdv_kernel, in whole tiles of 128 queries.  Odd queries are spoilt ones (what sees
+// them becomes NaN) and such as see no key but hold something non-finite: masked_dkdv_kernel keeps their rows out of
+// the sums that they have no part in.
 struct BwdStats {
-    float* stats;     // [B, Hq, tiles][2][128]: -lse (-inf: no weight), and -delta
+    float* stats;     // [B, Hq, tiles][2][128]: -lse (-inf: no weight; NaN: an odd query), and -delta
     int2* ranges;     // [B, tiles * 128]: visible keys
     int4* tiles;      // [B, tiles]: least lo, largest hi over rows that see something; largest lo, least hi over all rows
-    unsigned* amax;   // [B, Hq, tiles]: exponent field of the largest |dout| (fp16)
+    unsigned* amax;   // [B, Hq, tiles]: exponent field of the largest |dout| (fp16), plus 256 where the tile has an odd query
     int n;            // tiles of a sequence
 };
 
@@ -67,6 +69,30 @@ __device__ __forceinline__ float2 pair_weights(float2 t, float unit, float slope
     return make_float2(fast_exp2(s.x), fast_exp2(s.y));
 }
 
+// Rows of a block's tile that something non-finite reached (bits of `bad`, by warps of either half of the threads): once more, from
+// what they see alone, shared out over the block's warps.  A function of its own, which finds its place by itself:
+// nothing has to be kept for it while the block works.
+template <typename T, bool KEYS>
+__device__ __noinline__ void redo_rows(const MaskedParams& p, const unsigned* bad, int tiles) {
+    const int warp = threadIdx.x >> 5, heads = KEYS ? p.Hkv : p.Hq;
+    const int bh = blockIdx.x % (p.B * heads), b = bh / heads, h = bh % heads, block = (int)(blockIdx.x / (p.B * heads));
+    const int row0 = KEYS ? block * kTileK : (tiles - 1 - block) * kTileQ;
+    int turn = 0;
+    for (int quad = 0; quad < 4; ++quad)
+        for (unsigned rows = bad[quad] | bad[quad + 4]; rows; rows &= rows - 1) {
+            if (turn++ % (kBwdThreads / 32) != warp) continue;
+            const int row = row0 + quad * 32 + __ffs(rows) - 1;
+            if constexpr (KEYS) exact_row_dkdv<T>(p, b, h, row);
+            else exact_row_dq<T>(p, b, h, row);
+        }
+}
+__device__ __forceinline__ bool any_bad(const unsigned (&bad)[8]) {
+    unsigned any = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) any |= bad[i];
+    return any != 0u;
+}
+
 // d[128 x HD] (+)= w[128 x 128] b[128 x HD]; w's halves lie in columns 0 .. 31 and 64 .. 95 of its region, each
 // where the half of the scores was that the same threads have read.
 template <int HD>
@@ -89,7 +115,7 @@ masked_dq_kernel(const __grid_constant__ MaskedParams p, const __grid_constant__
     const uint32_t bar_q = bars, bar_s = bars + 8, bar_dp = bars + 24, bar_ds = bars + 32, bar_done = bars + 40, bar_full = bars + 48,
                    bar_empty = bar_full + 8 * L::kStages, slot = bar_empty + 8 * L::kStages;
     __shared__ int s_lo, s_hi, s_lomax, s_himin;
-    __shared__ unsigned s_top;
+    __shared__ unsigned s_top, s_odd;
     __shared__ float s_part[2][kTileQ];
     __shared__ unsigned char s_big[2][kTileQ];
     __shared__ unsigned s_bad[8];
@@ -99,7 +125,7 @@ masked_dq_kernel(const __grid_constant__ MaskedParams p, const __grid_constant__
     const int qt = st.n - 1 - (int)(blockIdx.x / (p.B * p.Hq)), q0 = qt * kTileQ;
 
     if (tid == 0) {
-        s_lo = 0x7fffffff; s_hi = 0; s_lomax = -1; s_himin = 0x7fffffff; s_top = 0;
+        s_lo = 0x7fffffff; s_hi = 0; s_lomax = -1; s_himin = 0x7fffffff; s_top = s_odd = 0;
         mbar_init(bar_q, 1);
         mbar_init(bar_s, 1);
         mbar_init(bar_s + 8, 1);
@@ -225,28 +251,46 @@ masked_dq_kernel(const __grid_constant__ MaskedParams p, const __grid_constant__
                     }
                 }
             }
+        } else if (row < p.Lq) {
+            // NaN where its rows hold something non-finite
+            const T* a = row_of<T>(p.q, p.sq, b, h, row);
+            const T* g = row_of<T>(p.dout, p.sdo, b, h, row);
+#pragma unroll
+            for (int z = 0; z < HD / 2; z += 8) {
+                const int d = half * (HD / 2) + z;
+                if (d < p.D) {
+                    float x[8], y[8];
+                    load8<T>(a + d, x);
+                    load8<T>(g + d, y);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) sum = fmaf(x[e], 0.0f, fmaf(y[e], 0.0f, sum));
+                }
+            }
         }
         s_part[half][in_tile] = sum;
         s_big[half][in_tile] = (unsigned char)(most >> 23);
         asm volatile("bar.sync 1, 256;" ::: "memory");
-        const float delta = s_part[0][in_tile] + s_part[1][in_tile];
+        float delta = s_part[0][in_tile] + s_part[1][in_tile];
         const unsigned big = max((unsigned)s_big[0][in_tile], (unsigned)s_big[1][in_tile]);
         const float sigma = kScaled ? scale_down(big) : 1.0f;
         const long long at = (long long)bh * p.Lq + row;
         float lse = sees ? p.lse[at] : kNegInf;
         if (lse == kNegInf) lse = -kNegInf;                 // weight exp2(s - inf) = 0
         if (half == 0) {
+            const bool odd = sees ? spoilt(lse, delta) : delta != delta;
+            if (odd) s_odd = 1;
             float* stats = st.stats + ((long long)bh * st.n + qt) * 2 * kTileQ + in_tile;
-            stats[0] = -lse;
-            stats[kTileQ] = -delta;
+            stats[0] = odd ? __int_as_float(0x7fffffff) : -lse;
+            stats[kTileQ] = odd || !sees ? 0.0f : -delta;
+            if (!sees) delta = 0.0f;
             if (h == 0) st.ranges[(long long)b * st.n * kTileQ + row] = r;
             if (row < p.Lq) p.delta[at] = delta;
             if (kScaled) {
-                const unsigned top = __reduce_max_sync(0xffffffffu, big);
+                const unsigned top = __reduce_max_sync(0xffffffffu, odd ? 0u : big);
                 if (lane == 0) atomicMax(&s_top, top);
             }
         }
-        const float ndelta = -delta * sigma;
+        const float ndelta = sees ? -delta * sigma : 0.0f;
         const int pos = row + (p.Lk - p.Lq);
         bool ok = true;
         for (int i = 0; i < n; ++i) {
@@ -327,7 +371,7 @@ masked_dq_kernel(const __grid_constant__ MaskedParams p, const __grid_constant__
                     }
                 }
             }
-            const unsigned bad = __ballot_sync(0xffffffffu, row < p.Lq && !fine);
+            const unsigned bad = __ballot_sync(0xffffffffu, n > 0 && row < p.Lq && !fine && !spoilt(lse, delta));
             if (lane == 0) s_bad[warp] = bad;
         } else if (lane == 0) s_bad[warp] = 0;
     }
@@ -335,16 +379,22 @@ masked_dq_kernel(const __grid_constant__ MaskedParams p, const __grid_constant__
     tc_fence_before();
     __syncthreads();
     if (warp == 9) tmem_free(tmem, 512);
-    if (kScaled && tid == 0) st.amax[(long long)bh * st.n + qt] = s_top;
-    // rows that something non-finite reached: once more, from the keys they see alone
-    if (n > 0 && warp < 4) {
-        unsigned bad = s_bad[warp] | s_bad[warp + 4];
-        while (bad) {
-            const int at = __ffs(bad) - 1;
-            bad &= bad - 1;
-            exact_row_dq<T>(p, b, h, row - lane + at);
-        }
+    if (tid == 0) st.amax[(long long)bh * st.n + qt] = s_top | s_odd << 8;
+    if (any_bad(s_bad)) redo_rows<T, false>(p, s_bad, st.n);
+}
+
+// The rows of a tile's odd queries to zero before any product reads them, by one thread: scores and dP^T of a query that a key does not
+// see are then finite whatever it holds, and the zeros of P^T and dS^T keep it out of the sums.
+template <int HD>
+__device__ __noinline__ void clear_odd_rows(uint32_t tile, uint32_t stats) {
+    for (int r = 0; r < kTileQ; ++r) {
+        float stat;
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(stat) : "r"(stats + r * 4) : "memory");
+        if (stat != stat)
+            for (int x = 0; x < HD / 8; ++x)
+                asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" :: "r"(tile + x / 8 * 128 * 128 + r * 128 + x % 8 * 16), "r"(0) : "memory");
     }
+    fence_proxy_async();
 }
 
 template <int HD>
@@ -369,7 +419,7 @@ masked_dkdv_kernel(const __grid_constant__ MaskedParams p, const __grid_constant
     const uint32_t bar_kv = bars, bar_qf = bars + 8, bar_qe = bars + 24, bar_of = bars + 40, bar_oe = bars + 56, bar_s = bars + 72,
                    bar_dp = bars + 80, bar_p = bars + 88, bar_ds = bars + 96, bar_done = bars + 104, slot = bars + 112;
     __shared__ int s_first, s_end;
-    __shared__ unsigned s_bad[8], s_top;
+    __shared__ unsigned s_bad[8], s_top, s_odd;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int bh = blockIdx.x % (p.B * p.Hkv), b = bh / p.Hkv, hk = bh % p.Hkv;
     const int k0 = (int)(blockIdx.x / (p.B * p.Hkv)) * kTileK;       // first keys first: with a causal mask most queries see them
@@ -378,7 +428,7 @@ masked_dkdv_kernel(const __grid_constant__ MaskedParams p, const __grid_constant
     auto tile_rows = [&](int e) { return sm_rows + (uint32_t)(e & 1) * 2 * L::kRowBytes; };
 
     if (tid == 0) {
-        s_first = 0x7fffffff; s_end = 0; s_top = 0;
+        s_first = 0x7fffffff; s_end = 0; s_top = s_odd = 0;
         mbar_init(bar_kv, 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(bar_qf + 8 * i, 1);
@@ -413,13 +463,16 @@ masked_dkdv_kernel(const __grid_constant__ MaskedParams p, const __grid_constant
     lo = warp_min(lo);
     hi = warp_max(hi);
     if (lane == 0) { atomicMin(&s_first, lo); atomicMax(&s_end, hi); }
-    if (kScaled) {
-        // the largest |dout| of the group's heads
+    {
+        // the largest |dout| of the group's heads, and whether they have odd queries
         const unsigned* from = st.amax + (long long)(b * p.Hq + hk * p.group) * st.n;
-        unsigned top = 0;
-        for (int i = tid; i < p.group * st.n; i += kBwdThreads) top = max(top, from[i]);
-        top = __reduce_max_sync(0xffffffffu, top);
-        if (lane == 0) atomicMax(&s_top, top);
+        unsigned top = 0, odd = 0;
+        for (int i = tid; i < p.group * st.n; i += kBwdThreads) { top = max(top, from[i] & 255u); odd |= from[i] >> 8; }
+        if (kScaled) {
+            top = __reduce_max_sync(0xffffffffu, top);
+            if (lane == 0) atomicMax(&s_top, top);
+        }
+        if (odd) s_odd = 1;
     }
     tc_fence_before();
     __syncthreads();
@@ -452,14 +505,20 @@ masked_dkdv_kernel(const __grid_constant__ MaskedParams p, const __grid_constant
             const uint32_t id_s = mma_desc<T>(kTileQ, false, negate != 0), id_dp = mma_desc<T>(kTileQ, false), id_g = mma_desc<T>(HD, true);
             const uint32_t t_dp = tmem + 128, t_dv = tmem + 256, t_dk = tmem + 384;
             bool ok = mbar_wait_bounded(bar_kv, 0, p.err) && n > 0;
+            auto clean = [&](int e, uint32_t tile) {
+                if (st.amax[((long long)b * p.Hq + hk * p.group + e / span) * st.n + first + e % span] >> 8) clear_odd_rows<HD>(tile, tile_rows(e));
+            };
+            const bool any_odd = s_odd != 0;
             auto score = [&](int e) {
                 if (!mbar_wait_bounded(bar_qf + 8 * (e & 1), (e >> 1) & 1, p.err)) return false;
+                if (any_odd) clean(e, tile_q(e));
                 mma_rows<HD>(tmem, sm_k, tile_q(e), kTileQ, id_s);
                 mma_commit(bar_s);
                 return true;
             };
             auto dprod = [&](int e) {
                 if (!mbar_wait_bounded(bar_of + 8 * (e & 1), (e >> 1) & 1, p.err)) return false;
+                if (any_odd) clean(e, tile_do(e));
                 mma_rows<HD>(t_dp, sm_v, tile_do(e), kTileQ, id_dp);
                 mma_commit(bar_dp);
                 return true;
@@ -592,7 +651,7 @@ masked_dkdv_kernel(const __grid_constant__ MaskedParams p, const __grid_constant
                     }
                 }
             }
-            const unsigned bad = __ballot_sync(0xffffffffu, key < p.Lk && !fine);
+            const unsigned bad = __ballot_sync(0xffffffffu, n > 0 && key < p.Lk && !fine);
             if (lane == 0) s_bad[warp] = bad;
         } else if (lane == 0) s_bad[warp] = 0;
     }
@@ -600,14 +659,7 @@ masked_dkdv_kernel(const __grid_constant__ MaskedParams p, const __grid_constant
     tc_fence_before();
     __syncthreads();
     if (warp == 9) tmem_free(tmem, 512);
-    if (n > 0 && warp < 4) {
-        unsigned bad = s_bad[warp] | s_bad[warp + 4];
-        while (bad) {
-            const int at = __ffs(bad) - 1;
-            bad &= bad - 1;
-            exact_row_dkdv<T>(p, b, hk, k0 + warp * 32 + at);
-        }
-    }
+    if (any_bad(s_bad)) redo_rows<T, true>(p, s_bad, 0);
 }
 
 }  // namespace dsdpa

@@ -37,8 +37,11 @@ struct FwdLayout {
 // exp2 of x <= 8, by the special-function unit.
 __device__ __forceinline__ float weight_exp2(float x) { return fast_exp2(x); }
 
+// The least positive number for 0, which it is in all but name for scores of any size.
+__device__ __forceinline__ float positive_scale(float sm_scale) { return fmaxf(fabsf(sm_scale) * kLog2e, __int_as_float(1)); }
+
 struct ScoreConsts {
-    float scale2;       // sm_scale log2(e), made positive (the sign is the matrix instruction's)
+    float scale2;       // sm_scale log2(e), made positive (the sign is the matrix instruction's); not 0: -inf times it is -inf
     float cap_in;       // 2 |sm_scale| / cap
     float cap_out;      // cap log2(e)
 };
@@ -92,6 +95,15 @@ __device__ __forceinline__ void add_bias(float (&s)[N], float unit, float slope2
     }
 }
 
+// A warp's rows whose values' sums something non-finite reached: once more, from the keys they see alone.  A function of its own, which
+// finds its place by itself: nothing has to be kept for it while the block works.
+template <typename T>
+__device__ __noinline__ void redo_rows_forward(const MaskedParams& p, const unsigned* bad, int qtiles) {
+    const int warp = threadIdx.x >> 5, bh = blockIdx.x % (p.B * p.Hq);
+    const int row0 = (qtiles - 1 - (int)(blockIdx.x / (p.B * p.Hq))) * 2 * kTileQ + warp * 32;
+    for (unsigned rows = bad[warp]; rows; rows &= rows - 1) exact_row_forward<T>(p, bh / p.Hq, bh % p.Hq, row0 + __ffs(rows) - 1);
+}
+
 __device__ __forceinline__ int warp_min(int x) { return __reduce_min_sync(0xffffffffu, x); }
 __device__ __forceinline__ int warp_max(int x) { return __reduce_max_sync(0xffffffffu, x); }
 
@@ -106,6 +118,7 @@ masked_fwd_kernel(const __grid_constant__ MaskedParams p, const __grid_constant_
     const uint32_t bar_q = bars, bar_s = bars + 8, bar_p = bars + 24, bar_o = bars + 40, bar_full = bars + 56,
                    bar_empty = bar_full + 8 * L::kStages, slot = bar_empty + 8 * L::kStages;
     __shared__ int s_lo[2], s_hi[2];
+    __shared__ unsigned s_bad[8];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     // longest rows first: with a causal mask these are the last ones
     const int bh = blockIdx.x % (p.B * p.Hq), b = bh / p.Hq, h = bh % p.Hq, hk = h / p.group;
@@ -237,7 +250,7 @@ masked_fwd_kernel(const __grid_constant__ MaskedParams p, const __grid_constant_
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;        // 32 lanes a warp, in the address's upper half
         const uint32_t s_at = tmem + tile * kTileK + lanes, o_at = tmem + 2 * kTileK + tile * HD + lanes;
         ScoreConsts c;
-        c.scale2 = fabsf(p.sm_scale) * kLog2e;
+        c.scale2 = positive_scale(p.sm_scale);
         c.cap_in = CAP ? 2.0f * fabsf(p.sm_scale) / p.cap : 0.0f;
         c.cap_out = CAP ? p.cap * kLog2e : 0.0f;
         const float unit = CAP ? c.cap_out : c.scale2;            // of what cap_scores, or the product, left: scores in base 2
@@ -383,20 +396,16 @@ masked_fwd_kernel(const __grid_constant__ MaskedParams p, const __grid_constant_
                 }
             }
             if (row < p.Lq) p.lse[(long long)bh * p.Lq + row] = l != 0.0f ? m + log2f(l) : kNegInf;
-            // rows that something non-finite reached: once more, from the keys they see alone
-            __syncwarp();
-            unsigned bad = __ballot_sync(0xffffffffu, row < p.Lq && !(fine && l == l));
-            while (bad) {
-                const int at = __ffs(bad) - 1;
-                bad &= bad - 1;
-                exact_row_forward<T>(p, b, h, row - lane + at);
-            }
-        }
+            // (a sum of weights that is NaN is the row's own)
+            const unsigned bad = __ballot_sync(0xffffffffu, row < p.Lq && !fine && l == l);
+            if (lane == 0) s_bad[warp] = bad;
+        } else if (lane == 0) s_bad[warp] = 0;
     }
     __syncwarp();
     tc_fence_before();
     __syncthreads();
     if (warp == 9) tmem_free(tmem, 512);
+    if (warp < 8 && s_bad[warp]) redo_rows_forward<T>(p, s_bad, qtiles);
 }
 
 }  // namespace dsdpa

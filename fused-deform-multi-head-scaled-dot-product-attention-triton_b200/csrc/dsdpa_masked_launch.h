@@ -24,13 +24,11 @@ template <typename T> cudaError_t launch_masked_bwd_simt(const MaskedParams& p, 
 struct MaskedBwdSpace {
     size_t stats, ranges, tiles, amax, bytes;
     int n;          // tiles of 128 queries
-    bool scaled;
 };
-inline MaskedBwdSpace masked_bwd_space(int dtype, int B, int Hq, int Lq) {
+inline MaskedBwdSpace masked_bwd_space(int B, int Hq, int Lq) {
     auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
     MaskedBwdSpace w{};
     w.n = (Lq + 127) / 128;
-    w.scaled = dtype == DSDPA_F16;
     w.stats = up((size_t)B * Hq * Lq * 4);
     w.ranges = w.stats + up((size_t)B * Hq * w.n * 128 * 8);
     w.tiles = w.ranges + up((size_t)B * w.n * 128 * 8);

@@ -311,7 +311,7 @@ masked_simt_fwd_kernel(const __grid_constant__ MaskedParams p, int qtiles) {
         const float nan = half_warp_sum(simt_store<T, HD>(out, acc[r], inv, p.D) + sum * 0.0f);
         if (i < p.Lq) {
             if (tx == 0) p.lse[(long long)bh * p.Lq + i] = sum != 0.0f ? m[r] + log2f(sum) : kNegInf;
-            if (nan != nan) bad |= 1u << r;
+            if (nan != nan && sum == sum) bad |= 1u << r;       // a sum of weights that is NaN is the row's own
         }
     }
     simt_redo<L::RM>(bad, [&](int r) { exact_row_forward<T>(p, b, h, q0 + r); });
@@ -400,7 +400,7 @@ masked_simt_dq_kernel(const __grid_constant__ MaskedParams p, int qtiles) {
         const int i = q0 + ty * L::RM + r;
         T* out = i < p.Lq ? row_of<T>(p.dq, p.sdq, b, h, i) : nullptr;
         const float nan = half_warp_sum(simt_store<T, HD>(out, acc[r], p.sm_scale, p.D));
-        if (i < p.Lq && nan != nan) bad |= 1u << r;
+        if (i < p.Lq && nan != nan && !spoilt(lse[r], delta[r])) bad |= 1u << r;
     }
     simt_redo<L::RM>(bad, [&](int r) { exact_row_dq<T>(p, b, h, q0 + r); });
 }
@@ -443,8 +443,18 @@ masked_simt_dkdv_kernel(const __grid_constant__ MaskedParams p) {
             const int q0 = t * L::BM;
             simt_load<T, HD, L::BM>(sq, row_of<T>(p.q, p.sq, b, h, 0), p.sq[2], q0, p.Lq, p.D);
             simt_load<T, HD, L::BM>(sg, row_of<T>(p.dout, p.sdo, b, h, 0), p.sdo[2], q0, p.Lq, p.D);
+            // queries without weight or spoilt: their rows, which may hold anything, out of the sums of rows to come
+            bool off = false;
+            if (tid < L::BM && q0 + tid < p.Lq) {
+                const long long row = ((long long)b * p.Hq + h) * p.Lq + q0 + tid;
+                off = p.lse[row] == kNegInf || spoilt(p.lse[row], p.delta[row]);
+            }
             simt_wait();
-            __syncthreads();
+            if (__syncthreads_or(off)) {
+                if (off)
+                    for (int d = 0; d < HD; ++d) sq[tid * L::S + d] = sg[tid * L::S + d] = 0.0f;
+                __syncthreads();
+            }
             float s[L::RM][4], dp[L::RM][4];
             simt_dot<HD>(sq, sk, s);
             simt_dot<HD>(sg, sv, dp);
@@ -458,8 +468,9 @@ masked_simt_dkdv_kernel(const __grid_constant__ MaskedParams p) {
                     rg = key_range(p, b, i);
                     const long long row = ((long long)b * p.Hq + h) * p.Lq + i;
                     lse = p.lse[row];
-                    if (lse == kNegInf) lse = -kNegInf;
                     delta = p.delta[row];
+                    if (spoilt(lse, delta)) lse = __int_as_float(0x7fffffff);       // all that sees it becomes NaN
+                    if (lse == kNegInf) lse = -kNegInf;
                 }
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {

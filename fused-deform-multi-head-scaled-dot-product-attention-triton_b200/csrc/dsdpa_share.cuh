@@ -146,7 +146,7 @@ __device__ __forceinline__ void find_share(const CacheParams& p, const TreeSplit
 // block of kCombineWarps: one where there are many rows, all where a few long caches leave many parts to each.
 constexpr int kCombineWarps = 8;
 template <typename T, typename Tile, int WARPS>
-__global__ void __launch_bounds__(kCombineWarps * 32) tree_combine_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeSplit sp) {
+__global__ void __launch_bounds__(kCombineWarps * 32, 3) tree_combine_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeSplit sp) {
     __shared__ __align__(16) float s_acc[WARPS > 1 ? kCombineWarps : 1][WARPS > 1 ? 256 : 1], s_sum[kCombineWarps];
     const int warp = threadIdx.x / 32, mine = warp % WARPS;           // the same row for all threads, or no barrier below
     const long long row = (long long)blockIdx.x * (kCombineWarps / WARPS) + warp / WARPS;

@@ -224,7 +224,7 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
         const int tile = warp >> 2, quad = warp & 3, in_tile = quad * 32 + lane;
         const uint32_t lanes = (uint32_t)quad << 21, s_col = tmem + tile * kTreeKeys + lanes, o_col = tmem + 256 + tile * HD + lanes;
         ScoreConsts c;
-        c.scale2 = fabsf(p.sm_scale) * kLog2e;
+        c.scale2 = positive_scale(p.sm_scale);
         c.cap_in = CAP ? 2.0f * fabsf(p.sm_scale) / p.cap : 0.0f;
         c.cap_out = CAP ? p.cap * kLog2e : 0.0f;
         const float unit = CAP ? c.cap_out : c.scale2;    // of what cap_scores, or the product, left: scores in base 2

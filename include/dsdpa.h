@@ -271,6 +271,9 @@ int dsdpa_describe_plan(const dsdpa_problem* p, char* text, size_t cap);
  * A query that sees no key gives out = 0 and lse = -inf, and zero gradients; so does one all of
  * whose scores are -inf.  Keys that a query does not see have no part in its results, whatever
  * they hold, NaN and infinity included; nor have queries that do not see a key in its gradients.
+ * Where something non-finite does have a part in a gradient -- a query whose row, or whose gradient, is
+ * not finite, in its dq and in dk and dv of all keys that it sees -- that row comes out non-finite, but
+ * which of its elements do, and whether as NaN or infinity, is not promised.
  * Strides are in elements; the last dimension (D) is contiguous.  Row starts are 16-byte aligned:
  * stride * element size is a multiple of 16 and so is every address.  D is a multiple of 8 up to 256.
  * Hq is a multiple of Hkv; query heads h*Hq/Hkv .. (h+1)*Hq/Hkv - 1 share key/value head h.

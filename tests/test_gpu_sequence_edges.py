@@ -192,3 +192,94 @@ def test_hidden_drafts_above_the_cap_change_no_bit(dtype, group, T, n):
     c.k[c.table[0, (n + T - 1) // 16].item(), :, (n + T - 1) % 16] = 300.0
     q[:, :, -1] = 300.0
     assert all(torch.equal(a, b) for a, b in zip(call(), want))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("where", ["dout", "dout element", "q", "out of nothing"])
+@pytest.mark.parametrize("softcap", [0.0, 5.0])
+def test_a_spoilt_query_spoils_what_it_sees_only(dtype, D, bad, where, softcap):
+    """Documents, causal: one query whose gradient or row is not finite.  Its own dq and the keys that it sees are not finite,
+    every other row is what it is without that query."""
+    vis = be.visible_ranges([130, 100, 70], prefix=[20, 0, 0], device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(D)
+    q, k, v, do = (torch.randn(1, h, 300, D, generator=g, device="cuda").to(dtype) for h in (4, 2, 2, 4))
+    sm, at, head = D ** -0.5, 180, 1
+    if where == "out of nothing":
+        vis[at] = 0                                           # the spoilt query sees no key at all: nobody is reached
+        do[0, head, at] = bad
+    elif where == "dout element":
+        do[0, head, at, 3] = bad
+    elif where == "dout":
+        do[0, head, at] = bad
+    clean_q, clean_do = q.clone(), do.clone()
+    if where == "q":
+        q[0, head, at] = bad
+    clean_do[0, head, at] = 0.0
+    kw = dict(visible=vis, softcap=softcap)
+    out, lse = be.masked_forward_raw(q, k, v, sm, **kw)
+    dq, dk, dv = be.masked_backward_raw(q, k, v, out, lse, do, sm, **kw)
+    res, tol = ref.masked(clean_q, k, v, sm, dout=clean_do, **kw)
+    own = torch.zeros(1, 4, 300, dtype=torch.bool, device="cuda")
+    own[0, head, at] = where != "out of nothing"
+    # with a cap an infinite q gives scores of plus and minus the cap: a row like any other until its gradient
+    rows = ~own
+    for n, t in (("out", out), ("lse", lse), ("dq", dq)):
+        ref.assert_within(t[rows], res[n][rows], tol[n][rows], n)
+    seen = torch.zeros(1, 2, 300, dtype=torch.bool, device="cuda")
+    if where != "out of nothing":
+        seen[0, head // 2, vis[at, 0]:vis[at, 1]] = True
+    for n, t in (("dk", dk), ("dv", dv)):
+        ref.assert_within(t[~seen], res[n][~seen], tol[n][~seen], n)
+    if where.startswith("dout"):
+        assert not torch.isfinite(dk[seen]).any() and not torch.isfinite(dq[own]).any()
+        assert not torch.isfinite(dv[seen][:, 3]).any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_an_infinite_value_spoils_one_column(dtype, D):
+    g = torch.Generator(device="cuda").manual_seed(D)
+    q, k, v, do = (torch.randn(1, h, 300, D, generator=g, device="cuda").to(dtype) for h in (4, 2, 2, 4))
+    clean = v.clone()
+    v[0, 1, 140, 5] = math.inf
+    out, lse = be.masked_forward_raw(q, k, v, D ** -0.5, causal=True)
+    res, tol = ref.masked(q, k, clean, D ** -0.5, causal=True)
+    bad = torch.zeros_like(out, dtype=torch.bool)
+    bad[0, 2:, 140:, 5] = True
+    ref.assert_within(out[~bad], res["out"][~bad], tol["out"][~bad], "out")
+    ref.assert_within(lse, res["lse"], tol["lse"], "lse")
+    assert (out[bad] == math.inf).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("what", ["one row", "one element", "all of it", "an element of each row"])
+def test_a_step_whose_loss_scale_overflowed_is_not_far_slower(dtype, what):
+    """Infinite gradients are an everyday thing where a 16-bit loss is scaled: the pass is to take a few times a finite one's
+    time, not hundreds of times it."""
+    L = 4096 if dtype == torch.float16 else 2048
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q, k, v, do = (torch.randn(1, h, L, 64, generator=g, device="cuda").to(dtype) for h in (8, 2, 2, 8))
+    out, lse = be.masked_forward_raw(q, k, v, 0.125, causal=True)
+
+    def time():
+        best = math.inf
+        for _ in range(4):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            be.masked_backward_raw(q, k, v, out, lse, do, 0.125, causal=True)
+            b.record()
+            torch.cuda.synchronize()
+            best = min(best, a.elapsed_time(b))
+        return best
+    usual = time()
+    if what == "one row":
+        do[0, 3, L // 2] = math.inf
+    elif what == "one element":
+        do[0, 3, L // 2, 7] = math.inf
+    elif what == "all of it":
+        do.fill_(math.inf)
+    else:
+        do[..., 7] = math.inf
+    assert time() < 40 * usual
