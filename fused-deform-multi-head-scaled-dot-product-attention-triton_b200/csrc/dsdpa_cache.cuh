@@ -91,6 +91,15 @@ __device__ __forceinline__ unsigned long long tokens_above(const CacheParams& p,
 }
 __device__ __forceinline__ int depth_of(unsigned long long above) { return __popcll(above) - 1; }
 __device__ __forceinline__ int first_position(const CacheParams& p, int b, int n) { return p.start ? __ldg(p.start + b) : n; }
+// Positions are taken from that of a drafted token without parent on: a drafted token's is then its depth, and a cached key's
+// far behind it, whatever the numbers themselves are, off by no more than the distance's own rounding to fp32.
+__device__ __forceinline__ float from_first(int at, int first) {       // the halves' differences are exact, and so is their sum up to one rounding
+    return fmaf((float)((at >> 16) - (first >> 16)), 65536.0f, (float)((at & 0xffff) - (first & 0xffff)));
+}
+// Position of cached key j of head hk.
+__device__ __forceinline__ float key_position(const CacheParams& p, int b, int hk, int j, int first) {
+    return from_first(p.positions ? __ldg(p.positions + ((long long)b * p.Hkv + hk) * p.slots + j) : j, first);
+}
 
 // out and lse of one drafted token, by one warp (as in dsdpa_masked.cuh).
 template <typename T>
@@ -104,7 +113,7 @@ __device__ __noinline__ void exact_row_tree(const CacheParams& p, int b, int h, 
     RowSoftmax sum;
     if (t < real) {
         const unsigned long long above = tokens_above(p, b, t);
-        const int base = first_position(p, b, n), pos = base + depth_of(above);
+        const int base = first_position(p, b, n), depth = depth_of(above);
         const T *k = row_of<T>(p.k, p.sk, 0, hk, 0), *v = row_of<T>(p.v, p.sv, 0, hk, 0);
         float q[8];
         load_piece<T>(row_of<T>(p.q, p.sq, b, h, t), rl.at, D, q);
@@ -132,10 +141,8 @@ __device__ __noinline__ void exact_row_tree(const CacheParams& p, int b, int h, 
                 const int j = j0 + e * rl.places + rl.place;
                 s[e] = soft_cap(sm_scale * s[e], cap);
                 if (p.slopes && on[e]) {
-                    int at = j;
-                    if (j >= n) at = base + depth_of(tokens_above(p, b, j - n));
-                    else if (p.positions) at = __ldg(p.positions + ((long long)b * p.Hkv + hk) * p.slots + j);
-                    s[e] -= slope * fabsf((float)(pos - at));
+                    const float at = j >= n ? (float)depth_of(tokens_above(p, b, j - n)) : key_position(p, b, hk, j, base);
+                    s[e] -= slope * fabsf((float)depth - at);
                 }
                 s[e] = on[e] ? s[e] * kLog2e : kNegInf;
             }

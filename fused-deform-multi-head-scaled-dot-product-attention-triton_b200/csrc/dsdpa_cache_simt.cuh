@@ -52,17 +52,15 @@ __device__ __forceinline__ void simt_tokens(const CacheParams& p, const TreeItem
 }
 
 // What a tile's keys are, by threads 0 .. 63: their pages (-1: absent) and positions.
-__device__ __forceinline__ void simt_keys(const CacheParams& p, const TreeItem& it, const SimtTokens& tokens, int k0, int* s_page, int* s_at) {
+__device__ __forceinline__ void simt_keys(const CacheParams& p, const TreeItem& it, const SimtTokens& tokens, int k0, int* s_page, float* s_at) {
     const int t = threadIdx.x;
     if (t >= kSimtKeys) return;
     const int j = k0 + t;
-    int page = -1, at = j;
+    int page = -1;
+    float at = 0.0f;
     if (j < it.n + it.real) {
         page = page_of(p.table, p.width, p.pages, p.err, it.b, page_index(p.div, j));
-        if (p.slopes) {
-            if (j >= it.n) at = first_position(p, it.b, it.n) + depth_of(tokens.above[j - it.n]);
-            else if (p.positions) at = __ldg(p.positions + ((long long)it.b * p.Hkv + it.hk) * p.slots + j);
-        }
+        if (p.slopes) at = j >= it.n ? (float)depth_of(tokens.above[j - it.n]) : key_position(p, it.b, it.hk, j, first_position(p, it.b, it.n));
     }
     s_page[t] = page;
     s_at[t] = at;
@@ -76,7 +74,8 @@ tree_simt_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ 
     using Tile = typename C::Tile;
     extern __shared__ float4 simt_smem[];
     float *sq = reinterpret_cast<float*>(simt_smem), *sk = sq + L::BM * L::S, *sv = sk + kSimtKeys * L::S, *sw = sv + kSimtKeys * L::S;
-    __shared__ int s_page[2][kSimtKeys], s_at[2][kSimtKeys];
+    __shared__ int s_page[2][kSimtKeys];
+    __shared__ float s_at[2][kSimtKeys];
     __shared__ TreeShare<kSimtThreads> share;
     __shared__ SimtTokens tokens;
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
@@ -103,7 +102,7 @@ tree_simt_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ 
             real[r] = in_tile < it.rows && t < it.real;
             above[r] = real[r] ? tokens.above[t] : 0ull;
             slope2[r] = p.slopes && real[r] ? __ldg(p.slopes + h) * kLog2e : 0.0f;
-            pos[r] = p.slopes && real[r] ? (float)(first_position(p, it.b, it.n) + depth_of(above[r])) : 0.0f;
+            pos[r] = p.slopes && real[r] ? (float)depth_of(above[r]) : 0.0f;
             m[r] = kNegInf;
             l[r] = 0.0f;
         }
@@ -134,7 +133,7 @@ tree_simt_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ 
                 for (int c = 0; c < 4; ++c) {
                     const int key = k0 + tx + 16 * c, draft = key - it.n;
                     float x = s[r][c] * unit;
-                    if (p.slopes) x = fmaf(-slope2[r], fabsf(pos[r] - (float)s_at[cur][tx + 16 * c]), x);
+                    if (p.slopes) x = fmaf(-slope2[r], fabsf(pos[r] - s_at[cur][tx + 16 * c]), x);
                     const bool sees = real[r] && s_page[cur][tx + 16 * c] >= 0 && (draft < 0 || (above[r] >> (draft & 63) & 1u));
                     s[r][c] = sees ? x : kNegInf;
                     top = fmaxf(top, s[r][c]);
@@ -191,7 +190,8 @@ weights_simt_kernel(const __grid_constant__ CacheParams p, const __grid_constant
     using Tile = typename C::Tile;
     extern __shared__ float4 simt_smem[];
     float *sq = reinterpret_cast<float*>(simt_smem), *sk = sq + L::BM * L::S, *part = sk + kSimtKeys * L::S;
-    __shared__ int s_page[kSimtKeys], s_at[kSimtKeys];
+    __shared__ int s_page[kSimtKeys];
+    __shared__ float s_at[kSimtKeys];
     __shared__ TreeShare<kSimtThreads> share;
     __shared__ SimtTokens tokens;
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
@@ -222,7 +222,7 @@ weights_simt_kernel(const __grid_constant__ CacheParams p, const __grid_constant
                     above[r] = tokens.above[t];
                     if (p.slopes) {
                         slope2[r] = __ldg(p.slopes + h) * kLog2e;
-                        pos[r] = (float)(first_position(p, it.b, it.n) + depth_of(above[r]));
+                        pos[r] = (float)depth_of(above[r]);
                     }
                 }
             }
@@ -256,7 +256,7 @@ weights_simt_kernel(const __grid_constant__ CacheParams p, const __grid_constant
                     for (int c = 0; c < 4; ++c) {
                         const int draft = k0 + tx + 16 * c - it.n;
                         float x = s[r][c] * unit;
-                        if (p.slopes) x = fmaf(-slope2[r], fabsf(pos[r] - (float)s_at[tx + 16 * c]), x);
+                        if (p.slopes) x = fmaf(-slope2[r], fabsf(pos[r] - s_at[tx + 16 * c]), x);
                         const bool sees = lse[r] != -kNegInf && (draft < 0 || (above[r] >> (draft & 63) & 1u));
                         sum[c] += sees ? fast_exp2(x - lse[r]) : 0.0f;
                     }

@@ -56,7 +56,7 @@ __device__ __forceinline__ void few_queries(const CacheParams& p, const TreeItem
         row[s].masked = valid && !row[s].real;
         row[s].above = row[s].real ? tokens_above(p, it.b, t) : 0ull;
         row[s].slope2 = p.slopes && valid ? __ldg(p.slopes + h) * kLog2e : 0.0f;
-        row[s].pos = p.slopes && row[s].real ? (float)(first_position(p, it.b, it.n) + depth_of(row[s].above)) : 0.0f;
+        row[s].pos = p.slopes && row[s].real ? (float)depth_of(row[s].above) : 0.0f;
         if (valid) src[s] = row_of<T>(p.q, p.sq, it.b, h, t);
     }
     __syncwarp();                                        // the last unit's are read
@@ -190,16 +190,17 @@ __device__ __forceinline__ void few_scores(const CacheParams& p, const TreeItem&
             for (int c = 0; c < 2 * NR; ++c) s[j][c] *= scale2;
     }
     if (p.slopes) {
+        const int base = first_position(p, it.b, it.n);
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int key = k0 + 8 * j + 2 * t4 + e;
-                int at = key;
-                if (key >= it.n) at = key < it.n + it.real ? first_position(p, it.b, it.n) + depth_of(tokens_above(p, it.b, key - it.n)) : 0;
-                else if (p.positions) at = __ldg(p.positions + ((long long)it.b * p.Hkv + it.hk) * p.slots + key);
+                float at = 0.0f;
+                if (key < it.n) at = key_position(p, it.b, it.hk, key, base);
+                else if (key < it.n + it.real) at = (float)depth_of(tokens_above(p, it.b, key - it.n));
 #pragma unroll
-                for (int r = 0; r < NR; ++r) s[j][2 * r + e] = fmaf(-row[r].slope2, fabsf(row[r].pos - (float)at), s[j][2 * r + e]);
+                for (int r = 0; r < NR; ++r) s[j][2 * r + e] = fmaf(-row[r].slope2, fabsf(row[r].pos - at), s[j][2 * r + e]);
             }
     }
     if (!__all_sync(0xffffffffu, there == 0xffffu && k0 + 16 <= it.n && !row[0].masked && !row[NR - 1].masked)) {

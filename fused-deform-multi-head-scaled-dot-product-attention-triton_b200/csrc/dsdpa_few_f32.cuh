@@ -49,7 +49,7 @@ struct F32Few {
             r.real = valid && t < it.real;
             r.above = r.real ? tokens_above(p, it.b, t) : 0ull;
             r.slope2 = p.slopes && valid ? __ldg(p.slopes + h) * kLog2e : 0.0f;
-            r.pos = p.slopes && r.real ? (float)(first_position(p, it.b, it.n) + depth_of(r.above)) : 0.0f;
+            r.pos = p.slopes && r.real ? (float)depth_of(r.above) : 0.0f;
             rows[lane] = r;
         }
 #pragma unroll
@@ -131,10 +131,9 @@ struct F32Few {
                 const bool sees = row.real && (now >> in_step & 1u) && (draft < 0 || (row.above >> (draft & 63) & 1u));
                 float y = soft_cap(p.sm_scale * x[v], p.cap) * kLog2e;
                 if (p.slopes && sees) {
-                    int where = j;
-                    if (draft >= 0) where = first_position(p, it.b, it.n) + depth_of(tokens_above(p, it.b, draft));
-                    else if (p.positions) where = __ldg(p.positions + ((long long)it.b * p.Hkv + it.hk) * p.slots + j);
-                    y = fmaf(-row.slope2, fabsf(row.pos - (float)where), y);
+                    const float where = draft >= 0 ? (float)depth_of(tokens_above(p, it.b, draft))
+                                                   : key_position(p, it.b, it.hk, j, first_position(p, it.b, it.n));
+                    y = fmaf(-row.slope2, fabsf(row.pos - where), y);
                 }
                 s[c][v] = sees ? y : kNegInf;
             }

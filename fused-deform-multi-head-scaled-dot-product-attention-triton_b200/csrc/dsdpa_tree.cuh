@@ -62,7 +62,7 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
     const uint32_t bar_s = bars, bar_p = bars + 16, bar_o = bars + 32, bar_qe = bars + 48, bar_full = bars + 64,
                    bar_empty = bar_full + 8 * L::kStages, slot = bar_empty + 8 * L::kStages;
     __shared__ unsigned s_valid[kInfo][4];                 // keys of a tile that are there
-    __shared__ float s_at[BIAS ? kInfo : 1][kTreeKeys];    // their positions
+    __shared__ float s_at[BIAS ? kInfo : 1][kTreeKeys];    // their positions, from the first drafted token's on
     __shared__ float s_m[2][kTreeRows], s_l[2][kTreeRows]; // what the streams tell one another
     __shared__ unsigned s_odd[4][2];
     __shared__ TreeShare<kTreeThreads> share;
@@ -185,12 +185,10 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
                     const unsigned valid = __ballot_sync(0xffffffffu, src != nullptr);
                     if (lane == 0) s_valid[info][w] = valid;
                     if (BIAS) {
-                        int pos = j;
-                        if (src != nullptr) {
-                            if (j >= it.n) pos = first_position(p, it.b, it.n) + depth_of(tokens_above(p, it.b, j - it.n));
-                            else if (p.positions) pos = __ldg(p.positions + ((long long)it.b * p.Hkv + it.hk) * p.slots + j);
-                        }
-                        s_at[info][w * 32 + lane] = (float)pos;
+                        float pos = 0.0f;
+                        if (src != nullptr)
+                            pos = j >= it.n ? (float)depth_of(tokens_above(p, it.b, j - it.n)) : key_position(p, it.b, it.hk, j, first_position(p, it.b, it.n));
+                        s_at[info][w * 32 + lane] = pos;
                     }
                     info = (info + 1) % kInfo;
                 }
@@ -237,7 +235,7 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
             const bool valid = in_tile < it.rows, real = valid && t < it.real;
             unsigned long long above = real ? tokens_above(p, it.b, t) : 0ull;
             const float slope2 = BIAS && valid ? __ldg(p.slopes + h) * kLog2e : 0.0f;
-            const float pos = BIAS && real ? (float)(first_position(p, it.b, it.n) + depth_of(above)) : 0.0f;
+            const float pos = BIAS && real ? (float)depth_of(above) : 0.0f;
             float m = kNegInf, l = 0.0f;
             int mine = 0;
             for (int i = tile; i < it.tiles; i += 2, ++mine) {
@@ -263,7 +261,7 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
                         if (BIAS) {
                             // cached keys at their own numbers lie before every query that starts behind them
                             if (linear) {
-                                add_bias(s, unit, slope2, pos - (float)(k0 + w * 32), true);
+                                add_bias(s, unit, slope2, pos - from_first(k0 + w * 32, it.n), true);
                             } else {
 #pragma unroll
                                 for (int x = 0; x < 32; ++x) s[x] = fmaf(-slope2, fabsf(pos - s_at[slot_i][w * 32 + x]), s[x] * unit);

@@ -111,7 +111,7 @@ weights_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ Tr
                 s_lse[buf][col] = lse;
                 s_above[buf][col] = above;
                 if (BIAS) {
-                    s_pos[buf][col] = above ? (float)(first_position(p, it.b, it.n) + depth_of(above)) : 0.0f;
+                    s_pos[buf][col] = above ? (float)depth_of(above) : 0.0f;
                     s_slope[buf][col] = valid ? __ldg(p.slopes + h) * kLog2e : 0.0f;
                 }
                 for (int i = 0; i < it.tiles; ++i) {
@@ -156,11 +156,9 @@ weights_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ Tr
                     // a drafted key that the table has no room for is behind the row of weights too
                     const bool exists = draft < it.real && j < p.width * p.page_size;
                     const float old = exists ? out[j] : 0.0f;
-                    float at = (float)j;
-                    if (BIAS && exists) {
-                        if (draft >= 0) at = (float)(first_position(p, it.b, it.n) + depth_of(tokens_above(p, it.b, draft)));
-                        else if (p.positions) at = (float)__ldg(p.positions + ((long long)it.b * p.Hkv + it.hk) * p.slots + j);
-                    }
+                    float at = 0.0f;
+                    if (BIAS && exists)
+                        at = draft >= 0 ? (float)depth_of(tokens_above(p, it.b, draft)) : key_position(p, it.b, it.hk, j, first_position(p, it.b, it.n));
                     const int buffer = side * 2 + (m & 1);
                     if (!(ok = mbar_wait_bounded(bar_s + 8 * buffer, (m >> 1) & 1, p.err))) break;
                     ++m;

@@ -8,7 +8,7 @@ import torch
 
 import ops
 import sequence_ref as ref
-from test_gpu_cache import Cache, as_int
+from test_gpu_cache import Cache, as_int, check, random_tree
 
 be = ops.backend
 cabi = be.cabi
@@ -283,3 +283,16 @@ def test_a_step_whose_loss_scale_overflowed_is_not_far_slower(dtype, what):
     else:
         do[..., 7] = math.inf
     assert time() < 40 * usual
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("group,T", ROWS)
+@pytest.mark.parametrize("n", [150, 3000])
+@pytest.mark.parametrize("first", [0, 2 ** 30 + 1, 2 ** 31 - 1, -2 ** 31 + 5000])
+def test_positions_far_from_zero(dtype, group, T, n, first):
+    """Distances count, not positions: numbers that fp32 cannot tell apart, and ones next to the ends of int32."""
+    c = Cache([n, 40], T, 2, 64, 16, dtype, seed=T + n)
+    ago = torch.sort(torch.randint(0, 4000, (2, 2, c.slots), generator=c.g, device="cuda"), -1, descending=True).values
+    positions = (first - ago).clamp_min(-2 ** 31).int()
+    check(c, c.q(2 * group, T), 0.125, parents=random_tree(2, T, n) if T > 1 else None, positions=positions, start=[first, first - 1],
+          slopes=torch.linspace(0.2, 0.001, 2 * group, device="cuda"))
