@@ -8,9 +8,9 @@
 //
 // Every gradient has one writer and one order of sums, so two runs give the same bits; the price, against
 // one kernel that adds dq up with atomics, is seven products a tile pair instead of five.  P and dS go to
-// tensor memory in the storage type, as operands; everything before them and every sum is fp32.  For
-// fp16 dS is scaled by a power of two (of the largest |dout|, of the row or of the whole group), since
-// a loss that is scaled far down would take it out of the type's range.
+// tensor memory in the storage type, as operands; everything before them and every sum is fp32.  For fp16 P^T is
+// scaled by 2^15 and dS by a power of two: dq's by the row's largest |dout|, dk's by a bound of what the key's row of dS^T can
+// hold, since even weights of many keys, or a loss that is scaled far down, would take them out of the type's range.
 // Both kernels: 8 warps of elementwise work (a thread has one row and 64 of its 128 columns), one warp of
 // TMA loads, one that issues the matrix instructions.
 //
@@ -43,13 +43,24 @@ struct BwdStats {
     float* stats;     // [B, Hq, tiles][2][128]: -lse (-inf: no weight; NaN: an odd query), and -delta
     int2* ranges;     // [B, tiles * 128]: visible keys
     int4* tiles;      // [B, tiles]: least lo, largest hi over rows that see something; largest lo, least hi over all rows
-    unsigned* amax;   // [B, Hq, tiles]: exponent field of the largest |dout| (fp16), plus 256 where the tile has an odd query
+    unsigned* amax;   // [B, Hq, tiles]: bit 8: the tile has an odd query; fp16: exponent fields of the largest |dout| (bits 0-7) and
+                      // the largest |delta| (bits 16-23) of the others
     int n;            // tiles of a sequence
 };
 
 // 2^-e for numbers in [2^e, 2^(e+1)), from their exponent field; 1 for zero, infinity and NaN.
 __device__ __forceinline__ float scale_down(unsigned e) {
     return e == 0 || e >= 254 ? 1.0f : __uint_as_float((unsigned)(254 - e) << 23);
+}
+
+// Power of two that P^T of fp16 is scaled by: weights are at most 1, the type's largest number is above 2^15.
+constexpr float kWeightBits = 15.0f, kWeightUp = 32768.0f;
+// Scale of dS of a key whose row of V has the sum of magnitudes `norm`, from the exponent fields of the largest |dout| and
+// |delta|: |dp - delta| < 2^(fields - 126) each way, so that dS, whose weights are at most 1, stays below 2^14.
+__device__ __forceinline__ float scale_up(float norm, unsigned dout, unsigned delta) {
+    const float most = fmaf(norm, __uint_as_float(min(dout + 1u, 254u) << 23), __uint_as_float(min(delta + 1u, 254u) << 23));
+    const unsigned e = __float_as_uint(most) >> 23;             // most < 2^(e - 126)
+    return e >= 254u ? 1.0f : __uint_as_float(min(267u - e, 200u) << 23);
 }
 
 // Two products that scale_scores has been at to tanh(x / cap); as they are where there is no cap.  Done pair by pair with what
@@ -115,7 +126,7 @@ masked_dq_kernel(const __grid_constant__ MaskedParams p, const __grid_constant__
     const uint32_t bar_q = bars, bar_s = bars + 8, bar_dp = bars + 24, bar_ds = bars + 32, bar_done = bars + 40, bar_full = bars + 48,
                    bar_empty = bar_full + 8 * L::kStages, slot = bar_empty + 8 * L::kStages;
     __shared__ int s_lo, s_hi, s_lomax, s_himin;
-    __shared__ unsigned s_top, s_odd;
+    __shared__ unsigned s_top, s_delta, s_odd;
     __shared__ float s_part[2][kTileQ];
     __shared__ unsigned char s_big[2][kTileQ];
     __shared__ unsigned s_bad[8];
@@ -125,7 +136,7 @@ masked_dq_kernel(const __grid_constant__ MaskedParams p, const __grid_constant__
     const int qt = st.n - 1 - (int)(blockIdx.x / (p.B * p.Hq)), q0 = qt * kTileQ;
 
     if (tid == 0) {
-        s_lo = 0x7fffffff; s_hi = 0; s_lomax = -1; s_himin = 0x7fffffff; s_top = s_odd = 0;
+        s_lo = 0x7fffffff; s_hi = 0; s_lomax = -1; s_himin = 0x7fffffff; s_top = s_delta = s_odd = 0;
         mbar_init(bar_q, 1);
         mbar_init(bar_s, 1);
         mbar_init(bar_s + 8, 1);
@@ -280,14 +291,15 @@ masked_dq_kernel(const __grid_constant__ MaskedParams p, const __grid_constant__
             const bool odd = sees ? spoilt(lse, delta) : delta != delta;
             if (odd) s_odd = 1;
             float* stats = st.stats + ((long long)bh * st.n + qt) * 2 * kTileQ + in_tile;
-            stats[0] = odd ? __int_as_float(0x7fffffff) : -lse;
+            stats[0] = odd ? __int_as_float(0x7fffffff) : kScaled ? kWeightBits - lse : -lse;
             stats[kTileQ] = odd || !sees ? 0.0f : -delta;
             if (!sees) delta = 0.0f;
             if (h == 0) st.ranges[(long long)b * st.n * kTileQ + row] = r;
             if (row < p.Lq) p.delta[at] = delta;
             if (kScaled) {
                 const unsigned top = __reduce_max_sync(0xffffffffu, odd ? 0u : big);
-                if (lane == 0) atomicMax(&s_top, top);
+                const unsigned most = __reduce_max_sync(0xffffffffu, odd ? 0u : (__float_as_uint(delta) & 0x7fffffffu) >> 23);
+                if (lane == 0) { atomicMax(&s_top, top); atomicMax(&s_delta, most); }
             }
         }
         const float ndelta = sees ? -delta * sigma : 0.0f;
@@ -379,7 +391,7 @@ masked_dq_kernel(const __grid_constant__ MaskedParams p, const __grid_constant__
     tc_fence_before();
     __syncthreads();
     if (warp == 9) tmem_free(tmem, 512);
-    if (tid == 0) st.amax[(long long)bh * st.n + qt] = s_top | s_odd << 8;
+    if (tid == 0) st.amax[(long long)bh * st.n + qt] = s_top | s_odd << 8 | s_delta << 16;
     if (any_bad(s_bad)) redo_rows<T, false>(p, s_bad, st.n);
 }
 
@@ -419,7 +431,7 @@ masked_dkdv_kernel(const __grid_constant__ MaskedParams p, const __grid_constant
     const uint32_t bar_kv = bars, bar_qf = bars + 8, bar_qe = bars + 24, bar_of = bars + 40, bar_oe = bars + 56, bar_s = bars + 72,
                    bar_dp = bars + 80, bar_p = bars + 88, bar_ds = bars + 96, bar_done = bars + 104, slot = bars + 112;
     __shared__ int s_first, s_end;
-    __shared__ unsigned s_bad[8], s_top, s_odd;
+    __shared__ unsigned s_bad[8], s_top, s_delta, s_odd;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int bh = blockIdx.x % (p.B * p.Hkv), b = bh / p.Hkv, hk = bh % p.Hkv;
     const int k0 = (int)(blockIdx.x / (p.B * p.Hkv)) * kTileK;       // first keys first: with a causal mask most queries see them
@@ -428,7 +440,7 @@ masked_dkdv_kernel(const __grid_constant__ MaskedParams p, const __grid_constant
     auto tile_rows = [&](int e) { return sm_rows + (uint32_t)(e & 1) * 2 * L::kRowBytes; };
 
     if (tid == 0) {
-        s_first = 0x7fffffff; s_end = 0; s_top = s_odd = 0;
+        s_first = 0x7fffffff; s_end = 0; s_top = s_delta = s_odd = 0;
         mbar_init(bar_kv, 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(bar_qf + 8 * i, 1);
@@ -454,26 +466,30 @@ masked_dkdv_kernel(const __grid_constant__ MaskedParams p, const __grid_constant
         }
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");      // masked_dq_kernel's results from here on
-    // the query tiles between the first and the last that see any of these keys
+    // the query tiles between the first and the last that see any of these keys; the largest |dout| and |delta| of those that do;
+    // whether any has odd queries
     int lo = 0x7fffffff, hi = 0;
+    const unsigned* amax = st.amax + (long long)(b * p.Hq + hk * p.group) * st.n;
+    unsigned top = 0, most = 0, odd = 0;
     for (int i = tid; i < st.n; i += kBwdThreads) {
         const int4 t = st.tiles[(long long)b * st.n + i];
-        if (t.x < k0 + kTileK && t.y > k0) { lo = min(lo, i); hi = max(hi, i + 1); }
+        const bool sees = t.x < k0 + kTileK && t.y > k0;
+        if (sees) { lo = min(lo, i); hi = max(hi, i + 1); }
+        for (int g = 0; g < p.group; ++g) {
+            const unsigned a = amax[(long long)g * st.n + i];
+            odd |= a >> 8 & 1u;
+            if (kScaled && sees) { top = max(top, a & 255u); most = max(most, a >> 16); }
+        }
     }
     lo = warp_min(lo);
     hi = warp_max(hi);
     if (lane == 0) { atomicMin(&s_first, lo); atomicMax(&s_end, hi); }
-    {
-        // the largest |dout| of the group's heads, and whether they have odd queries
-        const unsigned* from = st.amax + (long long)(b * p.Hq + hk * p.group) * st.n;
-        unsigned top = 0, odd = 0;
-        for (int i = tid; i < p.group * st.n; i += kBwdThreads) { top = max(top, from[i] & 255u); odd |= from[i] >> 8; }
-        if (kScaled) {
-            top = __reduce_max_sync(0xffffffffu, top);
-            if (lane == 0) atomicMax(&s_top, top);
-        }
-        if (odd) s_odd = 1;
+    if (kScaled) {
+        top = __reduce_max_sync(0xffffffffu, top);
+        most = __reduce_max_sync(0xffffffffu, most);
+        if (lane == 0) { atomicMax(&s_top, top); atomicMax(&s_delta, most); }
     }
+    if (odd) s_odd = 1;
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -506,7 +522,7 @@ masked_dkdv_kernel(const __grid_constant__ MaskedParams p, const __grid_constant
             const uint32_t t_dp = tmem + 128, t_dv = tmem + 256, t_dk = tmem + 384;
             bool ok = mbar_wait_bounded(bar_kv, 0, p.err) && n > 0;
             auto clean = [&](int e, uint32_t tile) {
-                if (st.amax[((long long)b * p.Hq + hk * p.group + e / span) * st.n + first + e % span] >> 8) clear_odd_rows<HD>(tile, tile_rows(e));
+                if (st.amax[((long long)b * p.Hq + hk * p.group + e / span) * st.n + first + e % span] >> 8 & 1u) clear_odd_rows<HD>(tile, tile_rows(e));
             };
             const bool any_odd = s_odd != 0;
             auto score = [&](int e) {
@@ -546,10 +562,24 @@ masked_dkdv_kernel(const __grid_constant__ MaskedParams p, const __grid_constant
         c.cap_in = CAP ? 2.0f * fabsf(p.sm_scale) / p.cap : 0.0f;
         c.cap_out = CAP ? p.cap * kLog2e : 0.0f;
         const float unit = CAP ? c.cap_out : c.scale2;
-        const float sigma = kScaled ? scale_down(s_top) : 1.0f;
         const uint32_t s_at = tmem + half * 64 + lanes, d_at = s_at + 128;
         bool ok = true;
-        for (int e = 0; e < n; ++e) {
+        float sigma = 1.0f;
+        if (kScaled && n > 0) {
+            // the key's row of V: its sum of magnitudes, pieces in an order that keeps lanes apart in the banks
+            float norm = 0.0f;
+            ok = mbar_wait_bounded(bar_kv, 0, p.err);
+#pragma unroll
+            for (int x = 0; x < HD / 8; ++x) {
+                float v[8];
+                unpack16(lds128(sm_v + x / 8 * 128 * 128 + in_tile * 128 + ((x + lane) & 7) * 16), v, (T*)nullptr);
+#pragma unroll
+                for (int y = 0; y < 8; ++y) norm += fabsf(v[y]);
+            }
+            sigma = scale_up(norm, s_top, s_delta);
+        }
+        const float dsigma = sigma / kWeightUp;                    // P^T has its own scale in it
+        for (int e = 0; e < n && ok; ++e) {
             const int qt = first + e % span, q0 = qt * kTileQ + half * 64;
             const float slope2 = BIAS ? __ldg(p.slopes + hk * p.group + e / span) * kLog2e : 0.0f;
             const int4 t = st.tiles[(long long)b * st.n + qt];          // written while this kernel was resident: not by the read-only path
@@ -612,7 +642,7 @@ masked_dkdv_kernel(const __grid_constant__ MaskedParams p, const __grid_constant
 #pragma unroll
                     for (int z = 0; z < 4; z += 2) {
                         float2 u = add2(make_float2(d[y + z], d[y + z + 1]), z ? make_float2(nd.z, nd.w) : make_float2(nd.x, nd.y));
-                        if (kScaled) u = mul2(u, make_float2(sigma, sigma));
+                        if (kScaled) u = mul2(u, make_float2(dsigma, dsigma));
                         const float2 ds = mul2(make_float2(w[x + y + z], w[x + y + z + 1]), u);
                         o[(y + z) / 2] = pack2<T>(ds.x, ds.y);
                     }
@@ -627,7 +657,7 @@ masked_dkdv_kernel(const __grid_constant__ MaskedParams p, const __grid_constant
         if (ok && n > 0) ok = mbar_wait_bounded(bar_done, 0, p.err);
         if (ok) {
             tc_fence_after();
-            const float back = p.sm_scale / sigma;
+            const float back = half ? p.sm_scale / sigma : kScaled ? 1.0f / kWeightUp : 1.0f;
             bool fine = true;
             // the first half of the threads has dv, the second dk
             T* out = key < p.Lk ? (half ? row_of<T>(p.dk, p.sdk, b, hk, key) : row_of<T>(p.dv, p.sdv, b, hk, key)) : nullptr;
@@ -644,7 +674,7 @@ masked_dkdv_kernel(const __grid_constant__ MaskedParams p, const __grid_constant
                         float v[8];
 #pragma unroll
                         for (int z = 0; z < 8; ++z) {
-                            v[z] = n > 0 ? (half ? o[y + z] * back : o[y + z]) : 0.0f;
+                            v[z] = n > 0 ? o[y + z] * back : 0.0f;
                             fine = fine && fabsf(v[z]) <= 3.0e38f;
                         }
                         if (x + y < p.D) stg128(out + x + y, pack16(v, (T*)nullptr));

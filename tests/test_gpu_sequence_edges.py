@@ -296,3 +296,45 @@ def test_positions_far_from_zero(dtype, group, T, n, first):
     positions = (first - ago).clamp_min(-2 ** 31).int()
     check(c, c.q(2 * group, T), 0.125, parents=random_tree(2, T, n) if T > 1 else None, positions=positions, start=[first, first - 1],
           slopes=torch.linspace(0.2, 0.001, 2 * group, device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [64, 128])
+def test_weights_far_below_the_range_of_fp16(dtype, D):
+    """Even weights of 277,309 keys, 60.5 of fp16's smallest steps each: dv is dout's sum over as many, to half a step of the
+    weights and of the result."""
+    Lk, Lq = 277309, 1024
+    g = torch.Generator(device="cuda").manual_seed(D)
+    q = torch.zeros(1, 1, Lq, D, dtype=dtype, device="cuda")
+    k, v = (torch.randn(1, 1, Lk, D, generator=g, device="cuda").to(dtype) for _ in range(2))
+    do = (torch.rand(1, 1, Lq, D, generator=g, device="cuda") + 1).mul(16).to(dtype)
+    out, lse = be.masked_forward_raw(q, k, v, 0.125)
+    dv = be.masked_backward_raw(q, k, v, out, lse, do, 0.125)[2]
+    want = (do.double().sum(2, keepdim=True) / Lk).expand_as(dv)
+    # lse is off by the sum of Lk weights (fp32, in groups of hundreds: 2^-20 is far above it) and a rounding near 18
+    rel = 2 * ref.half_step(dtype) + 2.0 ** -20 + 18 * ref.E32 + (Lq + 8) * ref.E32
+    ref.assert_within(dv, want, rel * want.abs(), "dv")
+
+
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("softcap", [0.0, 10.0])
+def test_a_document_with_far_smaller_gradients_keeps_them(D, softcap):
+    """fp16, two packed documents, the second one's dout 1e-5 of the first's: its gradients are those that it has alone, with the
+    precision of the type.  dk's operand may round below the normal range: by half of fp16's smallest step at the scale of
+    the key, which puts a bound of its row, 2 max |dout| |v|_1 + 2 max |delta|, between 2^13 and 2^14."""
+    lens, sm = [150, 120], D ** -0.5
+    vis = be.visible_ranges(lens, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(D)
+    q, k, v, do = (torch.randn(1, h, 270, D, generator=g, device="cuda") for h in (4, 2, 2, 4))
+    do[:, :, :150] *= 1000
+    do[:, :, 150:] *= 0.01
+    q, k, v, do = (t.half() for t in (q, k, v, do))
+    kw = dict(softcap=softcap)
+    out, lse = be.masked_forward_raw(q, k, v, sm, visible=vis, **kw)
+    got = be.masked_backward_raw(q, k, v, out, lse, do, sm, visible=vis, **kw)
+    for lo, hi in ((0, 150), (150, 270)):
+        res, tol = ref.masked(*(t[:, :, lo:hi] for t in (q, k, v)), sm, causal=True, dout=do[:, :, lo:hi], **kw)
+        most = do.double().abs().amax() * v[:, :, lo:hi].double().abs().sum(-1) + (out.double() * do.double()).sum(-1).abs().amax()
+        tol["dk"] = tol["dk"] + sm * 2.0 ** -25 * (2 * most / 2.0 ** 13)[..., None] * q[:, :, lo:hi].double().abs().view(1, 2, 2, hi - lo, D).sum((2, 3))[:, :, None]
+        for n, t in zip(("dq", "dk", "dv"), got):
+            ref.assert_within(t[:, :, lo:hi], res[n], tol[n], f"{n} of the document from {lo} on")
