@@ -5,7 +5,8 @@ contiguous and 16-byte aligned), and for every sequence a row of page numbers: i
 slot ``n % page_size`` of page ``page_table[b, n // page_size]``.  ``lens[b]`` keys are cached; the T drafted
 tokens' own keys are to be in the cache behind them, as keys ``lens[b] .. lens[b] + T - 1``.
 Formulas and limits are in ``include/dsdpa.h``.  Nothing here waits for the device; a page number or a parent
-out of range is left out on the device and reported by ``cabi.lib().dsdpa_device_error(device)``.
+out of range is left out on the device and reported by ``cabi.lib().dsdpa_device_error(device)``; with
+``op.check_device_errors`` every call waits for the device, asks it and raises.
 """
 from __future__ import annotations
 
@@ -122,8 +123,7 @@ def tree_sdpa(q, k_pages, v_pages, page_table, lens, sm_scale=None, *, parents=N
     ws = q.new_empty(n, dtype=torch.uint8) if n else None
     st = L.dsdpa_tree_forward(prob, tree, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), lens.data_ptr(),
                               out.data_ptr(), lse.data_ptr(), None if ws is None else ws.data_ptr(), n, dev, masked._raw_stream(dev))
-    if st:
-        cabi.check(st)
+    masked._done(st, dev)
     return out, lse
 
 
@@ -152,8 +152,7 @@ def cache_weights(weights, q, lse, k_pages, page_table, lens, sm_scale=None, *, 
     prob = _problem(q, k_pages, None, page_table, sm_scale, softcap, weights.shape[2])
     st = cabi.lib().dsdpa_cache_weights(prob, tree, q.data_ptr(), lse.data_ptr(), k_pages.data_ptr(), page_table.data_ptr(), lens.data_ptr(),
                                         None if take is None else take.data_ptr(), weights.data_ptr(), dev, masked._raw_stream(dev))
-    if st:
-        cabi.check(st)
+    masked._done(st, dev)
     return weights
 
 
@@ -202,6 +201,5 @@ def cache_evict(k_pages, v_pages, page_table, lens, weights, keep, *, sinks=0, r
             None if positions is None else positions.data_ptr(), keep, sinks, recent, out_table.data_ptr(), out_table.shape[1],
             kept.data_ptr(), new_lens.data_ptr(), new_weights.data_ptr(), None if positions is None else new_positions.data_ptr(),
             dev, masked._raw_stream(dev))
-        if st:
-            cabi.check(st)
+        masked._done(st, dev)
     return (new_lens, kept, new_weights) if positions is None else (new_lens, kept, new_weights, new_positions)

@@ -122,6 +122,14 @@ def _numbers(q, sm_scale, softcap):
     return sm_scale, softcap
 
 
+def _done(st, device):
+    """After a call of the library: its status, and with ``op.check_device_errors`` what the kernels recorded."""
+    if st:
+        cabi.check(st)
+    if op.check_device_errors:
+        cabi.check(cabi.lib().dsdpa_device_error(device))
+
+
 def masked_forward_raw(q, k, v, sm_scale=None, *, causal=False, visible=None, softcap=0.0, slopes=None):
     """Forward through the C ABI.  Returns ``(out, lse)``, lse fp32 [B, heads, Lq] in base 2; no autograd.
 
@@ -144,8 +152,7 @@ def masked_forward_raw(q, k, v, sm_scale=None, *, causal=False, visible=None, so
     st = cabi.lib().dsdpa_masked_forward(prob, q.data_ptr(), k.data_ptr(), v.data_ptr(),
                                          None if visible is None else visible.data_ptr(), None if slopes is None else slopes.data_ptr(),
                                          out.data_ptr(), lse.data_ptr(), dev, _raw_stream(dev))
-    if st:
-        cabi.check(st)
+    _done(st, dev)
     return out, lse
 
 
@@ -178,8 +185,7 @@ def masked_backward_raw(q, k, v, out, lse, dout, sm_scale=None, *, causal=False,
     st = L.dsdpa_masked_backward(prob, q.data_ptr(), k.data_ptr(), v.data_ptr(), None if visible is None else visible.data_ptr(),
                                  None if slopes is None else slopes.data_ptr(), out.data_ptr(), lse.data_ptr(), dout.data_ptr(),
                                  dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), None if ws is None else ws.data_ptr(), n, dev, _raw_stream(dev))
-    if st:
-        cabi.check(st)
+    _done(st, dev)
     return dq, dk, dv
 
 
@@ -187,8 +193,6 @@ def _grads(ctx, dout):
     q, k, v, out, lse, visible, slopes = ctx.saved_tensors
     dq, dk, dv = masked_backward_raw(q, k, v, out, lse, dout, ctx.sm_scale, causal=ctx.causal, visible=visible,
                                      softcap=ctx.softcap, slopes=slopes)
-    if op.check_device_errors:
-        cabi.check(cabi.lib().dsdpa_device_error(q.device.index))
     return dq, dk, dv, None, None, None, None, None
 
 

@@ -23,9 +23,10 @@ _DTYPES = {torch.float32: cabi.F32, torch.bfloat16: cabi.BF16, torch.float16: ca
 default_flags = 0
 
 # Debug aid, off by default: when set (or with DSDPA_CHECK_DEVICE_ERRORS=1 in the environment),
-# the autograd function synchronises the device after every backward and raises if a kernel
-# recorded that one of its bounded waits ran out (such a kernel returns without writing its
-# results).  Without it nobody looks at that record unless the caller polls
+# the autograd function synchronises the device after every backward, the sequence and cache operators
+# after every call, and they raise if a kernel recorded that one of its bounded waits ran out (such a
+# kernel returns without writing its results) or that a page table, a length or a tree holds a number
+# out of range.  Without it nobody looks at that record unless the caller polls
 # ``cabi.lib().dsdpa_device_error(device)`` itself.
 check_device_errors = os.environ.get("DSDPA_CHECK_DEVICE_ERRORS", "0") not in ("", "0")
 

@@ -338,3 +338,21 @@ def test_a_document_with_far_smaller_gradients_keeps_them(D, softcap):
         tol["dk"] = tol["dk"] + sm * 2.0 ** -25 * (2 * most / 2.0 ** 13)[..., None] * q[:, :, lo:hi].double().abs().view(1, 2, 2, hi - lo, D).sum((2, 3))[:, :, None]
         for n, t in zip(("dq", "dk", "dv"), got):
             ref.assert_within(t[:, :, lo:hi], res[n], tol[n], f"{n} of the document from {lo} on")
+
+
+def test_every_call_raises_what_the_device_recorded_where_that_is_asked_for(monkeypatch):
+    c = Cache([40, 40], 2, 1, 64, 16, torch.bfloat16, seed=1)
+    q, w = c.q(2, 2), torch.rand(2, 1, c.slots, device="cuda")
+    out, lse = be.tree_sdpa(q, c.k, c.v, c.table, c.lens, 0.125)
+    broken = c.table.clone()
+    broken[1, 1] = -1
+    monkeypatch.setattr(be.op, "check_device_errors", True)
+    calls = [lambda t: be.tree_sdpa(q, c.k, c.v, t, c.lens, 0.125), lambda t: be.cache_weights(w, q, lse, c.k, t, c.lens, 0.125),
+             lambda t: be.cache_evict(c.k.clone(), c.v.clone(), t, c.lens, w, 30)]
+    for call in calls:
+        call(c.table)
+        with pytest.raises(cabi.DsdpaError, match="out of range"):
+            call(broken)
+        call(c.table)
+    x = torch.randn(1, 2, 20, 64, device="cuda", requires_grad=True)
+    be.masked_sdpa(x, x, x, causal=True).sum().backward()
