@@ -10,7 +10,6 @@ out of range is left out on the device and reported by ``cabi.lib().dsdpa_device
 """
 from __future__ import annotations
 
-import math
 import struct
 
 import torch
@@ -78,7 +77,7 @@ def _tokens(q, k_pages, page_table, sm_scale, softcap, parents, drafted, slopes,
         raise ValueError(f"{name}: {Hq} query heads are no multiple of {Hkv} key/value heads")
     if T > cabi.TREE_MAX:
         raise ValueError(f"{name}: {T} drafted tokens, at most {cabi.TREE_MAX}")
-    if not (math.isfinite(sm_scale) and 0.0 <= softcap < math.inf):
+    if not masked._sound(sm_scale, softcap):
         masked._check_numbers(sm_scale, softcap, name)
     if parents is None and drafted is None and positions is None and start is None and slopes is None:
         return None, None

@@ -24,7 +24,7 @@ int check_tokens(const dsdpa_cache_problem* p) {
     if (st != DSDPA_OK) return st;
     if (p->Hq <= 0 || p->Hq % p->Hkv || (long long)p->B * p->Hq >= (1ll << 24) || p->T <= 0) return DSDPA_ERR_BAD_SHAPE;
     if (p->T > kTreeMax) return DSDPA_ERR_TOO_LARGE;
-    if (!isfinite(p->sm_scale) || !isfinite(p->softcap)) return DSDPA_ERR_BAD_SHAPE;
+    if (bad_score(p->sm_scale, p->softcap)) return DSDPA_ERR_BAD_SHAPE;
     return bad_stride(p->stride_q, p->dtype, p->B, p->Hq, p->T) ? DSDPA_ERR_MISALIGNED : DSDPA_OK;
 }
 bool odd4(const void* p) { return ((uintptr_t)p & 3) != 0; }

@@ -2,6 +2,8 @@
 #pragma once
 
 #include <cuda_runtime.h>
+#include <float.h>
+#include <math.h>
 #include <stdint.h>
 #include <atomic>
 
@@ -24,6 +26,14 @@ inline bool bad_stride(const long long (&st)[3], int dtype, int B, int H, int L)
     for (int i = 0; i < 3; ++i)
         if (n[i] > 1 && (st[i] <= 0 || (st[i] * (dtype == DSDPA_F32 ? 4 : 2)) % 16)) return true;
     return false;
+}
+
+// A scale or a cap that the kernels' fp32 cannot carry: they work with 2 |sm_scale| / softcap and softcap log2(e).
+inline bool bad_score(float sm_scale, float softcap) {
+    if (!isfinite(sm_scale) || !isfinite(softcap)) return true;
+    if (softcap <= 0.0f) return false;
+    const double in = 2.0 * fabs((double)sm_scale) / softcap;
+    return softcap < FLT_MIN || softcap > FLT_MAX / 2 || in > FLT_MAX || (sm_scale != 0.0f && in < FLT_MIN);
 }
 
 struct DeviceGuard {

@@ -54,7 +54,7 @@ int check(const dsdpa_masked_problem* p) {
     // positions are exact in fp32 and tile counts fit the grid
     if (p->Lq > (1 << 24) || p->Lk > (1 << 24) || (long long)p->B * p->Hq >= (1ll << 24)) return DSDPA_ERR_BAD_SHAPE;
     if (p->flags & ~DSDPA_MASKED_CAUSAL) return DSDPA_ERR_BAD_FLAGS;
-    if (!isfinite(p->sm_scale) || !isfinite(p->softcap)) return DSDPA_ERR_BAD_SHAPE;
+    if (bad_score(p->sm_scale, p->softcap)) return DSDPA_ERR_BAD_SHAPE;
     return DSDPA_OK;
 }
 

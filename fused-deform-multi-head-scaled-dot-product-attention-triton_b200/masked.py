@@ -6,7 +6,6 @@ The device work is libdeform_sdpa.so's, through the C ABI of ``include/dsdpa.h``
 """
 from __future__ import annotations
 
-import math
 import struct
 
 import torch
@@ -69,9 +68,19 @@ def _check_inputs(q, k, v, sm_scale, softcap, visible, slopes, name):
             raise ValueError(f"{name}: visible is on another device")
 
 
+_LEAST, _MOST = torch.finfo(torch.float32).tiny, torch.finfo(torch.float32).max
+
+
+def _sound(sm_scale, softcap):
+    """What the kernels' fp32 can carry: sm_scale itself, softcap log2(e) and 2 |sm_scale| / softcap."""
+    return -_MOST <= sm_scale <= _MOST and (softcap == 0.0 or (
+        _LEAST <= softcap <= _MOST / 2 and (sm_scale == 0.0 or _LEAST <= 2.0 * abs(sm_scale) / softcap <= _MOST)))
+
+
 def _check_numbers(sm_scale, softcap, name):
-    if not math.isfinite(sm_scale) or not math.isfinite(softcap) or softcap < 0:
-        raise ValueError(f"{name}: sm_scale must be finite and softcap finite and not negative")
+    if not _sound(sm_scale, softcap):
+        raise ValueError(f"{name}: sm_scale {sm_scale} must be a finite fp32 number and softcap {softcap} 0 or a positive one, "
+                         "neither so far from the other that 2 sm_scale / softcap leaves fp32")
 
 
 def _check_slopes(slopes, heads, device, name):
@@ -117,7 +126,7 @@ def _plain(q, k, v, visible, slopes):
 def _numbers(q, sm_scale, softcap):
     sm_scale = q.shape[-1] ** -0.5 if sm_scale is None else float(sm_scale)
     softcap = float(softcap)
-    if not (math.isfinite(sm_scale) and 0.0 <= softcap < math.inf):
+    if not _sound(sm_scale, softcap):
         _check_numbers(sm_scale, softcap, "masked_sdpa")
     return sm_scale, softcap
 

@@ -286,7 +286,7 @@ typedef struct dsdpa_masked_problem {
     int B, Hq, Hkv;
     int Lq, Lk;              /* 0 is allowed */
     int D;
-    float sm_scale, softcap; /* softcap <= 0: no cap */
+    float sm_scale, softcap; /* softcap <= 0: no cap; else 2 |sm_scale| / softcap and softcap log2(e) fit fp32 */
     int dtype;               /* of q, k, v, out, dout, dq, dk, dv */
     unsigned flags;
     long long stride_q[3], stride_k[3], stride_v[3];     /* batch, head, row */
@@ -328,7 +328,7 @@ typedef struct dsdpa_cache_problem {
     int B, Hq, Hkv, T, D;
     int pages, page_size, table_width;
     int slots;               /* row length of weights and positions: at least table_width * page_size */
-    float sm_scale, softcap;
+    float sm_scale, softcap; /* as above */
     int dtype;               /* of q, k_pages, v_pages, out */
     unsigned flags;          /* 0 */
     long long stride_q[3];                /* batch, head, token */

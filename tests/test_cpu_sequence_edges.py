@@ -1,13 +1,20 @@
 """What can be held without a GPU about the sequence operators' sources, build and argument checks."""
+import ctypes
 import importlib
+import math
 import os
 import re
 from pathlib import Path
 
 
+import pytest
+import torch
+
 import ops
+from test_cpu_sequence import cache_problem, masked_problem, tree_status
 
 be = ops.backend
+cabi = be.cabi
 PACKAGE = Path(be.__file__).resolve().parent
 CSRC = PACKAGE / "csrc"
 
@@ -39,3 +46,28 @@ def test_a_copied_tree_is_compiled_again(tmp_path, monkeypatch):
     monkeypatch.setattr(build, "HERE", tmp_path / "copy" / "package")
     assert build._newest_source(tmp_path / "copy" / "a.cu", dep) == float("inf")
     assert build._newest_source(tmp_path / "copy" / "a.cu", tmp_path / "none.d") == float("inf")
+
+
+@pytest.mark.parametrize("sm_scale,softcap", [(1e39, 0.0), (-math.inf, 0.0), (math.nan, 0.0), (0.125, math.nan), (0.125, -1.0), (0.125, math.inf),
+                                              (0.125, 1e39), (0.125, 3e38), (0.125, 1e-46), (0.125, 1e-40), (1e-8, 1e37), (1e10, 1e-30)])
+def test_numbers_that_fp32_cannot_carry_are_refused(sm_scale, softcap):
+    """Neither a silent infinity, nor a cap that becomes none, nor one whose ratio to the scale is lost."""
+    q = torch.zeros(1, 2, 4, 64)
+    with pytest.raises(ValueError, match="sm_scale"):
+        be.masked_sdpa(q, q, q, sm_scale, softcap=softcap)
+    with pytest.raises(ValueError, match="tree_sdpa: sm_scale"):
+        be.masked._check_numbers(sm_scale, softcap, "tree_sdpa")
+    if softcap < 0:                       # the C ABI's sign for no cap
+        return
+    as_float = [ctypes.c_float(x).value for x in (sm_scale, softcap)]
+    if softcap == 0.0 or as_float[1] != 0.0:
+        for p, call in ((masked_problem(sm_scale=as_float[0], softcap=as_float[1]), "dsdpa_masked_backward_workspace_bytes"),
+                        (cache_problem(sm_scale=as_float[0], softcap=as_float[1]), "dsdpa_tree_workspace_bytes")):
+            assert getattr(cabi.lib(), call)(ctypes.byref(p)) == 0
+    assert tree_status(cache_problem(sm_scale=as_float[0], softcap=as_float[1] or math.nan)) == cabi.ERR_BAD_SHAPE
+
+
+@pytest.mark.parametrize("sm_scale,softcap", [(0.125, 0.0), (0.0, 5.0), (-2.0, 1e30), (0.125, 50.0), (1e20, 1.0), (1e-20, 1.0)])
+def test_numbers_that_it_can_are_not(sm_scale, softcap):
+    be.masked._check_numbers(sm_scale, softcap, "masked_sdpa")
+    assert cabi.lib().dsdpa_masked_backward_workspace_bytes(ctypes.byref(masked_problem(sm_scale=sm_scale, softcap=softcap))) > 0
