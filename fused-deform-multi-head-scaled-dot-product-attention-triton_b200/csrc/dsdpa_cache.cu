@@ -150,6 +150,7 @@ int dsdpa_cache_evict(const dsdpa_cache_problem* p, void* k_pages, void* v_pages
     if (out_width <= 0 || (long long)out_width * p->page_size > (1ll << 30)) return DSDPA_ERR_BAD_SHAPE;
     const long long most = (long long)p->table_width * p->page_size < keep ? (long long)p->table_width * p->page_size : keep;
     if ((long long)out_width * p->page_size < most) return DSDPA_ERR_BAD_SHAPE;
+    if (new_lens == lens) return DSDPA_ERR_BAD_SHAPE;      // the blocks of a sequence's other heads still read it
     DeviceGuard guard(device);
     if (guard.err != cudaSuccess) return report_cuda_failure(guard.err);
     int* err = nullptr;

@@ -379,7 +379,8 @@ int dsdpa_cache_weights(const dsdpa_cache_problem* p, const dsdpa_cache_tree* tr
  * Their rows of k_pages and v_pages are copied to keys 0 .. new_lens-1 of out_table [B, out_width].  Where
  * out_table is page_table itself the sequence is compacted in place.  Otherwise the pages of out_table hold
  * none of the sequences' keys, and the old rows stay as they were.  Rows behind the last kept one
- * are left as they were.  p->T, Hq, sm_scale and softcap play no part.
+ * are left as they were.  new_lens, new_weights and new_positions are other memory than lens, weights and
+ * positions.  p->T, Hq, sm_scale and softcap play no part.
  */
 int dsdpa_cache_evict(const dsdpa_cache_problem* p, void* k_pages, void* v_pages, const int* page_table, const int* lens,
                       const float* weights, const int* positions, int keep, int sinks, int recent,

@@ -11,7 +11,7 @@ import pytest
 import torch
 
 import ops
-from test_cpu_sequence import cache_problem, masked_problem, tree_status
+from test_cpu_sequence import OK, cache_problem, evict_status, masked_problem, tree_status
 
 be = ops.backend
 cabi = be.cabi
@@ -71,3 +71,10 @@ def test_numbers_that_fp32_cannot_carry_are_refused(sm_scale, softcap):
 def test_numbers_that_it_can_are_not(sm_scale, softcap):
     be.masked._check_numbers(sm_scale, softcap, "masked_sdpa")
     assert cabi.lib().dsdpa_masked_backward_workspace_bytes(ctypes.byref(masked_problem(sm_scale=sm_scale, softcap=softcap))) > 0
+
+
+def test_an_eviction_does_not_write_over_the_lengths_it_reads():
+    p = cache_problem()
+    lens, other = ctypes.c_void_p(16384), ctypes.c_void_p(8192)
+    ptrs = [OK, OK, OK, lens, OK, None]
+    assert evict_status(p, ptrs=ptrs, more=(OK, lens, other, None)) == cabi.ERR_BAD_SHAPE
