@@ -98,7 +98,7 @@ __device__ __forceinline__ float from_first(int at, int first) {       // the ha
 }
 // Position of cached key j of head hk.
 __device__ __forceinline__ float key_position(const CacheParams& p, int b, int hk, int j, int first) {
-    return from_first(p.positions ? __ldg(p.positions + ((long long)b * p.Hkv + hk) * p.slots + j) : j, first);
+    return from_first(p.positions && in_range(j, p.slots, p.err) ? __ldg(p.positions + ((long long)b * p.Hkv + hk) * p.slots + j) : j, first);
 }
 
 // out and lse of one drafted token, by one warp (as in dsdpa_masked.cuh).

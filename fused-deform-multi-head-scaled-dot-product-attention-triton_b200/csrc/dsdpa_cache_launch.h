@@ -29,6 +29,7 @@ constexpr int few_blocks(int hd, int rows, bool weights) {
 struct TreePlan {
     bool whole;              // units are not cut
     int row_unit, row_tiles, part_rows, blocks, weight_blocks;
+    long long parts;         // places for them in the workspace
     size_t part, part_lse, bytes;      // workspace: the table of starts at 0
 };
 inline TreePlan plan_tree(const dsdpa_cache_problem& p) {
@@ -54,6 +55,7 @@ inline TreePlan plan_tree(const dsdpa_cache_problem& p) {
     const size_t parts = (size_t)t.blocks * workers * 2;
     if (!t.whole) {
         auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
+        t.parts = (long long)parts;
         t.part_lse = up(((size_t)p.B + 2) * 8);
         t.part = t.part_lse + up(parts * t.part_rows * 4);
         t.bytes = t.part + parts * t.part_rows * p.D * 4;

@@ -163,8 +163,8 @@ tree_simt_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ 
 #pragma unroll
         for (int r = 0; r < RM; ++r) {
             const int in_tile = ty * RM + r, gr = it.row0 + in_tile, t = gr / p.group, h = it.hk * p.group + gr % p.group;
-            const bool valid = in_tile < it.rows;
             const long long row = ((long long)it.b * p.Hq + h) * p.T + t, part = (long long)it.part * sp.part_rows + in_tile;
+            const bool valid = in_tile < it.rows && (it.part < 0 || in_range(part, sp.rows, p.err));
             const float sum = half_warp_sum(l[r]), inv = sum != 0.0f ? 1.0f / sum : 0.0f, lse = sum != 0.0f ? m[r] + log2f(sum) : kNegInf;
             float nan;
             if (it.part < 0) nan = simt_store<T, HD>(valid ? (T*)p.out + row * p.D : nullptr, acc[r], inv, p.D);
@@ -264,7 +264,7 @@ weights_simt_kernel(const __grid_constant__ CacheParams p, const __grid_constant
 #pragma unroll
             for (int c = 0; c < 4; ++c) part[ty * kSimtKeys + tx + 16 * c] = sum[c];
             __syncthreads();
-            if (tid < kSimtKeys && s_page[tid] >= 0) {
+            if (tid < kSimtKeys && s_page[tid] >= 0 && in_range(k0 + tid, p.slots, p.err)) {
                 float total = 0.0f;
 #pragma unroll
                 for (int y = 0; y < 16; ++y) total += part[y * kSimtKeys + tid];

@@ -57,6 +57,7 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __gr
     const int left = min(n, p.keep);
     if (h == 0 && tid == 0) p.new_lens[b] = left;
     auto put = [&](int at, int key) {
+        if (!in_range(at, min(p.keep, p.slots), p.err) || !in_range(key, p.slots, p.err)) return;
         kept[at] = key;
         nw[at] = w[key];
         if (np) np[at] = pos ? pos[key] : key;
@@ -154,7 +155,7 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __gr
             }
 #pragma unroll
             for (int e = 0; e < kBatch; ++e)
-                if (to[e] >= 0) {
+                if (to[e] >= 0 && in_range(to[e], min(p.keep, p.slots), p.err)) {
                     const int i = first + i0 + e * 32 + lane;
                     kept[to[e]] = i;
                     nw[to[e]] = val[e];

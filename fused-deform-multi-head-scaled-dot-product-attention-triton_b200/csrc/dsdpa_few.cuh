@@ -382,7 +382,7 @@ tree_few_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ T
                     }
                     if (valid && d < p.D) {
                         if (it.part < 0) store8<T>((T*)p.out + out_row * p.D + d, x);
-                        else store8<float>(sp.part + part * p.D + d, x);
+                        else if (in_range(part, sp.rows, p.err)) store8<float>(sp.part + part * p.D + d, x);
                     }
                 }
             nan = quad_sum(nan);
@@ -474,7 +474,7 @@ weights_few_kernel(const __grid_constant__ CacheParams p, const __grid_constant_
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int key = 2 * t4 + (e & 1) + 8 * (e >> 1);
-                old[e] = g == 0 && (now >> key & 1u) ? out[k0 + key] : 0.0f;
+                old[e] = g == 0 && (now >> key & 1u) && in_range(k0 + key, p.slots, p.err) ? out[k0 + key] : 0.0f;
             }
             float s[2][4];
             few_scores<T, HD, NR>(p, it, k0, lane, q, k, row, now, scale2, s);
@@ -492,7 +492,7 @@ weights_few_kernel(const __grid_constant__ CacheParams p, const __grid_constant_
                 x += __shfl_xor_sync(0xffffffffu, x, 8);
                 x += __shfl_xor_sync(0xffffffffu, x, 16);
                 const int key = 2 * t4 + (e & 1) + 8 * (e >> 1);
-                if (g == 0 && (now >> key & 1u)) out[k0 + key] = old[e] + x;
+                if (g == 0 && (now >> key & 1u) && in_range(k0 + key, p.slots, p.err)) out[k0 + key] = old[e] + x;
             }
         }
     }

@@ -15,7 +15,7 @@ cudaError_t tree(const CacheParams& p, const TreePlan& t, const TreeSplit& sp, c
 }
 template <int HD, int NC>
 cudaError_t weights(const CacheParams& p, const TreePlan& t, cudaStream_t s) {
-    const TreeSplit sp{ 0, 1, 0, nullptr, nullptr, nullptr };
+    const TreeSplit sp{ 0, 1, 0, nullptr, nullptr, nullptr, 0 };
     weights_few_f32_kernel<HD, NC><<<t.weight_blocks, kF32Warps * 32, 0, s>>>(p, sp);
     count_launches(1);
     return cudaGetLastError();

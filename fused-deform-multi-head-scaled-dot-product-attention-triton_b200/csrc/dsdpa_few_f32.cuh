@@ -279,6 +279,7 @@ tree_few_f32_kernel(const __grid_constant__ CacheParams p, const __grid_constant
                 }
                 if (gr < it.rows) {                      // the same for the whole warp
                     const long long out_row = ((long long)it.b * p.Hq + h) * p.T + t, part = (long long)it.part * sp.part_rows + gr;
+                    if (it.part >= 0 && !in_range(part, sp.rows, p.err)) continue;
                     if (few.group == 0 && few.at * 4 < p.D) store4<float>((it.part < 0 ? (float*)p.out + out_row * p.D : sp.part + part * p.D) + few.at * 4, x);
                     if (few.lane == 0) (it.part < 0 ? p.lse[out_row] : sp.part_lse[part]) = sum != 0.0f ? ref + log2f(sum) : kNegInf;
                     if (__any_sync(0xffffffffu, nan != nan) && it.part < 0) bad |= 1u << gr;
@@ -329,7 +330,7 @@ weights_few_f32_kernel(const __grid_constant__ CacheParams p, const __grid_const
         for (int i = 0; i < keys; i += F::kStep) {
             const int k0 = it.key0 + i, in_step = F::key_of(few.at * F::kHeld >> 2, few.group);
             // the first of the lanes that have a key's rows writes it
-            const bool writes = (few.at * F::kHeld & 3) == 0 && (few.there >> in_step & 1u);
+            const bool writes = (few.at * F::kHeld & 3) == 0 && (few.there >> in_step & 1u) && in_range(k0 + in_step, p.slots, p.err);
             const float old = writes ? out[k0 + in_step] : 0.0f;
             float s[NC][F::kHeld];
             few.scores(p, it, k0, k, rows, few.there, s);

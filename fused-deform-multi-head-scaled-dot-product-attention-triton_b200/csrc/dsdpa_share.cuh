@@ -24,6 +24,7 @@ struct TreeSplit {
     long long* start;     // null, or [B + 1]: key tiles of a head's query tile in the sequences before, and [B + 1]: a worker's share
     float* part;          // [workers * 2][part_rows][D], normalised
     float* part_lse;      // [workers * 2][part_rows]
+    long long rows;       // workers * 2 * part_rows
 };
 // Key tiles of a sequence: the same for all of its heads.
 template <typename Tile>
@@ -161,7 +162,8 @@ __global__ void __launch_bounds__(kCombineWarps * 32, 3) tree_combine_kernel(con
     if (c0 == c1) return;                                // written by the worker itself
     const int used = c1 - c0 + 1;                        // 0: a query that sees no key
     auto place = [&](int c) {                            // a worker's first part, or its second
-        return ((long long)(c0 + c) * 2 + ((c0 + c) * share >= from ? 0 : 1)) * sp.part_rows + gr % Tile::kRows;
+        const long long at = ((long long)(c0 + c) * 2 + ((c0 + c) * share >= from ? 0 : 1)) * sp.part_rows + gr % Tile::kRows;
+        return in_range(at, sp.rows, p.err) ? at : 0ll;
     };
     float m = kNegInf, kept = kNegInf;                    // kept: of this warp's first 32 parts
     bool nan = false;

@@ -8,7 +8,7 @@ namespace dsdpa {
 
 inline TreeSplit tree_split(const TreePlan& t, void* workspace) {
     char* at = (char*)workspace;
-    return TreeSplit{ t.whole, t.row_tiles, t.part_rows, (long long*)at, (float*)(at + t.part), (float*)(at + t.part_lse) };
+    return TreeSplit{ t.whole, t.row_tiles, t.part_rows, (long long*)at, (float*)(at + t.part), (float*)(at + t.part_lse), t.parts * t.part_rows };
 }
 
 // The second kernel's blocks are in place when the first one's end, and wait for its results there.

@@ -380,13 +380,13 @@ tree_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ TreeS
 #pragma unroll
                             for (int z = 0; z < 8; ++z) v[z] = o[y + z];
                             if (it.part < 0) store8<T>((T*)p.out + row * p.D + x + y, v);
-                            else store8<float>(sp.part + part * p.D + x + y, v);
+                            else if (in_range(part, sp.rows, p.err)) store8<float>(sp.part + part * p.D + x + y, v);
                         }
                 }
             }
             if (tile == 0 && valid) {
                 if (it.part < 0) p.lse[row] = lse;
-                else sp.part_lse[part] = lse;
+                else if (in_range(part, sp.rows, p.err)) sp.part_lse[part] = lse;
             }
             // rows that something non-finite reached are marked by an lse of NaN, which no other row has, and done once more
             // behind the loop: the other roles wait for this warp here, with limits

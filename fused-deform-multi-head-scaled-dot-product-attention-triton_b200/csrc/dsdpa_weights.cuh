@@ -155,7 +155,7 @@ weights_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ Tr
                     const int j = it.key0 + i * kTreeKeys + quad * 32 + lane, draft = j - it.n;
                     // a drafted key that the table has no room for is behind the row of weights too
                     const bool exists = draft < it.real && j < p.width * p.page_size;
-                    const float old = exists ? out[j] : 0.0f;
+                    const float old = exists && in_range(j, p.slots, p.err) ? out[j] : 0.0f;
                     float at = 0.0f;
                     if (BIAS && exists)
                         at = draft >= 0 ? (float)depth_of(tokens_above(p, it.b, draft)) : key_position(p, it.b, it.hk, j, first_position(p, it.b, it.n));
@@ -193,7 +193,7 @@ weights_kernel(const __grid_constant__ CacheParams p, const __grid_constant__ Tr
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(bar_r + 8 * buffer);
-                    if (exists && there) out[j] = old + sum;
+                    if (exists && there && in_range(j, p.slots, p.err)) out[j] = old + sum;
                 }
                 // a warp without a tile in this pass must not run ahead: its next arrival would count for this phase
                 ok = ok && mbar_wait_bounded(bar_qe + 8 * buf, ((pass >> 1) & 1) ^ 1, p.err);
