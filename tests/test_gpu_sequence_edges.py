@@ -356,3 +356,123 @@ def test_every_call_raises_what_the_device_recorded_where_that_is_asked_for(monk
         call(c.table)
     x = torch.randn(1, 2, 20, 64, device="cuda", requires_grad=True)
     be.masked_sdpa(x, x, x, causal=True).sum().backward()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("group,T", ROWS)
+@pytest.mark.parametrize("page,n", [(16, 100), (7, 100), (16, 3000), (64, 3001)])
+def test_absent_pages(dtype, group, T, page, n):
+    """Page numbers that are none, at the start, inside and at the end of a sequence: their keys count as absent, everywhere."""
+    c = Cache([n, 50, n - 30], T, 2, 64, page, dtype, seed=T + n + page)
+    q = c.q(2 * group, T)
+    broken = c.table.clone()
+    broken[0, 1], broken[0, (n + T - 1) // page], broken[2, 0] = -1, c.k.shape[0], 2 ** 31 - 1
+    out, lse = be.tree_sdpa(q, c.k, c.v, broken, c.lens, 0.125)
+    assert cabi.lib().dsdpa_device_error(0) == cabi.ERR_DEVICE_BOUNDS
+    w = torch.rand(3, 2, c.slots, generator=c.g, device="cuda")
+    before = w.clone()
+    be.cache_weights(w, q, lse, c.k, broken, c.lens, 0.125)
+    assert cabi.lib().dsdpa_device_error(0) == cabi.ERR_DEVICE_BOUNDS
+    for b, m in enumerate(c.lens.tolist()):
+        keys = present(c, b, m, T, broken)
+        res, tol, p, at = among(c, q, b, m, keys, 0.125, broken)
+        ref.assert_within(out[b], res["out"], tol["out"], f"out of sequence {b}")
+        ref.assert_within(lse[b], res["lse"], tol["lse"], f"lse of sequence {b}")
+        add = p.view(2, -1, *p.shape[-2:])
+        want = before[b][:, at].double() + add.sum((1, 2))
+        err = (add * (2 * tol["lse"].view(2, -1, T, 1) + 2.0 ** -19)).sum((1, 2))
+        ref.assert_within(w[b][:, at], want, err + (group * T + 2) * ref.E32 * want, f"weights of sequence {b}")
+        other = torch.ones(c.slots, dtype=torch.bool, device="cuda")
+        other[at] = False
+        assert torch.equal(w[b][:, other], before[b][:, other])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("group,T", ROWS)
+@pytest.mark.parametrize("n", [90, 3000])
+def test_strides_of_pages_and_queries(dtype, group, T, n):
+    """Keys and values interleaved in one pool, heads inside a slot, a wider table, queries of [B, T, heads, D] storage."""
+    c = Cache([n, 33], T, 2, 64, 16, dtype, seed=T + n)
+    q = c.q(2 * group, T)
+    want = be.tree_sdpa(q, c.k, c.v, c.table, c.lens, 0.125)
+    ww = be.cache_weights(torch.zeros(2, 2, c.slots, device="cuda"), q, want[1], c.k, c.table, c.lens, 0.125)
+    both = torch.stack([c.k.transpose(1, 2), c.v.transpose(1, 2)], 1).contiguous()
+    k, v = both[:, 0].transpose(1, 2), both[:, 1].transpose(1, 2)
+    qt = q.transpose(1, 2).contiguous().transpose(1, 2)
+    got = be.tree_sdpa(qt, k, v, c.table, c.lens, 0.125)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert torch.equal(be.cache_weights(torch.zeros(2, 2, c.slots, device="cuda"), qt, got[1], k, c.table, c.lens, 0.125), ww)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("group,T", ROWS)
+@pytest.mark.parametrize("longest", [200, 4000])
+def test_graphs_of_trees(dtype, group, T, longest):
+    """Lengths, trees, tables and queries change between the replays of two graphs that live side by side."""
+    c = Cache([longest, 60, longest // 2], T, 2, 64, 16, dtype, seed=T)
+    q, tree = c.q(2 * group, T), as_int(random_tree(3, T, 1))
+    kw = dict(parents=tree if T > 1 else None, slopes=torch.full((2 * group,), 0.05, device="cuda"), softcap=20.0)
+    w = torch.zeros(3, 2, c.slots, device="cuda")
+
+    def step():
+        out, lse = be.tree_sdpa(q, c.k, c.v, c.table, c.lens, 0.125, **kw)
+        return out, lse, be.cache_weights(w, q, lse, c.k, c.table, c.lens, 0.125, **kw)
+    step()
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            res = step()
+        graphs.append((graph, res))
+    g = torch.Generator(device="cuda").manual_seed(2)
+    for i, lens in enumerate([[longest, 60, 3], [0, 1, longest // 3], [longest - 1, 17, longest // 2]]):
+        c.lens.copy_(torch.tensor(lens))
+        tree.copy_(as_int(random_tree(3, T, 10 + i)))
+        q.copy_(torch.randn(q.shape, generator=g, device="cuda"))
+        c.table[0, :4] = c.table[0, :4].flip(0)
+        for graph, (out, lse, _) in graphs:
+            w.zero_()
+            graph.replay()
+            got = [t.clone() for t in (out, lse, w)]
+            w.zero_()
+            assert all(torch.equal(a, b) for a, b in zip(got, step()))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("group,T", ROWS)
+def test_streams_at_once(dtype, group, T):
+    c = Cache([3000, 900], T, 2, 64, 64, dtype, seed=T)
+    qs = [c.q(2 * group, T) for _ in range(3)]
+
+    def call(q):
+        out, lse = be.tree_sdpa(q, c.k, c.v, c.table, c.lens, 0.125)
+        return out, lse, be.cache_weights(torch.zeros(2, 2, c.slots, device="cuda"), q, lse, c.k, c.table, c.lens, 0.125)
+    want = [call(q) for q in qs]
+    streams = [torch.cuda.Stream() for _ in qs]
+    torch.cuda.synchronize()
+    got = [[] for _ in qs]
+    for _ in range(4):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(call(qs[i]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for i, runs in enumerate(got) for run in runs for a, b in zip(run, want[i]))
+
+
+def test_far_pages_of_trees():
+    """A pool of more than 2^31 elements under more than 16 rows."""
+    Hkv, page, D, T = 2, 512, 128, 9
+    pages = (1 << 31) // (Hkv * page * D) + 3
+    k = torch.zeros(pages, Hkv, page, D, dtype=torch.bfloat16, device="cuda")
+    v = torch.zeros_like(k)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    for i in (0, pages - 1):
+        k[i], v[i] = (torch.randn(Hkv, page, D, generator=g, device="cuda").to(torch.bfloat16) for _ in range(2))
+    table, lens = as_int([[pages - 1, 0]]), as_int([700])
+    q = torch.randn(1, 8, T, D, generator=g, device="cuda").to(torch.bfloat16)
+    out, lse = be.tree_sdpa(q, k, v, table, lens, 0.1)
+    res, tol = ref.tree_one(q[0], k, v, table[0], 700, 0.1)
+    ref.assert_within(out[0], res["out"], tol["out"], "out")
+    ref.assert_within(lse[0], res["lse"], tol["lse"], "lse")
+    w = be.cache_weights(torch.zeros(1, Hkv, 2 * page, device="cuda"), q, lse, k, table, lens, 0.1)
+    assert ((w.sum(-1) - 4 * T).abs() < 1e-3).all()
