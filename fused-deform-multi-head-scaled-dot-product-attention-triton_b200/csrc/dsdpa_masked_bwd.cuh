@@ -113,6 +113,30 @@ __device__ __forceinline__ void mma_halves(uint32_t d, uint32_t w, uint32_t b, u
         mma_ts(d, w + (s & 3) * 8 + (s >> 2) * 64, smem_desc(b + s * 2048, 128 * 128), idesc, add || s > 0);
 }
 
+// Sums of p dp and of p over this thread's 64 columns of the block's only key tile, whose scores and dP lie in tensor memory.
+template <bool CAP, bool BIAS>
+__device__ __noinline__ float2 weigh_dp(uint32_t s_at, uint32_t d_at, const ScoreConsts c, float lse, float slope2, float d0, int a, int e) {
+    const float unit = CAP ? c.cap_out : c.scale2;
+    float2 sum = make_float2(0.0f, 0.0f);
+#pragma unroll 1
+    for (int x = 0; x < 64; x += 32) {
+        float s[32], dp[32];
+        tmem_ld32(s_at + x, s);
+        tmem_ld32(d_at + x, dp);
+        tmem_wait_ld();
+        if (CAP) cap_scores(s, c);
+#pragma unroll
+        for (int y = 0; y < 32; y += 2) {
+            const float at = (float)(x + y);
+            float2 slope;
+            const float2 w = pair_weights<false, BIAS>(make_float2(s[y], s[y + 1]), unit, slope2, make_float2(d0 - at, d0 - at - 1.0f), make_float2(-lse, -lse), slope);
+            if (x + y >= a && x + y < e && w.x != 0.0f) { sum.x = fmaf(w.x, dp[y], sum.x); sum.y += w.x; }
+            if (x + y + 1 >= a && x + y + 1 < e && w.y != 0.0f) { sum.x = fmaf(w.y, dp[y + 1], sum.x); sum.y += w.y; }
+        }
+    }
+    return sum;
+}
+
 template <typename T, int HD, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 masked_dq_kernel(const __grid_constant__ MaskedParams p, const __grid_constant__ BwdStats st, const __grid_constant__ CUtensorMap mq,
@@ -282,11 +306,29 @@ masked_dq_kernel(const __grid_constant__ MaskedParams p, const __grid_constant__
         s_big[half][in_tile] = (unsigned char)(most >> 23);
         asm volatile("bar.sync 1, 256;" ::: "memory");
         float delta = s_part[0][in_tile] + s_part[1][in_tile];
+        const int pos = row + (p.Lk - p.Lq);
         const unsigned big = max((unsigned)s_big[0][in_tile], (unsigned)s_big[1][in_tile]);
         const float sigma = kScaled ? scale_down(big) : 1.0f;
         const long long at = (long long)bh * p.Lq + row;
         float lse = sees ? p.lse[at] : kNegInf;
         if (lse == kNegInf) lse = -kNegInf;                 // weight exp2(s - inf) = 0
+        bool ok = true;
+        if (n == 1) {
+            // A row of a few keys may have nearly all of its weight on one of them; its gradients are then differences in which out's
+            // rounding to storage shows (two keys, bf16: dq off by up to 5 %).  Where the keys are one tile delta comes from
+            // p and dp themselves.
+            const int n0 = first * kTileK + half * 64;
+            const uint32_t mine = sm_ring + 2 * L::kTileBytes + in_tile * 8;       // of the ring, which holds two tiles
+            ok = mbar_wait_bounded(bar_s, 0, p.err) && mbar_wait_bounded(bar_dp, 0, p.err);
+            tc_fence_after();
+            const float2 sum = weigh_dp<CAP, BIAS>(tmem + half * 64 + lanes, tmem + 256 + half * 64 + lanes, c, lse, slope2, (float)(pos - n0), r.x - n0, r.y - n0);
+            asm volatile("st.shared.v2.f32 [%0], {%1, %2};" :: "r"(mine + half * kTileQ * 8), "f"(sum.x), "f"(sum.y) : "memory");
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            float2 other;
+            asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(other.x), "=f"(other.y) : "r"(mine + (half ^ 1) * kTileQ * 8) : "memory");
+            const float all = half ? other.y + sum.y : sum.y + other.y;
+            if (sees && all != 0.0f) delta = (half ? other.x + sum.x : sum.x + other.x) / all;
+        }
         if (half == 0) {
             const bool odd = sees ? spoilt(lse, delta) : delta != delta;
             if (odd) s_odd = 1;
@@ -303,9 +345,7 @@ masked_dq_kernel(const __grid_constant__ MaskedParams p, const __grid_constant__
             }
         }
         const float ndelta = sees ? -delta * sigma : 0.0f;
-        const int pos = row + (p.Lk - p.Lq);
-        bool ok = true;
-        for (int i = 0; i < n; ++i) {
+        for (int i = 0; i < n && ok; ++i) {
             const uint32_t s_at = tmem + (i & 1) * kTileK + half * 64 + lanes, d_at = tmem + 256 + half * 64 + lanes;
             float w[64];
             if (!mbar_wait_bounded(bar_s + 8 * (i & 1), (i >> 1) & 1, p.err)) { ok = false; break; }

@@ -378,6 +378,25 @@ masked_simt_dq_kernel(const __grid_constant__ MaskedParams p, int qtiles) {
         simt_dot<HD>(sq, sk, s);
         simt_dot<HD>(sg, sv, dp);
         const float unit = simt_cap(s, p.sm_scale, p.cap);
+        if (sizeof(T) == 2 && end - first == 1) {
+            // the only tile: delta from p and dp themselves, as in masked_dq_kernel
+#pragma unroll
+            for (int r = 0; r < L::RM; ++r) {
+                const int i = q0 + ty * L::RM + r, pos = i + (p.Lk - p.Lq);
+                float sum = 0.0f, all = 0.0f;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const int key = n0 + tx + 16 * c;
+                    float w, ds;
+                    simt_grad(s[r][c], unit, false, p.slopes ? slope2 * fabsf((float)(pos - key)) : 0.0f, dp[r][c], lse[r], 0.0f, w, ds);
+                    if (key >= rg[r].x && key < rg[r].y && w != 0.0f) { sum += ds; all += w; }
+                }
+                sum = half_warp_sum(sum);
+                all = half_warp_sum(all);
+                if (all != 0.0f) delta[r] = sum / all;
+                if (tx == 0 && i < p.Lq) p.delta[(long long)bh * p.Lq + i] = delta[r];
+            }
+        }
 #pragma unroll
         for (int r = 0; r < L::RM; ++r) {
             const int pos = q0 + ty * L::RM + r + (p.Lk - p.Lq);

@@ -476,3 +476,52 @@ def test_far_pages_of_trees():
     ref.assert_within(lse[0], res["lse"], tol["lse"], "lse")
     w = be.cache_weights(torch.zeros(1, Hkv, 2 * page, device="cuda"), q, lse, k, table, lens, 0.1)
     assert ((w.sum(-1) - 4 * T).abs() < 1e-3).all()
+
+
+def few_key_bounds(q, k, v, do, sm, causal, cap, slopes):
+    """dq, dk in 64 bits and their bounds where delta is the weighted mean of dp in fp32: as in sequence_ref.attend, but
+    delta's own error is that of the weights, of the sums (N + 16 roundings of their terms) and of dp, with no rounding of out."""
+    storage, (B, H, M, D), N, g = q.dtype, q.shape, k.shape[2], q.shape[1] // k.shape[1]
+    u, e, a = ref.half_step(storage), ref.E32, abs(sm)
+    x = dict(causal=causal, softcap=cap, slopes=slopes)
+    res, tol = ref.masked(q, k, v, sm, dout=do, **x)
+    seen = ref.seen_mask(B, M, N, causal, None, q.device)[:, None]
+    dist = (torch.arange(M, device=q.device)[:, None] + (N - M) - torch.arange(N, device=q.device)).double().abs()
+    q, do, k, v = q.double(), do.double(), k.double().repeat_interleave(g, 1), v.double().repeat_interleave(g, 1)
+    s0 = sm * q @ k.transpose(-1, -2)
+    y = cap * torch.tanh(s0 / cap) if cap else s0
+    bias = slopes.double()[:, None, None] * dist if slopes is not None else torch.zeros_like(s0)
+    off = (D + 4) * e * a * (q.abs() @ k.abs().transpose(-1, -2)) + 8 * e * ((y - bias).abs() + y.abs() + bias) + 8 * e * cap
+    worst = 2 * torch.where(seen, off, torch.zeros_like(off)).amax(-1, keepdim=True)
+    p = torch.softmax((y - bias).masked_fill(~seen, -math.inf), -1)
+    dp = do @ v.transpose(-1, -2)
+    c = dp - (p * dp).sum(-1, keepdim=True)
+    slope = 1 - (y / cap) ** 2 if cap else torch.ones_like(y)
+    err_dp = (D + 2) * e * (do.abs() @ v.abs().transpose(-1, -2))
+    err_p = p * (2 * worst + 16 * e)
+    err_delta = (p * (err_dp + (N + 16) * e * dp.abs()) + err_p * c.abs()).sum(-1, keepdim=True)
+    ds = p * c * slope
+    err_ds = p * (err_delta + err_dp + c.abs() * 16 * e) + err_p * c.abs() + (u + 4 * e) * ds.abs()
+    if storage == torch.float16:
+        err_ds = err_ds + torch.where(seen, 2.0 ** -22, 0.0) * do.abs().amax()
+    dk = lambda z, w: a * (z.transpose(-1, -2) @ w).view(B, -1, g, N, D).sum(2)
+    tol["dq"] = ref.stored(res["dq"], storage) + a * (err_ds @ k.abs() + (N + 4) * e * (ds.abs() @ k.abs()))
+    tol["dk"] = ref.stored(res["dk"], storage) + dk(err_ds + (g * M + 4) * e * ds.abs(), q.abs())
+    return res, tol
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [16, 64, 128, 256])
+@pytest.mark.parametrize("Lq,Lk,causal", [(1, 1, True), (2, 2, True), (2, 2, False), (3, 3, True), (5, 4, False), (16, 16, True), (1, 64, False), (300, 2, False)])
+@pytest.mark.parametrize("softcap,bias", [(0.0, False), (4.0, True)])
+def test_gradients_of_rows_with_few_keys(dtype, D, Lq, Lk, causal, softcap, bias):
+    """Rows with nearly all of their weight on one key: gradients are small differences of large numbers."""
+    g = torch.Generator(device="cuda").manual_seed(D + Lq + Lk)
+    q, k, v, do = (torch.randn(4, h, n, D, generator=g, device="cuda").to(dtype) for h, n in ((4, Lq), (2, Lk), (2, Lk), (4, Lq)))
+    sm, slopes = 4 * D ** -0.5, torch.tensor([0.5, 0.1, 0.05, 0.01], device="cuda") if bias else None
+    kw = dict(causal=causal, softcap=softcap, slopes=slopes)
+    out, lse = be.masked_forward_raw(q, k, v, sm, **kw)
+    dq, dk, dv = be.masked_backward_raw(q, k, v, out, lse, do, sm, **kw)
+    res, tol = few_key_bounds(q, k, v, do, sm, causal, softcap, slopes)
+    for n, t in (("dq", dq), ("dk", dk), ("dv", dv)):
+        ref.assert_within(t, res[n], tol[n], n)
