@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const __gr
 // batch of rows loaded before any of it is stored the move is right in place too, and the blocks need
 // nothing from one another.  The next batch's key and page numbers are fetched while this one's rows
 // are on their way.  Bound by DRAM: every byte is read and written once.  Measured with the selection, 16 caches of up to
-// 16384 keys cut to 4096 (8 heads, D = 128): bf16 127 us (548 MB, 4.3 TB/s, of which the selection takes 20 us), fp32
+// 16384 keys cut to 4096 (8 heads, D = 128): bf16 130 us (548 MB, 4.2 TB/s, of which the selection takes 20 us), fp32
 // 214 us (5.1 TB/s).  Copies through a ring in shared memory took 140 us where this took 109.
 constexpr int kMoveThreads = 256, kMoveRows = 4, kMoveBlocks = 4;   // blocks an SM
 __global__ void __launch_bounds__(kMoveThreads, kMoveBlocks) evict_move_kernel(const __grid_constant__ EvictParams p, int width, int slices) {

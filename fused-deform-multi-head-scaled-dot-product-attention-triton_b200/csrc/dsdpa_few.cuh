@@ -9,8 +9,8 @@
 // instructions, with the queries arranged alike; and the value rows of two neighbouring keys, of which it
 // pairs up elements, as operands of eight.  The fifth-generation instructions, whose operands lie in shared
 // memory, need 128 rows and a pipeline of roles to do the same: for 64 caches of up to 8192 keys, 32 heads on 8, one
-// token each (D = 128, bf16) they take 254 us, this kernel 164 us (6.0 TB/s of the 6.5 that a copy reaches), and
-// weights_few_kernel 84 us (6.1 TB/s).  Bound by DRAM; a warp has 8 KB of loads in flight.
+// token each (D = 128, bf16) they take 254 us, this kernel 168 us (5.9 TB/s of the 6.5 that a copy reaches; capped 173, biased 194), and
+// weights_few_kernel 86 us (5.9 TB/s).  Bound by DRAM; a warp has 8 KB of loads in flight.
 #pragma once
 
 #include "dsdpa_cache_launch.h"

@@ -8,7 +8,7 @@
 // would take 32 log2(lanes)) and of which a lane then has 32 / lanes: the scores.  Their weights go through
 // shared memory back to all lanes.  The register tiles of dsdpa_cache_simt.cuh spend 16 rows' fmas on whatever rows
 // there are: for 64 caches of up to 8192 keys, 32 heads on 8, one token each (D = 128) they take 1150 us and
-// 723 us (weights), these kernels 320 us (6.2 TB/s of the 6.5 that a copy reaches) and 175 us (5.7).  Bound by DRAM;
+// 723 us (weights), these kernels 318 us (6.2 TB/s of the 6.5 that a copy reaches) and 174 us (5.7).  Bound by DRAM;
 // with 8 rows (522 us) by the arithmetic between the loads, two blocks an SM.
 #pragma once
 

@@ -119,7 +119,7 @@ __device__ __forceinline__ float rcp_approx(float x) {
 // tanh(a / 2), the cap's argument being a = 2 x / cap.  For |a| < 2 (scores below the cap) an odd polynomial, fitted to
 // the least largest relative error (5e-8; evaluated in fp32 1.5e-7): ten fma-pipe operations for two values where
 // the general form, 1 - 2 / (1 + e^a), takes four of the special-function unit, which is what these kernels run
-// out of: the capped backward over four sequences of 1571 image and text tokens (16 heads, D = 64) takes 245 us with
+// out of: the capped backward over four sequences of 1571 image and text tokens (16 heads, D = 64) took 245 us with
 // that form alone, 208 us with this one.
 constexpr int kTanhTerms = 7;
 __device__ __forceinline__ float tanh_term(int i) {
@@ -138,7 +138,7 @@ __device__ __forceinline__ bool is_small(float a) { return fabsf(a) < 2.0f; }
 // Any two values, each by the form that its own size asks for: what a score becomes does not depend on the others that a
 // warp happens to hold, hidden ones among them, and the general form, which is good to a step of 1, is not taken where
 // that is much of the result.  (Both forms for every value of a warp that has one above the cap: a forward all of whose
-// key tiles have some takes 224 us where the general form alone took 171, 4 x 16 heads of 2048, D = 64.)
+// key tiles have some takes 220 us where the general form alone took 171, 4 x 16 heads of 2048, D = 64.)
 __device__ __forceinline__ float2 half_tanh_any(float2 a) {
     const float2 t = half_tanh_small(a);
     return make_float2(is_small(a.x) ? t.x : half_tanh(a.x), is_small(a.y) ? t.y : half_tanh(a.y));

@@ -14,8 +14,8 @@
 // Both kernels: 8 warps of elementwise work (a thread has one row and 64 of its 128 columns), one warp of
 // TMA loads, one that issues the matrix instructions.
 //
-// Measured, 32 heads on 8 of 8192 x 8192, bf16, D = 128: 3.01 ms, 0.91 PFLOP/s by the formula's five products and 1.28
-// by the seven done; causal 1.63 ms (0.85); capped 4.13 ms; 4 x 16 heads of 2048, D = 64: 339 us (0.51).  D = 128 is near the
+// Measured, 32 heads on 8 of 8192 x 8192, bf16, D = 128: 3.14-3.29 ms, 0.86 PFLOP/s by the formula's five products and 1.20
+// by the seven done; causal 1.64 ms (0.84); capped 4.33-4.42 ms; 4 x 16 heads of 2048, D = 64: 345 us (0.50).  D = 128 is near the
 // products' rate; at D = 64 these are half as long and the elementwise work between them bounds.
 // Tiles of 64 columns, one for each half of the threads and half a turn apart, were slower: products of that
 // width wait for shared memory (3473 -> 4074 us, D = 128).

@@ -10,8 +10,8 @@
 // the other tile's products do, so that both units stay busy.  (Two query tiles in turn, rescaling only past a
 // threshold and the hand-over of registers are a published method of attention on this chip.)
 //
-// Measured, 32 heads on 8 of 8192 x 8192, bf16: D = 128 832-848 us (1.30 PFLOP/s, 0.79 of a large library matrix product's
-// rate), causal 457 us (1.20), capped 1.42 ms (0.77), causal with a bias 585 us (0.94); D = 64 0.79-0.94 ms.
+// Measured, 32 heads on 8 of 8192 x 8192, bf16: D = 128 842-845 us (1.30 PFLOP/s, 0.79 of a large library matrix product's
+// rate), causal 526-536 us (1.04), capped 1.35-1.37 ms (0.81), causal with a bias 611-614 us (0.90); D = 64 0.83-0.85 ms.
 // Bound by the softmax: of the special-function unit's time 0.63 is used at D = 64, since a scheduler has two
 // warps only and their chains (load, maximum, exp2, store) leave gaps.  A quarter of exp2 moved to the fma
 // pipes did not help (832 -> 875 us at D = 128, 813 -> 791 at 64), nor did going through capped scores 32 or 64 columns

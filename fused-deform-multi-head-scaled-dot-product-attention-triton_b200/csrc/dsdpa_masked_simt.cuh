@@ -4,7 +4,7 @@
 // (sums of rows).  A block has 64 queries (32 for 256 elements) and goes over keys 64 at a time, or has 64
 // keys and goes over queries.  The 16 threads that share a row exchange its maximum and sum by shuffles.
 // Bound by the fma pipe: a thread issues 32 packed fmas for eight 16-byte loads.  Measured, 8 heads of 2816 tokens, an image
-// prefix of 700, capped, D = 32: forward 208 us, backward 643 us (0.28 and 0.22 of the pipe's rate for the products
+// prefix of 700, capped, D = 32: forward 206 us, backward 655 us (0.28 and 0.22 of the pipe's rate for the products
 // alone; at D = 32 the cap, exp2 and masks are as much again).
 #pragma once
 

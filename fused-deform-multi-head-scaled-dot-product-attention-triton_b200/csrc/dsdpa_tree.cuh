@@ -7,7 +7,7 @@
 // accumulator (tensor memory holds both), joined at the end: one stream's softmax runs while the other's
 // products do, which matters when a handful of rows leaves a single warp with all of the softmax.
 // Taken for more than 16 rows (dsdpa_few.cuh has the others).  Measured, three caches of up to 65536 keys, 32 heads on 8, trees of
-// 29 tokens (116 rows), D = 128, fp16: 146 us without cap or bias (4.6 TB/s), 164 us biased, 181 us capped, 206 us
+// 29 tokens (116 rows), D = 128, fp16: 149 us without cap or bias (4.5 TB/s), 168 us biased, 184 us capped, 207 us
 // both, where reading the cache takes 103 us: bound by DRAM's latency and, with a cap, by the softmax's
 // arithmetic.  Loads by TMA, a box for each page, were slower (254 -> 320 us then): boxes are issued one by one.
 // Roles: warps 0-3 and 4-7 the streams' softmax, 8-11 copy rows (cp.async: any page size and stride, rows
