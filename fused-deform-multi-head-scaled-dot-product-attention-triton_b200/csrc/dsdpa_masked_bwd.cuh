@@ -511,14 +511,15 @@ masked_dkdv_kernel(const __grid_constant__ MaskedParams p, const __grid_constant
     int lo = 0x7fffffff, hi = 0;
     const unsigned* amax = st.amax + (long long)(b * p.Hq + hk * p.group) * st.n;
     unsigned top = 0, most = 0, odd = 0;
-    for (int i = tid; i < st.n; i += kBwdThreads) {
-        const int4 t = st.tiles[(long long)b * st.n + i];
-        const bool sees = t.x < k0 + kTileK && t.y > k0;
-        if (sees) { lo = min(lo, i); hi = max(hi, i + 1); }
-        for (int g = 0; g < p.group; ++g) {
-            const unsigned a = amax[(long long)g * st.n + i];
-            odd |= a >> 8 & 1u;
-            if (kScaled && sees) { top = max(top, a & 255u); most = max(most, a >> 16); }
+    for (int i = tid; i < p.group * st.n; i += kBwdThreads) {          // a head's tile a step: one wait for memory, mostly
+        const int tile = i % st.n;
+        const int4 t = st.tiles[(long long)b * st.n + tile];
+        const unsigned a = amax[i];
+        odd |= a >> 8 & 1u;
+        if (t.x < k0 + kTileK && t.y > k0) {
+            lo = min(lo, tile);
+            hi = max(hi, tile + 1);
+            if (kScaled) { top = max(top, a & 255u); most = max(most, a >> 16); }
         }
     }
     lo = warp_min(lo);

@@ -96,10 +96,10 @@ __device__ __forceinline__ void add_bias(float (&s)[N], float unit, float slope2
 // A warp's rows whose values' sums something non-finite reached: once more, from the keys they see alone.  A function of its own, which
 // finds its place by itself: nothing has to be kept for it while the block works.
 template <typename T>
-__device__ __noinline__ void redo_rows_forward(const MaskedParams& p, const unsigned* bad, int qtiles) {
+__device__ __noinline__ void redo_rows_forward(const MaskedParams& p, unsigned rows, int qtiles) {
     const int warp = threadIdx.x >> 5, bh = blockIdx.x % (p.B * p.Hq);
     const int row0 = (qtiles - 1 - (int)(blockIdx.x / (p.B * p.Hq))) * 2 * kTileQ + warp * 32;
-    for (unsigned rows = bad[warp]; rows; rows &= rows - 1) exact_row_forward<T>(p, bh / p.Hq, bh % p.Hq, row0 + __ffs(rows) - 1);
+    for (; rows; rows &= rows - 1) exact_row_forward<T>(p, bh / p.Hq, bh % p.Hq, row0 + __ffs(rows) - 1);
 }
 
 __device__ __forceinline__ int warp_min(int x) { return __reduce_min_sync(0xffffffffu, x); }
@@ -116,7 +116,6 @@ masked_fwd_kernel(const __grid_constant__ MaskedParams p, const __grid_constant_
     const uint32_t bar_q = bars, bar_s = bars + 8, bar_p = bars + 24, bar_o = bars + 40, bar_full = bars + 56,
                    bar_empty = bar_full + 8 * L::kStages, slot = bar_empty + 8 * L::kStages;
     __shared__ int s_lo[2], s_hi[2];
-    __shared__ unsigned s_bad[8];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     // longest rows first: with a causal mask these are the last ones
     const int bh = blockIdx.x % (p.B * p.Hq), b = bh / p.Hq, h = bh % p.Hq, hk = h / p.group;
@@ -396,14 +395,14 @@ masked_fwd_kernel(const __grid_constant__ MaskedParams p, const __grid_constant_
             if (row < p.Lq) p.lse[(long long)bh * p.Lq + row] = l != 0.0f ? m + log2f(l) : kNegInf;
             // (a sum of weights that is NaN is the row's own)
             const unsigned bad = __ballot_sync(0xffffffffu, row < p.Lq && !fine && l == l);
-            if (lane == 0) s_bad[warp] = bad;
-        } else if (lane == 0) s_bad[warp] = 0;
+            __syncwarp();
+            if (bad) redo_rows_forward<T>(p, bad, qtiles);
+        }
     }
     __syncwarp();
     tc_fence_before();
     __syncthreads();
     if (warp == 9) tmem_free(tmem, 512);
-    if (warp < 8 && s_bad[warp]) redo_rows_forward<T>(p, s_bad, qtiles);
 }
 
 }  // namespace dsdpa
