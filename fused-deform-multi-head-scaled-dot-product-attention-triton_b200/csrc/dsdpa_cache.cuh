@@ -117,7 +117,8 @@ __device__ __noinline__ void exact_row_tree(const CacheParams& p, int b, int h, 
         const T *k = row_of<T>(p.k, p.sk, 0, hk, 0), *v = row_of<T>(p.v, p.sv, 0, hk, 0);
         float q[8];
         load_piece<T>(row_of<T>(p.q, p.sq, b, h, t), rl.at, D, q);
-        for (int j0 = 0; j0 < n + real; j0 += kSteps * rl.places) {
+        // (a sum of weights that is NaN stays one, and out and lse with it)
+        for (int j0 = 0; j0 < n + real && !__any_sync(0xffffffffu, sum.l != sum.l); j0 += kSteps * rl.places) {
             RowPiece<T> kr[kSteps], vr[kSteps];
             float s[kSteps], w[kSteps], f[8];
             bool on[kSteps];
